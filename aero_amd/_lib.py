@@ -42,6 +42,13 @@ class AttnInput(ctypes.Structure):
                 ("k_norm_w", vp), ("qk_eps", c_float), ("qk_flags", c_int)]
 
 
+class KvPool(ctypes.Structure):
+    """aero_kv_pool_t of include/aero_hip.h, field for field."""
+    _fields_ = [("kv_dt", c_int), ("page", c_int64), ("n_layers", c_int64),
+                ("n_pages", c_int64), ("n_head_kv", c_int64), ("head_dim", c_int64),
+                ("value_dim", c_int64), ("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp)]
+
+
 # name -> (restype, argtypes), exactly the prototypes of include/aero_hip.h
 PROTOTYPES = {
     # reference-compatible host ABI
@@ -189,6 +196,20 @@ PROTOTYPES = {
     "aero_hip_attention": (c_int, [vp, c_int, vp, vp, vp, vp, vp, c_int64, c_int64, c_int64,
                                    c_int64, c_int64, c_float, vp, vp, c_int64, c_int, vp,
                                    c_int64, vp]),
+    "aero_hip_attention_sinks_workspace": (c_int64, [c_int] + [c_int64] * 6 + [c_int, c_int]),
+    "aero_hip_attention_sinks": (c_int, [vp, c_int, vp, vp, vp, vp, vp, c_int64, c_int64,
+                                         c_int64, c_int64, c_int64, c_float, vp, vp, c_int64,
+                                         c_int, c_int, vp, c_int64, vp]),
+    "aero_hip_paged_attention_workspace": (c_int64, [POINTER(KvPool)] + [c_int64] * 4),
+    "aero_hip_paged_attention": (c_int, [POINTER(KvPool), c_int64, vp, vp, vp, c_int64, vp,
+                                         c_int64, c_int64, c_int64, c_float, c_int, c_int, vp,
+                                         vp, c_int64, vp]),
+    "aero_hip_paged_kv_write": (c_int, [POINTER(KvPool), c_int64, vp, vp, vp, c_int64, vp,
+                                        c_int64, c_int64, vp, vp]),
+    "aero_hip_paged_kv_read": (c_int, [POINTER(KvPool), c_int64, vp, vp, vp, c_int64, vp,
+                                       c_int64, c_int64, vp, vp]),
+    "aero_hip_kv_pages_copy": (c_int, [POINTER(KvPool), ip, ip, c_int64, vp]),
+    "aero_hip_write_i32": (c_int, [vp, c_int64, POINTER(c_int64), ip, c_int64, vp]),
     "aero_hip_kv_write": (c_int, [c_int, vp, c_int64, c_int64, c_int64, c_int64, c_int64, vp,
                                   vp, vp]),
     "aero_hip_softmax_rows": (c_int, [vp, vp, c_int64, c_int64, vp]),

@@ -24,7 +24,7 @@
 //
 // Results differ from the reference's serial loops in summation order and in
 // the exp of the GPU's math library: <= 1e-5 relative to the output's scale.
-#include "common.hpp"
+#include "attn_common.hpp"
 #include "aero_hip.h"
 
 #include <cmath>
@@ -251,9 +251,6 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attn_kernel(AttnParams p) {
 // key tile of the chunk (balanced under a causal mask); their (m, l, acc) are
 // merged through LDS. Workgroups run the last query tiles (in causal prefill
 // the longest) first.
-template <int DT>
-constexpr int kv_bits() { return DT == 0 ? 32 : (DT == 1 ? 8 : 4); }
-
 // Loaded in place of an absent position array: the loads of positions stay
 // unconditional (a load under a branch makes the compiler wait for every
 // load in flight where the branches join) and the value is selected after.
@@ -263,42 +260,6 @@ __device__ __forceinline__ int32_t position_or(const int32_t* pos, int64_t i, in
     const int32_t* a = pos ? pos + i : &g_no_position;
     const int32_t v = *a;
     return pos ? v : (int32_t)dflt;
-}
-
-// N bytes (4-byte multiple, or 2) at p into words.
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
-    if constexpr (N % 16 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 16; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(p + 16 * i);
-            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-        }
-    } else if constexpr (N % 8 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 8; ++i) {
-            const uint2 x = *reinterpret_cast<const uint2*>(p + 8 * i);
-            w[2 * i] = x.x; w[2 * i + 1] = x.y;
-        }
-    } else if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-    } else {
-        static_assert(N == 2, "slice size");
-        w[0] = *reinterpret_cast<const uint16_t*>(p);
-    }
-}
-
-// element e of a slice held as words: fp32 bits, int8 or int4 (low nibble first)
-template <int DT>
-__device__ __forceinline__ float slice_elem(const uint32_t* w, int e) {
-    if constexpr (DT == 0) {
-        return __uint_as_float(w[e]);
-    } else if constexpr (DT == 1) {
-        return (float)((int32_t)(w[e >> 2] << (24 - 8 * (e & 3))) >> 24);
-    } else {
-        return (float)((int32_t)(w[e >> 3] << (28 - 4 * (e & 7))) >> 28);
-    }
 }
 
 template <int DT, int D, int DV>
@@ -581,67 +542,6 @@ __global__ __launch_bounds__(256) void attn_mfma_kernel(AttnParams p) {
 //    value tile, lane group g's k-slots being keys 4g..4g+3 of each half:
 //    the probabilities the lane holds after the scores, and the codes of
 //    those keys' value rows it loaded.
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef unsigned int v2u __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ h2 u32_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
-__device__ __forceinline__ uint32_t h2_u32(h2 h) { return __builtin_bit_cast(uint32_t, h); }
-
-// the 8 codes of key-slice step s as fp16, in the order described above
-template <int DT>
-__device__ __forceinline__ h8 key_codes(const uint32_t* k, int s) {
-    constexpr uint32_t E = 0x64646464u;
-    if constexpr (DT == 1) {
-        const h2 off = h2{(_Float16)-1152.f, (_Float16)-1152.f};
-        const uint32_t u0 = k[2 * s] ^ 0x80808080u, u1 = k[2 * s + 1] ^ 0x80808080u;
-        const h2 a0 = u32_h2(__builtin_amdgcn_perm(E, u0, 0x04010400u)) + off;
-        const h2 a1 = u32_h2(__builtin_amdgcn_perm(E, u0, 0x04030402u)) + off;
-        const h2 a2 = u32_h2(__builtin_amdgcn_perm(E, u1, 0x04010400u)) + off;
-        const h2 a3 = u32_h2(__builtin_amdgcn_perm(E, u1, 0x04030402u)) + off;
-        return __builtin_bit_cast(h8, make_uint4(h2_u32(a0), h2_u32(a1), h2_u32(a2), h2_u32(a3)));
-    } else {
-        const h2 off = h2{(_Float16)-1032.f, (_Float16)-1032.f};
-        const uint32_t u = k[s] ^ 0x88888888u;
-        const uint32_t lo = u & 0x0F0F0F0Fu, hi = (u >> 4) & 0x0F0F0F0Fu;
-        const h2 a0 = u32_h2(__builtin_amdgcn_perm(E, lo, 0x04020400u)) + off;  // 0, 4
-        const h2 a1 = u32_h2(__builtin_amdgcn_perm(E, lo, 0x04030401u)) + off;  // 2, 6
-        const h2 a2 = u32_h2(__builtin_amdgcn_perm(E, hi, 0x04020400u)) + off;  // 1, 5
-        const h2 a3 = u32_h2(__builtin_amdgcn_perm(E, hi, 0x04030401u)) + off;  // 3, 7
-        return __builtin_bit_cast(h8, make_uint4(h2_u32(a0), h2_u32(a1), h2_u32(a2), h2_u32(a3)));
-    }
-}
-
-// element i of a key-slice operand is slice element 8s + key_order(i)
-template <int DT>
-__device__ __forceinline__ constexpr int key_order(int i) {
-    return DT == 1 ? i : ((i & 1) ? 4 : 0) + ((i >> 1) & 1) * 2 + (i >> 2);
-}
-
-// codes of element t of two value rows (words a, b of those rows) as fp16
-// (code_a, code_b)
-template <int DT>
-__device__ __forceinline__ uint32_t value_pair(const uint32_t* a, const uint32_t* b, int t) {
-    if constexpr (DT == 1) {
-        const uint32_t byte = (uint32_t)(t & 3);
-        const uint32_t sel = 0x0C000C00u | ((4u + byte) << 16) | byte;
-        const uint32_t x = __builtin_amdgcn_perm(b[t >> 2], a[t >> 2], sel) ^ 0x64806480u;
-        return h2_u32(u32_h2(x) + h2{(_Float16)-1152.f, (_Float16)-1152.f});
-    } else {
-        const uint32_t byte = (uint32_t)((t >> 1) & 3);
-        const uint32_t sel = 0x0C000C00u | ((4u + byte) << 16) | byte;
-        uint32_t x = __builtin_amdgcn_perm(b[t >> 3], a[t >> 3], sel);
-        x = ((t & 1) ? (x >> 4) : x) & 0x000F000Fu;
-        return h2_u32(u32_h2(x ^ 0x64086408u) + h2{(_Float16)-1032.f, (_Float16)-1032.f});
-    }
-}
-
-// v = 2^scale-shifted value split into fp16 hi and lo
-__device__ __forceinline__ void split2(float v, _Float16& hi, _Float16& lo) {
-    hi = (_Float16)v;
-    lo = (_Float16)(v - (float)hi);
-}
-
 // One kv head's keys [c0, c0 + n) of an integer cache, read through buffer
 // descriptors. A 16-key tile's descriptors start at its first key and end at
 // the chunk's last one, so a lane's byte offsets within a tile are fixed (no
@@ -750,12 +650,6 @@ struct IntKv {
         }
     }
 };
-
-// 2^e as a float, e in [-126, 127]
-__device__ __forceinline__ float pow2i(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // Per 32-key step:
 //  * the scores are kept in log2 units (the softmax scale times log2(e)
@@ -1489,6 +1383,67 @@ bool attention_dev(const float* q, int kv_dt, const void* k, const float* k_scal
     return true;
 }
 
+// (attn_rows.hip)
+int64_t rows_sinks_workspace(int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_dim,
+                             int64_t value_dim, int64_t n_kv, int window, int sinks, int kv_dt);
+bool rows_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_scale, const void* v,
+                    const float* v_scale, float* out, int64_t n_q, int64_t n_head,
+                    int64_t n_head_kv, int64_t head_dim, int64_t value_dim, float scale,
+                    const int32_t* qpos, const int32_t* kpos, int64_t n_kv, int window, int sinks,
+                    void* ws, int64_t ws_bytes, hipStream_t s);
+
+// Sizes that attention_sinks takes (as attention_dev, and 32-bit key places)
+bool sinks_sizes_ok(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_dim,
+                    int64_t value_dim, int64_t n_kv, int sinks) {
+    if (n_q <= 0 || n_head <= 0 || n_head_kv <= 0 || head_dim <= 0 || value_dim <= 0 ||
+        n_kv <= 0 || n_head % n_head_kv || head_dim > 256 || value_dim > 256 || kv_dt < 0 ||
+        kv_dt > 2 || (kv_dt == 0 && (head_dim % 4 || value_dim % 4)) ||
+        (kv_dt == 2 && (head_dim % 2 || value_dim % 2)) || sinks < 0 ||
+        n_kv >= (int64_t(1) << 30) || n_q > (int64_t(1) << 28) / n_head ||
+        n_head_kv > (int64_t(1) << 16)) {
+        set_error("attention_sinks: bad sizes (kv_dt=%d n_q=%lld n_head=%lld n_head_kv=%lld "
+                  "head_dim=%lld value_dim=%lld n_kv=%lld sinks=%d)", kv_dt, (long long)n_q,
+                  (long long)n_head, (long long)n_head_kv, (long long)head_dim,
+                  (long long)value_dim, (long long)n_kv, sinks);
+        return false;
+    }
+    return true;
+}
+
+int64_t attn_sinks_workspace_bytes(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv,
+                                   int64_t head_dim, int64_t value_dim, int64_t n_kv, int window,
+                                   int sinks) {
+    if (!sinks_sizes_ok(kv_dt, n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, sinks))
+        return -1;
+    if (window <= 0 || sinks == 0)
+        return attn_workspace_bytes(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv);
+    return rows_sinks_workspace(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks,
+                                kv_dt);
+}
+
+// attention_dev with the keys at positions below `sinks` kept by the window too.
+// Without a window, or without sinks, it is attention_dev's call.
+bool attention_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_scale,
+                         const void* v, const float* v_scale, float* out, int64_t n_q,
+                         int64_t n_head, int64_t n_head_kv, int64_t head_dim, int64_t value_dim,
+                         float scale, const int32_t* qpos, const int32_t* kpos, int64_t n_kv,
+                         int window, int sinks, void* ws, int64_t ws_bytes, hipStream_t s) {
+    if (!sinks_sizes_ok(kv_dt, n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, sinks))
+        return false;
+    if (window <= 0 || sinks == 0)
+        return attention_dev(q, kv_dt, k, k_scale, v, v_scale, out, n_q, n_head, n_head_kv,
+                             head_dim, value_dim, scale, qpos, kpos, n_kv, window, ws, ws_bytes,
+                             s);
+    if (q == nullptr || k == nullptr || v == nullptr || out == nullptr ||
+        (kv_dt != 0 && (k_scale == nullptr || v_scale == nullptr)) ||
+        (kv_dt == 0 && (!aligned16(k) || !aligned16(v)))) {
+        set_error("attention_sinks: null pointer, or fp32 K / V that are not 16-byte aligned");
+        return false;
+    }
+    return rows_sinks_dev(q, kv_dt, k, k_scale, v, v_scale, out, n_q, n_head, n_head_kv, head_dim,
+                          value_dim, scale, qpos, kpos, n_kv, window, sinks, ws, ws_bytes, s);
+}
+
 bool kv_write_dev(int dt, const float* x, int64_t n_tok, int64_t heads, int64_t dim,
                   int64_t phys0, int64_t cap, void* q, float* scale, hipStream_t s) {
     if (x == nullptr || q == nullptr || n_tok < 0 || heads <= 0 || dim <= 0 || cap <= 0 ||
@@ -1545,6 +1500,28 @@ int aero_hip_attention(const float* q, int kv_dt, const void* k, const float* k_
     return aero::attention_dev(q, kv_dt, k, k_scale, v, v_scale, out, n_q, n_head, n_head_kv,
                                head_dim, value_dim, scale, qpos, kpos, n_kv, window, workspace,
                                ws_bytes, (hipStream_t)stream) ? 1 : 0;
+}
+
+int64_t aero_hip_attention_sinks_workspace(int kv_dt, int64_t n_q, int64_t n_head,
+                                           int64_t n_head_kv, int64_t head_dim,
+                                           int64_t value_dim, int64_t n_kv, int window,
+                                           int sinks) {
+    aero::clear_error();
+    return aero::attn_sinks_workspace_bytes(kv_dt, n_q, n_head, n_head_kv, head_dim, value_dim,
+                                            n_kv, window, sinks);
+}
+
+int aero_hip_attention_sinks(const float* q, int kv_dt, const void* k, const float* k_scale,
+                             const void* v, const float* v_scale, float* out, int64_t n_q,
+                             int64_t n_head, int64_t n_head_kv, int64_t head_dim,
+                             int64_t value_dim, float scale, const int32_t* qpos,
+                             const int32_t* kpos, int64_t n_kv, int window, int sinks,
+                             void* workspace, int64_t ws_bytes, void* stream) {
+    aero::clear_error();
+    return aero::attention_sinks_dev(q, kv_dt, k, k_scale, v, v_scale, out, n_q, n_head,
+                                     n_head_kv, head_dim, value_dim, scale, qpos, kpos, n_kv,
+                                     window, sinks, workspace, ws_bytes,
+                                     (hipStream_t)stream) ? 1 : 0;
 }
 
 int aero_hip_kv_write(int dt, const float* x, int64_t n_tok, int64_t heads, int64_t dim,

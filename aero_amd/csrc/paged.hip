@@ -1,0 +1,338 @@
+// A paged KV cache's rows and pages: new keys and values into their pages
+// (quantised as include/aero/kv.hpp:62-92), rows back as fp32 (src/kv.cpp:30-46),
+// pages copied for forks and compaction, table entries written in stream order.
+//
+// A vector (token, kv head) of position pos of sequence s lies in page
+// table[s][pos / page], row pos % page of the head's [page, dim] block.
+#include "paged.hpp"
+
+#include <climits>
+#include <cmath>
+#include <memory>
+#include <new>
+
+namespace aero {
+
+bool pool_ok(const aero_kv_pool_t& p, const char* what) {
+    if (p.kv_dt < 0 || p.kv_dt > 2 || p.page < 16 || p.page > 256 || (p.page & (p.page - 1)) ||
+        p.n_layers <= 0 || p.n_pages <= 0 || p.n_head_kv <= 0 || p.head_dim <= 0 ||
+        p.value_dim <= 0 || p.head_dim > 256 || p.value_dim > 256 || p.n_pages > INT_MAX ||
+        p.n_layers > (1 << 20) || p.n_head_kv > 65535 ||
+        (p.kv_dt == 0 && (p.head_dim % 4 || p.value_dim % 4)) ||
+        (p.kv_dt == 2 && (p.head_dim % 2 || p.value_dim % 2))) {
+        set_error("%s: bad pool (kv_dt=%d page=%lld layers=%lld pages=%lld heads=%lld "
+                  "head_dim=%lld value_dim=%lld; pages of 16-256 tokens, a power of two; dims up "
+                  "to 256, a multiple of 4 in fp32, of 2 in int4)", what, p.kv_dt,
+                  (long long)p.page, (long long)p.n_layers, (long long)p.n_pages,
+                  (long long)p.n_head_kv, (long long)p.head_dim, (long long)p.value_dim);
+        return false;
+    }
+    if (p.k == nullptr || p.v == nullptr || !aligned16(p.k) || !aligned16(p.v) ||
+        (p.kv_dt != 0 && (p.k_scale == nullptr || p.v_scale == nullptr ||
+                          !aligned16(p.k_scale) || !aligned16(p.v_scale)))) {
+        set_error("%s: the pool's K, V and scales must be there and 16-byte aligned", what);
+        return false;
+    }
+    return true;
+}
+
+namespace {
+
+struct RowsIo {
+    float* rows[2];        // k, v: [n_seq, n_q, heads, dim]
+    uint8_t* pages[2];
+    float* scales[2];
+    const int32_t* table;
+    const int32_t* lens;
+    int32_t* bad;
+    int32_t dim[2];
+    int32_t n_q, heads, n_pages, max_pages, shift;
+    int64_t n_rows;        // n_seq * n_q * heads
+};
+
+// The vector of the pool that row r is; -1: no token, or no page
+__device__ __forceinline__ int64_t pool_vector(const RowsIo& p, int64_t r) {
+    const int64_t tok = r / p.heads;
+    const int h = (int)(r - tok * p.heads);
+    const int64_t s = tok / p.n_q;
+    const int64_t pos = (int64_t)p.lens[s] - p.n_q + (tok - s * p.n_q);
+    if (pos < 0) return -1;
+    const int64_t col = pos >> p.shift;
+    const int32_t page = col < p.max_pages ? p.table[s * p.max_pages + col] : -1;
+    if (page < 0 || page >= p.n_pages) {
+        if (p.bad != nullptr) *p.bad = 1;
+        return -1;
+    }
+    return (((int64_t)page * p.heads + h) << p.shift) + (pos & ((1 << p.shift) - 1));
+}
+
+// A wave a row of K (blockIdx.y 0) or V (1), element by element.
+template <int DT>
+__global__ __launch_bounds__(64) void paged_write_kernel(RowsIo p) {
+    const int w = blockIdx.y, dim = p.dim[w], lane = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    const int64_t vec = pool_vector(p, r);
+    if (vec < 0) return;
+    const float* x = p.rows[w] + r * dim;
+    if constexpr (DT == 0) {
+        float* o = reinterpret_cast<float*>(p.pages[w]) + vec * dim;
+        for (int i = lane; i < dim; i += 64) o[i] = x[i];
+    } else {
+        float amax = 0.0f;
+        for (int i = lane; i < dim; i += 64) amax = fmaxf(amax, fabsf(x[i]));
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
+        constexpr float top = DT == 1 ? 127.0f : 7.0f;
+        const float sc = amax > 0.0f ? amax / top : 1.0f;
+        if (lane == 0) p.scales[w][vec] = sc;
+        auto code = [&](float v) { return (int)fminf(fmaxf(roundf(v / sc), -top), top); };
+        if constexpr (DT == 1) {
+            int8_t* o = reinterpret_cast<int8_t*>(p.pages[w]) + vec * dim;
+            for (int i = lane; i < dim; i += 64) o[i] = (int8_t)code(x[i]);
+        } else {
+            uint8_t* o = p.pages[w] + vec * (dim / 2);
+            for (int i = lane; i < dim / 2; i += 64)
+                o[i] = (uint8_t)((code(x[2 * i]) & 15) | ((code(x[2 * i + 1]) & 15) << 4));
+        }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(64) void paged_read_kernel(RowsIo p) {
+    const int w = blockIdx.y, dim = p.dim[w], lane = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    const int64_t vec = pool_vector(p, r);
+    float* o = p.rows[w] + r * dim;
+    const float sc = DT != 0 && vec >= 0 ? p.scales[w][vec] : 0.0f;
+    for (int i = lane; i < dim; i += 64) {
+        float v = 0.0f;
+        if (vec >= 0) {
+            if constexpr (DT == 0) {
+                v = reinterpret_cast<const float*>(p.pages[w])[vec * dim + i];
+            } else if constexpr (DT == 1) {
+                v = (float)reinterpret_cast<const int8_t*>(p.pages[w])[vec * dim + i] * sc;
+            } else {
+                const uint8_t b = p.pages[w][vec * (dim / 2) + i / 2];
+                const int n = (i & 1) ? b >> 4 : b & 15;
+                v = (float)(n >= 8 ? n - 16 : n) * sc;
+            }
+        }
+        o[i] = v;
+    }
+}
+
+bool rows_io(const aero_kv_pool_t& pool, int64_t layer, float* k, float* v, const int32_t* table,
+             int64_t max_pages, const int32_t* lens, int64_t n_seq, int64_t n_q, int32_t* bad,
+             const char* what, RowsIo& p) {
+    if (!pool_ok(pool, what)) return false;
+    if (layer < 0 || layer >= pool.n_layers || n_seq < 0 || n_q <= 0 || max_pages <= 0 ||
+        max_pages > (int64_t(1) << 30) / pool.page || n_q > (int64_t(1) << 30) ||
+        n_seq > INT_MAX / (n_q * pool.n_head_kv)) {
+        set_error("%s: bad sizes (layer=%lld n_seq=%lld n_q=%lld max_pages=%lld)", what,
+                  (long long)layer, (long long)n_seq, (long long)n_q, (long long)max_pages);
+        return false;
+    }
+    if (n_seq > 0 && (k == nullptr || v == nullptr || table == nullptr || lens == nullptr)) {
+        set_error("%s: null pointer", what);
+        return false;
+    }
+    const PoolLayer at = pool_layer(pool, layer);
+    p.rows[0] = k; p.rows[1] = v;
+    p.pages[0] = at.k; p.pages[1] = at.v;
+    p.scales[0] = at.ks; p.scales[1] = at.vs;
+    p.table = table; p.lens = lens; p.bad = bad;
+    p.dim[0] = (int32_t)pool.head_dim; p.dim[1] = (int32_t)pool.value_dim;
+    p.n_q = (int32_t)n_q; p.heads = (int32_t)pool.n_head_kv;
+    p.n_pages = (int32_t)pool.n_pages; p.max_pages = (int32_t)max_pages;
+    p.shift = 0;
+    while ((1 << p.shift) < pool.page) ++p.shift;
+    p.n_rows = n_seq * n_q * pool.n_head_kv;
+    return true;
+}
+
+// ------------------------------------------------------------------- pages
+constexpr int kCopyPairs = 256;   // pairs a launch (by value: 2 KB of arguments)
+
+struct PageCopy {
+    uint8_t* base[4];        // K, V, their scales
+    int64_t bytes[4];        // of a page in one layer (0: no such plane)
+    int64_t layer[4];        // from a layer to the next
+    int32_t src[kCopyPairs], dst[kCopyPairs];
+};
+
+// Workgroup (x, pair, layer): 16-byte pieces of the page's planes, one after the
+// other, 256 at a time.
+__global__ __launch_bounds__(256) void pages_copy_kernel(PageCopy p) {
+    const int64_t src = p.src[blockIdx.y], dst = p.dst[blockIdx.y];
+    const int64_t step = (int64_t)gridDim.x * 256;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const v4u* a = reinterpret_cast<const v4u*>(p.base[x] + blockIdx.z * p.layer[x] +
+                                                    src * p.bytes[x]);
+        v4u* b = reinterpret_cast<v4u*>(p.base[x] + blockIdx.z * p.layer[x] + dst * p.bytes[x]);
+        for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < p.bytes[x] / 16; i += step)
+            b[i] = a[i];
+    }
+}
+
+constexpr int kEdits = 256;
+struct Edits {
+    int32_t* base;
+    int64_t at[kEdits];
+    int32_t value[kEdits];
+    int32_t n;
+};
+__global__ __launch_bounds__(256) void write_i32_kernel(Edits e) {
+    const int i = threadIdx.x;
+    if (i < e.n) e.base[e.at[i]] = e.value[i];
+}
+
+bool pages_copy_dev(const aero_kv_pool_t& pool, const int32_t* src, const int32_t* dst, int64_t n,
+                    hipStream_t s) {
+    if (!pool_ok(pool, "kv_pages_copy")) return false;
+    if (n < 0 || (n > 0 && (src == nullptr || dst == nullptr)) || n > pool.n_pages ||
+        pool.n_layers > 65535) {
+        set_error("kv_pages_copy: bad list of %lld pairs (a pool of %lld pages, at most 65535 "
+                  "layers)", (long long)n, (long long)pool.n_pages);
+        return false;
+    }
+    // every destination once, and none of them a source: the copies then have no
+    // order among them
+    std::unique_ptr<uint8_t[]> seen(new (std::nothrow) uint8_t[(size_t)pool.n_pages]());
+    if (!seen) {
+        set_error("kv_pages_copy: out of host memory");
+        return false;
+    }
+    for (int64_t i = 0; i < n; ++i) {
+        if (src[i] < 0 || src[i] >= pool.n_pages || dst[i] < 0 || dst[i] >= pool.n_pages) {
+            set_error("kv_pages_copy: pair %lld (%d -> %d) is outside the pool's %lld pages",
+                      (long long)i, src[i], dst[i], (long long)pool.n_pages);
+            return false;
+        }
+        seen[src[i]] |= 1;
+        if (seen[dst[i]] & 2) {
+            set_error("kv_pages_copy: page %d is a destination twice", dst[i]);
+            return false;
+        }
+        seen[dst[i]] |= 2;
+    }
+    for (int64_t i = 0; i < n; ++i)
+        if (seen[dst[i]] & 1) {
+            set_error("kv_pages_copy: page %d is a source and a destination", dst[i]);
+            return false;
+        }
+    PageCopy p{};
+    const PoolLayer l0 = pool_layer(pool, 0);
+    const int64_t vecs = pool.n_head_kv * pool.page;
+    void* base[4] = {l0.k, l0.v, l0.ks, l0.vs};
+    const int64_t bytes[4] = {vecs * kv_vec_bytes(pool.kv_dt, pool.head_dim),
+                              vecs * kv_vec_bytes(pool.kv_dt, pool.value_dim),
+                              pool.kv_dt ? vecs * 4 : 0, pool.kv_dt ? vecs * 4 : 0};
+    int64_t most = 0;
+    for (int x = 0; x < 4; ++x) {
+        p.base[x] = static_cast<uint8_t*>(base[x]);
+        p.bytes[x] = bytes[x];
+        p.layer[x] = bytes[x] * pool.n_pages;
+        most = bytes[x] > most ? bytes[x] : most;
+    }
+    const unsigned gx = (unsigned)((most + 4095) / 4096);
+    for (int64_t i = 0; i < n; i += kCopyPairs) {
+        const int m = (int)(n - i < kCopyPairs ? n - i : kCopyPairs);
+        for (int x = 0; x < m; ++x) {
+            p.src[x] = src[i + x];
+            p.dst[x] = dst[i + x];
+        }
+        if (!launch("pages_copy_kernel", pages_copy_kernel,
+                    dim3(gx, (unsigned)m, (unsigned)pool.n_layers), dim3(256), 0, s, p))
+            return false;
+    }
+    return true;
+}
+
+}  // namespace
+}  // namespace aero
+
+extern "C" {
+
+int aero_hip_paged_kv_write(const aero_kv_pool_t* pool, int64_t layer, const float* k,
+                            const float* v, const int32_t* table, int64_t max_pages,
+                            const int32_t* lens, int64_t n_seq, int64_t n_q, int32_t* bad,
+                            void* stream) {
+    using namespace aero;
+    clear_error();
+    RowsIo p{};
+    if (pool == nullptr) {
+        set_error("paged_kv_write: null pool");
+        return 0;
+    }
+    if (!rows_io(*pool, layer, const_cast<float*>(k), const_cast<float*>(v), table, max_pages,
+                 lens, n_seq, n_q, bad, "paged_kv_write", p))
+        return 0;
+    if (p.n_rows == 0) return 1;
+    return launch("paged_write_kernel",
+                  pool->kv_dt == 0 ? paged_write_kernel<0>
+                                   : (pool->kv_dt == 1 ? paged_write_kernel<1>
+                                                       : paged_write_kernel<2>),
+                  dim3((unsigned)p.n_rows, 2), dim3(64), 0, (hipStream_t)stream, p) ? 1 : 0;
+}
+
+int aero_hip_paged_kv_read(const aero_kv_pool_t* pool, int64_t layer, float* k, float* v,
+                           const int32_t* table, int64_t max_pages, const int32_t* lens,
+                           int64_t n_seq, int64_t n_q, int32_t* bad, void* stream) {
+    using namespace aero;
+    clear_error();
+    RowsIo p{};
+    if (pool == nullptr) {
+        set_error("paged_kv_read: null pool");
+        return 0;
+    }
+    if (!rows_io(*pool, layer, k, v, table, max_pages, lens, n_seq, n_q, bad, "paged_kv_read", p))
+        return 0;
+    if (p.n_rows == 0) return 1;
+    return launch("paged_read_kernel",
+                  pool->kv_dt == 0 ? paged_read_kernel<0>
+                                   : (pool->kv_dt == 1 ? paged_read_kernel<1>
+                                                       : paged_read_kernel<2>),
+                  dim3((unsigned)p.n_rows, 2), dim3(64), 0, (hipStream_t)stream, p) ? 1 : 0;
+}
+
+int aero_hip_kv_pages_copy(const aero_kv_pool_t* pool, const int32_t* src, const int32_t* dst,
+                           int64_t n, void* stream) {
+    aero::clear_error();
+    if (pool == nullptr) {
+        aero::set_error("kv_pages_copy: null pool");
+        return 0;
+    }
+    return aero::pages_copy_dev(*pool, src, dst, n, (hipStream_t)stream) ? 1 : 0;
+}
+
+int aero_hip_write_i32(int32_t* base, int64_t n_base, const int64_t* at, const int32_t* value,
+                       int64_t n, void* stream) {
+    using namespace aero;
+    clear_error();
+    if (n < 0 || n_base < 0 || (n > 0 && (base == nullptr || at == nullptr || value == nullptr))) {
+        set_error("write_i32: bad arguments");
+        return 0;
+    }
+    for (int64_t i = 0; i < n; ++i)
+        if (at[i] < 0 || at[i] >= n_base || (i > 0 && at[i] <= at[i - 1])) {
+            set_error("write_i32: index %lld outside %lld elements, or not above the one before "
+                      "it", (long long)at[i], (long long)n_base);
+            return 0;
+        }
+    Edits e{};
+    e.base = base;
+    for (int64_t i = 0; i < n; i += kEdits) {
+        e.n = (int32_t)(n - i < kEdits ? n - i : kEdits);
+        for (int x = 0; x < e.n; ++x) {
+            e.at[x] = at[i + x];
+            e.value[x] = value[i + x];
+        }
+        if (!launch("write_i32_kernel", write_i32_kernel, dim3(1), dim3(256), 0,
+                    (hipStream_t)stream, e))
+            return 0;
+    }
+    return 1;
+}
+
+}  // extern "C"

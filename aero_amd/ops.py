@@ -574,17 +574,21 @@ def kv_write(dt: int, x: DeviceArray, n_tok: int, heads: int, dim: int, q: Devic
 
 
 _attn_ws = Workspace("attention chunk partials")
+_rows_ws = Workspace("attention row parts")
 
 
 def attention(q: DeviceArray, k: DeviceArray, v: DeviceArray, out: DeviceArray, n_q: int,
               n_head: int, n_head_kv: int, head_dim: int, value_dim: int, n_kv: int,
               scale: float, qpos: DeviceArray | None = None, kpos: DeviceArray | None = None,
               window: int = 0, kv_dt: int = KV_F32, k_scale: DeviceArray | None = None,
-              v_scale: DeviceArray | None = None, stream: Stream | None = None) -> None:
+              v_scale: DeviceArray | None = None, stream: Stream | None = None,
+              sinks: int = 0) -> None:
     """GQA attention with an online softmax over a KV cache
     (src/transformer.cpp:120-214): q [n_q, n_head, head_dim] -> out
-    [n_q, n_head, value_dim]; K / V [n_kv, n_head_kv, dim] in kv_dt. The
-    decode split's workspace is allocated once per size and reused."""
+    [n_q, n_head, value_dim]; K / V [n_kv, n_head_kv, dim] in kv_dt. A query at
+    position qp keeps keys at positions kp <= qp with qp - kp < window (0: all)
+    or kp < sinks. The decode split's workspace is allocated once per size and
+    reused."""
     _need(q, n_q * n_head * head_dim, np.float32, "q")
     _need(out, n_q * n_head * value_dim, np.float32, "out")
     _need(qpos, n_q, np.int32, "qpos")
@@ -599,6 +603,17 @@ def attention(q: DeviceArray, k: DeviceArray, v: DeviceArray, out: DeviceArray, 
         _need(k_scale, n_kv * n_head_kv, np.float32, "k_scale")
         _need(v_scale, n_kv * n_head_kv, np.float32, "v_scale")
     L = _lib.lib()
+    if sinks != 0:
+        sizes = (n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, int(window), int(sinks))
+        wsb = int(L.aero_hip_attention_sinks_workspace(kv_dt, *sizes))
+        _lib.check(wsb >= 0, "attention")
+        ws = _rows_ws.get(wsb)
+        _lib.check(L.aero_hip_attention_sinks(
+            q.ptr, kv_dt, k.ptr, as_ptr(k_scale), v.ptr, as_ptr(v_scale), out.ptr, n_q, n_head,
+            n_head_kv, head_dim, value_dim, float(scale), as_ptr(qpos), as_ptr(kpos), n_kv,
+            int(window), int(sinks), as_ptr(ws), ws.nbytes if ws is not None else 0, _s(stream)),
+            "attention")
+        return
     wsb = int(L.aero_hip_attention_workspace(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv))
     ws = _attn_ws.get(wsb)
     _lib.check(L.aero_hip_attention(q.ptr, kv_dt, k.ptr, as_ptr(k_scale), v.ptr,
@@ -606,6 +621,109 @@ def attention(q: DeviceArray, k: DeviceArray, v: DeviceArray, out: DeviceArray, 
                                     value_dim, float(scale), as_ptr(qpos), as_ptr(kpos), n_kv,
                                     int(window), as_ptr(ws), ws.nbytes if ws is not None else 0,
                                     _s(stream)), "attention")
+
+
+def _paged(pool, table: DeviceArray, lens: DeviceArray, n_seq: int, bad: DeviceArray | None):
+    """max_pages of a call's table, its arrays checked."""
+    if len(table.shape) != 2:
+        raise ValueError(f"table: shape {table.shape}, expected [sequences, max_pages]")
+    _need(table, n_seq * table.shape[1], np.int32, "table")
+    _need(lens, n_seq, np.int32, "lens")
+    _need(bad, 1, np.int32, "bad")
+    return table.shape[1]
+
+
+def paged_kv_write(pool, layer: int, k: DeviceArray, v: DeviceArray, table: DeviceArray,
+                   lens: DeviceArray, n_seq: int, n_q: int = 1, bad: DeviceArray | None = None,
+                   stream: Stream | None = None) -> None:
+    """The n_q newest tokens' rows k [n_seq, n_q, n_head_kv, head_dim] and v
+    (value_dim) of sequences 0 .. n_seq-1 into their pages of one layer of a
+    paged.KvPool, quantised as kv_write does. Row s of table [rows, max_pages]
+    lists the sequence's pages and lens[s] counts its tokens, the new ones
+    included; where lens[s] - n_q + t is negative there is no token t (a padding
+    row: lens 0). A page id outside the pool is not followed: the row is not
+    written and bad[0] becomes 1."""
+    max_pages = _paged(pool, table, lens, n_seq, bad)
+    rows = n_seq * n_q * pool.n_head_kv
+    _need(k, rows * pool.head_dim, np.float32, "k")
+    _need(v, rows * pool.value_dim, np.float32, "v")
+    _lib.check(_lib.lib().aero_hip_paged_kv_write(
+        pool.ref, layer, k.ptr, v.ptr, table.ptr, max_pages, lens.ptr, n_seq, n_q, as_ptr(bad),
+        _s(stream)), "paged_kv_write")
+
+
+def paged_kv_read(pool, layer: int, k: DeviceArray, v: DeviceArray, table: DeviceArray,
+                  lens: DeviceArray, n_seq: int, n_q: int = 1, bad: DeviceArray | None = None,
+                  stream: Stream | None = None) -> None:
+    """Such rows back as fp32 into k and v: the values the cache holds (code *
+    scale), zeros where there is no token or no page."""
+    max_pages = _paged(pool, table, lens, n_seq, bad)
+    rows = n_seq * n_q * pool.n_head_kv
+    _need(k, rows * pool.head_dim, np.float32, "k")
+    _need(v, rows * pool.value_dim, np.float32, "v")
+    _lib.check(_lib.lib().aero_hip_paged_kv_read(
+        pool.ref, layer, k.ptr, v.ptr, table.ptr, max_pages, lens.ptr, n_seq, n_q, as_ptr(bad),
+        _s(stream)), "paged_kv_read")
+
+
+def paged_attention(pool, layer: int, q: DeviceArray, out: DeviceArray, table: DeviceArray,
+                    lens: DeviceArray, n_seq: int, n_head: int, scale: float, n_q: int = 1,
+                    window: int = 0, sinks: int = 0, bad: DeviceArray | None = None,
+                    stream: Stream | None = None) -> None:
+    """Attention of each sequence's n_q newest tokens (their rows written before)
+    over its pages: q [n_seq, n_q, n_head, head_dim] -> out [n_seq, n_q, n_head,
+    value_dim], table and lens as paged_kv_write, the mask as attention with
+    window and sinks. Rows without a token, or that see nothing, become zeros;
+    keys of a page id outside the pool are not seen, and bad[0] becomes 1. The
+    launch does not depend on the lengths, so a plan that recorded it stays
+    right as the sequences grow. The workspace is allocated once per size and
+    reused: calls on different streams must not overlap."""
+    max_pages = _paged(pool, table, lens, n_seq, bad)
+    rows = n_seq * n_q * n_head
+    _need(q, rows * pool.head_dim, np.float32, "q")
+    _need(out, rows * pool.value_dim, np.float32, "out")
+    L = _lib.lib()
+    wsb = int(L.aero_hip_paged_attention_workspace(pool.ref, n_seq, n_q, n_head, max_pages))
+    _lib.check(wsb >= 0, "paged_attention")
+    ws = _rows_ws.get(wsb)
+    _lib.check(L.aero_hip_paged_attention(
+        pool.ref, layer, q.ptr, out.ptr, table.ptr, max_pages, lens.ptr, n_seq, n_q, n_head,
+        float(scale), int(window), int(sinks), as_ptr(bad), as_ptr(ws),
+        ws.nbytes if ws is not None else 0, _s(stream)), "paged_attention")
+
+
+def _ints(a, dtype) -> np.ndarray:
+    a = np.asarray(a)
+    if a.size and a.dtype.kind not in "iu":
+        raise TypeError(f"expected integers, got {a.dtype}")
+    b = np.ascontiguousarray(a, dtype).reshape(-1)
+    if not np.array_equal(b, a.reshape(-1)):
+        raise ValueError(f"values outside {np.dtype(dtype)}")
+    return b
+
+
+def kv_pages_copy(pool, src, dst, stream: Stream | None = None) -> None:
+    """Page dst[i] = page src[i] in every layer of a paged.KvPool (K, V and
+    scales). Host lists; a destination may be named once and may not be a source
+    too, so the copies have no order among them."""
+    src, dst = _ints(src, np.int32), _ints(dst, np.int32)
+    if src.size != dst.size:
+        raise ValueError(f"{src.size} sources for {dst.size} destinations")
+    _lib.check(_lib.lib().aero_hip_kv_pages_copy(
+        pool.ref, src.ctypes.data_as(_lib.ip), dst.ctypes.data_as(_lib.ip), src.size, _s(stream)),
+        "kv_pages_copy")
+
+
+def write_i32(a: DeviceArray, items, stream: Stream | None = None) -> None:
+    """a.flat[i] = value for (i, value) in items (i ascending), in stream order:
+    no blocking copy."""
+    _need(a, 0, np.int32, "a")
+    items = list(items)
+    at = _ints([i for i, _ in items], np.int64)
+    val = _ints([x for _, x in items], np.int32)
+    _lib.check(_lib.lib().aero_hip_write_i32(
+        a.ptr, a.size, at.ctypes.data_as(ctypes.POINTER(ctypes.c_int64)),
+        val.ctypes.data_as(_lib.ip), at.size, _s(stream)), "write_i32")
 
 
 def softmax_rows(x: DeviceArray, y: DeviceArray, n_rows: int, n_cols: int,

@@ -614,6 +614,89 @@ int aero_hip_kv_write(int dt, const float* x, int64_t n_tok, int64_t heads, int6
 int aero_hip_softmax_rows(const float* x, float* y, int64_t n_rows, int64_t n_cols,
                           void* stream);
 
+/* aero_hip_attention with sinks: key j (position kp = kpos[j] or j) is kept for a
+ * query at qp when kp <= qp and (window <= 0, or qp - kp < window, or kp < sinks),
+ * so the first tokens stay visible to a sliding window. With window <= 0 or
+ * sinks 0 it is aero_hip_attention's call. A cache that keeps the sinks and a
+ * ring of the window passes the positions of its slots in kpos. n_kv below
+ * 2^30. Workspace: aero_hip_attention_sinks_workspace bytes (-1: bad sizes),
+ * 16-byte aligned. No counterpart in the reference. */
+int64_t aero_hip_attention_sinks_workspace(int kv_dt, int64_t n_q, int64_t n_head,
+                                           int64_t n_head_kv, int64_t head_dim,
+                                           int64_t value_dim, int64_t n_kv, int window,
+                                           int sinks);
+int aero_hip_attention_sinks(const float* q, int kv_dt, const void* k, const float* k_scale,
+                             const void* v, const float* v_scale, float* out, int64_t n_q,
+                             int64_t n_head, int64_t n_head_kv, int64_t head_dim,
+                             int64_t value_dim, float scale, const int32_t* qpos,
+                             const int32_t* kpos, int64_t n_kv, int window, int sinks,
+                             void* workspace, int64_t ws_bytes, void* stream);
+
+/* A paged KV cache: the keys and values of many sequences in pages of `page`
+ * tokens (a power of two, 16-256) of one pool, in all layers alike. K is
+ * [n_layers][n_pages][n_head_kv][page][head_dim] in kv_dt (as
+ * aero_hip_attention), V the same of value_dim, the scales of integer types
+ * [n_layers][n_pages][n_head_kv][page] fp32; all 16-byte aligned. Dims up to
+ * 256, a multiple of 4 in fp32 and of 2 in int4.
+ * A call's sequences are rows 0 .. n_seq-1 of table [n_seq][max_pages] (the
+ * page of tokens page*c .. page*(c+1)-1 in column c) and of lens [n_seq],
+ * int32 on the device, read when the kernel runs: a recorded plan follows the
+ * sequences as they grow. lens counts the call's n_q new tokens: token t of
+ * sequence s has position lens[s] - n_q + t, and is no token when that is
+ * negative (a padding row: lens 0). A length past max_pages * page is taken
+ * as that many tokens. Page ids outside the pool are never followed: such a
+ * page's keys are not seen, its rows not written and read as zeros, and *bad
+ * (int32 on the device, or NULL) is set to 1. No counterpart in the
+ * reference, which keeps one contiguous slot a sequence (src/kv.cpp). */
+typedef struct aero_kv_pool {
+    int kv_dt;
+    int64_t page;
+    int64_t n_layers;
+    int64_t n_pages;
+    int64_t n_head_kv;
+    int64_t head_dim;
+    int64_t value_dim;
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+} aero_kv_pool_t;
+
+/* Attention of each sequence's n_q newest tokens over its pages: q [n_seq, n_q,
+ * n_head, head_dim] -> out [n_seq, n_q, n_head, value_dim], the mask of
+ * aero_hip_attention_sinks (window 0: none) by token positions. Pages that no
+ * token sees (between the sinks and the window) are not read and need no
+ * entry. Rows without tokens or visible keys become zeros. Workspace:
+ * aero_hip_paged_attention_workspace bytes (-1: bad sizes), 16-byte aligned,
+ * its contents free between calls; calls that share it must be ordered. */
+int64_t aero_hip_paged_attention_workspace(const aero_kv_pool_t* pool, int64_t n_seq, int64_t n_q,
+                                           int64_t n_head, int64_t max_pages);
+int aero_hip_paged_attention(const aero_kv_pool_t* pool, int64_t layer, const float* q, float* out,
+                             const int32_t* table, int64_t max_pages, const int32_t* lens,
+                             int64_t n_seq, int64_t n_q, int64_t n_head, float scale, int window,
+                             int sinks, int32_t* bad, void* ws, int64_t ws_bytes, void* stream);
+/* The new tokens' rows k [n_seq, n_q, n_head_kv, head_dim] and v (value_dim)
+ * into their pages of one layer, quantised as aero_hip_kv_write; and such rows
+ * back as fp32 (code * scale; zeros where there is no token). Sequences that
+ * write must not share the pages written. */
+int aero_hip_paged_kv_write(const aero_kv_pool_t* pool, int64_t layer, const float* k,
+                            const float* v, const int32_t* table, int64_t max_pages,
+                            const int32_t* lens, int64_t n_seq, int64_t n_q, int32_t* bad,
+                            void* stream);
+int aero_hip_paged_kv_read(const aero_kv_pool_t* pool, int64_t layer, float* k, float* v,
+                           const int32_t* table, int64_t max_pages, const int32_t* lens,
+                           int64_t n_seq, int64_t n_q, int32_t* bad, void* stream);
+/* Pages copied in every layer, K, V and scales: dst[i] = src[i], i < n. src and
+ * dst are host arrays, read during the call. A destination may be named once and
+ * may not be a source too (refused: such copies would have an order). */
+int aero_hip_kv_pages_copy(const aero_kv_pool_t* pool, const int32_t* src, const int32_t* dst,
+                           int64_t n, void* stream);
+/* base[at[i]] = value[i] in stream order, i < n; at and value are host arrays,
+ * read during the call, at ascending: page tables and lengths change between
+ * two kernels without a blocking copy. */
+int aero_hip_write_i32(int32_t* base, int64_t n_base, const int64_t* at, const int32_t* value,
+                       int64_t n, void* stream);
+
 /* Plain fp32 copy kernel (dst = src, n elements): the known-size reference
  * workload used to calibrate HBM byte counters. */
 int aero_hip_copy_f32(const float* src, float* dst, int64_t n, void* stream);

@@ -1,0 +1,159 @@
+"""GPU: attention with a sliding window and sinks over contiguous caches
+(ops.attention with sinks, aero_hip_attention_sinks) against plain attention in
+64 bits, within 1e-5 of the output's scale (the contiguous attention's
+tolerance; tests/test_gpu_paged.py has the arithmetic)."""
+import numpy as np
+import pytest
+
+import paged_ref as R
+from conftest import RTOL, bits_equal, rel_to_scale
+from aero_amd import ops
+from aero_amd.device import DeviceArray as DA, Plan, Stream, synchronize
+
+pytestmark = pytest.mark.gpu
+
+
+def cache(rng, n_kv, HK, D, dt):
+    """(device array, scales or None, the values stored in float64)"""
+    x = rng.standard_normal((n_kv, HK, D)).astype(np.float32)
+    if dt == 0:
+        return DA.from_numpy(x), None, x.astype(np.float64)
+    c, s = R.quantise(x, dt)
+    return (DA.from_numpy(R.pack(c, dt)), DA.from_numpy(s),
+            c.astype(np.float64) * s[..., None].astype(np.float64))
+
+
+def call(q, k, v, n_kv, HK, window, sinks, dt, qpos=None, kpos=None, scale=0.1, DV=None,
+         stream=None):
+    T, H, D = q.shape
+    DV = DV or D
+    out = DA.from_numpy(np.full((T, H, DV), 7.0, np.float32))
+    dev = lambda a: None if a is None else DA.from_numpy(np.asarray(a, np.int32))
+    ops.attention(DA.from_numpy(q), k[0], v[0], out, T, H, HK, D, DV, n_kv, scale, qpos=dev(qpos),
+                  kpos=dev(kpos), window=window, kv_dt=dt, k_scale=k[1], v_scale=v[1],
+                  stream=stream, sinks=sinks)
+    if stream is not None:
+        stream.synchronize()
+    return out.numpy()
+
+
+SHAPES = [
+    # H, HK, D, DV, n_q, n_kv, window, sinks
+    (32, 8, 128, 128, 1, 5000, 1000, 4), (32, 8, 128, 128, 1, 1, 1, 1), (14, 2, 64, 64, 1, 333, 64, 16),
+    (8, 4, 256, 256, 1, 2052, 512, 4), (16, 2, 256, 256, 3, 700, 100, 33), (20, 1, 64, 64, 2, 90, 7, 1),
+    (8, 8, 128, 128, 5, 300, 16, 16), (32, 8, 128, 128, 4, 4000, 33, 300), (4, 4, 80, 48, 1, 200, 30, 3),
+    (4, 1, 32, 32, 70, 100, 11, 2), (6, 2, 20, 100, 9, 50, 49, 1), (32, 8, 64, 64, 257, 300, 100, 4),
+    (32, 8, 128, 128, 200, 200, 1000, 4), (8, 4, 256, 256, 130, 600, 64, 5),
+    (32, 8, 128, 128, 700, 700, 128, 20), (14, 2, 64, 64, 1001, 2500, 300, 64),
+    (8, 4, 256, 256, 1400, 1400, 200, 4), (64, 8, 128, 128, 333, 3000, 90, 2000),
+]
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("shape", SHAPES, ids=["-".join(map(str, s)) for s in SHAPES])
+def test_sinks(hip, shape, dt):
+    H, HK, D, DV, T, n_kv, window, sinks = shape
+    rng = np.random.default_rng([H, D, T, dt])
+    k, v = cache(rng, n_kv, HK, D, dt), cache(rng, n_kv, HK, DV, dt)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    qpos = np.arange(n_kv - T, n_kv)
+    got = call(q, k, v, n_kv, HK, window, sinks, dt, qpos, DV=DV)
+    keep = R.seen(qpos, np.arange(n_kv), window, sinks)
+    assert rel_to_scale(got, R.attention(q, k[2], v[2], keep, 0.1)) <= RTOL
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("D,T", [(64, 5), (128, 3), (256, 2), (48, 4), (128, 400)])
+def test_positions(hip, D, T, dt):
+    """Query positions in any order, before every key, at the sinks, past the
+    cache; key positions of a ring and shuffled ones; absent positions."""
+    rng = np.random.default_rng([D, T, dt])
+    HK, H, n_kv, window, sinks = 2, 8, 400, 60, 6
+    k, v = cache(rng, n_kv, HK, D, dt), cache(rng, n_kv, HK, D, dt)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    ring = np.arange(n_kv)
+    ring[sinks:] = 1000 + (ring[sinks:] * 7) % (n_kv - sinks)
+    for qpos in (None, rng.integers(-3, 900, T), np.full(T, 5), np.full(T, -1), np.full(T, 2**31 - 1),
+                 np.resize([0, 399, 58, 1400], T)):
+        for kpos in (None, ring, rng.permutation(n_kv)):
+            got = call(q, k, v, n_kv, HK, window, sinks, dt, qpos, kpos)
+            keep = R.seen(np.arange(T) if qpos is None else qpos,
+                          np.arange(n_kv) if kpos is None else kpos, window, sinks)
+            want = R.attention(q, k[2], v[2], keep, 0.1)
+            assert np.isfinite(got).all()
+            assert not got[~keep.any(1)].any()
+            if want.any():
+                assert rel_to_scale(got, want) <= RTOL
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 48])
+@pytest.mark.parametrize("T", [1, 4, 40, 600])
+def test_values_that_no_query_may_see(hip, D, T):
+    """NaN and infinities in keys and values that some or all queries do not keep
+    reach none of those; one that a query keeps reaches that query."""
+    rng = np.random.default_rng([D, T])
+    H, HK, n_kv, window, sinks = 16, 4, 700, 50, 3
+    k = rng.standard_normal((n_kv, HK, D)).astype(np.float32)
+    v = rng.standard_normal((n_kv, HK, D)).astype(np.float32)
+    q = rng.standard_normal((T, H, D)).astype(np.float32)
+    qpos = np.arange(n_kv - T, n_kv)
+    hidden = ~R.seen(qpos, np.arange(n_kv), window, sinks).any(0)
+    k[hidden], v[hidden] = np.nan, np.inf
+    v[n_kv - 1] = np.inf                      # only the last query keeps it
+    k[n_kv - 1, 1] = np.nan
+    dev = lambda x: (DA.from_numpy(x), None)
+    got = call(q, dev(k), dev(v), n_kv, HK, window, sinks, 0, qpos)
+    keep = R.seen(qpos, np.arange(n_kv), window, sinks)
+    if T > 1:
+        want = R.attention(q[:-1], k, v, keep[:-1], 0.1)
+        assert np.isfinite(got[:-1]).all()
+        assert rel_to_scale(got[:-1], want) <= RTOL
+    assert not np.isfinite(got[-1]).any()
+
+
+@pytest.mark.parametrize("dt", [0, 1], ids=["fp32", "int8"])
+def test_without_window_or_sinks_it_is_attention(hip, dt):
+    rng = np.random.default_rng(dt)
+    k, v = cache(rng, 500, 2, 128, dt), cache(rng, 500, 2, 128, dt)
+    q = rng.standard_normal((3, 8, 128)).astype(np.float32)
+    qpos = np.arange(497, 500)
+    a = call(q, k, v, 500, 2, 0, 0, dt, qpos)
+    assert bits_equal(a, call(q, k, v, 500, 2, 0, 9, dt, qpos))
+    # sinks past the window's first key add nothing to its keys
+    want = R.attention(q, k[2], v[2], R.seen(qpos, np.arange(500), 1 << 30, 7), 0.1)
+    assert rel_to_scale(call(q, k, v, 500, 2, 1 << 30, 7, dt, qpos), want) <= RTOL
+    # the same bits twice, and on another stream
+    b = call(q, k, v, 500, 2, 100, 4, dt, qpos)
+    s = Stream()
+    assert bits_equal(b, call(q, k, v, 500, 2, 100, 4, dt, qpos))
+    assert bits_equal(b, call(q, k, v, 500, 2, 100, 4, dt, qpos, stream=s))
+    s.destroy()
+
+
+@pytest.mark.parametrize("dt", [0, 1], ids=["fp32", "int8"])
+def test_recorded_step(hip, dt):
+    """One token's step over a ring with sinks, recorded; positions move on
+    between the replays."""
+    rng = np.random.default_rng(40 + dt)
+    H, HK, D, window, sinks = 32, 8, 128, 512, 4
+    n_kv = window + sinks
+    k, v = cache(rng, n_kv, HK, D, dt), cache(rng, n_kv, HK, D, dt)
+    q = rng.standard_normal((1, H, D)).astype(np.float32)
+    dq, out = DA.from_numpy(q), DA.empty((1, H, D))
+    qp, kp = DA.empty(1, np.int32), DA.empty(n_kv, np.int32)
+    plan = Plan()
+    with plan:
+        ops.attention(dq, k[0], v[0], out, 1, H, HK, D, D, n_kv, 0.1, qpos=qp, kpos=kp,
+                      window=window, kv_dt=dt, k_scale=k[1], v_scale=v[1], sinks=sinks)
+    slots = np.arange(n_kv)
+    for last in (600, 601, 1300, 5000):
+        newest = last - (last - sinks - (slots - sinks)) % window
+        kpos = np.where(slots < sinks, slots, newest)
+        qp.copy_from(np.asarray([last], np.int32))
+        kp.copy_from(kpos.astype(np.int32))
+        plan.launch()
+        want = R.attention(q, k[2], v[2], R.seen([last], kpos, window, sinks), 0.1)
+        got = out.numpy()
+        assert rel_to_scale(got, want) <= RTOL
+        assert bits_equal(got, call(q, k, v, n_kv, HK, window, sinks, dt, [last], kpos))
+    plan.destroy()
