@@ -126,6 +126,7 @@ template <int DT, int E, bool PAGED>
 struct VecCore {
     static constexpr int VEC = 4;            // query vectors an item
     static constexpr int UNIT = 4;           // key tiles a unit
+    static constexpr int EU = 1;
     static constexpr int DVP = 16 * E;
     struct Shared {
         float m[16][VEC], l[16][VEC], acc[16][VEC][DVP];
@@ -257,6 +258,706 @@ struct VecCore {
     }
 };
 
+// ---------------------------------------------------------------- matrix cores
+// A 16-vector query tile on the matrix cores, as attention.hip lays it out: lane
+// (g, c) = (l / 16, l % 16) holds of a 16-key tile D/4 elements of key c (the
+// scores' operand) and D/16 elements of the values of keys 4g .. 4g + 3, so the
+// scores a lane receives are the value sum's operand as they come. Each of the
+// four waves takes every fourth step of the item's list; their sums meet in LDS.
+enum Source { kPaged, kLinear, kLinearPos };
+
+// One kv head's tiles in memory, through buffer descriptors: lane offsets within
+// a tile are fixed, the tile's place is wave-uniform, and what lies past the
+// cache's end, or on a bad page, reads as zeros.
+template <int DT, int D, Source SRC>
+struct Tiles {
+    static constexpr int KVEC = D * kv_bits<DT>() / 8;   // bytes of a vector
+    static constexpr int KS = D / 4, VS = D / 16;        // elements a lane holds
+    static constexpr int KB = KVEC / 4, VB = KVEC / 16;
+    static constexpr int KLB = KB < 16 ? KB : 16, KNI = KB / KLB, KLE = KLB * 8 / kv_bits<DT>();
+    static constexpr int VLB = VB < 16 ? VB : 16, VNI = VB / VLB, VLE = VLB * 8 / kv_bits<DT>();
+    // head dimension of element j of lane group g's key slice, value dimension
+    // of element t of lane c's value slice: pieces of the lanes interleave, so a
+    // load instruction reads whole runs of a vector
+    static __device__ __forceinline__ int kdim(int g, int j) {
+        return (j / KLE) * (4 * KLE) + g * KLE + j % KLE;
+    }
+    static __device__ __forceinline__ int vdim(int c, int t) {
+        return (t / VLE) * (16 * VLE) + c * VLE + t % VLE;
+    }
+    // a tile's place in memory (wave-uniform)
+    struct Place {
+        int64_t vec;     // its first vector
+        int32_t kb;      // its first key
+        int32_t left;    // keys there are from it on (0: no such tile, or no page)
+    };
+    struct K {
+        uint32_t k[(KB + 3) / 4];
+        float s[DT ? 4 : 1];                      // scales of keys 4g .. 4g + 3
+    };
+    struct V {
+        int32_t kp[SRC == kLinearPos ? 4 : 1];    // positions of keys 4g .. 4g + 3
+        float s[DT ? 4 : 1];
+        uint32_t v[4][(VB + 3) / 4];
+    };
+
+    const RowsParams& p;
+    int kh, g, c;
+    uint32_t stride;     // from a key to the next
+    static constexpr int kIds = 4;
+    int32_t ids[kIds];   // paged: ids of 64 kIds pages of the list, a lane each
+    int32_t place0;
+
+    __device__ __forceinline__ Tiles(const RowsParams& p_, int kh_, int g_, int c_)
+        : p(p_), kh(kh_), g(g_), c(c_) {
+        stride = SRC == kPaged ? KVEC : (uint32_t)(p.n_head_kv * KVEC);
+    }
+    // tiles that a set of ids is sure to cover (a multiple of 8; the sinks' and
+    // the window's first and last pages may be partly used)
+    static constexpr int kIdTiles = 64 * kIds - 8;
+
+    // ids for places x .. of the list (x1: its end)
+    __device__ __forceinline__ void pages(const Item& it, int x, int x1) {
+        if constexpr (SRC == kPaged) {
+            const int shift = p.page_shift - 4, lane = threadIdx.x & 63;
+            place0 = it.kt.page_place(x, shift);
+            const int n = it.kt.page_place(x1 - 1, shift) - place0 + 1;
+            bool bad = false;
+#pragma unroll
+            for (int r = 0; r < kIds; ++r) {
+                const int i = 64 * r + lane;
+                const int32_t col = it.kt.column(place0 + i, shift);
+                int32_t id = -1;
+                if (i < n && col < p.max_pages) id = p.table[(int64_t)it.s * p.max_pages + col];
+                const bool ok = id >= 0 && id < p.n_pages;
+                bad = bad || (i < n && !ok);
+                ids[r] = ok ? id : -1;
+            }
+            if (p.bad != nullptr && __any(bad)) *p.bad = 1;
+        }
+    }
+    __device__ __forceinline__ int32_t id(int i) const {
+        int32_t x = __builtin_amdgcn_readlane(ids[0], i & 63);
+#pragma unroll
+        for (int r = 1; r < kIds; ++r)
+            x = (i >> 6) == r ? __builtin_amdgcn_readlane(ids[r], i & 63) : x;
+        return x;
+    }
+
+    template <int N>
+    static __device__ __forceinline__ void words(__amdgpu_buffer_rsrc_t r, uint32_t off,
+                                                 uint32_t* w) {
+        if constexpr (N == 16) {
+            const v4u x = __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+        } else if constexpr (N == 8) {
+            const v2u x = __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0);
+            w[0] = x.x; w[1] = x.y;
+        } else if constexpr (N == 4) {
+            w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
+        } else {
+            static_assert(N == 2, "slice size");
+            w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, 0);
+        }
+    }
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, int64_t off,
+                                                                  uint32_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(static_cast<const uint8_t*>(base)) + off, 0, (int)bytes,
+            kBufferDword3);
+    }
+
+    // place x of the list (none at or past x1); x wave-uniform
+    __device__ __forceinline__ Place locate(const Item& it, int x, int x1) const {
+        const int tile = it.kt.at(x);
+        Place l;
+        l.kb = 16 * tile;
+        if constexpr (SRC == kPaged) {
+            const int shift = p.page_shift - 4;
+            const int32_t page = x < x1 ? id(it.kt.page_place(x, shift) - place0) : -1;
+            l.left = page >= 0 ? 16 : 0;
+            l.vec = (((int64_t)max(page, 0) * p.n_head_kv + kh) << p.page_shift) +
+                    16 * (tile & ((1 << shift) - 1));
+        } else {
+            l.left = x < x1 ? min(it.len - l.kb, 16) : 0;
+            l.vec = l.left > 0 ? (int64_t)l.kb * p.n_head_kv + kh : 0;
+        }
+        return l;
+    }
+    __device__ __forceinline__ uint32_t bytes(const Place& l) const {
+        return l.left > 0 ? (uint32_t)(l.left - 1) * stride + KVEC : 0u;
+    }
+    // scales of keys 4g .. 4g + 3 (paged: a head's scales of a page lie together)
+    __device__ __forceinline__ void load_scales(float (&o)[4], const float* s,
+                                                const Place& l) const {
+        if constexpr (SRC == kPaged) {
+            uint32_t w[4];
+            words<16>(rsrc(s, l.vec * 4, 4 * l.left), 16 * g, w);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = __uint_as_float(w[r]);
+        } else {
+            const __amdgpu_buffer_rsrc_t b = rsrc(
+                s, l.vec * 4, l.left > 0 ? ((uint32_t)(l.left - 1) * p.n_head_kv + 1) * 4 : 0u);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                o[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                    b, (4 * g + r) * p.n_head_kv * 4, 0, 0));
+        }
+    }
+    __device__ __forceinline__ void load(K& t, const Place& l) const {
+        const __amdgpu_buffer_rsrc_t r = rsrc(p.k, l.vec * KVEC, bytes(l));
+#pragma unroll
+        for (int i = 0; i < KNI; ++i)
+            words<KLB>(r, (uint32_t)c * stride + (uint32_t)((4 * i + g) * KLB), t.k + i * KLB / 4);
+        if constexpr (DT != 0) load_scales(t.s, p.ks, l);
+    }
+    __device__ __forceinline__ void load(V& t, const Place& l) const {
+        if constexpr (SRC == kLinearPos) {
+            const __amdgpu_buffer_rsrc_t b = rsrc(p.kpos, l.left > 0 ? (int64_t)l.kb * 4 : 0,
+                                                  4 * max(l.left, 0));
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                t.kp[r] = (int32_t)__builtin_amdgcn_raw_buffer_load_b32(b, (4 * g + r) * 4, 0, 0);
+        }
+        if constexpr (DT != 0) load_scales(t.s, p.vs, l);
+        const __amdgpu_buffer_rsrc_t b = rsrc(p.v, l.vec * KVEC, bytes(l));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < VNI; ++i)
+                words<VLB>(b, (uint32_t)(4 * g + r) * stride + (uint32_t)((16 * i + c) * VLB),
+                           t.v[r] + i * VLB / 4);
+    }
+};
+
+// A tile's query vectors: column c's row, position and the keys it sees
+template <Source SRC>
+struct Columns {
+    int rows;            // vectors there are
+    int64_t qrow;
+    int32_t qp, klo;     // kept: kp <= qp and (kp >= klo or kp < sinks)
+    int32_t qmin, klo_max;
+    bool mixed;          // positions differ
+
+    __device__ __forceinline__ Columns(const RowsParams& p, const Item& it, int c) {
+        const int n_vec = p.n_q * p.rep;
+        rows = min(n_vec - 16 * it.z, 16);
+        // (a column past the last vector is a copy of that one, never written)
+        const int u = min(16 * it.z + c, n_vec - 1);
+        const int t = u / p.rep;
+        qrow = ((int64_t)it.s * p.n_q + t) * p.n_head + it.kh * p.rep + u % p.rep;
+        qp = SRC == kPaged ? it.pos0 + t : (p.qpos ? p.qpos[t] : t);
+        klo = p.window > 0 ? (int32_t)max<int64_t>((int64_t)qp - p.window + 1, INT32_MIN)
+                           : INT32_MIN;
+        int32_t lo = qp, hi = qp;
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) {
+            lo = min(lo, __shfl_xor(lo, off, 16));
+            hi = max(hi, __shfl_xor(hi, off, 16));
+        }
+        qmin = __builtin_amdgcn_readfirstlane(lo);
+        const int32_t qmax = __builtin_amdgcn_readfirstlane(hi);
+        klo_max = p.window > 0 ? (int32_t)max<int64_t>((int64_t)qmax - p.window + 1, INT32_MIN)
+                               : INT32_MIN;
+        mixed = qmin != qmax;
+    }
+    // every column keeps every key of the tile at kb (left keys there are)
+    __device__ __forceinline__ bool whole(const RowsParams& p, const Item& it, int32_t kb,
+                                          int32_t left) const {
+        return SRC != kLinearPos && left > 0 && kb + 16 <= it.len && kb + 15 <= qmin &&
+               (kb >= klo_max || kb + 16 <= p.sinks);
+    }
+    // whether column c keeps key 4g + r of it (kp: its position)
+    __device__ __forceinline__ bool keeps(const RowsParams& p, const Item& it, int32_t kb,
+                                          int32_t left, int g, int r, int32_t kp) const {
+        const int32_t kj = kb + 4 * g + r;
+        if (SRC != kLinearPos) kp = kj;
+        return left > 0 && kj < it.len && kp <= qp && (kp >= klo || kp < p.sinks);
+    }
+};
+
+template <int D>
+struct TileShared {
+    float m[4][16], l[4][16], w[4][16], mt[16], lt[16];
+    float acc[4][16][D + 4];
+};
+
+// The four waves' (m, l, acc) of a tile joined through LDS; its rows written out
+// (row < 0) or as a part. Lane (g, c) holds acc of query 4g + r, dimension
+// vdim(c, t), and (m, l) of query c, l a share.
+template <typename TL, int D>
+__device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it, int rows, float m,
+                                            float ls, const v4f (&acc)[D / 16], int64_t row,
+                                            TileShared<D>& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    ls += __shfl_xor(ls, 16);
+    ls += __shfl_xor(ls, 32);
+    __syncthreads();     // (the item before is read)
+    if (g == 0) {
+        sh.m[wave][c] = m;
+        sh.l[wave][c] = ls;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (4 * g + r < rows) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) sh.acc[wave][4 * g + r][TL::vdim(c, t)] = acc[t][r];
+        }
+    __syncthreads();
+    if (tid < 64) {
+        const int x = tid >> 4, i = tid & 15;
+        const float mt = fmaxf(fmaxf(sh.m[0][i], sh.m[1][i]), fmaxf(sh.m[2][i], sh.m[3][i]));
+        const float w = sh.m[x][i] == -INFINITY ? 0.0f : expf(sh.m[x][i] - mt);
+        sh.w[x][i] = w;
+        float lw = sh.l[x][i] * w;
+        lw += __shfl_xor(lw, 16);
+        lw += __shfl_xor(lw, 32);
+        if (x == 0) {
+            sh.mt[i] = mt;
+            sh.lt[i] = lw;
+        }
+    }
+    __syncthreads();
+    for (int x = tid; x < rows * (D / 4); x += 256) {
+        const int i = x / (D / 4), d = 4 * (x % (D / 4));
+        v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const v4f a = *reinterpret_cast<const v4f*>(&sh.acc[y][i][d]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a[e], sh.w[y][i], o[e]);
+        }
+        if (row < 0) {
+            const int u = 16 * it.z + i;
+            const int64_t r = ((int64_t)it.s * p.n_q + u / p.rep) * p.n_head + it.kh * p.rep +
+                              u % p.rep;
+            const float inv = 1.0f / fmaxf(sh.lt[i], 1e-30f);
+            *reinterpret_cast<v4f*>(p.out + r * D + d) =
+                v4f{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        } else {
+            *reinterpret_cast<v4f*>(part_row(p, row + i) + d) = o;
+            if (d == 0) *part_ml(p, 16, row + i) = make_float2(sh.mt[i], sh.lt[i]);
+        }
+    }
+}
+
+// Integer caches on the fp16 matrix cores (v_mfma_f32_16x16x32_f16): the codes are
+// exact in fp16; q, scaled per query to below 2^15, and the probabilities times
+// the value scales, scaled by the largest value scale so far, go in two fp16 parts
+// (hi, lo = v - hi: 22 bits), so every product is exact and added in fp32. 32 keys
+// a step, scores in log2 units, sums rescaled only when a query's maximum passes
+// the reference by 2^8 or the scales' exponent moves (as attention.hip's kernel).
+template <int DT, int D, Source SRC>
+struct F16Core {
+    static constexpr int VEC = 16;
+    static constexpr int UNIT = 8;
+    static constexpr int EU = D == 256 ? 1 : 2;
+    using TL = Tiles<DT, D, SRC>;
+    using Shared = TileShared<D>;
+    static constexpr int KS = TL::KS, VS = TL::VS, NS = KS / 8;
+
+    const RowsParams& p;
+    const Item& it;
+    Shared& sh;
+    int g, c;
+    Columns<SRC> col;
+    float m = -INFINITY, ls = 0.0f;
+    int e_acc = -1000;
+    v4f acc[VS];
+    h8 qhi[NS], qlo[NS];
+    float qsl;
+
+    __device__ __forceinline__ F16Core(const RowsParams& p_, const Item& it_, Shared& sh_)
+        : p(p_), it(it_), sh(sh_), g((threadIdx.x >> 4) & 3), c(threadIdx.x & 15),
+          col(p_, it_, threadIdx.x & 15) {
+#pragma unroll
+        for (int t = 0; t < VS; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    static __device__ __forceinline__ void reach(const RowsParams& p, int z, int64_t& lo,
+                                                 int64_t& hi) {
+        const int u = min(z * 16 + (int)(threadIdx.x & 15), p.n_q * p.rep - 1);
+        const int t = u / p.rep;
+        int32_t a = p.qpos ? p.qpos[t] : t, b = a;
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) {
+            a = min(a, __shfl_xor(a, off, 16));
+            b = max(b, __shfl_xor(b, off, 16));
+        }
+        lo = a;
+        hi = b;
+    }
+
+    __device__ __forceinline__ void split_query(const float (&qs)[KS]) {
+        float qmax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < KS; ++e) qmax = fmaxf(qmax, fabsf(qs[e]));
+        qmax = fmaxf(qmax, __shfl_xor(qmax, 16));
+        qmax = fmaxf(qmax, __shfl_xor(qmax, 32));
+        int eq = 0;
+        if (qmax > 0.0f && qmax <= 3.4028235e38f) frexpf(qmax, &eq);
+        const float qsc = ldexpf(1.0f, 14 - eq);
+        qsl = ldexpf(p.scale * kLog2e, eq - 14);
+#pragma unroll
+        for (int st = 0; st < NS; ++st)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                _Float16 hi, lo;
+                split2(qs[8 * st + key_order<DT>(i)] * qsc, hi, lo);
+                qhi[st][i] = hi;
+                qlo[st][i] = lo;
+            }
+    }
+
+    // scores of keys 4g + r of both tiles, in log2 units
+    __device__ __forceinline__ void scores(const typename TL::K& A, const typename TL::K& B,
+                                           float (&sc)[8]) const {
+        v4f sa = {0.f, 0.f, 0.f, 0.f}, sb = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+            const h8 ka = key_codes<DT>(A.k, st), kb = key_codes<DT>(B.k, st);
+            sa = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[st], sa, 0, 0, 0);
+            sb = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qlo[st], sb, 0, 0, 0);
+            sa = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[st], sa, 0, 0, 0);
+            sb = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qhi[st], sb, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            sc[r] = sa[r] * (qsl * A.s[r]);
+            sc[4 + r] = sb[r] * (qsl * B.s[r]);
+        }
+    }
+
+    // the scores' probabilities times the values (la, lb: the tiles' places)
+    __device__ __forceinline__ void values(float (&sc)[8], const typename TL::V& A,
+                                           const typename TL::V& B, const typename TL::Place& la,
+                                           const typename TL::Place& lb) {
+        float vs[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            vs[r] = A.s[r];
+            vs[4 + r] = B.s[r];
+        }
+        const bool full = col.whole(p, it, la.kb, la.left) && col.whole(p, it, lb.kb, lb.left);
+        if (!full) {
+            // what lies in a key that a query does not keep (a scale that is not
+            // finite, say) is nothing to it
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const int r = x & 3, i = SRC == kLinearPos ? r : 0;
+                const bool keep = x < 4 ? col.keeps(p, it, la.kb, la.left, g, r, A.kp[i])
+                                        : col.keeps(p, it, lb.kb, lb.left, g, r, B.kp[i]);
+                sc[x] = keep ? sc[x] : -INFINITY;
+                vs[x] = keep ? vs[x] : 0.0f;
+            }
+        }
+        float tm = sc[0], vmax = vs[0];
+#pragma unroll
+        for (int x = 1; x < 8; ++x) {
+            tm = fmaxf(tm, sc[x]);
+            vmax = fmaxf(vmax, vs[x]);
+        }
+        tm = fmaxf(tm, __shfl_xor(tm, 16));
+        tm = fmaxf(tm, __shfl_xor(tm, 32));
+        vmax = fmaxf(vmax, __shfl_xor(vmax, 16));
+        vmax = fmaxf(vmax, __shfl_xor(vmax, 32));
+        if (!full) {
+#pragma unroll
+            for (int off = 8; off >= 1; off >>= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, off));
+        }
+        int ev = 0;
+        if (vmax > 0.0f && vmax <= 3.4028235e38f) frexpf(vmax, &ev);
+        ev = __builtin_amdgcn_readfirstlane(ev);
+        int e_new = e_acc;
+        if (ev > e_acc) {
+            e_new = ev;
+        } else if (ev < e_acc - 8) {
+            // down to ev, as far as the sums stay below 2^100
+            float amax = 0.0f;
+#pragma unroll
+            for (int t = 0; t < VS; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) amax = fmaxf(amax, fabsf(acc[t][r]));
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+            int ea = -1000;
+            if (amax > 0.0f) frexpf(amax, &ea);
+            ea = __builtin_amdgcn_readfirstlane(ea);
+            e_new = max(ev, e_acc - (100 - ea));
+        }
+        e_new = min(max(e_new, -120), 128);   // 2^(6 - e) and 2^(e - 6) normal
+        if (__any(tm > m + 8.0f) || e_new != e_acc) {
+            const float mn = fmaxf(m, tm);
+            if (e_acc != -1000) {     // (before the first step all sums are zero)
+                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                ls = ls * alpha;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float ar = __shfl(alpha, 4 * g + r);
+#pragma unroll
+                    for (int t = 0; t < VS; ++t) acc[t][r] *= ar;
+                }
+                const int d = e_acc - e_new;
+                if (d != 0) {
+#pragma unroll
+                    for (int t = 0; t < VS; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[t][r] = ldexpf(acc[t][r], d);
+                }
+            }
+            m = mn;
+            e_acc = e_new;
+        }
+        const float msafe = m == -INFINITY ? 0.0f : m;
+        const float psc = pow2i(6 - e_acc);
+        h8 phi, plo;
+        float psum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const float pr = __builtin_amdgcn_exp2f(sc[x] - msafe);
+            psum += pr;
+            _Float16 hi, lo;
+            split2(pr * vs[x] * psc, hi, lo);
+            phi[x] = hi;
+            plo[x] = lo;
+        }
+        ls += psum;
+#pragma unroll
+        for (int t = 0; t < VS; ++t) {
+            const h8 v = __builtin_bit_cast(
+                h8, make_uint4(value_pair<DT>(A.v[0], A.v[1], t), value_pair<DT>(A.v[2], A.v[3], t),
+                               value_pair<DT>(B.v[0], B.v[1], t), value_pair<DT>(B.v[2], B.v[3], t)));
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(plo, v, acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(phi, v, acc[t], 0, 0, 0);
+        }
+    }
+
+    __device__ __forceinline__ void walk(int x0, int x1) {
+        if (x0 >= x1) return;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        TL tl(p, it.kh, g, c);
+        float qs[KS];
+        const float* src = p.q + col.qrow * D;
+#pragma unroll
+        for (int e = 0; e < KS; e += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src + TL::kdim(g, e));
+            qs[e] = f.x; qs[e + 1] = f.y; qs[e + 2] = f.z; qs[e + 3] = f.w;
+        }
+        const int span = SRC == kPaged ? TL::kIdTiles << (p.page_shift - 4) : x1 - x0;
+        for (int xb = x0; xb < x1; xb += span) {
+            const int xe = min(x1, xb + span);
+            tl.pages(it, xb, xe);
+            typename TL::K ka, kb;
+            typename TL::V va, vb;
+            int x = xb + 2 * wave;
+            typename TL::Place la = tl.locate(it, x, xe), lb = tl.locate(it, x + 1, xe);
+            if (x < xe) {
+                tl.load(ka, la);
+                tl.load(kb, lb);
+                tl.load(va, la);
+                tl.load(vb, lb);
+            }
+            if (xb == x0) split_query(qs);
+            // the next step's keys are on their way during this one's softmax and
+            // value sum, its values during the next scores
+            while (x < xe) {
+                float sc[8];
+                scores(ka, kb, sc);
+                const typename TL::Place na = tl.locate(it, x + 8, xe),
+                                         nb = tl.locate(it, x + 9, xe);
+                __builtin_amdgcn_sched_barrier(0);
+                tl.load(ka, na);
+                tl.load(kb, nb);
+                __builtin_amdgcn_sched_barrier(0);
+                values(sc, va, vb, la, lb);
+                __builtin_amdgcn_sched_barrier(0);
+                tl.load(va, na);
+                tl.load(vb, nb);
+                __builtin_amdgcn_sched_barrier(0);
+                la = na;
+                lb = nb;
+                x += 8;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void finish(int64_t row) {
+        const float back = e_acc < -120 ? 0.0f : pow2i(e_acc - 6);
+#pragma unroll
+        for (int t = 0; t < VS; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][r] *= back;
+        finish_tile<TL, D>(p, it, col.rows, m * kLn2, ls, acc, row, sh);
+    }
+};
+
+// fp32 caches on the fp32 matrix cores (v_mfma_f32_16x16x4_f32): 16 keys a step.
+template <int D, Source SRC>
+struct F32Core {
+    static constexpr int VEC = 16;
+    static constexpr int UNIT = 4;
+    static constexpr int EU = D == 256 ? 1 : 2;
+    using TL = Tiles<0, D, SRC>;
+    using Shared = TileShared<D>;
+    static constexpr int KS = TL::KS, VS = TL::VS;
+
+    const RowsParams& p;
+    const Item& it;
+    Shared& sh;
+    int g, c;
+    Columns<SRC> col;
+    float m = -INFINITY, ls = 0.0f;    // (log2 units)
+    v4f acc[VS];
+    float qs[KS];
+
+    __device__ __forceinline__ F32Core(const RowsParams& p_, const Item& it_, Shared& sh_)
+        : p(p_), it(it_), sh(sh_), g((threadIdx.x >> 4) & 3), c(threadIdx.x & 15),
+          col(p_, it_, threadIdx.x & 15) {
+#pragma unroll
+        for (int t = 0; t < VS; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    static __device__ __forceinline__ void reach(const RowsParams& p, int z, int64_t& lo,
+                                                 int64_t& hi) {
+        F16Core<1, 64, SRC>::reach(p, z, lo, hi);
+    }
+
+    __device__ __forceinline__ void scores(const typename TL::K& t, float (&sc)[4]) const {
+        v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KS; j += 2) {
+            s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.k[j]), qs[j], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.k[j + 1]), qs[j + 1], s1,
+                                                      0, 0, 0);
+        }
+        const float c0 = p.scale * kLog2e;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[r] = (s0[r] + s1[r]) * c0;
+    }
+
+    __device__ __forceinline__ void values(float (&sc)[4], typename TL::V& t,
+                                           const typename TL::Place& l) {
+        bool leak = false;
+        uint64_t kept[4] = {~0ull, ~0ull, ~0ull, ~0ull};
+        if (!col.whole(p, it, l.kb, l.left)) {
+            // Values of keys that no query keeps become zeros; where some do and
+            // some do not and a value is not finite, 0 times it would reach the
+            // others: such a tile's value sum is done lane by lane.
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool keep = col.keeps(p, it, l.kb, l.left, g, r,
+                                            t.kp[SRC == kLinearPos ? r : 0]);
+                sc[r] = keep ? sc[r] : -INFINITY;
+                kept[r] = __ballot(keep);
+                const uint32_t mine = (uint32_t)(kept[r] >> (16 * g)) & 0xffffu;
+#pragma unroll
+                for (int e = 0; e < VS; ++e) {
+                    t.v[r][e] = mine == 0 ? 0u : t.v[r][e];
+                    leak = leak || (mine != 0xffffu &&
+                                    !(fabsf(__uint_as_float(t.v[r][e])) <= 3.4028235e38f));
+                }
+            }
+            leak = col.mixed && __any(leak);
+        }
+        float tm = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        tm = fmaxf(tm, __shfl_xor(tm, 16));
+        tm = fmaxf(tm, __shfl_xor(tm, 32));
+        // the sums move when a query's maximum passes the reference by 2^8
+        if (__any(tm > m + 8.0f)) {
+            const float mn = fmaxf(m, tm);
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            ls = ls * alpha;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float ar = __shfl(alpha, 4 * g + r);
+#pragma unroll
+                for (int e = 0; e < VS; ++e) acc[e][r] *= ar;
+            }
+            m = mn;
+        }
+        const float msafe = m == -INFINITY ? 0.0f : m;
+        float pr[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            pr[r] = __builtin_amdgcn_exp2f(sc[r] - msafe);
+            ls += pr[r];
+        }
+        if (leak) {
+            leaky_values(t, pr, kept);
+            return;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < VS; ++e)
+                acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pr[r], __uint_as_float(t.v[r][e]),
+                                                              acc[e], 0, 0, 0);
+    }
+
+    // acc[query 4g + r] += p v over the keys that the query keeps, by shuffles
+    // (a value at a time: it is rare, and must not hold registers)
+    __device__ __forceinline__ void leaky_values(const typename TL::V& t, const float (&pr)[4],
+                                                 const uint64_t (&kept)[4]) {
+#pragma unroll 1
+        for (int gk = 0; gk < 4; ++gk)
+#pragma unroll
+            for (int rk = 0; rk < 4; ++rk)
+#pragma unroll
+                for (int e = 0; e < VS; ++e) {
+                    const float v = __shfl(__uint_as_float(t.v[rk][e]), 16 * gk + c);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int q = 4 * g + r;
+                        const float w = __shfl(pr[rk], 16 * gk + q);
+                        const bool keep = (kept[rk] >> (16 * gk + q)) & 1;
+                        acc[e][r] = keep ? __builtin_fmaf(w, v, acc[e][r]) : acc[e][r];
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+    }
+
+    __device__ __forceinline__ void walk(int x0, int x1) {
+        if (x0 >= x1) return;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        TL tl(p, it.kh, g, c);
+        const float* src = p.q + col.qrow * D;
+#pragma unroll
+        for (int e = 0; e < KS; e += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src + TL::kdim(g, e));
+            qs[e] = f.x; qs[e + 1] = f.y; qs[e + 2] = f.z; qs[e + 3] = f.w;
+        }
+        const int span = SRC == kPaged ? TL::kIdTiles << (p.page_shift - 4) : x1 - x0;
+        for (int xb = x0; xb < x1; xb += span) {
+            const int xe = min(x1, xb + span);
+            tl.pages(it, xb, xe);
+            typename TL::K k;
+            typename TL::V v;
+            int x = xb + wave;
+            typename TL::Place l = tl.locate(it, x, xe);
+            if (x < xe) {
+                tl.load(k, l);
+                tl.load(v, l);
+            }
+            while (x < xe) {
+                float sc[4];
+                scores(k, sc);
+                const typename TL::Place n = tl.locate(it, x + 4, xe);
+                __builtin_amdgcn_sched_barrier(0);
+                tl.load(k, n);
+                __builtin_amdgcn_sched_barrier(0);
+                values(sc, v, l);
+                __builtin_amdgcn_sched_barrier(0);
+                tl.load(v, n);
+                __builtin_amdgcn_sched_barrier(0);
+                l = n;
+                x += 4;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void finish(int64_t row) {
+        finish_tile<TL, D>(p, it, col.rows, m * kLn2, ls, acc, row, sh);
+    }
+};
+
 // Inclusive sums over the wave's lanes
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
 #pragma unroll
@@ -285,7 +986,8 @@ __device__ __forceinline__ KeyTiles seq_tiles(const RowsParams& p, int32_t len) 
 // the span from the lengths by itself: a sum over the lanes, a scan over the 64
 // sequences around the span's begin.
 template <typename Core>
-__global__ __launch_bounds__(256) void rows_paged_kernel(RowsParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Core::EU))) void
+rows_paged_kernel(RowsParams p) {
     __shared__ typename Core::Shared sh;
     const int lane = threadIdx.x & 63;
     const int32_t per_seq = p.n_head_kv * p.tiles;
@@ -356,7 +1058,8 @@ __global__ __launch_bounds__(256) void rows_paged_kernel(RowsParams p) {
 // Contiguous: chunk blockIdx.x of n_chunks of item (kv head blockIdx.y, query
 // tile), the last query tiles (a prompt's longest) first.
 template <typename Core>
-__global__ __launch_bounds__(256) void rows_linear_kernel(RowsParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Core::EU))) void
+rows_linear_kernel(RowsParams p) {
     __shared__ typename Core::Shared sh;
     Item it;
     it.s = 0;
@@ -469,31 +1172,55 @@ __global__ __launch_bounds__(512) void rows_join_kernel(RowsParams p) {
 // ------------------------------------------------------------------- host
 using RowsKernel = void (*)(RowsParams);
 
-// A variant of the kernels: query vectors an item, key tiles a unit
+// A variant of the kernels: query vectors an item, key tiles a unit, workgroups
+// that fill the chip (two a CU, or one where a wave has a SIMD to itself)
 struct RowsVariant {
     const char* name;
-    int vec, unit;
-    RowsKernel paged, linear;
+    int vec, unit, workers;
+    RowsKernel paged, linear, linear_pos;
 };
+
+template <int DT, int E>
+RowsVariant vec_variant() {
+    return {"rows_vec_kernel", 4, 4, 512, rows_paged_kernel<VecCore<DT, E, true>>,
+            rows_linear_kernel<VecCore<DT, E, false>>, rows_linear_kernel<VecCore<DT, E, false>>};
+}
 
 template <int DT>
 RowsVariant vec_variant(int width) {
-    if (width <= 64)
-        return {"rows_vec_kernel", 4, 4, rows_paged_kernel<VecCore<DT, 4, true>>,
-                rows_linear_kernel<VecCore<DT, 4, false>>};
-    if (width <= 128)
-        return {"rows_vec_kernel", 4, 4, rows_paged_kernel<VecCore<DT, 8, true>>,
-                rows_linear_kernel<VecCore<DT, 8, false>>};
-    return {"rows_vec_kernel", 4, 4, rows_paged_kernel<VecCore<DT, 16, true>>,
-            rows_linear_kernel<VecCore<DT, 16, false>>};
+    return width <= 64 ? vec_variant<DT, 4>()
+                       : (width <= 128 ? vec_variant<DT, 8>() : vec_variant<DT, 16>());
 }
 
-RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim) {
+template <int DT, int D>
+RowsVariant f16_variant() {
+    return {"rows_f16_kernel", 16, 8, D == 256 ? 256 : 512,
+            rows_paged_kernel<F16Core<DT, D, kPaged>>, rows_linear_kernel<F16Core<DT, D, kLinear>>,
+            rows_linear_kernel<F16Core<DT, D, kLinearPos>>};
+}
+
+template <int D>
+RowsVariant f32_variant() {
+    return {"rows_f32_kernel", 16, 4, D == 256 ? 256 : 512, rows_paged_kernel<F32Core<D, kPaged>>,
+            rows_linear_kernel<F32Core<D, kLinear>>, rows_linear_kernel<F32Core<D, kLinearPos>>};
+}
+
+template <int D>
+RowsVariant mfma_variant(int dt) {
+    return dt == 0 ? f32_variant<D>() : (dt == 1 ? f16_variant<1, D>() : f16_variant<2, D>());
+}
+
+// The matrix cores take head_dim == value_dim of 64, 128 and 256 with 16-byte
+// aligned rows; any other width, or alignment, the vector kernel.
+RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool aligned) {
+    if (aligned && head_dim == value_dim && tune("rows_mfma", 1) != 0) {
+        if (head_dim == 64) return mfma_variant<64>(dt);
+        if (head_dim == 128) return mfma_variant<128>(dt);
+        if (head_dim == 256) return mfma_variant<256>(dt);
+    }
     const int width = (int)std::max(head_dim, value_dim);
     return dt == 0 ? vec_variant<0>(width) : (dt == 1 ? vec_variant<1>(width) : vec_variant<2>(width));
 }
-
-constexpr int kRowsWorkers = 512;   // workgroups that fill the chip
 
 // Bytes of the parts and spans: parts (16-byte aligned), (m, l), spans
 int64_t rows_workspace(const RowsVariant& k, int64_t workers, int64_t items, int64_t pitch) {
@@ -525,7 +1252,7 @@ struct PagedPlan {
 };
 
 bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t n_head,
-                int64_t max_pages, PagedPlan& pl) {
+                int64_t max_pages, bool aligned, PagedPlan& pl) {
     if (!pool_ok(pool, "paged_attention")) return false;
     if (n_seq < 0 || n_q <= 0 || n_head <= 0 || n_head % pool.n_head_kv || max_pages <= 0 ||
         max_pages > (int64_t(1) << 30) / pool.page) {
@@ -535,7 +1262,7 @@ bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t 
                   (long long)pool.page);
         return false;
     }
-    pl.k = pick_variant(pool.kv_dt, pool.head_dim, pool.value_dim);
+    pl.k = pick_variant(pool.kv_dt, pool.head_dim, pool.value_dim, aligned);
     const int64_t n_vec = n_q * (n_head / pool.n_head_kv);
     pl.tiles = (n_vec + pl.k.vec - 1) / pl.k.vec;
     if (n_q > (int64_t(1) << 24) || n_vec > (int64_t(1) << 28) || n_seq > (int64_t(1) << 24) ||
@@ -548,7 +1275,7 @@ bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t 
     const int64_t units = std::max<int64_t>(1, (max_pages * pool.page / 16 + pl.k.unit - 1) /
                                                    pl.k.unit);
     pl.cut = units > 1;
-    pl.workers = std::min<int64_t>(kRowsWorkers, pl.items * units);
+    pl.workers = std::min<int64_t>(pl.k.workers, pl.items * units);
     pl.bytes = rows_workspace(pl.k, pl.workers, pl.items, (pool.value_dim + 3) / 4 * 4);
     return true;
 }
@@ -558,7 +1285,8 @@ bool paged_attention_dev(const aero_kv_pool_t& pool, int64_t layer, const float*
                          int64_t n_seq, int64_t n_q, int64_t n_head, float scale, int window,
                          int sinks, int32_t* bad, void* ws, int64_t ws_bytes, hipStream_t s) {
     PagedPlan pl;
-    if (!paged_plan(pool, n_seq, n_q, n_head, max_pages, pl)) return false;
+    if (!paged_plan(pool, n_seq, n_q, n_head, max_pages, aligned16(q) && aligned16(out), pl))
+        return false;
     if (layer < 0 || layer >= pool.n_layers || window < 0 || sinks < 0) {
         set_error("paged_attention: bad layer %lld, window %d or sinks %d", (long long)layer,
                   window, sinks);
@@ -602,16 +1330,16 @@ struct LinearPlan {
 };
 
 bool linear_plan(int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_dim,
-                 int64_t value_dim, int64_t n_kv, int window, int sinks, int kv_dt,
+                 int64_t value_dim, int64_t n_kv, int window, int sinks, int kv_dt, bool aligned,
                  LinearPlan& pl) {
-    pl.k = pick_variant(kv_dt, head_dim, value_dim);
+    pl.k = pick_variant(kv_dt, head_dim, value_dim, aligned);
     const int64_t rep = n_head / n_head_kv;
     pl.tiles = (n_q * rep + pl.k.vec - 1) / pl.k.vec;
     // about the key tiles of an item, and enough chunks of them to fill the chip
     const int64_t keys = std::min<int64_t>(n_kv, (int64_t)window + sinks + pl.k.vec / rep + 32);
     const int64_t units = (keys + 16 * pl.k.unit - 1) / (16 * pl.k.unit);
     const int64_t base = n_head_kv * pl.tiles;
-    pl.n_chunks = std::max<int64_t>(1, std::min<int64_t>(units, kRowsWorkers / base));
+    pl.n_chunks = std::max<int64_t>(1, std::min<int64_t>(units, pl.k.workers / base));
     pl.bytes = pl.n_chunks > 1 ? rows_workspace(pl.k, base * pl.n_chunks, base,
                                                 (value_dim + 3) / 4 * 4) : 0;
     return true;
@@ -621,9 +1349,10 @@ bool linear_plan(int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_di
 
 int64_t rows_sinks_workspace(int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_dim,
                              int64_t value_dim, int64_t n_kv, int window, int sinks, int kv_dt) {
-    LinearPlan pl;
-    linear_plan(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks, kv_dt, pl);
-    return pl.bytes;
+    LinearPlan a, b;     // (whichever the pointers' alignment will choose)
+    linear_plan(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks, kv_dt, true, a);
+    linear_plan(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks, kv_dt, false, b);
+    return std::max(a.bytes, b.bytes);
 }
 
 // (sizes and pointers checked by the caller)
@@ -633,7 +1362,8 @@ bool rows_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_sca
                     const int32_t* qpos, const int32_t* kpos, int64_t n_kv, int window, int sinks,
                     void* ws, int64_t ws_bytes, hipStream_t s) {
     LinearPlan pl;
-    linear_plan(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks, kv_dt, pl);
+    linear_plan(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks, kv_dt,
+                aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), pl);
     if (pl.bytes > 0 && (ws == nullptr || ws_bytes < pl.bytes || !aligned16(ws))) {
         set_error("attention_sinks: workspace %lld bytes < %lld needed (16-byte aligned)",
                   (long long)ws_bytes, (long long)pl.bytes);
@@ -660,7 +1390,7 @@ bool rows_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_sca
     p.workers = (int32_t)(n_head_kv * pl.tiles * pl.n_chunks);
     p.scale = scale;
     if (pl.n_chunks > 1) place_workspace(p, pl.k, ws);
-    if (!launch(pl.k.name, pl.k.linear,
+    if (!launch(pl.k.name, kpos == nullptr ? pl.k.linear : pl.k.linear_pos,
                 dim3((unsigned)pl.n_chunks, (unsigned)n_head_kv, (unsigned)pl.tiles), dim3(256), 0,
                 s, p))
         return false;
@@ -674,9 +1404,11 @@ extern "C" {
 int64_t aero_hip_paged_attention_workspace(const aero_kv_pool_t* pool, int64_t n_seq, int64_t n_q,
                                            int64_t n_head, int64_t max_pages) {
     aero::clear_error();
-    aero::PagedPlan pl;
-    if (pool == nullptr || !aero::paged_plan(*pool, n_seq, n_q, n_head, max_pages, pl)) return -1;
-    return pl.bytes;
+    aero::PagedPlan a, b;    // (whichever the pointers' alignment will choose)
+    if (pool == nullptr || !aero::paged_plan(*pool, n_seq, n_q, n_head, max_pages, true, a) ||
+        !aero::paged_plan(*pool, n_seq, n_q, n_head, max_pages, false, b))
+        return -1;
+    return std::max(a.bytes, b.bytes);
 }
 
 int aero_hip_paged_attention(const aero_kv_pool_t* pool, int64_t layer, const float* q, float* out,
