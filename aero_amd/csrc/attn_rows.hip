@@ -12,12 +12,13 @@
 //
 // Work (paged_sched.hpp): an item is a sequence, a kv head and a tile of query
 // vectors (token t, head kh rep + r: every head of the group shares the keys);
-// its key tiles are cut into units.
-//  * paged: a fixed number of workgroups take equal spans of all items' units,
-//    read from the lengths on the device: a batch of ragged lengths is balanced,
-//    and a recorded plan stays right as the sequences grow. An item cut by a
-//    span's end leaves parts that rows_join_kernel joins.
-//  * contiguous: every item's units go to n_chunks workgroups.
+// its key tiles are cut into chunks, one a workgroup.
+//  * paged: workgroups find their chunk from the lengths on the device: items are
+//    cut so that all chunks are about as long, and the grid has room for as many
+//    as there can be, so a batch of ragged lengths is balanced and a recorded plan
+//    stays right as the sequences grow.
+//  * contiguous: every item has n_chunks.
+// The parts of an item of several chunks are joined by rows_join_kernel.
 // Page ids are checked against the pool: tiles of a bad page are not seen.
 #include "attn_common.hpp"
 #include "paged_sched.hpp"
@@ -43,14 +44,16 @@ struct RowsParams {
     const int32_t* qpos;   // contiguous: [n_q] or null (= t)
     const int32_t* kpos;   // contiguous: [n_kv] or null (= j)
     int32_t* bad;          // set to 1 when a bad page was met, or null
-    float* part;           // [workers][2][VEC] rows of pitch floats, then (m, l) of each
-    int2* spans;           // [items]: first and last worker of the item
+    float* part;           // [parts][VEC] rows of pitch floats, then (m, l) of each
+    int2* spans;           // [items]: the item's first part, and how many
     int32_t n_seq, n_q, n_head, n_head_kv, rep, head_dim, value_dim, pitch;
     int32_t n_pages, max_pages, page_shift;
     int32_t n_kv;          // contiguous: keys; paged: the table's room in tokens
     int32_t tiles;         // query tiles a kv head and sequence
     int32_t window, sinks;
-    int32_t workers, n_chunks;
+    int32_t parts;         // room for
+    int32_t target;        // paged: chunks that fill the chip
+    int32_t n_chunks;      // contiguous
     float scale;
 };
 
@@ -74,7 +77,7 @@ __device__ __forceinline__ float* part_row(const RowsParams& p, int64_t row) {
     return p.part + row * p.pitch;
 }
 __device__ __forceinline__ float2* part_ml(const RowsParams& p, int vec, int64_t row) {
-    return reinterpret_cast<float2*>(p.part + (int64_t)p.workers * 2 * vec * p.pitch) + row;
+    return reinterpret_cast<float2*>(p.part + (int64_t)p.parts * vec * p.pitch) + row;
 }
 
 // The page of table column col of sequence s, or -1 (none, or not of the pool)
@@ -265,6 +268,7 @@ struct VecCore {
 // scores a lane receives are the value sum's operand as they come. Each of the
 // four waves takes every fourth step of the item's list; their sums meet in LDS.
 enum Source { kPaged, kLinear, kLinearPos };
+constexpr int kIds = 1024;   // page ids a workgroup holds at a time
 
 // One kv head's tiles in memory, through buffer descriptors: lane offsets within
 // a tile are fixed, the tile's place is wave-uniform, and what lies past the
@@ -304,44 +308,29 @@ struct Tiles {
     const RowsParams& p;
     int kh, g, c;
     uint32_t stride;     // from a key to the next
-    static constexpr int kIds = 4;
-    int32_t ids[kIds];   // paged: ids of 64 kIds pages of the list, a lane each
+    const int32_t* ids;  // paged: in LDS, the pages of the list from place0 on
     int32_t place0;
 
-    __device__ __forceinline__ Tiles(const RowsParams& p_, int kh_, int g_, int c_)
-        : p(p_), kh(kh_), g(g_), c(c_) {
+    __device__ __forceinline__ Tiles(const RowsParams& p_, const int32_t* ids_, int kh_, int g_,
+                                     int c_)
+        : p(p_), kh(kh_), g(g_), c(c_), ids(ids_) {
         stride = SRC == kPaged ? KVEC : (uint32_t)(p.n_head_kv * KVEC);
     }
-    // tiles that a set of ids is sure to cover (a multiple of 8; the sinks' and
-    // the window's first and last pages may be partly used)
-    static constexpr int kIdTiles = 64 * kIds - 8;
 
-    // ids for places x .. of the list (x1: its end)
-    __device__ __forceinline__ void pages(const Item& it, int x, int x1) {
+    // the ids for places x .. x1 - 1 of the list into LDS (no more than
+    // id_tiles() places; the workgroup's threads, between barriers)
+    __device__ __forceinline__ void pages(const Item& it, int x, int x1, int32_t* to) {
         if constexpr (SRC == kPaged) {
-            const int shift = p.page_shift - 4, lane = threadIdx.x & 63;
+            const int shift = p.page_shift - 4;
             place0 = it.kt.page_place(x, shift);
             const int n = it.kt.page_place(x1 - 1, shift) - place0 + 1;
-            bool bad = false;
-#pragma unroll
-            for (int r = 0; r < kIds; ++r) {
-                const int i = 64 * r + lane;
-                const int32_t col = it.kt.column(place0 + i, shift);
-                int32_t id = -1;
-                if (i < n && col < p.max_pages) id = p.table[(int64_t)it.s * p.max_pages + col];
-                const bool ok = id >= 0 && id < p.n_pages;
-                bad = bad || (i < n && !ok);
-                ids[r] = ok ? id : -1;
-            }
-            if (p.bad != nullptr && __any(bad)) *p.bad = 1;
+            for (int i = threadIdx.x; i < n; i += 256)
+                to[i] = page_at(p, it.s, it.kt.column(place0 + i, shift));
         }
     }
-    __device__ __forceinline__ int32_t id(int i) const {
-        int32_t x = __builtin_amdgcn_readlane(ids[0], i & 63);
-#pragma unroll
-        for (int r = 1; r < kIds; ++r)
-            x = (i >> 6) == r ? __builtin_amdgcn_readlane(ids[r], i & 63) : x;
-        return x;
+    // (the sinks' and the window's first and last pages may be partly used)
+    __device__ __forceinline__ int id_tiles(int all) const {
+        return SRC == kPaged ? (kIds - 8) << (p.page_shift - 4) : all;
     }
 
     template <int N>
@@ -374,7 +363,9 @@ struct Tiles {
         l.kb = 16 * tile;
         if constexpr (SRC == kPaged) {
             const int shift = p.page_shift - 4;
-            const int32_t page = x < x1 ? id(it.kt.page_place(x, shift) - place0) : -1;
+            const int32_t page = x < x1 ? __builtin_amdgcn_readfirstlane(
+                                              ids[it.kt.page_place(x, shift) - place0])
+                                        : -1;
             l.left = page >= 0 ? 16 : 0;
             l.vec = (((int64_t)max(page, 0) * p.n_head_kv + kh) << p.page_shift) +
                     16 * (tile & ((1 << shift) - 1));
@@ -430,11 +421,17 @@ struct Tiles {
     }
 };
 
-// A tile's query vectors: column c's row, position and the keys it sees
+// the row of q and out of query vector i of an item's tile (a copy of the last
+// one past it)
+__device__ __forceinline__ int64_t query_row(const RowsParams& p, const Item& it, int i) {
+    const int u = min(16 * it.z + i, p.n_q * p.rep - 1);
+    return ((int64_t)it.s * p.n_q + u / p.rep) * p.n_head + it.kh * p.rep + u % p.rep;
+}
+
+// A tile's query vectors: column c's position and the keys it sees
 template <Source SRC>
 struct Columns {
     int rows;            // vectors there are
-    int64_t qrow;
     int32_t qp, klo;     // kept: kp <= qp and (kp >= klo or kp < sinks)
     int32_t qmin, klo_max;
     bool mixed;          // positions differ
@@ -445,7 +442,6 @@ struct Columns {
         // (a column past the last vector is a copy of that one, never written)
         const int u = min(16 * it.z + c, n_vec - 1);
         const int t = u / p.rep;
-        qrow = ((int64_t)it.s * p.n_q + t) * p.n_head + it.kh * p.rep + u % p.rep;
         qp = SRC == kPaged ? it.pos0 + t : (p.qpos ? p.qpos[t] : t);
         klo = p.window > 0 ? (int32_t)max<int64_t>((int64_t)qp - p.window + 1, INT32_MIN)
                            : INT32_MIN;
@@ -479,7 +475,14 @@ struct Columns {
 template <int D>
 struct TileShared {
     float m[4][16], l[4][16], w[4][16], mt[16], lt[16];
-    float acc[4][16][D + 4];
+    float qscale[16];
+    int32_t ids[kIds];
+    union {
+        float acc[4][16][D + 4];
+        // the queries in the order that the lanes' matrix operands have
+        v4f q[D / 16][64];        // fp32: elements 4j .. 4j + 3 of lane l's slice
+        h8 qh[D / 32][2][64];     // fp16 parts: elements 8j .. 8j + 7
+    };
 };
 
 // The four waves' (m, l, acc) of a tile joined through LDS; its rows written out
@@ -551,7 +554,7 @@ template <int DT, int D, Source SRC>
 struct F16Core {
     static constexpr int VEC = 16;
     static constexpr int UNIT = 8;
-    static constexpr int EU = D == 256 ? 1 : 2;
+    static constexpr int EU = D == 256 ? 2 : 3;
     using TL = Tiles<DT, D, SRC>;
     using Shared = TileShared<D>;
     static constexpr int KS = TL::KS, VS = TL::VS, NS = KS / 8;
@@ -564,7 +567,6 @@ struct F16Core {
     float m = -INFINITY, ls = 0.0f;
     int e_acc = -1000;
     v4f acc[VS];
-    h8 qhi[NS], qlo[NS];
     float qsl;
 
     __device__ __forceinline__ F16Core(const RowsParams& p_, const Item& it_, Shared& sh_)
@@ -587,25 +589,51 @@ struct F16Core {
         hi = b;
     }
 
-    __device__ __forceinline__ void split_query(const float (&qs)[KS]) {
+    // The queries' parts into LDS: 16 lanes a row, a row's 4 NS operands (step
+    // st, lane group) among them, scaled by a power of two per row.
+    static constexpr int QI = (4 * NS + 15) / 16;
+    __device__ __forceinline__ void load_query(float (&f)[QI][8]) const {
+        const int row = threadIdx.x >> 4;
+        const int64_t qrow = query_row(p, it, row);
+#pragma unroll
+        for (int i = 0; i < QI; ++i) {
+            const int x = min(16 * i + (int)(threadIdx.x & 15), 4 * NS - 1);
+            const float* src = p.q + qrow * D + TL::kdim(x & 3, 8 * (x >> 2));
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src + e);
+                f[i][e] = v.x; f[i][e + 1] = v.y; f[i][e + 2] = v.z; f[i][e + 3] = v.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void split_query(const float (&f)[QI][8]) {
+        const int row = threadIdx.x >> 4;
         float qmax = 0.0f;
 #pragma unroll
-        for (int e = 0; e < KS; ++e) qmax = fmaxf(qmax, fabsf(qs[e]));
-        qmax = fmaxf(qmax, __shfl_xor(qmax, 16));
-        qmax = fmaxf(qmax, __shfl_xor(qmax, 32));
+        for (int i = 0; i < QI; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qmax = fmaxf(qmax, fabsf(f[i][e]));
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) qmax = fmaxf(qmax, __shfl_xor(qmax, off, 16));
         int eq = 0;
         if (qmax > 0.0f && qmax <= 3.4028235e38f) frexpf(qmax, &eq);
         const float qsc = ldexpf(1.0f, 14 - eq);
-        qsl = ldexpf(p.scale * kLog2e, eq - 14);
+        if ((threadIdx.x & 15) == 0) sh.qscale[row] = ldexpf(p.scale * kLog2e, eq - 14);
 #pragma unroll
-        for (int st = 0; st < NS; ++st)
+        for (int i = 0; i < QI; ++i) {
+            const int x = 16 * i + (threadIdx.x & 15);
+            if (x >= 4 * NS) break;
+            h8 hi, lo;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                _Float16 hi, lo;
-                split2(qs[8 * st + key_order<DT>(i)] * qsc, hi, lo);
-                qhi[st][i] = hi;
-                qlo[st][i] = lo;
+            for (int e = 0; e < 8; ++e) {
+                _Float16 a, b;
+                split2(f[i][key_order<DT>(e)] * qsc, a, b);
+                hi[e] = a;
+                lo[e] = b;
             }
+            sh.qh[x >> 2][0][16 * (x & 3) + row] = hi;
+            sh.qh[x >> 2][1][16 * (x & 3) + row] = lo;
+        }
     }
 
     // scores of keys 4g + r of both tiles, in log2 units
@@ -614,11 +642,12 @@ struct F16Core {
         v4f sa = {0.f, 0.f, 0.f, 0.f}, sb = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
+            const h8 qhi = sh.qh[st][0][threadIdx.x & 63], qlo = sh.qh[st][1][threadIdx.x & 63];
             const h8 ka = key_codes<DT>(A.k, st), kb = key_codes<DT>(B.k, st);
-            sa = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo[st], sa, 0, 0, 0);
-            sb = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qlo[st], sb, 0, 0, 0);
-            sa = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi[st], sa, 0, 0, 0);
-            sb = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qhi[st], sb, 0, 0, 0);
+            sa = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qlo, sa, 0, 0, 0);
+            sb = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qlo, sb, 0, 0, 0);
+            sa = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qhi, sa, 0, 0, 0);
+            sb = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qhi, sb, 0, 0, 0);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -734,18 +763,17 @@ struct F16Core {
     __device__ __forceinline__ void walk(int x0, int x1) {
         if (x0 >= x1) return;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        TL tl(p, it.kh, g, c);
-        float qs[KS];
-        const float* src = p.q + col.qrow * D;
-#pragma unroll
-        for (int e = 0; e < KS; e += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src + TL::kdim(g, e));
-            qs[e] = f.x; qs[e + 1] = f.y; qs[e + 2] = f.z; qs[e + 3] = f.w;
-        }
-        const int span = SRC == kPaged ? TL::kIdTiles << (p.page_shift - 4) : x1 - x0;
+        TL tl(p, sh.ids, it.kh, g, c);
+        float f[QI][8];
+        load_query(f);
+        const int span = tl.id_tiles(x1 - x0);
         for (int xb = x0; xb < x1; xb += span) {
             const int xe = min(x1, xb + span);
-            tl.pages(it, xb, xe);
+            __syncthreads();     // (what was in LDS is read)
+            tl.pages(it, xb, xe, sh.ids);
+            if (xb == x0) split_query(f);
+            __syncthreads();
+            qsl = sh.qscale[c];
             typename TL::K ka, kb;
             typename TL::V va, vb;
             int x = xb + 2 * wave;
@@ -756,14 +784,13 @@ struct F16Core {
                 tl.load(va, la);
                 tl.load(vb, lb);
             }
-            if (xb == x0) split_query(qs);
             // the next step's keys are on their way during this one's softmax and
             // value sum, its values during the next scores
             while (x < xe) {
-                float sc[8];
-                scores(ka, kb, sc);
                 const typename TL::Place na = tl.locate(it, x + 8, xe),
                                          nb = tl.locate(it, x + 9, xe);
+                float sc[8];
+                scores(ka, kb, sc);
                 __builtin_amdgcn_sched_barrier(0);
                 tl.load(ka, na);
                 tl.load(kb, nb);
@@ -795,7 +822,7 @@ template <int D, Source SRC>
 struct F32Core {
     static constexpr int VEC = 16;
     static constexpr int UNIT = 4;
-    static constexpr int EU = D == 256 ? 1 : 2;
+    static constexpr int EU = D == 256 ? 1 : (D == 128 ? 2 : 3);
     using TL = Tiles<0, D, SRC>;
     using Shared = TileShared<D>;
     static constexpr int KS = TL::KS, VS = TL::VS;
@@ -807,7 +834,6 @@ struct F32Core {
     Columns<SRC> col;
     float m = -INFINITY, ls = 0.0f;    // (log2 units)
     v4f acc[VS];
-    float qs[KS];
 
     __device__ __forceinline__ F32Core(const RowsParams& p_, const Item& it_, Shared& sh_)
         : p(p_), it(it_), sh(sh_), g((threadIdx.x >> 4) & 3), c(threadIdx.x & 15),
@@ -823,10 +849,15 @@ struct F32Core {
     __device__ __forceinline__ void scores(const typename TL::K& t, float (&sc)[4]) const {
         v4f s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < KS; j += 2) {
-            s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.k[j]), qs[j], s0, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.k[j + 1]), qs[j + 1], s1,
-                                                      0, 0, 0);
+        for (int j = 0; j < KS; j += 4) {
+            const v4f q = sh.q[j / 4][threadIdx.x & 63];
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.k[j + e]), q[e], s0, 0,
+                                                          0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.k[j + e + 1]),
+                                                          q[e + 1], s1, 0, 0, 0);
+            }
         }
         const float c0 = p.scale * kLog2e;
 #pragma unroll
@@ -917,17 +948,30 @@ struct F32Core {
     __device__ __forceinline__ void walk(int x0, int x1) {
         if (x0 >= x1) return;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        TL tl(p, it.kh, g, c);
-        const float* src = p.q + col.qrow * D;
+        TL tl(p, sh.ids, it.kh, g, c);
+        // the queries into LDS: 16 lanes a row
+        constexpr int QI = D / 64;
+        const int row = threadIdx.x >> 4;
+        const float* src = p.q + query_row(p, it, row) * D;
+        v4f f[QI];
 #pragma unroll
-        for (int e = 0; e < KS; e += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src + TL::kdim(g, e));
-            qs[e] = f.x; qs[e + 1] = f.y; qs[e + 2] = f.z; qs[e + 3] = f.w;
+        for (int i = 0; i < QI; ++i) {
+            const int x = 16 * i + (threadIdx.x & 15);
+            f[i] = *reinterpret_cast<const v4f*>(src + TL::kdim(x & 3, 4 * (x >> 2)));
         }
-        const int span = SRC == kPaged ? TL::kIdTiles << (p.page_shift - 4) : x1 - x0;
+        const int span = tl.id_tiles(x1 - x0);
         for (int xb = x0; xb < x1; xb += span) {
             const int xe = min(x1, xb + span);
-            tl.pages(it, xb, xe);
+            __syncthreads();     // (what was in LDS is read)
+            tl.pages(it, xb, xe, sh.ids);
+            if (xb == x0) {
+#pragma unroll
+                for (int i = 0; i < QI; ++i) {
+                    const int x = 16 * i + (threadIdx.x & 15);
+                    sh.q[x >> 2][16 * (x & 3) + row] = f[i];
+                }
+            }
+            __syncthreads();
             typename TL::K k;
             typename TL::V v;
             int x = xb + wave;
@@ -937,9 +981,9 @@ struct F32Core {
                 tl.load(v, l);
             }
             while (x < xe) {
+                const typename TL::Place n = tl.locate(it, x + 4, xe);
                 float sc[4];
                 scores(k, sc);
-                const typename TL::Place n = tl.locate(it, x + 4, xe);
                 __builtin_amdgcn_sched_barrier(0);
                 tl.load(k, n);
                 __builtin_amdgcn_sched_barrier(0);
@@ -958,17 +1002,20 @@ struct F32Core {
     }
 };
 
-// Inclusive sums over the wave's lanes
-__device__ __forceinline__ int64_t wave_scan(int64_t v) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int64_t o = __shfl_up(v, off, 64);
-        if ((int)(threadIdx.x & 63) >= off) v += o;
-    }
-    return v;
+// Inclusive sums over the wave's lanes, by lane moves within rows of 16 and from
+// a row's last lane to the next rows
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t moved(int32_t v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ int64_t wave_value(int64_t v, int lane) {
-    return __shfl(v, lane, 64);
+__device__ __forceinline__ int32_t wave_scan(int32_t v) {
+    v += moved<0x111, 0xf>(v);    // from 1, 2, 4, 8 lanes below
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);    // lane 15 to row 1, 47 to row 3
+    v += moved<0x143, 0xc>(v);    // lane 31 to rows 2 and 3
+    return v;
 }
 __device__ __forceinline__ int64_t uniform64(int64_t v) {
     return (int64_t)(((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32)) << 32) |
@@ -982,77 +1029,59 @@ __device__ __forceinline__ KeyTiles seq_tiles(const RowsParams& p, int32_t len) 
     return key_tiles((int64_t)len - p.n_q, (int64_t)len - 1, len, p.window, p.sinks);
 }
 
-// Paged: worker blockIdx.x's span of units, item by item. Every wave works out
-// the span from the lengths by itself: a sum over the lanes, a scan over the 64
-// sequences around the span's begin.
+// Paged: workgroup blockIdx.x's chunk. Every wave finds it by itself: all items'
+// units summed over the lanes, then the chunks of 64 sequences at a time.
 template <typename Core>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Core::EU))) void
 rows_paged_kernel(RowsParams p) {
     __shared__ typename Core::Shared sh;
     const int lane = threadIdx.x & 63;
     const int32_t per_seq = p.n_head_kv * p.tiles;
-    int64_t total = 0;
+    // (the host keeps the units that the table has room for below 2^31)
+    int32_t total = 0;
     for (int s = lane; s < p.n_seq; s += 64)
-        total += (int64_t)item_units(seq_tiles(p, seq_len(p, s)).n, Core::UNIT) * per_seq;
-    total = uniform64(wave_value(wave_scan(total), 63));
-    const int64_t g = total < p.workers ? total : p.workers;
-    const int w = blockIdx.x;
-    if (w >= g) return;
-    int64_t u = span_begin(w, total, g);
-    const int64_t u_end = span_begin(w + 1, total, g);
-    // the sequence of unit u, and the units before it
-    int64_t base = 0;
-    int s = 0;
-    for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
+        total += item_units(seq_tiles(p, seq_len(p, s)).n, Core::UNIT) * per_seq;
+    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
+    int32_t b = blockIdx.x, part = 0;    // the chunk's place from a sequence's first on
+    int s0 = 0, s = -1;
+    for (; s0 < p.n_seq; s0 += 64) {
         const int x = s0 + lane;
-        const int64_t n = x < p.n_seq
-                              ? (int64_t)item_units(seq_tiles(p, seq_len(p, x)).n, Core::UNIT) *
-                                    per_seq
-                              : 0;
-        const int64_t upto = wave_scan(n);
-        const uint64_t past = __ballot(base + upto > u);
+        const int32_t n =
+            x < p.n_seq ? item_chunks(item_units(seq_tiles(p, seq_len(p, x)).n, Core::UNIT), total,
+                                      p.target) * per_seq
+                        : 0;
+        const int32_t m = n > per_seq ? n : 0;   // (an item of one chunk has no parts)
+        const int32_t upto = wave_scan(n), parts = wave_scan(m);
+        const uint64_t past = __ballot(upto > b);
         if (past != 0) {
             const int f = __ffsll((unsigned long long)past) - 1;
             s = s0 + f;
-            base = uniform64(base + wave_value(upto - n, f));
+            b -= __builtin_amdgcn_readlane(upto - n, f);
+            part += __builtin_amdgcn_readlane(parts - m, f);
             break;
         }
-        base += uniform64(wave_value(upto, 63));
+        b -= __builtin_amdgcn_readlane(upto, 63);
+        part += __builtin_amdgcn_readlane(parts, 63);
     }
-    s = __builtin_amdgcn_readfirstlane(s);
-
-    while (u < u_end && s < p.n_seq) {
-        Item it;
-        it.s = s;
-        it.len = __builtin_amdgcn_readfirstlane(seq_len(p, s));
-        it.pos0 = it.len - p.n_q;
-        it.kt = seq_tiles(p, it.len);
-        const int units = item_units(it.kt.n, Core::UNIT);
-        const int64_t end = base + (int64_t)units * per_seq;
-        while (u < u_end && u < end) {
-            const int64_t rel = u - base;
-            const int64_t item = rel / units;
-            const int a = (int)(rel % units);
-            const int b = (int)min<int64_t>(units, a + (u_end - u));
-            it.kh = (int)(item / p.tiles);
-            it.z = (int)(item % p.tiles);
-            // (keys past the tile's own last position are not walked)
-            const int t_last = min(it.z * Core::VEC + Core::VEC - 1, p.n_q * p.rep - 1) / p.rep;
-            const int x1 = min(b * Core::UNIT, it.kt.upto(it.pos0 + t_last));
-            Core core(p, it, sh);
-            core.walk(a * Core::UNIT, x1);
-            const bool whole = a == 0 && b == units;
-            core.finish(whole ? -1 : ((int64_t)w * 2 + (a == 0 ? 1 : 0)) * Core::VEC);
-            if (a == 0 && threadIdx.x == 0) {
-                const int64_t first = base + item * units;
-                p.spans[item_index(p, it)] =
-                    make_int2(w, (int)span_of(first + units - 1, total, g));
-            }
-            u += b - a;
-        }
-        base = end;
-        ++s;
-    }
+    if (s < 0) return;
+    Item it;
+    it.s = __builtin_amdgcn_readfirstlane(s);
+    it.len = __builtin_amdgcn_readfirstlane(seq_len(p, it.s));
+    it.pos0 = it.len - p.n_q;
+    it.kt = seq_tiles(p, it.len);
+    const int32_t units = item_units(it.kt.n, Core::UNIT);
+    const int32_t chunks = item_chunks(units, total, p.target);
+    const int32_t item = b / chunks, c = b % chunks;
+    it.kh = item / p.tiles;
+    it.z = item % p.tiles;
+    // (keys past the tile's own last position are not walked)
+    const int t_last = min(it.z * Core::VEC + Core::VEC - 1, p.n_q * p.rep - 1) / p.rep;
+    const int x1 = min(chunk_begin(c + 1, chunks, units) * Core::UNIT,
+                       it.kt.upto(it.pos0 + t_last));
+    Core core(p, it, sh);
+    core.walk(chunk_begin(c, chunks, units) * Core::UNIT, x1);
+    core.finish(chunks == 1 ? -1 : (int64_t)(part + b) * Core::VEC);
+    if (c == 0 && threadIdx.x == 0) p.spans[item_index(p, it)] = make_int2(part + b, chunks);
 }
 
 // Contiguous: chunk blockIdx.x of n_chunks of item (kv head blockIdx.y, query
@@ -1076,60 +1105,59 @@ rows_linear_kernel(RowsParams p) {
     }
     const int units = item_units(it.kt.n, Core::UNIT);
     const int c = blockIdx.x;
-    const int a = (int)((int64_t)c * units / p.n_chunks);
-    const int b = (int)((int64_t)(c + 1) * units / p.n_chunks);
+    const int a = chunk_begin(c, p.n_chunks, units), b = chunk_begin(c + 1, p.n_chunks, units);
     const int64_t item = item_index(p, it);
     Core core(p, it, sh);
     core.walk(a * Core::UNIT, min(b * Core::UNIT, it.kt.n));
-    core.finish(p.n_chunks == 1 ? -1
-                                : ((item * p.n_chunks + c) * 2 + (c == 0 ? 1 : 0)) * Core::VEC);
+    core.finish(p.n_chunks == 1 ? -1 : (item * p.n_chunks + c) * Core::VEC);
     if (c == 0 && threadIdx.x == 0 && p.n_chunks > 1)
-        p.spans[item] = make_int2((int)(item * p.n_chunks), (int)((item + 1) * p.n_chunks - 1));
+        p.spans[item] = make_int2((int)(item * p.n_chunks), p.n_chunks);
 }
 
-// The parts of one row (row blockIdx.x % VEC of item blockIdx.x / VEC) joined: a
-// group of pitch / 4 lanes takes every G-th part, then the groups meet in LDS.
-// The first worker's part is its slot 1 (it begins the item), the others' 0.
+// The parts of an item's rows joined: `groups` groups of pitch / 4 lanes a row
+// take every groups-th part, then the groups meet in LDS; 256 threads do as many
+// rows as fit.
 template <int VEC>
-__global__ __launch_bounds__(512) void rows_join_kernel(RowsParams p) {
-    __shared__ float sm[512], sl[512];
-    __shared__ float4 sa[512];
-    const int64_t item = blockIdx.x / VEC;
-    const int i = blockIdx.x % VEC;
+__global__ __launch_bounds__(256) void rows_join_kernel(RowsParams p, int32_t rows, int32_t groups) {
+    __shared__ float sm[256], sl[256];
+    __shared__ float4 sa[256];
+    const int tid = threadIdx.x;
+    const int lpr = p.pitch / 4, lanes = lpr * groups, per = 256 / lanes;
+    const int sub = (rows + per - 1) / per;      // workgroups an item
+    const int64_t item = blockIdx.x / sub;
+    const int2 span = p.spans[item];
+    const int n = span.y;
+    if (n <= 1) return;
+    const int i = (int)(blockIdx.x % sub) * per + tid / lanes;
+    const int d4 = tid % lpr, grp = tid % lanes / lpr;
     const int z = (int)(item % p.tiles);
     const int u = z * VEC + i;
-    if (u >= p.n_q * p.rep) return;
-    const int2 span = p.spans[item];
-    const int n = span.y - span.x + 1;
-    if (n <= 1) return;
-    const int tid = threadIdx.x;
-    const int lpr = p.pitch / 4, G = 512 / lpr;
-    const int d4 = tid % lpr, grp = tid / lpr;
+    const bool ok = tid < per * lanes && i < rows && u < p.n_q * p.rep;
     float M = -INFINITY, L = 0.0f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int B = 4;
-    if (grp < G) {
-        for (int c0 = grp; c0 < n; c0 += B * G) {
+    if (ok) {
+        for (int c0 = grp; c0 < n; c0 += B * groups) {
             float2 ml[B];
             float4 a[B];
 #pragma unroll
             for (int x = 0; x < B; ++x) {
-                const int c = min(c0 + x * G, n - 1);
-                const int64_t row = ((int64_t)(span.x + c) * 2 + (c == 0 ? 1 : 0)) * VEC + i;
+                const int c = min(c0 + x * groups, n - 1);
+                const int64_t row = (int64_t)(span.x + c) * VEC + i;
                 ml[x] = *part_ml(p, VEC, row);
                 a[x] = *reinterpret_cast<const float4*>(part_row(p, row) + 4 * d4);
             }
             float mb = M;
 #pragma unroll
             for (int x = 0; x < B; ++x)
-                if (c0 + x * G < n) mb = fmaxf(mb, ml[x].x);
+                if (c0 + x * groups < n) mb = fmaxf(mb, ml[x].x);
             const float sc = M == -INFINITY ? 0.0f : expf(M - mb);
             L *= sc;
             A.x *= sc; A.y *= sc; A.z *= sc; A.w *= sc;
 #pragma unroll
             for (int x = 0; x < B; ++x) {
-                // (a part without keys holds zeros; not so one that is no part)
-                if (c0 + x * G >= n || ml[x].x == -INFINITY) continue;
+                // (a part without keys holds zeros; a copy of the last is no part)
+                if (c0 + x * groups >= n || ml[x].x == -INFINITY) continue;
                 const float w = expf(ml[x].x - mb);
                 L = __builtin_fmaf(ml[x].y, w, L);
                 A.x = __builtin_fmaf(a[x].x, w, A.x);
@@ -1139,33 +1167,34 @@ __global__ __launch_bounds__(512) void rows_join_kernel(RowsParams p) {
             }
             M = mb;
         }
-        if (d4 == 0) sm[grp] = M;
     }
+    sm[tid] = M;
+    sl[tid] = L;
+    sa[tid] = A;
     __syncthreads();
-    if (grp < G) {
-        float mt = -INFINITY;
-        for (int k = 0; k < G; ++k) mt = fmaxf(mt, sm[k]);
-        const float w = M == -INFINITY ? 0.0f : expf(M - mt);
-        sa[tid] = make_float4(A.x * w, A.y * w, A.z * w, A.w * w);
-        if (d4 == 0) sl[grp] = L * w;
-    }
-    __syncthreads();
-    if (tid < lpr) {
+    if (ok && grp == 0) {
+        float mt = M;
+        for (int k = 1; k < groups; ++k) mt = fmaxf(mt, sm[tid + k * lpr]);
         float lt = 0.0f;
         float4 at = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < G; ++k) {
-            const float4 a = sa[k * lpr + tid];
-            lt += sl[k];
-            at.x += a.x; at.y += a.y; at.z += a.z; at.w += a.w;
+        for (int k = 0; k < groups; ++k) {
+            const int x = tid + k * lpr;
+            const float w = sm[x] == -INFINITY ? 0.0f : expf(sm[x] - mt);
+            const float4 a = sa[x];
+            lt = __builtin_fmaf(sl[x], w, lt);
+            at.x = __builtin_fmaf(a.x, w, at.x);
+            at.y = __builtin_fmaf(a.y, w, at.y);
+            at.z = __builtin_fmaf(a.z, w, at.z);
+            at.w = __builtin_fmaf(a.w, w, at.w);
         }
         const float r = 1.0f / fmaxf(lt, 1e-30f);
         const int64_t s = item / ((int64_t)p.n_head_kv * p.tiles);
         const int kh = (int)(item / p.tiles % p.n_head_kv);
         float* o = p.out + ((s * p.n_q + u / p.rep) * p.n_head + (int64_t)kh * p.rep + u % p.rep) *
-                               p.value_dim + 4 * tid;
+                               p.value_dim + 4 * d4;
         const float v[4] = {at.x * r, at.y * r, at.z * r, at.w * r};
         for (int x = 0; x < 4; ++x)
-            if (4 * tid + x < p.value_dim) o[x] = v[x];
+            if (4 * d4 + x < p.value_dim) o[x] = v[x];
     }
 }
 
@@ -1194,14 +1223,14 @@ RowsVariant vec_variant(int width) {
 
 template <int DT, int D>
 RowsVariant f16_variant() {
-    return {"rows_f16_kernel", 16, 8, D == 256 ? 256 : 512,
+    return {"rows_f16_kernel", 16, 8, 256 * F16Core<DT, D, kPaged>::EU,
             rows_paged_kernel<F16Core<DT, D, kPaged>>, rows_linear_kernel<F16Core<DT, D, kLinear>>,
             rows_linear_kernel<F16Core<DT, D, kLinearPos>>};
 }
 
 template <int D>
 RowsVariant f32_variant() {
-    return {"rows_f32_kernel", 16, 4, D == 256 ? 256 : 512, rows_paged_kernel<F32Core<D, kPaged>>,
+    return {"rows_f32_kernel", 16, 4, 256 * F32Core<D, kPaged>::EU, rows_paged_kernel<F32Core<D, kPaged>>,
             rows_linear_kernel<F32Core<D, kLinear>>, rows_linear_kernel<F32Core<D, kLinearPos>>};
 }
 
@@ -1222,19 +1251,27 @@ RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool align
     return dt == 0 ? vec_variant<0>(width) : (dt == 1 ? vec_variant<1>(width) : vec_variant<2>(width));
 }
 
-// Bytes of the parts and spans: parts (16-byte aligned), (m, l), spans
-int64_t rows_workspace(const RowsVariant& k, int64_t workers, int64_t items, int64_t pitch) {
-    return workers * 2 * k.vec * (pitch + 2) * 4 + items * 8;
+// Bytes of the parts (16-byte aligned), their (m, l), and the spans
+int64_t rows_workspace(const RowsVariant& k, int64_t parts, int64_t items, int64_t pitch) {
+    return parts * k.vec * (pitch + 2) * 4 + items * 8;
 }
 
 void place_workspace(RowsParams& p, const RowsVariant& k, void* ws) {
     p.part = static_cast<float*>(ws);
-    p.spans = reinterpret_cast<int2*>(p.part + (int64_t)p.workers * 2 * k.vec * (p.pitch + 2));
+    p.spans = reinterpret_cast<int2*>(p.part + (int64_t)p.parts * k.vec * (p.pitch + 2));
 }
 
 bool join(const RowsVariant& k, int64_t items, const RowsParams& p, hipStream_t s) {
+    // a group of lanes for each part that an item has on the average, as far as a
+    // row's groups fit a workgroup
+    const int lpr = p.pitch / 4;
+    const int rows = std::min(k.vec, p.n_q * p.rep);
+    int groups = 1;
+    while (groups < p.parts / items && 2 * groups * lpr <= 256) groups *= 2;
+    const int per = 256 / (lpr * groups);
+    const int64_t grid = items * ((rows + per - 1) / per);
     return launch("rows_join_kernel", k.vec == 4 ? rows_join_kernel<4> : rows_join_kernel<16>,
-                  dim3((unsigned)(items * k.vec)), dim3(512), 0, s, p);
+                  dim3((unsigned)grid), dim3(256), 0, s, p, rows, groups);
 }
 
 int log2_of(int64_t x) {
@@ -1247,8 +1284,8 @@ int log2_of(int64_t x) {
 // not possible. (Pointers are checked apart.)
 struct PagedPlan {
     RowsVariant k;
-    int64_t tiles, items, workers, bytes;
-    bool cut;   // some item may have more than one unit
+    int64_t tiles, items, target, bytes;
+    bool cut;   // some item may have more than one chunk
 };
 
 bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t n_head,
@@ -1271,12 +1308,22 @@ bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t 
                   (long long)n_seq, (long long)n_vec);
         return false;
     }
-    pl.items = n_seq * pool.n_head_kv * pl.tiles;
+    pl.items = std::max<int64_t>(n_seq * pool.n_head_kv * pl.tiles, 1);
     const int64_t units = std::max<int64_t>(1, (max_pages * pool.page / 16 + pl.k.unit - 1) /
                                                    pl.k.unit);
+    if (units > INT_MAX / pl.items) {
+        set_error("paged_attention: a table of %lld pages for %lld sequences has room for more "
+                  "work than one call takes", (long long)max_pages, (long long)n_seq);
+        return false;
+    }
     pl.cut = units > 1;
-    pl.workers = std::min<int64_t>(pl.k.workers, pl.items * units);
-    pl.bytes = rows_workspace(pl.k, pl.workers, pl.items, (pool.value_dim + 3) / 4 * 4);
+    // few items: all chunks run at once; else more chunks than fit, so that those
+    // of short sequences make room early
+    const int64_t fill = pl.k.workers;
+    const int64_t target = pl.items <= fill / 8 ? fill - pl.items
+                                                : (pl.items < fill ? 2 * fill : fill);
+    pl.target = std::min<int64_t>(target, pl.items * units);
+    pl.bytes = rows_workspace(pl.k, 2 * pl.target, pl.items, (pool.value_dim + 3) / 4 * 4);
     return true;
 }
 
@@ -1315,10 +1362,12 @@ bool paged_attention_dev(const aero_kv_pool_t& pool, int64_t layer, const float*
     p.n_kv = (int32_t)(max_pages * pool.page);
     p.tiles = (int32_t)pl.tiles;
     p.window = window; p.sinks = sinks;
-    p.workers = (int32_t)pl.workers;
+    p.target = (int32_t)pl.target;
+    p.parts = (int32_t)(2 * pl.target);
     p.scale = scale;
     place_workspace(p, pl.k, ws);
-    if (!launch(pl.k.name, pl.k.paged, dim3((unsigned)pl.workers), dim3(256), 0, s, p))
+    // (as many workgroups as there can be chunks)
+    if (!launch(pl.k.name, pl.k.paged, dim3((unsigned)(pl.target + pl.items)), dim3(256), 0, s, p))
         return false;
     return !pl.cut || join(pl.k, pl.items, p, s);
 }
@@ -1387,7 +1436,7 @@ bool rows_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_sca
     p.tiles = (int32_t)pl.tiles;
     p.window = window; p.sinks = sinks;
     p.n_chunks = (int32_t)pl.n_chunks;
-    p.workers = (int32_t)(n_head_kv * pl.tiles * pl.n_chunks);
+    p.parts = (int32_t)(n_head_kv * pl.tiles * pl.n_chunks);
     p.scale = scale;
     if (pl.n_chunks > 1) place_workspace(p, pl.k, ws);
     if (!launch(pl.k.name, kpos == nullptr ? pl.k.linear : pl.k.linear_pos,

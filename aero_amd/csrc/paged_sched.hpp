@@ -6,8 +6,9 @@
 // first key on (one run where the two meet), else all up to q_hi. A tile lies
 // in one page (pages are 16 tokens or more, a power of two).
 //
-// The tiles of an item (sequence, kv head, query tile) are cut into units; the
-// units of all items, in order, into equal spans, one a worker.
+// The tiles of an item (sequence, kv head, query tile) are grouped into units,
+// the units into chunks, one a workgroup: as many of about the same size as fill
+// the chip, whatever the items' lengths.
 #pragma once
 
 #include <cstdint>
@@ -74,15 +75,23 @@ AERO_HD KeyTiles key_tiles(int64_t q_lo, int64_t q_hi, int64_t n_kv, int32_t win
     return t;
 }
 
-// units of an item: at least one, so that some worker writes its rows
+// units of an item: at least one, so that some workgroup writes its rows
 AERO_HD int32_t item_units(int32_t n_tiles, int32_t tiles_a_unit) {
     const int32_t u = (n_tiles + tiles_a_unit - 1) / tiles_a_unit;
     return u > 0 ? u : 1;
 }
 
-// worker w of g takes units [span_begin(w), span_begin(w + 1)) of u
-AERO_HD int64_t span_begin(int64_t w, int64_t u, int64_t g) { return w * u / g; }
-// the worker of unit x
-AERO_HD int64_t span_of(int64_t x, int64_t u, int64_t g) { return ((x + 1) * g - 1) / u; }
+// The chunks of an item of u units where all items' units, `total`, are to make
+// about `target` chunks: at most total / target units each (rounded up), so no
+// more than target + items in all, and no more than 2 target in the items that
+// have several.
+AERO_HD int32_t item_chunks(int32_t u, int32_t total, int32_t target) {
+    const int32_t most = (total - 1) / target + 1;
+    return (u - 1) / most + 1;
+}
+// chunk c of n takes units [chunk_begin(c), chunk_begin(c + 1)) of u
+AERO_HD int32_t chunk_begin(int32_t c, int32_t n, int32_t u) {
+    return (int32_t)((int64_t)c * u / n);
+}
 
 }  // namespace aero

@@ -29,8 +29,8 @@ int tiles(long long lo, long long hi, long long n_kv, int window, int sinks, int
     return t.n;
 }
 int units(int n, int u) { return item_units(n, u); }
-long long begin(long long w, long long u, long long g) { return span_begin(w, u, g); }
-long long of(long long x, long long u, long long g) { return span_of(x, u, g); }
+int chunks(int u, int total, int target) { return item_chunks(u, total, target); }
+int begin(int c, int n, int u) { return chunk_begin(c, n, u); }
 }
 """
 
@@ -46,8 +46,6 @@ def sched(tmp_path_factory):
     L = ctypes.CDLL(str(so))
     i64, i32p = ctypes.c_int64, ctypes.POINTER(ctypes.c_int32)
     L.tiles.argtypes = [i64, i64, i64, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [i32p] * 4 + [i64]
-    L.begin.argtypes = L.of.argtypes = [i64, i64, i64]
-    L.begin.restype = L.of.restype = i64
     return L
 
 
@@ -81,20 +79,24 @@ def test_key_tiles_are_those_of_the_seen_keys(sched):
         assert upto.value == sum(16 * t <= q for t in got)
 
 
-def test_spans_cover_every_unit_once(sched):
+def test_chunks_cover_every_unit_once(sched):
+    """An item's chunks are its units, none empty, none longer than the share of a
+    chunk; all items' chunks fit the grid and the room for parts."""
     rng = random.Random(2)
     assert [sched.units(n, 8) for n in (0, 1, 8, 9)] == [1, 1, 1, 2]
-    for _ in range(500):
-        u = rng.choice((1, 2, 511, 512, 513, rng.randint(1, 10**7)))
-        g = min(u, rng.choice((1, 7, 256, 512)))
-        cuts = [sched.begin(w, u, g) for w in range(g + 1)]
-        assert cuts[0] == 0 and cuts[-1] == u and all(a < b for a, b in zip(cuts, cuts[1:]))
-        for x in {0, u - 1, rng.randrange(u), *(c for c in cuts[1:-1][:20]),
-                  *(c - 1 for c in cuts[1:][:20])}:
-            w = sched.of(x, u, g)
-            assert cuts[w] <= x < cuts[w + 1]
-    big = 1 << 40
-    assert sched.of(big - 1, big, 512) == 511 and sched.begin(512, big, 512) == big
+    for _ in range(400):
+        items = [rng.choice((1, 2, rng.randint(1, 40), rng.randint(1, 3000)))
+                 for _ in range(rng.randint(1, 60))]
+        total, target = sum(items), rng.choice((1, 5, 256, 768))
+        n = [sched.chunks(u, total, target) for u in items]
+        assert sum(n) <= target + len(items) and sum(x for x in n if x > 1) <= 2 * target
+        for u, c in zip(items, n):
+            cuts = [sched.begin(i, c, u) for i in range(c + 1)]
+            assert cuts[0] == 0 and cuts[-1] == u
+            assert all(0 < b - a <= -(-total // target) for a, b in zip(cuts, cuts[1:]))
+    big = 2**31 - 1
+    n = sched.chunks(big, big, 768)
+    assert n <= 769 and sched.begin(n, n, big) == big and sched.begin(1, n, big) > 0
 
 
 def test_kv_pool_struct_layout(tmp_path):
