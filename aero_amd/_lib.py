@@ -208,7 +208,7 @@ PROTOTYPES = {
                                         c_int64, c_int64, vp, vp]),
     "aero_hip_paged_kv_read": (c_int, [POINTER(KvPool), c_int64, vp, vp, vp, c_int64, vp,
                                        c_int64, c_int64, vp, vp]),
-    "aero_hip_kv_pages_copy": (c_int, [POINTER(KvPool), ip, ip, c_int64, vp]),
+    "aero_hip_kv_pages_copy": (c_int, [POINTER(KvPool), vp, vp, c_int64, vp]),
     "aero_hip_write_i32": (c_int, [vp, c_int64, POINTER(c_int64), ip, c_int64, vp]),
     "aero_hip_kv_write": (c_int, [c_int, vp, c_int64, c_int64, c_int64, c_int64, c_int64, vp,
                                   vp, vp]),

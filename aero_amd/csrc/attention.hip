@@ -55,6 +55,7 @@ struct AttnParams {
     float scale;
     int64_t chunk_len;     // keys per chunk (a multiple of the kernel's keys per step)
     int n_chunks;
+    int sinks;             // attention_sinks: keys at positions below it stay visible
 };
 
 // E consecutive elements [e0, e0+E) of vector `vec` of a cache side, as fp32
@@ -96,6 +97,12 @@ __device__ __forceinline__ bool key_kept(int64_t kp, int64_t qp, int window) {
     bool keep = kp <= qp;
     if (window > 0) keep = keep && (qp - kp) < window;
     return keep;
+}
+
+template <bool SINK>
+__device__ __forceinline__ bool key_kept(const AttnParams& p, int64_t kp, int64_t qp) {
+    if constexpr (SINK) return kp <= qp && (p.window <= 0 || qp - kp < p.window || kp < p.sinks);
+    return key_kept(kp, qp, p.window);
 }
 
 // MERGE_OUT: one chunk, write out directly; else write the chunk's partials.
@@ -381,7 +388,7 @@ __device__ __forceinline__ void merge_tile(const AttnParams& p, float m, float l
 
 // One 16-key tile (first key kb, keys at or past c1 masked) against a wave's
 // 16 queries: scores, running max and sum, value sum.
-template <int DT, int D, int DV>
+template <int DT, int D, int DV, bool SINK = false>
 __device__ __forceinline__ void mfma_step(const AttnParams& p, const KvTile<DT, D, DV>& tl,
                                           const float (&qs)[D / 4], int64_t kb, int64_t c1,
                                           int64_t qp, bool qok, int g, float& m, float& ls,
@@ -401,7 +408,7 @@ __device__ __forceinline__ void mfma_step(const AttnParams& p, const KvTile<DT, 
     for (int r = 0; r < 4; ++r) {
         const int64_t kj = kb + 4 * g + r;
         const int64_t kp = p.kpos ? (int64_t)__shfl(tl.kp, 4 * g + r) : kj;
-        const bool keep = qok && kj < c1 && key_kept(kp, qp, p.window);
+        const bool keep = qok && kj < c1 && key_kept<SINK>(p, kp, qp);
         float y = (s0[r] + s1[r]);
         if constexpr (DT != 0) y *= __shfl(tl.ks, 4 * g + r);
         sc[r] = keep ? y * p.scale : -INFINITY;
@@ -1124,11 +1131,12 @@ AttnKernel pick_f16(int dt, int D, bool merge_out, bool kpos) {
                    : (dt == 2 ? pick_f16_dt<2>(D, merge_out, kpos) : nullptr);
 }
 
+template <bool SINK>
 AttnKernel pick_split(int D, bool kpos) {
     switch (D) {
-    case 64: return kpos ? attn_split_kernel<64, true> : attn_split_kernel<64, false>;
-    case 128: return kpos ? attn_split_kernel<128, true> : attn_split_kernel<128, false>;
-    case 256: return kpos ? attn_split_kernel<256, true> : attn_split_kernel<256, false>;
+    case 64: return kpos ? attn_split_kernel<64, true, SINK> : attn_split_kernel<64, false, SINK>;
+    case 128: return kpos ? attn_split_kernel<128, true, SINK> : attn_split_kernel<128, false, SINK>;
+    case 256: return kpos ? attn_split_kernel<256, true, SINK> : attn_split_kernel<256, false, SINK>;
     default: return nullptr;
     }
 }
@@ -1363,9 +1371,9 @@ bool attention_dev(const float* q, int kv_dt, const void* k, const float* k_scal
     plan_split(n_q, n_head, n_head_kv, head_dim, n_kv, window, kv_dt, kpos != nullptr, pl);
     AttnParams p{q, k, k_scale, v, v_scale, out, static_cast<float*>(workspace), qpos, kpos,
                  n_q, n_head, n_head_kv, head_dim, value_dim, n_kv,
-                 (int)(n_head / n_head_kv), window, scale, pl.chunk_len, pl.n_chunks};
+                 (int)(n_head / n_head_kv), window, scale, pl.chunk_len, pl.n_chunks, 0};
     const bool one = pl.n_chunks == 1;
-    AttnKernel kern = pl.split ? pick_split((int)head_dim, kpos != nullptr)
+    AttnKernel kern = pl.split ? pick_split<false>((int)head_dim, kpos != nullptr)
                       : pl.f16 ? pick_f16(kv_dt, (int)head_dim, one, kpos != nullptr)
                       : pl.mfma ? pick_mfma(kv_dt, (int)head_dim, one)
                                 : pick_attn(kv_dt, pl.E, one);
@@ -1421,6 +1429,19 @@ int64_t attn_sinks_workspace_bytes(int kv_dt, int64_t n_q, int64_t n_head, int64
                                 kv_dt);
 }
 
+// Whether a call with sinks goes to attn_split_kernel.
+bool split_sinks(const float* q, int kv_dt, const void* k, const void* v, const float* out,
+                 int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_dim,
+                 int64_t value_dim, int64_t n_kv, int window, int sinks, bool kpos) {
+    if (kv_dt != 0 || head_dim != value_dim ||
+        (head_dim != 64 && head_dim != 128 && head_dim != 256) || !aligned16(q) || !aligned16(k) ||
+        !aligned16(v) || !aligned16(out) || n_head_kv > 65535 ||
+        n_head_kv * head_dim * 4 * 128 >= (int64_t(1) << 31))
+        return false;
+    const int64_t tiles = (n_q * (n_head / n_head_kv) + kSplitVecs - 1) / kSplitVecs;
+    return tiles <= 65535 && n_head_kv * tiles >= tune("sinks_split", 128);
+}
+
 // attention_dev with the keys at positions below `sinks` kept by the window too.
 // Without a window, or without sinks, it is attention_dev's call.
 bool attention_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_scale,
@@ -1439,6 +1460,18 @@ bool attention_sinks_dev(const float* q, int kv_dt, const void* k, const float* 
         (kv_dt == 0 && (!aligned16(k) || !aligned16(v)))) {
         set_error("attention_sinks: null pointer, or fp32 K / V that are not 16-byte aligned");
         return false;
+    }
+    if (split_sinks(q, kv_dt, k, v, out, n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window,
+                    sinks, kpos != nullptr)) {
+        AttnParams p{};
+        p.q = q; p.k = k; p.v = v; p.out = out; p.qpos = qpos; p.kpos = kpos;
+        p.n_q = n_q; p.n_head = n_head; p.n_head_kv = n_head_kv; p.head_dim = head_dim;
+        p.value_dim = value_dim; p.n_kv = n_kv; p.rep = (int)(n_head / n_head_kv);
+        p.window = window; p.scale = scale; p.chunk_len = n_kv; p.n_chunks = 1; p.sinks = sinks;
+        const int64_t tiles = (n_q * p.rep + kSplitVecs - 1) / kSplitVecs;
+        return launch("attn_split_kernel", pick_split<true>((int)head_dim, kpos != nullptr),
+                      dim3(1, (unsigned)n_head_kv, (unsigned)tiles),
+                      dim3(64 * split_waves((int)head_dim)), 0, s, p);
     }
     return rows_sinks_dev(q, kv_dt, k, k_scale, v, v_scale, out, n_q, n_head, n_head_kv, head_dim,
                           value_dim, scale, qpos, kpos, n_kv, window, sinks, ws, ws_bytes, s);

@@ -167,7 +167,7 @@ __device__ __forceinline__ int block_exp(float amax) {
 // the other in plain fp32, so that a value that is not finite reaches only the
 // queries that keep its key. 64 keys a step, a lane a key for the scores, a
 // lane D / 64 dimensions for the value sum.
-template <int D>
+template <int D, bool SINK>
 __device__ __forceinline__ void attn_rows_plain(const AttnParams& p, int64_t u0, int n, int kh,
                                                 int j0, int j1) {
     constexpr int E = D / 64;
@@ -188,7 +188,7 @@ __device__ __forceinline__ void attn_rows_plain(const AttnParams& p, int64_t u0,
 #pragma unroll 4
             for (int d = 0; d < D; ++d) s = __builtin_fmaf(q[d], kv[d], s);
             const int64_t kp = p.kpos ? (int64_t)p.kpos[j] : j;
-            const bool keep = jb + lane < j1 && key_kept(kp, qp, p.window);
+            const bool keep = jb + lane < j1 && key_kept<SINK>(p, kp, qp);
             s = keep ? s * p.scale : -INFINITY;
             float mn = fmaxf(m, s);
             for (int off = 32; off >= 1; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off));
@@ -223,7 +223,7 @@ struct TileSums {
     float acc[4][16][D + 4];
 };
 
-template <int D>
+template <int D, bool SINK>
 __device__ __forceinline__ void attn_tile_fp32(const AttnParams& p, int64_t tile, int kh,
                                                TileSums<D>& sums) {
     using Tile = KvTile<0, D, D>;
@@ -258,12 +258,20 @@ __device__ __forceinline__ void attn_tile_fp32(const AttnParams& p, int64_t tile
         i_hi = min(i_hi, max<int64_t>(0, (qmax + 16) / 16));
         if (p.window > 0) i_lo = max<int64_t>(0, (qmin - p.window + 1) / 16);
     }
+    // (with sinks: their tiles, then the window's)
+    int64_t i_gap = 0, i_after = 0;
+    if constexpr (SINK) {
+        i_gap = min<int64_t>(((int64_t)p.sinks + 15) / 16, i_lo);
+        i_after = i_lo;
+        i_lo = 0;
+    }
     float m = -INFINITY, ls = 0.0f;
     v4f acc[VS];
 #pragma unroll
     for (int t = 0; t < VS; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
     bool leak = false;
     for (int64_t i = i_lo + w; i < i_hi; i += 4) {
+        if (SINK && i >= i_gap && i < i_after) continue;
         Tile tl;
         tl.load(p, 16 * i, p.n_kv, g, c, kh);
         bool part = false;
@@ -271,7 +279,7 @@ __device__ __forceinline__ void attn_tile_fp32(const AttnParams& p, int64_t tile
         for (int r = 0; r < 4; ++r) {
             const int64_t kj = 16 * i + 4 * g + r;
             const int64_t kp = p.kpos ? (int64_t)__shfl(tl.kp, 4 * g + r) : kj;
-            part = part || (qok && !(kj < p.n_kv && key_kept(kp, qp, p.window)));
+            part = part || (qok && !(kj < p.n_kv && key_kept<SINK>(p, kp, qp)));
         }
         if (__any(part)) {
 #pragma unroll
@@ -280,7 +288,7 @@ __device__ __forceinline__ void attn_tile_fp32(const AttnParams& p, int64_t tile
                 for (int t = 0; t < VS; ++t)
                     leak = leak || !(fabsf(slice_elem<0>(tl.v[r], t)) <= 3.4028235e38f);
         }
-        mfma_step<0, D, D>(p, tl, qs, 16 * i, p.n_kv, qp, qok, g, m, ls, acc);
+        mfma_step<0, D, D, SINK>(p, tl, qs, 16 * i, p.n_kv, qp, qok, g, m, ls, acc);
     }
     ls += __shfl_xor(ls, 16);
     ls += __shfl_xor(ls, 32);
@@ -298,7 +306,7 @@ __device__ __forceinline__ void attn_tile_fp32(const AttnParams& p, int64_t tile
                 v4f{acc[t][r], acc[t + 1][r], acc[t + 2][r], acc[t + 3][r]};
     __syncthreads();
     if (sums.leak[0] | sums.leak[1] | sums.leak[2] | sums.leak[3]) {
-        attn_rows_plain<D>(p, u0 + 4 * w, (int)max<int64_t>(0, min<int64_t>(4, n_vec - u0 - 4 * w)),
+        attn_rows_plain<D, SINK>(p, u0 + 4 * w, (int)max<int64_t>(0, min<int64_t>(4, n_vec - u0 - 4 * w)),
                            kh, (int)(16 * i_lo), (int)min<int64_t>(16 * i_hi, p.n_kv));
         return;
     }
@@ -349,7 +357,9 @@ constexpr int kSpreadCh = 14;
 // steps / split: product 2^12 3e-8 / 2.7e-7, 2^14 6e-9 / 1.2e-6.
 constexpr int kScoreExp = 12;
 
-template <int D, bool KPOS>
+// SINK: keys at positions below p.sinks are kept by the window too. The walk then
+// goes over the sinks' tiles, and from the window's first tile on.
+template <int D, bool KPOS, bool SINK = false>
 __global__ __launch_bounds__(64 * SplitCfg<D>::NW)
 __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(AttnParams p) {
     using C = SplitCfg<D>;
@@ -424,6 +434,17 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
         if (p.window > 0)
             i_lo = (int)max<int64_t>(0, ((int64_t)wmin - p.window + 1) / C::KT);
     }
+    // step i of the walk [i_lo, i_hi) takes tile tile_at(i)
+    int sink_tiles = 0, skip = 0;
+    if constexpr (SINK && !KPOS) {
+        sink_tiles = min((int)(((int64_t)p.sinks + C::KT - 1) / C::KT), i_lo);
+        skip = i_lo - sink_tiles;
+        i_hi = max(i_hi - skip, 0);
+        i_lo = 0;
+    }
+    auto tile_at = [&](int i) __attribute__((always_inline)) {
+        return SINK && !KPOS && i >= sink_tiles ? i + skip : i;
+    };
 
     // A tile on its way to LDS, through buffer descriptors of the tile (keys
     // at or past n_kv read as zeros): of a wave's KW keys, lane (lane / LK,
@@ -459,13 +480,13 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
         if (x < 2 * C::NK) {
             kr[x >> 1][x & 1] = __builtin_bit_cast(
                 v4f, __builtin_amdgcn_raw_buffer_load_b128(
-                         rsrc(kbase, i * C::KT + (x >> 1) * C::PK), (int)(koff + 2u * D * (x & 1)),
+                         rsrc(kbase, tile_at(i) * C::KT + (x >> 1) * C::PK), (int)(koff + 2u * D * (x & 1)),
                          0, 0));
         } else {
             const int e = (x - 2 * C::NK) & 7, c = (x - 2 * C::NK) >> 3;
             vr[c][e] = __builtin_bit_cast(
                 v2f, __builtin_amdgcn_raw_buffer_load_b64(
-                         rsrc(vbase, i * C::KT + (e >> 2) * 8 + (e & 3)), (int)(voff + 512u * c),
+                         rsrc(vbase, tile_at(i) * C::KT + (e >> 2) * 8 + (e & 3)), (int)(voff + 512u * c),
                          0, 0));
         }
         if constexpr (KPOS) {   // (lane's key of the wave's KW)
@@ -485,16 +506,18 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
 #pragma unroll
     for (int x = 0; x < C::CV; ++x) vch[x][0] = vch[x][1] = 0.0f;
     auto scales = [&](int b, int i) __attribute__((always_inline)) {
-        const int first = i * C::KT + wave * C::KW;
+        const int tl = tile_at(i), first = tl * C::KT + wave * C::KW;
         // keys of the tile that no query of the workgroup keeps become zeros
         auto visible = [&](int key, int32_t kp) __attribute__((always_inline)) {
-            return key < n_kv && kp <= wmax && (p.window <= 0 || (int64_t)wmin - kp < p.window);
+            return key < n_kv && kp <= wmax &&
+                   (p.window <= 0 || (int64_t)wmin - kp < p.window || (SINK && kp < p.sinks));
         };
         if constexpr (KPOS) {
             if (lane < C::KW) s_kp[b][wave * C::KW + lane] = kpr;
         }
-        if (KPOS || (i + 1) * C::KT - 1 > wmax ||
-            (p.window > 0 && (int64_t)wmin - i * C::KT >= p.window)) {
+        if (KPOS || (tl + 1) * C::KT - 1 > wmax ||
+            (p.window > 0 && (int64_t)wmin - tl * C::KT >= p.window &&
+             !(SINK && (tl + 1) * C::KT <= p.sinks))) {
             asm volatile("");
 #pragma unroll
             for (int x = 0; x < C::NK; ++x) {
@@ -508,7 +531,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int key = i * C::KT + vk + (e >> 2) * 8 + (e & 3);
+                const int key = tl * C::KT + vk + (e >> 2) * 8 + (e & 3);
                 int32_t kp = key;
                 if constexpr (KPOS) kp = p.kpos[min(key, n_kv - 1)];
                 const bool vis = visible(key, kp);
@@ -699,7 +722,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
     // after it loaded
     auto compute = [&](auto conv, int b, int sub, int i) __attribute__((always_inline)) {
         constexpr bool CONV = decltype(conv)::value;
-        const int kb = i * C::KT + 32 * sub;
+        const int kb = tile_at(i) * C::KT + 32 * sub;
         constexpr int PS = 4 * C::NP / NS;   // pairs split a step
         const _Float16* kl = smem[b] + (32 * sub + n) * C::KP + 8 * h;
         // (the small products in sums of their own: their roundings vanish,
@@ -750,7 +773,8 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
             c[j] = fmaxf(s_kf[b][(32 * sub + 8 * j) / C::KW] * qsc, 1.17549435e-38f);
             evt = max(evt, __builtin_amdgcn_readfirstlane(s_ev[b][(4 * sub + j) / C::OW]));
         }
-        if (KPOS || kb + 31 > min(qmin, n_kv - 1) || kb < klo_max) {
+        if (KPOS || kb + 31 > min(qmin, n_kv - 1) ||
+            (kb < klo_max && !(SINK && kb + 32 <= p.sinks))) {
             asm volatile("");   // (a branch: most steps skip this)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -760,9 +784,11 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
                     bool keep;
                     if constexpr (KPOS) {
                         const int32_t kp = s_kp[b][32 * sub + i + 4 * h];
-                        keep = kp <= qp && kp >= klo && kb + i + 4 * h < n_kv;
+                        keep = kp <= qp && (kp >= klo || (SINK && kp < p.sinks)) &&
+                               kb + i + 4 * h < n_kv;
                     } else {
-                        keep = i <= khi - kb - 4 * h && i >= klo - kb - 4 * h;
+                        keep = i <= khi - kb - 4 * h &&
+                               (i >= klo - kb - 4 * h || (SINK && i < p.sinks - kb - 4 * h));
                     }
                     s[4 * j + r] = keep ? s[4 * j + r] : -INFINITY;
                 }
@@ -973,7 +999,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
 #pragma unroll 1
         for (int x = gk; x < kSplitVecs / 16; x += C::GK) {
             __syncthreads();
-            attn_tile_fp32<D>(p, (int64_t)tile * (kSplitVecs / 16) + x, kh, sums[gk]);
+            attn_tile_fp32<D, SINK>(p, (int64_t)tile * (kSplitVecs / 16) + x, kh, sums[gk]);
         }
     }
 }

@@ -66,9 +66,84 @@ __device__ __forceinline__ int64_t pool_vector(const RowsIo& p, int64_t r) {
     return (((int64_t)page * p.heads + h) << p.shift) + (pos & ((1 << p.shift) - 1));
 }
 
-// A wave a row of K (blockIdx.y 0) or V (1), element by element.
+// A row (a vector of K or V) is L lanes' work, four elements each at a time: a
+// workgroup takes 256 / L rows of K (blockIdx.y 0) or V (1). The rows come and go
+// in fp32 as 16-byte pieces and in the pages as whole words. L is the lanes a row
+// of dim / 4 pieces fills, or 64 (several pieces a lane).
+struct Codes {
+    float top, scale;
+    __device__ __forceinline__ int operator()(float v) const {
+        return (int)fminf(fmaxf(roundf(v / scale), -top), top);
+    }
+};
+
+template <int DT, int L>
+__global__ __launch_bounds__(256) void paged_write_kernel(RowsIo p) {
+    const int w = blockIdx.y, dim = p.dim[w], li = threadIdx.x % L;
+    const int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (r >= p.n_rows) return;
+    const float* x = p.rows[w] + r * dim;
+    // (the row is on its way while its place is looked up; dim <= 256: a lane of
+    // 64 has one piece, and no row two)
+    const bool in = 4 * li < dim;
+    const float4 f = in ? *reinterpret_cast<const float4*>(x + 4 * li)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+    const int64_t vec = pool_vector(p, r);
+    if (vec < 0) return;
+    if constexpr (DT == 0) {
+        if (in) *reinterpret_cast<float4*>(p.pages[w] + (vec * dim + 4 * li) * 4) = f;
+    } else {
+        float amax = fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w)));
+#pragma unroll
+        for (int off = L / 2; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, L));
+        constexpr float top = DT == 1 ? 127.0f : 7.0f;
+        const float sc = amax > 0.0f ? amax / top : 1.0f;
+        if (li == 0) p.scales[w][vec] = sc;
+        const Codes code{top, sc};
+        const int a = code(f.x), b = code(f.y), c = code(f.z), d = code(f.w);
+        if (!in) return;
+        if constexpr (DT == 1)
+            *reinterpret_cast<uint32_t*>(p.pages[w] + vec * dim + 4 * li) =
+                (a & 255) | ((b & 255) << 8) | ((c & 255) << 16) | ((uint32_t)(d & 255) << 24);
+        else
+            *reinterpret_cast<uint16_t*>(p.pages[w] + vec * (dim / 2) + 2 * li) =
+                (uint16_t)((a & 15) | ((b & 15) << 4) | ((c & 15) << 8) | ((d & 15) << 12));
+    }
+}
+
+template <int DT, int L>
+__global__ __launch_bounds__(256) void paged_read_kernel(RowsIo p) {
+    const int w = blockIdx.y, dim = p.dim[w], li = threadIdx.x % L;
+    const int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (r >= p.n_rows || 4 * li >= dim) return;
+    const int64_t vec = pool_vector(p, r);
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (vec >= 0) {
+        if constexpr (DT == 0) {
+            f = *reinterpret_cast<const float4*>(p.pages[w] + (vec * dim + 4 * li) * 4);
+        } else {
+            const float sc = p.scales[w][vec];
+            int n[4];
+            if constexpr (DT == 1) {
+                const uint32_t c = *reinterpret_cast<const uint32_t*>(p.pages[w] + vec * dim + 4 * li);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) n[e] = (int32_t)(c << (24 - 8 * e)) >> 24;
+            } else {
+                const uint32_t c =
+                    *reinterpret_cast<const uint16_t*>(p.pages[w] + vec * (dim / 2) + 2 * li);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) n[e] = (int32_t)(c << (28 - 4 * e)) >> 28;
+            }
+            f = make_float4((float)n[0] * sc, (float)n[1] * sc, (float)n[2] * sc, (float)n[3] * sc);
+        }
+    }
+    *reinterpret_cast<float4*>(p.rows[w] + r * dim + 4 * li) = f;
+}
+
+// The same for dims that are no multiple of 4, or rows that are not 16-byte
+// aligned: a wave a row, element by element.
 template <int DT>
-__global__ __launch_bounds__(64) void paged_write_kernel(RowsIo p) {
+__global__ __launch_bounds__(64) void paged_write_any_kernel(RowsIo p) {
     const int w = blockIdx.y, dim = p.dim[w], lane = threadIdx.x;
     const int64_t r = blockIdx.x;
     const int64_t vec = pool_vector(p, r);
@@ -85,7 +160,7 @@ __global__ __launch_bounds__(64) void paged_write_kernel(RowsIo p) {
         constexpr float top = DT == 1 ? 127.0f : 7.0f;
         const float sc = amax > 0.0f ? amax / top : 1.0f;
         if (lane == 0) p.scales[w][vec] = sc;
-        auto code = [&](float v) { return (int)fminf(fmaxf(roundf(v / sc), -top), top); };
+        const Codes code{top, sc};
         if constexpr (DT == 1) {
             int8_t* o = reinterpret_cast<int8_t*>(p.pages[w]) + vec * dim;
             for (int i = lane; i < dim; i += 64) o[i] = (int8_t)code(x[i]);
@@ -98,7 +173,7 @@ __global__ __launch_bounds__(64) void paged_write_kernel(RowsIo p) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(64) void paged_read_kernel(RowsIo p) {
+__global__ __launch_bounds__(64) void paged_read_any_kernel(RowsIo p) {
     const int w = blockIdx.y, dim = p.dim[w], lane = threadIdx.x;
     const int64_t r = blockIdx.x;
     const int64_t vec = pool_vector(p, r);
@@ -119,6 +194,42 @@ __global__ __launch_bounds__(64) void paged_read_kernel(RowsIo p) {
         }
         o[i] = v;
     }
+}
+
+using RowsIoKernel = void (*)(RowsIo);
+
+// the kernel for rows of dims d0 and d1 and its rows a workgroup
+template <int DT>
+RowsIoKernel rows_io_kernel(bool write, bool vector, int most, int& rows, int& threads) {
+    threads = 256;
+    if (vector && most <= 64) {
+        rows = 16;
+        return write ? paged_write_kernel<DT, 16> : paged_read_kernel<DT, 16>;
+    }
+    if (vector && most <= 128) {
+        rows = 8;
+        return write ? paged_write_kernel<DT, 32> : paged_read_kernel<DT, 32>;
+    }
+    if (vector) {
+        rows = 4;
+        return write ? paged_write_kernel<DT, 64> : paged_read_kernel<DT, 64>;
+    }
+    rows = 1;
+    threads = 64;
+    return write ? paged_write_any_kernel<DT> : paged_read_any_kernel<DT>;
+}
+
+bool launch_rows_io(const RowsIo& p, int dt, bool write, hipStream_t s) {
+    if (p.n_rows == 0) return true;
+    const bool vector = p.dim[0] % 4 == 0 && p.dim[1] % 4 == 0 && aligned16(p.rows[0]) &&
+                        aligned16(p.rows[1]);
+    const int most = p.dim[0] > p.dim[1] ? p.dim[0] : p.dim[1];
+    int rows, threads;
+    RowsIoKernel k = dt == 0 ? rows_io_kernel<0>(write, vector, most, rows, threads)
+                             : (dt == 1 ? rows_io_kernel<1>(write, vector, most, rows, threads)
+                                        : rows_io_kernel<2>(write, vector, most, rows, threads));
+    return launch(write ? "paged_write_kernel" : "paged_read_kernel", k,
+                  dim3((unsigned)((p.n_rows + rows - 1) / rows), 2), dim3(threads), 0, s, p);
 }
 
 bool rows_io(const aero_kv_pool_t& pool, int64_t layer, float* k, float* v, const int32_t* table,
@@ -268,12 +379,7 @@ int aero_hip_paged_kv_write(const aero_kv_pool_t* pool, int64_t layer, const flo
     if (!rows_io(*pool, layer, const_cast<float*>(k), const_cast<float*>(v), table, max_pages,
                  lens, n_seq, n_q, bad, "paged_kv_write", p))
         return 0;
-    if (p.n_rows == 0) return 1;
-    return launch("paged_write_kernel",
-                  pool->kv_dt == 0 ? paged_write_kernel<0>
-                                   : (pool->kv_dt == 1 ? paged_write_kernel<1>
-                                                       : paged_write_kernel<2>),
-                  dim3((unsigned)p.n_rows, 2), dim3(64), 0, (hipStream_t)stream, p) ? 1 : 0;
+    return launch_rows_io(p, pool->kv_dt, true, (hipStream_t)stream) ? 1 : 0;
 }
 
 int aero_hip_paged_kv_read(const aero_kv_pool_t* pool, int64_t layer, float* k, float* v,
@@ -288,12 +394,7 @@ int aero_hip_paged_kv_read(const aero_kv_pool_t* pool, int64_t layer, float* k, 
     }
     if (!rows_io(*pool, layer, k, v, table, max_pages, lens, n_seq, n_q, bad, "paged_kv_read", p))
         return 0;
-    if (p.n_rows == 0) return 1;
-    return launch("paged_read_kernel",
-                  pool->kv_dt == 0 ? paged_read_kernel<0>
-                                   : (pool->kv_dt == 1 ? paged_read_kernel<1>
-                                                       : paged_read_kernel<2>),
-                  dim3((unsigned)p.n_rows, 2), dim3(64), 0, (hipStream_t)stream, p) ? 1 : 0;
+    return launch_rows_io(p, pool->kv_dt, false, (hipStream_t)stream) ? 1 : 0;
 }
 
 int aero_hip_kv_pages_copy(const aero_kv_pool_t* pool, const int32_t* src, const int32_t* dst,

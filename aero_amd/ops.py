@@ -694,6 +694,8 @@ def paged_attention(pool, layer: int, q: DeviceArray, out: DeviceArray, table: D
 
 def _ints(a, dtype) -> np.ndarray:
     a = np.asarray(a)
+    if a.dtype == dtype and a.ndim == 1 and a.flags.c_contiguous:
+        return a
     if a.size and a.dtype.kind not in "iu":
         raise TypeError(f"expected integers, got {a.dtype}")
     b = np.ascontiguousarray(a, dtype).reshape(-1)
@@ -710,8 +712,7 @@ def kv_pages_copy(pool, src, dst, stream: Stream | None = None) -> None:
     if src.size != dst.size:
         raise ValueError(f"{src.size} sources for {dst.size} destinations")
     _lib.check(_lib.lib().aero_hip_kv_pages_copy(
-        pool.ref, src.ctypes.data_as(_lib.ip), dst.ctypes.data_as(_lib.ip), src.size, _s(stream)),
-        "kv_pages_copy")
+        pool.ref, src.ctypes.data, dst.ctypes.data, src.size, _s(stream)), "kv_pages_copy")
 
 
 def write_i32(a: DeviceArray, items, stream: Stream | None = None) -> None:

@@ -279,7 +279,7 @@ def test_bad_pools_are_refused(bad):
     L, p = _lib.load(), c_pool(**bad)
     r = ctypes.byref(p)
     idx = np.zeros(1, np.int32)
-    ip = idx.ctypes.data_as(_lib.ip)
+    ip = idx.ctypes.data
     assert L.aero_hip_paged_attention_workspace(r, 1, 1, 4, 4) == (
         -1)
     assert L.aero_hip_paged_attention(r, 0, 16, 16, 16, 4, 16, 1, 1, 4, 1.0, 0, 0, None, 16,
@@ -317,8 +317,7 @@ def test_bad_calls_are_refused():
 
     def copy(src, dst):
         a, b = np.asarray(src, np.int32), np.asarray(dst, np.int32)
-        return L.aero_hip_kv_pages_copy(r, a.ctypes.data_as(_lib.ip), b.ctypes.data_as(_lib.ip),
-                                        a.size, None)
+        return L.aero_hip_kv_pages_copy(r, a.ctypes.data, b.ctypes.data, a.size, None)
 
     for src, dst, word in (([0], [8], "outside"), ([-1], [1], "outside"), ([8], [1], "outside"),
                            ([0, 1], [5, 5], "twice"), ([0, 1], [1, 2], "a source and"),
