@@ -25,8 +25,10 @@
 // Results differ from the reference's serial loops in summation order and in
 // the exp of the GPU's math library: <= 1e-5 relative to the output's scale.
 #include "attn_common.hpp"
+#include "paged_sched.hpp"
 #include "aero_hip.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -925,6 +927,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 }
 
 #include "attn_split.hpp"
+#include "attn_prompt.hpp"
 
 // Merge the chunks' (m, l, acc) of one (token, head) row per workgroup. Thread
 // (part q, element d) loads (m, l, acc[d]) of chunks q, q + P, ... all at once
@@ -1131,12 +1134,11 @@ AttnKernel pick_f16(int dt, int D, bool merge_out, bool kpos) {
                    : (dt == 2 ? pick_f16_dt<2>(D, merge_out, kpos) : nullptr);
 }
 
-template <bool SINK>
 AttnKernel pick_split(int D, bool kpos) {
     switch (D) {
-    case 64: return kpos ? attn_split_kernel<64, true, SINK> : attn_split_kernel<64, false, SINK>;
-    case 128: return kpos ? attn_split_kernel<128, true, SINK> : attn_split_kernel<128, false, SINK>;
-    case 256: return kpos ? attn_split_kernel<256, true, SINK> : attn_split_kernel<256, false, SINK>;
+    case 64: return kpos ? attn_split_kernel<64, true> : attn_split_kernel<64, false>;
+    case 128: return kpos ? attn_split_kernel<128, true> : attn_split_kernel<128, false>;
+    case 256: return kpos ? attn_split_kernel<256, true> : attn_split_kernel<256, false>;
     default: return nullptr;
     }
 }
@@ -1373,7 +1375,7 @@ bool attention_dev(const float* q, int kv_dt, const void* k, const float* k_scal
                  n_q, n_head, n_head_kv, head_dim, value_dim, n_kv,
                  (int)(n_head / n_head_kv), window, scale, pl.chunk_len, pl.n_chunks, 0};
     const bool one = pl.n_chunks == 1;
-    AttnKernel kern = pl.split ? pick_split<false>((int)head_dim, kpos != nullptr)
+    AttnKernel kern = pl.split ? pick_split((int)head_dim, kpos != nullptr)
                       : pl.f16 ? pick_f16(kv_dt, (int)head_dim, one, kpos != nullptr)
                       : pl.mfma ? pick_mfma(kv_dt, (int)head_dim, one)
                                 : pick_attn(kv_dt, pl.E, one);
@@ -1418,6 +1420,61 @@ bool sinks_sizes_ok(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv, i
     return true;
 }
 
+// The prompt kernels' shape for a call with sinks: GK waves a query group, tiles of
+// 32 keys there is room for, workspace bytes; gk 0 where the call is not theirs
+// (attn_rows.hip's kernels take it).
+struct PromptPlan {
+    int gk = 0;
+    int64_t vecs, cap, bytes, image, record, channel;
+};
+
+using PromptKernel = void (*)(PromptParams);
+
+template <int D>
+PromptKernel prompt_kernel(int gk, bool kpos) {
+    if constexpr (D == 64) {
+        if (gk == 4) return kpos ? attn_prompt_kernel<D, 4, true> : attn_prompt_kernel<D, 4, false>;
+    }
+    if constexpr (D != 256) {
+        if (gk == 2) return kpos ? attn_prompt_kernel<D, 2, true> : attn_prompt_kernel<D, 2, false>;
+    }
+    return kpos ? attn_prompt_kernel<D, 1, true> : attn_prompt_kernel<D, 1, false>;
+}
+
+template <int D>
+PromptKernel parts_kernel(bool kpos) {
+    return kpos ? prompt_parts_kernel<D, true> : prompt_parts_kernel<D, false>;
+}
+
+PromptPlan prompt_plan(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv,
+                       int64_t head_dim, int64_t value_dim, int64_t n_kv, int window, int sinks) {
+    PromptPlan pl;
+    if (kv_dt != 0 || head_dim != value_dim ||
+        (head_dim != 64 && head_dim != 128 && head_dim != 256) || n_head_kv > 65535)
+        return pl;
+    const int64_t n_vec = n_q * (n_head / n_head_kv);
+    const int waves = head_dim == 256 ? 4 : 8;
+    const int most = head_dim == 64 ? 4 : (head_dim == 128 ? 2 : 1);
+    int gk = 1;
+    auto wgs = [&](int g) {
+        const int64_t vecs = 32 * waves / g;
+        return n_head_kv * ((n_vec + vecs - 1) / vecs);
+    };
+    while (gk < most && wgs(gk) < tune("prompt_fill", 200)) gk *= 2;
+    if (wgs(gk) < tune("prompt_wgs", 64)) return pl;
+    // (where the positions are consecutive; tiles past the room are noticed)
+    pl.cap = std::min<int64_t>((n_kv + 31) / 32, ((int64_t)window + n_q + sinks + 31) / 32 + 4);
+    pl.image = 256;
+    pl.record = pl.image + n_head_kv * pl.cap * 256 * head_dim;
+    pl.channel = pl.record + n_head_kv * pl.cap * (int64_t)sizeof(PromptTile);
+    pl.bytes = pl.channel + n_head_kv * pl.cap * head_dim * 4;
+    if (pl.bytes > (int64_t(4) << 30)) return pl;
+    pl.vecs = 32 * waves / gk;
+    if ((n_vec + pl.vecs - 1) / pl.vecs > 65535) return pl;
+    pl.gk = gk;
+    return pl;
+}
+
 int64_t attn_sinks_workspace_bytes(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv,
                                    int64_t head_dim, int64_t value_dim, int64_t n_kv, int window,
                                    int sinks) {
@@ -1425,21 +1482,11 @@ int64_t attn_sinks_workspace_bytes(int kv_dt, int64_t n_q, int64_t n_head, int64
         return -1;
     if (window <= 0 || sinks == 0)
         return attn_workspace_bytes(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv);
-    return rows_sinks_workspace(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks,
-                                kv_dt);
-}
-
-// Whether a call with sinks goes to attn_split_kernel.
-bool split_sinks(const float* q, int kv_dt, const void* k, const void* v, const float* out,
-                 int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_dim,
-                 int64_t value_dim, int64_t n_kv, int window, int sinks, bool kpos) {
-    if (kv_dt != 0 || head_dim != value_dim ||
-        (head_dim != 64 && head_dim != 128 && head_dim != 256) || !aligned16(q) || !aligned16(k) ||
-        !aligned16(v) || !aligned16(out) || n_head_kv > 65535 ||
-        n_head_kv * head_dim * 4 * 128 >= (int64_t(1) << 31))
-        return false;
-    const int64_t tiles = (n_q * (n_head / n_head_kv) + kSplitVecs - 1) / kSplitVecs;
-    return tiles <= 65535 && n_head_kv * tiles >= tune("sinks_split", 128);
+    const PromptPlan pl = prompt_plan(kv_dt, n_q, n_head, n_head_kv, head_dim, value_dim, n_kv,
+                                      window, sinks);
+    return std::max(pl.gk != 0 ? pl.bytes : 0,
+                    rows_sinks_workspace(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window,
+                                         sinks, kv_dt));
 }
 
 // attention_dev with the keys at positions below `sinks` kept by the window too.
@@ -1461,17 +1508,39 @@ bool attention_sinks_dev(const float* q, int kv_dt, const void* k, const float* 
         set_error("attention_sinks: null pointer, or fp32 K / V that are not 16-byte aligned");
         return false;
     }
-    if (split_sinks(q, kv_dt, k, v, out, n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window,
-                    sinks, kpos != nullptr)) {
-        AttnParams p{};
+    const PromptPlan pl = prompt_plan(kv_dt, n_q, n_head, n_head_kv, head_dim, value_dim, n_kv,
+                                      window, sinks);
+    if (pl.gk != 0 && aligned16(q) && aligned16(out) &&
+        (kpos == nullptr || (n_kv + 31) / 32 <= pl.cap)) {
+        if (ws == nullptr || ws_bytes < pl.bytes || !aligned16(ws)) {
+            set_error("attention_sinks: workspace %lld bytes < %lld needed (16-byte aligned)",
+                      (long long)ws_bytes, (long long)pl.bytes);
+            return false;
+        }
+        PromptParams pp{};
+        AttnParams& p = pp.a;
         p.q = q; p.k = k; p.v = v; p.out = out; p.qpos = qpos; p.kpos = kpos;
         p.n_q = n_q; p.n_head = n_head; p.n_head_kv = n_head_kv; p.head_dim = head_dim;
         p.value_dim = value_dim; p.n_kv = n_kv; p.rep = (int)(n_head / n_head_kv);
         p.window = window; p.scale = scale; p.chunk_len = n_kv; p.n_chunks = 1; p.sinks = sinks;
-        const int64_t tiles = (n_q * p.rep + kSplitVecs - 1) / kSplitVecs;
-        return launch("attn_split_kernel", pick_split<true>((int)head_dim, kpos != nullptr),
-                      dim3(1, (unsigned)n_head_kv, (unsigned)tiles),
-                      dim3(64 * split_waves((int)head_dim)), 0, s, p);
+        uint8_t* w = static_cast<uint8_t*>(ws);
+        pp.list = reinterpret_cast<KeyTiles*>(w);
+        pp.image = w + pl.image;
+        pp.tile = reinterpret_cast<PromptTile*>(w + pl.record);
+        pp.channel = reinterpret_cast<uint32_t*>(w + pl.channel);
+        pp.cap = (int32_t)pl.cap;
+        const bool kp = kpos != nullptr;
+        const PromptKernel parts = head_dim == 64    ? parts_kernel<64>(kp)
+                                   : head_dim == 128 ? parts_kernel<128>(kp)
+                                                     : parts_kernel<256>(kp);
+        const PromptKernel main = head_dim == 64    ? prompt_kernel<64>(pl.gk, kp)
+                                  : head_dim == 128 ? prompt_kernel<128>(pl.gk, kp)
+                                                    : prompt_kernel<256>(pl.gk, kp);
+        const int64_t tiles = (n_q * p.rep + pl.vecs - 1) / pl.vecs;
+        return launch("prompt_parts_kernel", parts, dim3((unsigned)pl.cap, (unsigned)n_head_kv),
+                      dim3(256), 0, s, pp) &&
+               launch("attn_prompt_kernel", main, dim3(1, (unsigned)n_head_kv, (unsigned)tiles),
+                      dim3(head_dim == 256 ? 256 : 512), 0, s, pp);
     }
     return rows_sinks_dev(q, kv_dt, k, k_scale, v, v_scale, out, n_q, n_head, n_head_kv, head_dim,
                           value_dim, scale, qpos, kpos, n_kv, window, sinks, ws, ws_bytes, s);

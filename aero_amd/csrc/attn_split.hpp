@@ -357,9 +357,7 @@ constexpr int kSpreadCh = 14;
 // steps / split: product 2^12 3e-8 / 2.7e-7, 2^14 6e-9 / 1.2e-6.
 constexpr int kScoreExp = 12;
 
-// SINK: keys at positions below p.sinks are kept by the window too. The walk then
-// goes over the sinks' tiles, and from the window's first tile on.
-template <int D, bool KPOS, bool SINK = false>
+template <int D, bool KPOS>
 __global__ __launch_bounds__(64 * SplitCfg<D>::NW)
 __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(AttnParams p) {
     using C = SplitCfg<D>;
@@ -434,17 +432,6 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
         if (p.window > 0)
             i_lo = (int)max<int64_t>(0, ((int64_t)wmin - p.window + 1) / C::KT);
     }
-    // step i of the walk [i_lo, i_hi) takes tile tile_at(i)
-    int sink_tiles = 0, skip = 0;
-    if constexpr (SINK && !KPOS) {
-        sink_tiles = min((int)(((int64_t)p.sinks + C::KT - 1) / C::KT), i_lo);
-        skip = i_lo - sink_tiles;
-        i_hi = max(i_hi - skip, 0);
-        i_lo = 0;
-    }
-    auto tile_at = [&](int i) __attribute__((always_inline)) {
-        return SINK && !KPOS && i >= sink_tiles ? i + skip : i;
-    };
 
     // A tile on its way to LDS, through buffer descriptors of the tile (keys
     // at or past n_kv read as zeros): of a wave's KW keys, lane (lane / LK,
@@ -480,13 +467,13 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
         if (x < 2 * C::NK) {
             kr[x >> 1][x & 1] = __builtin_bit_cast(
                 v4f, __builtin_amdgcn_raw_buffer_load_b128(
-                         rsrc(kbase, tile_at(i) * C::KT + (x >> 1) * C::PK), (int)(koff + 2u * D * (x & 1)),
+                         rsrc(kbase, i * C::KT + (x >> 1) * C::PK), (int)(koff + 2u * D * (x & 1)),
                          0, 0));
         } else {
             const int e = (x - 2 * C::NK) & 7, c = (x - 2 * C::NK) >> 3;
             vr[c][e] = __builtin_bit_cast(
                 v2f, __builtin_amdgcn_raw_buffer_load_b64(
-                         rsrc(vbase, tile_at(i) * C::KT + (e >> 2) * 8 + (e & 3)), (int)(voff + 512u * c),
+                         rsrc(vbase, i * C::KT + (e >> 2) * 8 + (e & 3)), (int)(voff + 512u * c),
                          0, 0));
         }
         if constexpr (KPOS) {   // (lane's key of the wave's KW)
@@ -506,18 +493,16 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
 #pragma unroll
     for (int x = 0; x < C::CV; ++x) vch[x][0] = vch[x][1] = 0.0f;
     auto scales = [&](int b, int i) __attribute__((always_inline)) {
-        const int tl = tile_at(i), first = tl * C::KT + wave * C::KW;
+        const int first = i * C::KT + wave * C::KW;
         // keys of the tile that no query of the workgroup keeps become zeros
         auto visible = [&](int key, int32_t kp) __attribute__((always_inline)) {
-            return key < n_kv && kp <= wmax &&
-                   (p.window <= 0 || (int64_t)wmin - kp < p.window || (SINK && kp < p.sinks));
+            return key < n_kv && kp <= wmax && (p.window <= 0 || (int64_t)wmin - kp < p.window);
         };
         if constexpr (KPOS) {
             if (lane < C::KW) s_kp[b][wave * C::KW + lane] = kpr;
         }
-        if (KPOS || (tl + 1) * C::KT - 1 > wmax ||
-            (p.window > 0 && (int64_t)wmin - tl * C::KT >= p.window &&
-             !(SINK && (tl + 1) * C::KT <= p.sinks))) {
+        if (KPOS || (i + 1) * C::KT - 1 > wmax ||
+            (p.window > 0 && (int64_t)wmin - i * C::KT >= p.window)) {
             asm volatile("");
 #pragma unroll
             for (int x = 0; x < C::NK; ++x) {
@@ -531,7 +516,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int key = tl * C::KT + vk + (e >> 2) * 8 + (e & 3);
+                const int key = i * C::KT + vk + (e >> 2) * 8 + (e & 3);
                 int32_t kp = key;
                 if constexpr (KPOS) kp = p.kpos[min(key, n_kv - 1)];
                 const bool vis = visible(key, kp);
@@ -722,7 +707,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
     // after it loaded
     auto compute = [&](auto conv, int b, int sub, int i) __attribute__((always_inline)) {
         constexpr bool CONV = decltype(conv)::value;
-        const int kb = tile_at(i) * C::KT + 32 * sub;
+        const int kb = i * C::KT + 32 * sub;
         constexpr int PS = 4 * C::NP / NS;   // pairs split a step
         const _Float16* kl = smem[b] + (32 * sub + n) * C::KP + 8 * h;
         // (the small products in sums of their own: their roundings vanish,
@@ -773,8 +758,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
             c[j] = fmaxf(s_kf[b][(32 * sub + 8 * j) / C::KW] * qsc, 1.17549435e-38f);
             evt = max(evt, __builtin_amdgcn_readfirstlane(s_ev[b][(4 * sub + j) / C::OW]));
         }
-        if (KPOS || kb + 31 > min(qmin, n_kv - 1) ||
-            (kb < klo_max && !(SINK && kb + 32 <= p.sinks))) {
+        if (KPOS || kb + 31 > min(qmin, n_kv - 1) || kb < klo_max) {
             asm volatile("");   // (a branch: most steps skip this)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -784,11 +768,9 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
                     bool keep;
                     if constexpr (KPOS) {
                         const int32_t kp = s_kp[b][32 * sub + i + 4 * h];
-                        keep = kp <= qp && (kp >= klo || (SINK && kp < p.sinks)) &&
-                               kb + i + 4 * h < n_kv;
+                        keep = kp <= qp && kp >= klo && kb + i + 4 * h < n_kv;
                     } else {
-                        keep = i <= khi - kb - 4 * h &&
-                               (i >= klo - kb - 4 * h || (SINK && i < p.sinks - kb - 4 * h));
+                        keep = i <= khi - kb - 4 * h && i >= klo - kb - 4 * h;
                     }
                     s[4 * j + r] = keep ? s[4 * j + r] : -INFINITY;
                 }
@@ -999,7 +981,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_split_kernel(At
 #pragma unroll 1
         for (int x = gk; x < kSplitVecs / 16; x += C::GK) {
             __syncthreads();
-            attn_tile_fp32<D, SINK>(p, (int64_t)tile * (kSplitVecs / 16) + x, kh, sums[gk]);
+            attn_tile_fp32<D, false>(p, (int64_t)tile * (kSplitVecs / 16) + x, kh, sums[gk]);
         }
     }
 }

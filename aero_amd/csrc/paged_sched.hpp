@@ -28,6 +28,8 @@ struct KeyTiles {
 
     // the 16-key tile at place x of the list
     AERO_HD int32_t at(int32_t x) const { return x < n_sink ? x : x - n_sink + first; }
+    // the place of tile x (one of the list's)
+    AERO_HD int32_t place(int32_t x) const { return x < n_sink ? x : x - first + n_sink; }
     // the places whose tiles begin at or before position q_hi
     AERO_HD int32_t upto(int64_t q_hi) const {
         if (q_hi < 0) return 0;
@@ -52,18 +54,18 @@ struct KeyTiles {
 };
 
 // Keys below n_kv seen from positions q_lo .. q_hi (q_hi < q_lo or q_hi < 0:
-// none). Positions are those of the keys' places.
+// none), in tiles of `tile` keys. Positions are those of the keys' places.
 AERO_HD KeyTiles key_tiles(int64_t q_lo, int64_t q_hi, int64_t n_kv, int32_t window,
-                           int32_t sinks) {
+                           int32_t sinks, int32_t tile = 16) {
     KeyTiles t{0, 0, 0};
     const int64_t hi = q_hi + 1 < n_kv ? q_hi + 1 : n_kv;   // keys 0 .. hi - 1
     if (hi <= 0 || q_lo > q_hi) return t;
-    const int32_t last = (int32_t)((hi + 15) / 16);
+    const int32_t last = (int32_t)((hi + tile - 1) / tile);
     if (window > 0) {
         int64_t lo = q_lo - window + 1;
         lo = lo < 0 ? 0 : (lo < hi ? lo : hi);
         const int64_t s = sinks < lo ? sinks : lo;
-        const int32_t ns = (int32_t)((s + 15) / 16), first = (int32_t)(lo / 16);
+        const int32_t ns = (int32_t)((s + tile - 1) / tile), first = (int32_t)(lo / tile);
         if (ns < first) {
             t.n_sink = ns;
             t.first = first;
