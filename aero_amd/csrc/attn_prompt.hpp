@@ -57,9 +57,16 @@ __device__ __forceinline__ void call_reach(const AttnParams& p, int32_t* s, int3
         hi = (int32_t)p.n_q - 1;
         return;
     }
-    for (int64_t t = threadIdx.x; t < p.n_q; t += 256) {
-        lo = min(lo, p.qpos[t]);
-        hi = max(hi, p.qpos[t]);
+    // (loads of 8 at a time: one memory round trip for most prompts)
+    for (int64_t t0 = threadIdx.x; t0 < p.n_q; t0 += 8 * 256) {
+        int32_t q[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) q[x] = p.qpos[min(t0 + 256 * x, p.n_q - 1)];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            lo = min(lo, q[x]);
+            hi = max(hi, q[x]);
+        }
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) {
@@ -81,11 +88,12 @@ template <int D, bool KPOS>
 __global__ __launch_bounds__(256) void prompt_parts_kernel(PromptParams pp) {
     const AttnParams& p = pp.a;
     constexpr int NS = D / 16, RC = D / 64;     // K steps; 8-element chunks a lane of 8 takes
-    __shared__ int32_t s_reach[8], s_kp[32];
-    __shared__ uint32_t s_row[32], s_ch[D], s_bad, s_kmax;
+    __shared__ int32_t s_reach[8];
+    __shared__ float s_row[2][32];
+    __shared__ uint32_t s_ch[D], s_bad, s_seen;
     const int tid = threadIdx.x, place = blockIdx.x, kh = blockIdx.y;
     if (tid < D) s_ch[tid] = 0;
-    if (tid == 0) s_bad = s_kmax = 0;
+    if (tid == 0) s_bad = 0;
     int32_t qmin, qmax;
     call_reach(p, s_reach, qmin, qmax);
     const int32_t n_kv = (int32_t)p.n_kv;
@@ -94,27 +102,43 @@ __global__ __launch_bounds__(256) void prompt_parts_kernel(PromptParams pp) {
     if (place == 0 && kh == 0 && tid == 0) *pp.list = list;
     if (place >= list.n) return;
     const int32_t key0 = 32 * list.at(place);
-    if (tid < 32) s_kp[tid] = KPOS ? p.kpos[min(key0 + tid, n_kv - 1)] : key0 + tid;
-    __syncthreads();
-
-    // row tid / 8, chunks tid % 8 + 8 i of 8 dimensions
-    const int row = tid >> 3, key = key0 + row;
-    const int32_t kp = s_kp[row];
-    const bool seen = key < n_kv && kp <= qmax &&
-                      (p.window <= 0 || (int64_t)qmin - kp < p.window || kp < p.sinks);
-    const float* kr = static_cast<const float*>(p.k) +
-                      ((int64_t)min(key, n_kv - 1) * p.n_head_kv + kh) * D;
-    const float* vr = static_cast<const float*>(p.v) +
-                      ((int64_t)min(key, n_kv - 1) * p.n_head_kv + kh) * D;
+    const float* kb = static_cast<const float*>(p.k) + (int64_t)kh * D;
+    const float* vb = static_cast<const float*>(p.v) + (int64_t)kh * D;
+    auto row_of = [&](int x) __attribute__((always_inline)) {
+        return (int64_t)min(key0 + x, n_kv - 1) * p.n_head_kv * D;
+    };
+    // K and V by rows (row tid / 8, chunks tid % 8 + 8 i of 8 dimensions), V by
+    // columns too (dimension d, the 8 keys 16 s + 8 b + 4 h + r of an operand)
+    const int row = tid >> 3;
     v4f k[RC][2], v[RC][2];
 #pragma unroll
     for (int i = 0; i < RC; ++i)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int d = 8 * ((tid & 7) + 8 * i) + 4 * x;
-            k[i][x] = *reinterpret_cast<const v4f*>(kr + d);
-            v[i][x] = *reinterpret_cast<const v4f*>(vr + d);
+            k[i][x] = *reinterpret_cast<const v4f*>(kb + row_of(row) + d);
+            v[i][x] = *reinterpret_cast<const v4f*>(vb + row_of(row) + d);
         }
+    constexpr int VC = 4 * D / 256;
+    float f[VC][8];
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+        const int x = tid + 256 * i, d = x % D, s = (x / D) >> 1, h = (x / D) & 1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = vb[row_of(16 * s + 8 * (e >> 2) + 4 * h + (e & 3)) + d];
+    }
+    auto is_seen = [&](int x, int32_t kp) __attribute__((always_inline)) {
+        return key0 + x < n_kv && kp <= qmax &&
+               (p.window <= 0 || (int64_t)qmin - kp < p.window || kp < p.sinks);
+    };
+    if (tid < 64) {     // which of the 32 keys are seen
+        const int x = tid & 31;
+        const uint64_t m = __ballot(is_seen(x, KPOS ? p.kpos[min(key0 + x, n_kv - 1)] : key0 + x));
+        if (tid == 0) s_seen = (uint32_t)m;
+    }
+    __syncthreads();
+    const uint32_t seen_rows = s_seen;
+    const bool seen = (seen_rows >> row) & 1;
     float ak = 0.0f, av = 0.0f;
     bool bad = false;
 #pragma unroll
@@ -135,24 +159,21 @@ __global__ __launch_bounds__(256) void prompt_parts_kernel(PromptParams pp) {
         av = fmaxf(av, __shfl_xor(av, off));
     }
     if ((tid & 7) == 0) {
-        s_row[row] = __builtin_bit_cast(uint32_t, av);
-        atomicMax(&s_kmax, __builtin_bit_cast(uint32_t, ak));
+        s_row[0][row] = ak;
+        s_row[1][row] = av;
     }
     if (bad) s_bad = 1;
     __syncthreads();
-    float vmax = 0.0f, vmin = INFINITY;
-    uint32_t seen_rows = 0;
+    // (32 rows in each half of a wave)
+    float kmax = s_row[0][tid & 31], vmax = s_row[1][tid & 31];
+    float vmin = vmax > 0.0f ? vmax : INFINITY;
 #pragma unroll
-    for (int x = 0; x < 32; ++x) {
-        const float m = __builtin_bit_cast(float, s_row[x]);
-        vmax = fmaxf(vmax, m);
-        vmin = m > 0.0f ? fminf(vmin, m) : vmin;
-        const int32_t q = s_kp[x];
-        const bool s = key0 + x < n_kv && q <= qmax &&
-                       (p.window <= 0 || (int64_t)qmin - q < p.window || q < p.sinks);
-        seen_rows |= s ? 1u << x : 0u;
+    for (int off = 16; off >= 1; off >>= 1) {
+        kmax = fmaxf(kmax, __shfl_xor(kmax, off));
+        vmax = fmaxf(vmax, __shfl_xor(vmax, off));
+        vmin = fminf(vmin, __shfl_xor(vmin, off));
     }
-    const int ek = block_exp(__builtin_bit_cast(float, s_kmax)), ev = block_exp(vmax);
+    const int ek = block_exp(kmax), ev = block_exp(vmax);
     const bool finite = s_bad == 0;     // (else the image is not read)
     const float fk = finite ? pow2i(14 - ek) : 0.0f, fv = finite ? pow2i(14 - ev) : 0.0f;
 
@@ -171,24 +192,22 @@ __global__ __launch_bounds__(256) void prompt_parts_kernel(PromptParams pp) {
         ki[(2 * st + 1) * 64 + row + 32 * h] = __builtin_bit_cast(
             h8, make_uint4(h2_u32(lo[0]), h2_u32(lo[1]), h2_u32(lo[2]), h2_u32(lo[3])));
     }
-    // V^T: dimension d, the 8 keys 16 s + 8 b + 4 h + r of a lane's operand (read
-    // again, by columns now: it is in the cache)
     h8* vi = ki + 2 * NS * 64;
-    for (int x = tid; x < 4 * D; x += 256) {
-        const int d = x % D, s = (x / D) >> 1, h = (x / D) & 1;
-        float f[8], m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+        const int x = tid + 256 * i, d = x % D, s = (x / D) >> 1, h = (x / D) & 1;
+        float m = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int r = 16 * s + 8 * (e >> 2) + 4 * h + (e & 3);
-            const float y = static_cast<const float*>(
-                p.v)[((int64_t)min(key0 + r, n_kv - 1) * p.n_head_kv + kh) * D + d];
-            f[e] = (seen_rows >> r) & 1 ? y : 0.0f;
-            m = fmaxf(m, fabsf(f[e]));
+            f[i][e] = (seen_rows >> r) & 1 ? f[i][e] : 0.0f;
+            m = fmaxf(m, fabsf(f[i][e]));
         }
         atomicMax(&s_ch[d], __builtin_bit_cast(uint32_t, m));
         h2 hi[4], lo[4];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) split_pair(f[2 * y] * fv, f[2 * y + 1] * fv, hi[y], lo[y]);
+        for (int y = 0; y < 4; ++y)
+            split_pair(f[i][2 * y] * fv, f[i][2 * y + 1] * fv, hi[y], lo[y]);
         const int at = ((2 * (d >> 5) + s) * 2) * 64 + (d & 31) + 32 * h;
         vi[at] = __builtin_bit_cast(
             h8, make_uint4(h2_u32(hi[0]), h2_u32(hi[1]), h2_u32(hi[2]), h2_u32(hi[3])));
@@ -203,14 +222,18 @@ __global__ __launch_bounds__(256) void prompt_parts_kernel(PromptParams pp) {
                        vmin < INFINITY ? block_exp(vmin) : 1000, finite ? 0 : 1, {0, 0, 0}};
 }
 
-template <int D>
+// GK waves on the same queries; TS tiles a step of a workgroup (one a wave of a
+// group, or two), NB steps in LDS: the one in use and NB - 1 on their way
+template <int D, int GK>
 struct PromptCfg {
-    static constexpr int NW = D == 256 ? 4 : 8;                  // waves
-    static constexpr int SUBS = D == 64 ? 4 : (D == 128 ? 2 : 1);   // tiles a step
-    static constexpr int IMG = 256 * D;                          // bytes of a tile's image
-    // (a buffer also holds the sums of an fp32 tile)
-    static constexpr int BUF = SUBS * IMG > (int)sizeof(TileSums<D>) ? SUBS * IMG
-                                                                     : (int)sizeof(TileSums<D>);
+    static constexpr int NW = D == 256 ? 4 : 8;       // waves
+    static constexpr int IMG = 256 * D;               // bytes of a tile's image
+    static constexpr int TS = D == 64 && GK == 1 ? 2 : GK;
+    static constexpr int NB = TS * IMG <= 32768 ? 4 : 2;
+    static constexpr int LOADS = TS * IMG / (NW * 1024) + 1;   // a wave's, a step
+    // (two of the buffers also hold the sums of an fp32 tile)
+    static constexpr int BUF = TS * IMG > (int)sizeof(TileSums<D>) ? TS * IMG
+                                                                   : (int)sizeof(TileSums<D>);
 };
 
 // A tile's record and its keys' positions, as they are in LDS
@@ -221,16 +244,15 @@ struct PromptLds {
 
 // GK waves on the same queries, 32 NW / GK query vectors a workgroup
 template <int D, int GK, bool KPOS>
-__global__ __launch_bounds__(64 * PromptCfg<D>::NW)
+__global__ __launch_bounds__((64 * PromptCfg<D, GK>::NW))
 __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(PromptParams pp) {
-    using C = PromptCfg<D>;
+    using C = PromptCfg<D, GK>;
     const AttnParams& p = pp.a;
     constexpr int NT = D / 32, NS = D / 16, GQ = C::NW / GK, QV = 32 * GQ;
-    static_assert(GK <= C::SUBS, "a tile a wave");
-    // (two objects each, so that reads of one need not wait for loads into the other)
-    __shared__ __attribute__((aligned(16))) uint8_t buf0[C::BUF];
-    __shared__ __attribute__((aligned(16))) uint8_t buf1[C::BUF];
-    __shared__ PromptLds rec0[C::SUBS], rec1[C::SUBS];
+    // (objects of their own, so that reads of one need not wait for loads into another)
+    __shared__ __attribute__((aligned(16))) uint8_t buf0[C::BUF], buf1[C::BUF],
+        buf2[C::NB > 2 ? C::BUF : 16], buf3[C::NB > 2 ? C::BUF : 16];
+    __shared__ PromptLds rec0[C::TS], rec1[C::TS], rec2[C::TS], rec3[C::TS];
     __shared__ uint32_t s_ch[D];
     __shared__ int32_t s_lo[C::NW], s_hi[C::NW], s_eq[C::NW];
     __shared__ int s_bad, s_emax, s_lomin, s_ekmax;
@@ -260,19 +282,21 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
     qmin = __builtin_amdgcn_readfirstlane(qmin);
     qmax = __builtin_amdgcn_readfirstlane(qmax);
 
-    // the query's parts, times scale * log2(e) (its product with two floats):
-    // dimensions 16 st + 8 h .. + 7 of step st, scaled by a power of two
-    h8 qhi[NS], qlo[NS];
-    float qsc;
-    int eq;
+    // the query, on its way; then its parts, times scale * log2(e) (its product with
+    // two floats): dimensions 16 st + 8 h .. + 7 of step st, scaled by a power of two
+    v4f f[NS][2];
     {
         const float* src = p.q + (int64_t)qrow * D + 8 * h;
-        v4f f[NS][2];
 #pragma unroll
         for (int st = 0; st < NS; ++st)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
                 f[st][x] = *reinterpret_cast<const v4f*>(src + 16 * st + 4 * x);
+    }
+    const KeyTiles call = *pp.list;
+    h8 qhi[NS], qlo[NS];
+    float qsc;
+    auto split_query = [&]() __attribute__((always_inline)) {
         float am = 0.0f;
 #pragma unroll
         for (int st = 0; st < NS; ++st)
@@ -287,7 +311,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
         am = fmaxf(am, __shfl_xor(am, 32));
         const float c0 = p.scale * kLog2e;
         const float c1 = __builtin_fmaf(p.scale, kLog2e, -c0) + p.scale * kLog2eLo;
-        eq = block_exp(am * fabsf(c0) * 1.0001f);
+        int eq = block_exp(am * fabsf(c0) * 1.0001f);
         const float f0 = pow2i(14 - min(eq, 128));
         qsc = pow2i(min(eq, 128) - 14);
 #pragma unroll
@@ -304,15 +328,14 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
             qlo[st] = __builtin_bit_cast(
                 h8, make_uint4(h2_u32(lo[0]), h2_u32(lo[1]), h2_u32(lo[2]), h2_u32(lo[3])));
         }
-    }
-    int eqm = eq;
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) eqm = max(eqm, __shfl_xor(eqm, off));
+        for (int off = 16; off >= 1; off >>= 1) eq = max(eq, __shfl_xor(eq, off));
+        if (lane == 0) s_eq[wave] = eq;
+    };
     for (int d = threadIdx.x; d < D; d += 64 * C::NW) s_ch[d] = 0;
     if (lane == 0) {
         s_lo[wave] = qmin;
         s_hi[wave] = qmax;
-        s_eq[wave] = eqm;
         if (wave == 0) {
             s_bad = 0;
             s_emax = -112;
@@ -321,52 +344,101 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
         }
     }
     __syncthreads();
-    int32_t wmin = s_lo[0], wmax = s_hi[0], wq = s_eq[0];
+    int32_t wmin = s_lo[0], wmax = s_hi[0];
 #pragma unroll
     for (int x = 1; x < C::NW; ++x) {
         wmin = min(wmin, s_lo[x]);
         wmax = max(wmax, s_hi[x]);
-        wq = max(wq, s_eq[x]);
     }
     wmin = __builtin_amdgcn_readfirstlane(wmin);
     wmax = __builtin_amdgcn_readfirstlane(wmax);
 
     // the workgroup's tiles, and their places among the call's
-    const KeyTiles call = *pp.list;
     const KeyTiles kt = KPOS ? call : key_tiles(wmin, wmax, n_kv, p.window, p.sinks, 32);
     const int64_t head0 = (int64_t)kh * pp.cap;
-    const uint32_t bound = (uint32_t)pp.cap;
-    {
-        // their records: the walk's exponents, and whether the parts carry it
-        int em = -112, lo = 1000, ekm = -112, bad = 0;
-        for (int x = threadIdx.x; x < kt.n; x += 64 * C::NW) {
-            const uint32_t pl = (uint32_t)call.place(kt.at(x));
-            if (pl >= bound) {
-                bad = 1;
-                continue;
-            }
-            const PromptTile r = pp.tile[head0 + pl];
+    const int steps = (kt.n + C::TS - 1) / C::TS;
+
+    // step i of the walk, tiles TS i .. of the list, into b and rec (tiles past the
+    // list's end are its last; past the room, noticed below, what is there)
+    auto fetch = [&](int i, uint8_t* b, PromptLds* rec) __attribute__((always_inline)) {
+        constexpr int W = C::IMG / (C::NW * 1024);      // KB of a tile's image a wave
+#pragma unroll
+        for (int sub = 0; sub < C::TS; ++sub) {
+            const int x = min(C::TS * i + sub, kt.n - 1);
+            const int64_t pl = head0 + min(call.place(kt.at(x)), pp.cap - 1);
+            const uint8_t* src = pp.image + pl * C::IMG + wave * (W * 1024) + lane * 16;
+            uint8_t* dst = b + sub * C::IMG + wave * (W * 1024);
+#pragma unroll
+            for (int y = 0; y < W; ++y)
+                __builtin_amdgcn_global_load_lds(
+                    src + y * 1024,
+                    (__attribute__((address_space(3))) void*)(dst + y * 1024), 16, 0, 0);
+        }
+        if (lane < (KPOS ? 40 : 8)) {     // (a record a wave, some twice)
+            const int x = min(C::TS * i + wave % C::TS, kt.n - 1), tl = kt.at(x);
+            const int64_t pl = head0 + min(call.place(tl), pp.cap - 1);
+            const int32_t* src = reinterpret_cast<const int32_t*>(pp.tile + pl) + lane;
+            if (KPOS && lane >= 8) src = p.kpos + min(32 * tl + lane - 8, n_kv - 1);
+            __builtin_amdgcn_global_load_lds(
+                src, (__attribute__((address_space(3))) void*)(rec + wave % C::TS), 4, 0, 0);
+        }
+    };
+    // The tiles' records: the walk's exponents, the largest value of each dimension,
+    // and whether the parts carry it. (The first of each thread go out ahead of the
+    // walk's loads, which they then need not wait for.)
+    constexpr int G = 64 * C::NW / D, CL = 4;
+    auto place = [&](int x) __attribute__((always_inline)) {
+        return call.place(kt.at(max(min(x, kt.n - 1), 0)));
+    };
+    const int pl0 = place(threadIdx.x);
+    const PromptTile r0 = pp.tile[head0 + min(max(pl0, 0), pp.cap - 1)];
+    uint32_t c0[CL];
+#pragma unroll
+    for (int y = 0; y < CL; ++y)
+        c0[y] = pp.channel[(head0 + min(max(place(threadIdx.x / D + G * y), 0), pp.cap - 1)) * D +
+                           threadIdx.x % D];
+    __builtin_amdgcn_sched_barrier(0);
+    if (steps > 0) fetch(0, buf0, rec0);
+    if constexpr (C::NB > 2) {
+        if (steps > 1) fetch(1, buf1, rec1);
+        if (steps > 2) fetch(2, buf2, rec2);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (kt.n > 0) {
+        int em = r0.ev, lo = r0.ev_lo, ekm = r0.ek;
+        bool bad = r0.bad != 0 || pl0 >= pp.cap;
+        for (int x = threadIdx.x + 64 * C::NW; x < kt.n; x += 64 * C::NW) {
+            const int pl = place(x);
+            const PromptTile r = pp.tile[head0 + min(pl, pp.cap - 1)];
             em = max(em, r.ev);
             lo = min(lo, r.ev_lo);
             ekm = max(ekm, r.ek);
-            bad |= r.bad;
+            bad = bad || r.bad != 0 || pl >= pp.cap;
         }
-        // and the largest value of each dimension
-        constexpr int G = 64 * C::NW / D;
-        uint32_t c = 0;
+        uint32_t c = max(max(c0[0], c0[1]), max(c0[2], c0[3]));
 #pragma unroll 4
-        for (int x = threadIdx.x / D; x < kt.n; x += G) {
-            const uint32_t pl = min((uint32_t)call.place(kt.at(x)), bound - 1);
-            c = max(c, pp.channel[(head0 + pl) * D + threadIdx.x % D]);
-        }
+        for (int x = threadIdx.x / D + G * CL; x < kt.n; x += G)
+            c = max(c, pp.channel[(head0 + min(place(x), pp.cap - 1)) * D + threadIdx.x % D]);
         atomicMax(&s_ch[threadIdx.x % D], c);
-        atomicMax(&s_emax, em);
-        atomicMin(&s_lomin, lo);
-        atomicMax(&s_ekmax, ekm);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) {
+            em = max(em, __shfl_xor(em, off));
+            lo = min(lo, __shfl_xor(lo, off));
+            ekm = max(ekm, __shfl_xor(ekm, off));
+        }
+        if (lane == 0) {
+            atomicMax(&s_emax, em);
+            atomicMin(&s_lomin, lo);
+            atomicMax(&s_ekmax, ekm);
+        }
         if (bad) s_bad = 1;
     }
+    split_query();
     __syncthreads();
     const int E = __builtin_amdgcn_readfirstlane(s_emax);
+    int wq = s_eq[0];
+#pragma unroll
+    for (int x = 1; x < C::NW; ++x) wq = max(wq, s_eq[x]);
     bool redo = s_bad != 0 || E > 128 || E - s_lomin > kRowSpread || wq > 128 ||
                 s_ekmax + wq > kScoreExp;
     // (a dimension of V far below the others; one of zeros is exact)
@@ -379,6 +451,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
     if (redo) {
         constexpr int PAIR = C::NW / 4;       // four waves a 16-query tile
         TileSums<D>* mine = reinterpret_cast<TileSums<D>*>(wave < 4 ? buf0 : buf1);
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // (the buffers are still being filled)
 #pragma unroll 1
         for (int x = wave / 4; x < QV / 16; x += PAIR) {
             __syncthreads();
@@ -393,6 +466,9 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
     const int32_t klo_max =
         p.window > 0 ? (int32_t)max<int64_t>((int64_t)qmax - p.window + 1, INT32_MIN) : INT32_MIN;
 
+    const int32_t klo_min =
+        p.window > 0 ? (int32_t)max<int64_t>((int64_t)qmin - p.window + 1, INT32_MIN) : INT32_MIN;
+
     int m = kNoMax;
     float ls = 0.0f;
     v16f acc[NT];
@@ -401,52 +477,49 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
 #pragma unroll
         for (int x = 0; x < 16; ++x) acc[t][x] = 0.0f;
 
-    // step i of the walk: tiles SUBS i .. of the list, into b
-    const int steps = (kt.n + C::SUBS - 1) / C::SUBS;
-    auto fetch = [&](int i, uint8_t* b, PromptLds* rec) __attribute__((always_inline)) {
-        constexpr int W = C::IMG / (C::NW * 1024);      // KB of a tile's image a wave
-#pragma unroll
-        for (int sub = 0; sub < C::SUBS; ++sub) {
-            const int x = min(C::SUBS * i + sub, kt.n - 1);
-            const uint8_t* src = pp.image + (head0 + call.place(kt.at(x))) * C::IMG +
-                                 wave * (W * 1024) + lane * 16;
-            uint8_t* dst = b + sub * C::IMG + wave * (W * 1024);
-#pragma unroll
-            for (int y = 0; y < W; ++y)
-                __builtin_amdgcn_global_load_lds(
-                    src + y * 1024,
-                    (__attribute__((address_space(3))) void*)(dst + y * 1024), 16, 0, 0);
-        }
-        if (wave < C::SUBS && lane < (KPOS ? 40 : 8)) {
-            const int x = min(C::SUBS * i + wave, kt.n - 1), tl = kt.at(x);
-            const int32_t* src =
-                reinterpret_cast<const int32_t*>(pp.tile + head0 + call.place(tl)) + lane;
-            if (KPOS && lane >= 8) src = p.kpos + min(32 * tl + lane - 8, n_kv - 1);
-            __builtin_amdgcn_global_load_lds(
-                src, (__attribute__((address_space(3))) void*)(rec + wave), 4, 0, 0);
-        }
-    };
     auto compute = [&](int i, const uint8_t* b, const PromptLds* recs) __attribute__((always_inline)) {
 #pragma unroll 1
-        for (int sub = gk; sub < C::SUBS; sub += GK) {
-            const int x = C::SUBS * i + sub;
+        for (int sub = gk; sub < C::TS; sub += GK) {
+            const int x = C::TS * i + sub;
             if (x >= kt.n) break;
             const int kb = 32 * kt.at(x);
+            // (nothing of it for the wave's queries)
+            if (!KPOS && (kb > qmax || (kb + 31 < klo_min && kb >= p.sinks))) continue;
+            const h8* ki = reinterpret_cast<const h8*>(b + sub * C::IMG) + lane;
+            const h8* vi = ki + 2 * NS * 64;
+            // operands are read two steps ahead
+            h8 ah[3], al[3];
+            auto key_parts = [&](int st) __attribute__((always_inline)) {
+                ah[st % 3] = ki[2 * st * 64];
+                al[st % 3] = ki[(2 * st + 1) * 64];
+            };
+            auto value_parts = [&](int y) __attribute__((always_inline)) {   // y = 2 t + k
+                ah[y % 3] = vi[2 * y * 64];
+                al[y % 3] = vi[(2 * y + 1) * 64];
+            };
+            key_parts(0);
+            key_parts(1);
             const float kf = recs[sub].tile.kf;
             const int ev = __builtin_amdgcn_readfirstlane(recs[sub].tile.ev);
-            const h8* ki = reinterpret_cast<const h8*>(b + sub * C::IMG) + lane;
-            v16f s;
+            v16f s, sl;
 #pragma unroll
-            for (int y = 0; y < 16; ++y) s[y] = 0.0f;
-            // the small products first
+            for (int y = 0; y < 16; ++y) s[y] = sl[y] = 0.0f;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int st = 0; st < NS; ++st) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ki[(2 * st + 1) * 64], qhi[st], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ki[2 * st * 64], qlo[st], s, 0, 0, 0);
+                if (st + 2 < NS) key_parts(st + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[st % 3], qhi[st], sl, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[st % 3], qhi[st], s, 0, 0, 0);
+                sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[st % 3], qlo[st], sl, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
+            value_parts(0);
+            value_parts(1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int st = 0; st < NS; ++st)
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ki[2 * st * 64], qhi[st], s, 0, 0, 0);
+            for (int y = 0; y < 16; ++y) s[y] += sl[y];
             // (at least the smallest normal: -inf times c stays -inf)
             const float c = fmaxf(kf * qsc, 1.17549435e-38f);
             if (KPOS || kb + 31 > min(qmin, n_kv - 1) ||
@@ -481,7 +554,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
             const int fe = max(ev - E, -kRowSpread) + 12;
             const float off = (float)fe - (m == kNoMax ? 0.0f : (float)m);
             h8 phi[2], plo[2];
-            float sum = 0.0f;
+            float sum[4];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 h2 hi[4], lo[4];
@@ -490,7 +563,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
                     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * k + 2 * y], c, off));
                     const float p1 =
                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * k + 2 * y + 1], c, off));
-                    sum += p0 + p1;
+                    sum[y] = k == 0 ? p0 + p1 : sum[y] + (p0 + p1);
                     split_pair(p0, p1, hi[y], lo[y]);
                 }
                 phi[k] = __builtin_bit_cast(h8, make_uint4(h2_u32(hi[0]), h2_u32(hi[1]),
@@ -498,35 +571,60 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
                 plo[k] = __builtin_bit_cast(h8, make_uint4(h2_u32(lo[0]), h2_u32(lo[1]),
                                                            h2_u32(lo[2]), h2_u32(lo[3])));
             }
-            ls += sum * pow2i(-fe);
-            const h8* vi = ki + 2 * NS * 64;
+            ls += ((sum[0] + sum[1]) + (sum[2] + sum[3])) * pow2i(-fe);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const h8 vh = vi[((2 * t + k) * 2) * 64], vl = vi[((2 * t + k) * 2 + 1) * 64];
-                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, phi[k], acc[t], 0, 0, 0);
-                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, plo[k], acc[t], 0, 0, 0);
-                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, phi[k], acc[t], 0, 0, 0);
-                }
+            for (int y = 0; y < 2 * NT; ++y) {
+                const int t = y >> 1, k = y & 1;
+                if (y + 2 < 2 * NT) value_parts(y + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[y % 3], phi[k], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[y % 3], plo[k], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[y % 3], phi[k], acc[t], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
         }
     };
-    // at a barrier a wave's own loads into LDS have landed; those of a step are
-    // issued when every wave is done with the buffer, a step ahead
-    auto landed = [&]() __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0)
-        __syncthreads();
+    // A step begins when its loads have landed (those of the NB - 2 steps after it
+    // may be on their way) and every wave is done with the step before, whose
+    // buffer is then filled again.
+    // (the copies of this code are marked apart: merged, they would read a buffer that
+    // the compiler cannot tell from the one being filled, and wait for the loads)
+    auto step = [&](auto k, int i, const uint8_t* b, const PromptLds* recs, uint8_t* nb,
+                    PromptLds* nrec) __attribute__((always_inline)) {
+        constexpr int N = (C::NB - 2) * C::LOADS;
+        if (i + C::NB - 2 < steps)
+            __builtin_amdgcn_s_waitcnt((N & 15) | 0x0f70 | ((N >> 4) << 14));
+        else
+            __builtin_amdgcn_s_waitcnt(0x0f70);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (i + C::NB - 1 < steps) fetch(i + C::NB - 1, nb, nrec);
+        asm volatile("; buffer %0" ::"n"(decltype(k)::value) : "memory");
+        compute(i, b, recs);
+        asm volatile("; buffer %0 done" ::"n"(decltype(k)::value) : "memory");
     };
-    __syncthreads();
-    if (steps > 0) fetch(0, buf0, rec0);
-    for (int i = 0; i < steps; i += 2) {
-        landed();
-        if (i + 1 < steps) fetch(i + 1, buf1, rec1);
-        compute(i, buf0, rec0);
-        if (i + 1 >= steps) break;
-        landed();
-        if (i + 2 < steps) fetch(i + 2, buf0, rec0);
-        compute(i + 1, buf1, rec1);
+    using K0 = std::integral_constant<int, 0>;
+    using K1 = std::integral_constant<int, 1>;
+    using K2 = std::integral_constant<int, 2>;
+    using K3 = std::integral_constant<int, 3>;
+    for (int i = 0; i < steps; i += C::NB) {
+        if constexpr (C::NB > 2) {
+            step(K0{}, i, buf0, rec0, buf3, rec3);
+            if (i + 1 >= steps) break;
+            step(K1{}, i + 1, buf1, rec1, buf0, rec0);
+            if (i + 2 >= steps) break;
+            step(K2{}, i + 2, buf2, rec2, buf1, rec1);
+            if (i + 3 >= steps) break;
+            step(K3{}, i + 3, buf3, rec3, buf2, rec2);
+        } else {
+            step(K0{}, i, buf0, rec0, buf1, rec1);
+            if (i + 1 >= steps) break;
+            step(K1{}, i + 1, buf1, rec1, buf0, rec0);
+        }
     }
 
     // the halves of a column added; the groups' sums joined
