@@ -52,7 +52,7 @@ struct RowsParams {
     int32_t tiles;         // query tiles a kv head and sequence
     int32_t window, sinks;
     int32_t parts;         // room for
-    int32_t target;        // paged: chunks that fill the chip
+    int32_t target;        // paged: chunks that fill the chip (0: an item is one chunk)
     int32_t n_chunks;      // contiguous
     float scale;
 };
@@ -1029,6 +1029,10 @@ __device__ __forceinline__ KeyTiles seq_tiles(const RowsParams& p, int32_t len) 
     return key_tiles((int64_t)len - p.n_q, (int64_t)len - 1, len, p.window, p.sinks);
 }
 
+__device__ __forceinline__ int32_t chunks_of(const RowsParams& p, int32_t units, int32_t total) {
+    return p.target == 0 ? 1 : item_chunks(units, total, p.target);
+}
+
 // Paged: workgroup blockIdx.x's chunk. Every wave finds it by itself: all items'
 // units summed over the lanes, then the chunks of 64 sequences at a time.
 template <typename Core>
@@ -1039,7 +1043,7 @@ rows_paged_kernel(RowsParams p) {
     const int32_t per_seq = p.n_head_kv * p.tiles;
     // (the host keeps the units that the table has room for below 2^31)
     int32_t total = 0;
-    for (int s = lane; s < p.n_seq; s += 64)
+    for (int s = lane; s < p.n_seq && p.target != 0; s += 64)
         total += item_units(seq_tiles(p, seq_len(p, s)).n, Core::UNIT) * per_seq;
     total = __builtin_amdgcn_readlane(wave_scan(total), 63);
     int32_t b = blockIdx.x, part = 0;    // the chunk's place from a sequence's first on
@@ -1047,8 +1051,8 @@ rows_paged_kernel(RowsParams p) {
     for (; s0 < p.n_seq; s0 += 64) {
         const int x = s0 + lane;
         const int32_t n =
-            x < p.n_seq ? item_chunks(item_units(seq_tiles(p, seq_len(p, x)).n, Core::UNIT), total,
-                                      p.target) * per_seq
+            x < p.n_seq ? chunks_of(p, item_units(seq_tiles(p, seq_len(p, x)).n, Core::UNIT), total) *
+                              per_seq
                         : 0;
         const int32_t m = n > per_seq ? n : 0;   // (an item of one chunk has no parts)
         const int32_t upto = wave_scan(n), parts = wave_scan(m);
@@ -1070,7 +1074,7 @@ rows_paged_kernel(RowsParams p) {
     it.pos0 = it.len - p.n_q;
     it.kt = seq_tiles(p, it.len);
     const int32_t units = item_units(it.kt.n, Core::UNIT);
-    const int32_t chunks = item_chunks(units, total, p.target);
+    const int32_t chunks = chunks_of(p, units, total);
     const int32_t item = b / chunks, c = b % chunks;
     it.kh = item / p.tiles;
     it.z = item % p.tiles;
@@ -1081,7 +1085,8 @@ rows_paged_kernel(RowsParams p) {
     Core core(p, it, sh);
     core.walk(chunk_begin(c, chunks, units) * Core::UNIT, x1);
     core.finish(chunks == 1 ? -1 : (int64_t)(part + b) * Core::VEC);
-    if (c == 0 && threadIdx.x == 0) p.spans[item_index(p, it)] = make_int2(part + b, chunks);
+    if (c == 0 && threadIdx.x == 0 && p.target != 0)
+        p.spans[item_index(p, it)] = make_int2(part + b, chunks);
 }
 
 // Contiguous: chunk blockIdx.x of n_chunks of item (kv head blockIdx.y, query
@@ -1106,18 +1111,15 @@ rows_linear_kernel(RowsParams p) {
     const int units = item_units(it.kt.n, Core::UNIT);
     const int c = blockIdx.x;
     const int a = chunk_begin(c, p.n_chunks, units), b = chunk_begin(c + 1, p.n_chunks, units);
-    const int64_t item = item_index(p, it);
     Core core(p, it, sh);
     core.walk(a * Core::UNIT, min(b * Core::UNIT, it.kt.n));
-    core.finish(p.n_chunks == 1 ? -1 : (item * p.n_chunks + c) * Core::VEC);
-    if (c == 0 && threadIdx.x == 0 && p.n_chunks > 1)
-        p.spans[item] = make_int2((int)(item * p.n_chunks), p.n_chunks);
+    core.finish(p.n_chunks == 1 ? -1 : (item_index(p, it) * p.n_chunks + c) * Core::VEC);
 }
 
 // The parts of an item's rows joined: `groups` groups of pitch / 4 lanes a row
 // take every groups-th part, then the groups meet in LDS; 256 threads do as many
-// rows as fit.
-template <int VEC>
+// rows as fit. B: parts that a group has in flight.
+template <int VEC, int B>
 __global__ __launch_bounds__(256) void rows_join_kernel(RowsParams p, int32_t rows, int32_t groups) {
     __shared__ float sm[256], sl[256];
     __shared__ float4 sa[256];
@@ -1125,7 +1127,9 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsParams p, int32_t ro
     const int lpr = p.pitch / 4, lanes = lpr * groups, per = 256 / lanes;
     const int sub = (rows + per - 1) / per;      // workgroups an item
     const int64_t item = blockIdx.x / sub;
-    const int2 span = p.spans[item];
+    // (contiguous: every item has n_chunks)
+    const int2 span = p.n_chunks > 0 ? make_int2((int)(item * p.n_chunks), p.n_chunks)
+                                     : p.spans[item];
     const int n = span.y;
     if (n <= 1) return;
     const int i = (int)(blockIdx.x % sub) * per + tid / lanes;
@@ -1135,7 +1139,6 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsParams p, int32_t ro
     const bool ok = tid < per * lanes && i < rows && u < p.n_q * p.rep;
     float M = -INFINITY, L = 0.0f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int B = 4;
     if (ok) {
         for (int c0 = grp; c0 < n; c0 += B * groups) {
             float2 ml[B];
@@ -1251,6 +1254,11 @@ RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool align
     return dt == 0 ? vec_variant<0>(width) : (dt == 1 ? vec_variant<1>(width) : vec_variant<2>(width));
 }
 
+// Items of no more units than this are not cut: a unit more takes a workgroup less
+// than the parts and their join do. One sequence of 333 int8 tokens, two kv heads of
+// dim 64 (3 units): cut 11.9 us, whole 8.9.
+constexpr int kWholeUnits = 4;
+
 // Bytes of the parts (16-byte aligned), their (m, l), and the spans
 int64_t rows_workspace(const RowsVariant& k, int64_t parts, int64_t items, int64_t pitch) {
     return parts * k.vec * (pitch + 2) * 4 + items * 8;
@@ -1270,7 +1278,10 @@ bool join(const RowsVariant& k, int64_t items, const RowsParams& p, hipStream_t 
     while (groups < p.parts / items && 2 * groups * lpr <= 256) groups *= 2;
     const int per = 256 / (lpr * groups);
     const int64_t grid = items * ((rows + per - 1) / per);
-    return launch("rows_join_kernel", k.vec == 4 ? rows_join_kernel<4> : rows_join_kernel<16>,
+    const bool many = p.parts / items > 2 * groups;
+    return launch("rows_join_kernel",
+                  k.vec == 4 ? (many ? rows_join_kernel<4, 8> : rows_join_kernel<4, 2>)
+                             : (many ? rows_join_kernel<16, 8> : rows_join_kernel<16, 2>),
                   dim3((unsigned)grid), dim3(256), 0, s, p, rows, groups);
 }
 
@@ -1289,7 +1300,7 @@ struct PagedPlan {
 };
 
 bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t n_head,
-                int64_t max_pages, bool aligned, PagedPlan& pl) {
+                int64_t max_pages, int window, int sinks, bool aligned, PagedPlan& pl) {
     if (!pool_ok(pool, "paged_attention")) return false;
     if (n_seq < 0 || n_q <= 0 || n_head <= 0 || n_head % pool.n_head_kv || max_pages <= 0 ||
         max_pages > (int64_t(1) << 30) / pool.page) {
@@ -1316,14 +1327,19 @@ bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t 
                   "work than one call takes", (long long)max_pages, (long long)n_seq);
         return false;
     }
-    pl.cut = units > 1;
+    // (a window's keys, and what is left of the tiles at the runs' ends)
+    const int64_t seen = window > 0 ? std::min<int64_t>(max_pages * pool.page, (int64_t)window +
+                                                        sinks + n_q + 45)
+                                    : max_pages * pool.page;
+    pl.cut = (seen + 16 * pl.k.unit - 1) / (16 * pl.k.unit) > kWholeUnits;
     // few items: all chunks run at once; else more chunks than fit, so that those
     // of short sequences make room early
     const int64_t fill = pl.k.workers;
     const int64_t target = pl.items <= fill / 8 ? fill - pl.items
                                                 : (pl.items < fill ? 2 * fill : fill);
-    pl.target = std::min<int64_t>(target, pl.items * units);
-    pl.bytes = rows_workspace(pl.k, 2 * pl.target, pl.items, (pool.value_dim + 3) / 4 * 4);
+    pl.target = pl.cut ? std::min<int64_t>(target, pl.items * units) : 0;
+    pl.bytes = pl.cut ? rows_workspace(pl.k, 2 * pl.target, pl.items, (pool.value_dim + 3) / 4 * 4)
+                      : 0;
     return true;
 }
 
@@ -1332,7 +1348,8 @@ bool paged_attention_dev(const aero_kv_pool_t& pool, int64_t layer, const float*
                          int64_t n_seq, int64_t n_q, int64_t n_head, float scale, int window,
                          int sinks, int32_t* bad, void* ws, int64_t ws_bytes, hipStream_t s) {
     PagedPlan pl;
-    if (!paged_plan(pool, n_seq, n_q, n_head, max_pages, aligned16(q) && aligned16(out), pl))
+    if (!paged_plan(pool, n_seq, n_q, n_head, max_pages, window, sinks,
+                    aligned16(q) && aligned16(out), pl))
         return false;
     if (layer < 0 || layer >= pool.n_layers || window < 0 || sinks < 0) {
         set_error("paged_attention: bad layer %lld, window %d or sinks %d", (long long)layer,
@@ -1340,8 +1357,8 @@ bool paged_attention_dev(const aero_kv_pool_t& pool, int64_t layer, const float*
         return false;
     }
     if (n_seq == 0) return true;
-    if (q == nullptr || out == nullptr || table == nullptr || lens == nullptr || ws == nullptr ||
-        ws_bytes < pl.bytes || !aligned16(ws)) {
+    if (q == nullptr || out == nullptr || table == nullptr || lens == nullptr ||
+        (pl.bytes > 0 && (ws == nullptr || ws_bytes < pl.bytes || !aligned16(ws)))) {
         set_error("paged_attention: null pointer, or a workspace of %lld bytes < %lld needed "
                   "(16-byte aligned)", (long long)ws_bytes, (long long)pl.bytes);
         return false;
@@ -1365,7 +1382,7 @@ bool paged_attention_dev(const aero_kv_pool_t& pool, int64_t layer, const float*
     p.target = (int32_t)pl.target;
     p.parts = (int32_t)(2 * pl.target);
     p.scale = scale;
-    place_workspace(p, pl.k, ws);
+    if (pl.cut) place_workspace(p, pl.k, ws);
     // (as many workgroups as there can be chunks)
     if (!launch(pl.k.name, pl.k.paged, dim3((unsigned)(pl.target + pl.items)), dim3(256), 0, s, p))
         return false;
@@ -1388,7 +1405,8 @@ bool linear_plan(int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_di
     const int64_t keys = std::min<int64_t>(n_kv, (int64_t)window + sinks + pl.k.vec / rep + 32);
     const int64_t units = (keys + 16 * pl.k.unit - 1) / (16 * pl.k.unit);
     const int64_t base = n_head_kv * pl.tiles;
-    pl.n_chunks = std::max<int64_t>(1, std::min<int64_t>(units, pl.k.workers / base));
+    pl.n_chunks = units <= kWholeUnits
+                      ? 1 : std::max<int64_t>(1, std::min<int64_t>(units, pl.k.workers / base));
     pl.bytes = pl.n_chunks > 1 ? rows_workspace(pl.k, base * pl.n_chunks, base,
                                                 (value_dim + 3) / 4 * 4) : 0;
     return true;
@@ -1454,8 +1472,9 @@ int64_t aero_hip_paged_attention_workspace(const aero_kv_pool_t* pool, int64_t n
                                            int64_t n_head, int64_t max_pages) {
     aero::clear_error();
     aero::PagedPlan a, b;    // (whichever the pointers' alignment will choose)
-    if (pool == nullptr || !aero::paged_plan(*pool, n_seq, n_q, n_head, max_pages, true, a) ||
-        !aero::paged_plan(*pool, n_seq, n_q, n_head, max_pages, false, b))
+    if (pool == nullptr ||
+        !aero::paged_plan(*pool, n_seq, n_q, n_head, max_pages, 0, 0, true, a) ||
+        !aero::paged_plan(*pool, n_seq, n_q, n_head, max_pages, 0, 0, false, b))
         return -1;
     return std::max(a.bytes, b.bytes);
 }

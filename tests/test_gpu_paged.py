@@ -155,6 +155,19 @@ def test_many_ragged_sequences(hip, dt):
     assert bits_equal(got, c.attend(q, 0.125))
 
 
+def test_thousands_of_sequences(hip):
+    """Most of them empty or of a few tokens, two long."""
+    n_seq = 2060
+    rng = np.random.default_rng(n_seq)
+    lens = rng.integers(0, 5, n_seq).tolist()
+    lens[3], lens[n_seq - 1] = 2500, 1700
+    c = Cache(rng, 1, 16, 8, 64, 64, lens)
+    q = rng.standard_normal((n_seq, 1, 8, 64)).astype(np.float32)
+    got = c.attend(q, 0.125)
+    check(got, c.ref(q, 0.125), lens, 1)
+    assert bits_equal(got, c.attend(q, 0.125))
+
+
 @pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
 def test_pages_given_up_and_bad_pages(hip, dt):
     """Pages between the sinks and the window need no entry; ids outside the pool

@@ -294,9 +294,9 @@ def test_bad_pools_are_refused(bad):
 def test_bad_calls_are_refused():
     L, p = _lib.load(), c_pool()
     r = ctypes.byref(p)
-    need = L.aero_hip_paged_attention_workspace(r, 3, 1, 4, 4)
+    need = L.aero_hip_paged_attention_workspace(r, 3, 1, 4, 400)
     assert need > 0
-    ok = dict(layer=0, q=16, out=16, table=16, max_pages=4, lens=16, n_seq=3, n_q=1, n_head=4,
+    ok = dict(layer=0, q=16, out=16, table=16, max_pages=400, lens=16, n_seq=3, n_q=1, n_head=4,
               scale=1.0, window=0, sinks=0, bad=None, ws=16, ws_bytes=need)
     for k in (dict(layer=2), dict(layer=-1), dict(q=None), dict(out=None), dict(table=None),
               dict(lens=None), dict(ws=None), dict(ws=24), dict(ws_bytes=need - 1),
