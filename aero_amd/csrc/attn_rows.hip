@@ -1254,10 +1254,12 @@ RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool align
     return dt == 0 ? vec_variant<0>(width) : (dt == 1 ? vec_variant<1>(width) : vec_variant<2>(width));
 }
 
-// Items of no more units than this are not cut: a unit more takes a workgroup less
-// than the parts and their join do. One sequence of 333 int8 tokens, two kv heads of
-// dim 64 (3 units): cut 11.9 us, whole 8.9.
-constexpr int kWholeUnits = 4;
+// Items of no more keys than this (whole units) are not cut: a unit more takes a
+// workgroup less than the parts and their join do. One sequence of 333 int8 tokens,
+// two kv heads of dim 64: cut 11.9 us, whole 8.5. More where the items fill half of
+// the chip: 64 sequences in a window of 1024, four kv heads of dim 256, 3 tokens each,
+// int8 38.3 / 29.0, fp32 100 / 80.9; in a window of 4096 cutting is as good.
+constexpr int kWholeKeys = 512, kWholeKeysMany = 2176;
 
 // Bytes of the parts (16-byte aligned), their (m, l), and the spans
 int64_t rows_workspace(const RowsVariant& k, int64_t parts, int64_t items, int64_t pitch) {
@@ -1331,10 +1333,10 @@ bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t 
     const int64_t seen = window > 0 ? std::min<int64_t>(max_pages * pool.page, (int64_t)window +
                                                         sinks + n_q + 45)
                                     : max_pages * pool.page;
-    pl.cut = (seen + 16 * pl.k.unit - 1) / (16 * pl.k.unit) > kWholeUnits;
+    const int64_t fill = pl.k.workers, most = (seen + 16 * pl.k.unit - 1) / (16 * pl.k.unit);
+    pl.cut = most * 16 * pl.k.unit > (2 * pl.items >= fill ? kWholeKeysMany : kWholeKeys);
     // few items: all chunks run at once; else more chunks than fit, so that those
     // of short sequences make room early
-    const int64_t fill = pl.k.workers;
     const int64_t target = pl.items <= fill / 8 ? fill - pl.items
                                                 : (pl.items < fill ? 2 * fill : fill);
     pl.target = pl.cut ? std::min<int64_t>(target, pl.items * units) : 0;
@@ -1405,7 +1407,7 @@ bool linear_plan(int64_t n_q, int64_t n_head, int64_t n_head_kv, int64_t head_di
     const int64_t keys = std::min<int64_t>(n_kv, (int64_t)window + sinks + pl.k.vec / rep + 32);
     const int64_t units = (keys + 16 * pl.k.unit - 1) / (16 * pl.k.unit);
     const int64_t base = n_head_kv * pl.tiles;
-    pl.n_chunks = units <= kWholeUnits
+    pl.n_chunks = units * 16 * pl.k.unit <= kWholeKeys
                       ? 1 : std::max<int64_t>(1, std::min<int64_t>(units, pl.k.workers / base));
     pl.bytes = pl.n_chunks > 1 ? rows_workspace(pl.k, base * pl.n_chunks, base,
                                                 (value_dim + 3) / 4 * 4) : 0;
