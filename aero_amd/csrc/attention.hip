@@ -1446,6 +1446,16 @@ PromptKernel parts_kernel(bool kpos) {
     return kpos ? prompt_parts_kernel<D, true> : prompt_parts_kernel<D, false>;
 }
 
+// A workgroup walks all keys of its queries: the time of the prompt kernels is that of
+// one walk until the chip is full. So GK doubles until most of the CUs have one (8 kv
+// heads, 4 queries each, dim 128, window 512, 1024 tokens: 128 workgroups of GK 1
+// 59.7 us, 256 of GK 2 46.4; 2048 tokens: 256 of GK 1 72.2), and fewer workgroups than
+// kPromptLeast leave more CUs idle than attn_rows.hip's, which cut the keys. Rows /
+// prompt, us, in a window of 1024 behind 4096 keys: dim 128, 64 workgroups 54.4 / 63.3,
+// 128: 103 / 67.8; dim 256, 64: 134 / 140, 128: 251 / 142; dim 64, 56: 23.7 / 29.0,
+// 112: 31.0 / 30.0, 128: 31.3 / 30.8, 224: 51.9 / 32.7.
+constexpr int64_t kPromptFill = 200, kPromptLeast = 128;
+
 PromptPlan prompt_plan(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv,
                        int64_t head_dim, int64_t value_dim, int64_t n_kv, int window, int sinks) {
     PromptPlan pl;
@@ -1460,8 +1470,8 @@ PromptPlan prompt_plan(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv
         const int64_t vecs = 32 * waves / g;
         return n_head_kv * ((n_vec + vecs - 1) / vecs);
     };
-    while (gk < most && wgs(gk) < tune("prompt_fill", 200)) gk *= 2;
-    if (wgs(gk) < tune("prompt_wgs", 64)) return pl;
+    while (gk < most && wgs(gk) < kPromptFill) gk *= 2;
+    if (wgs(gk) < kPromptLeast) return pl;
     // (where the positions are consecutive; tiles past the room are noticed)
     pl.cap = std::min<int64_t>((n_kv + 31) / 32, ((int64_t)window + n_q + sinks + 31) / 32 + 4);
     pl.image = 256;

@@ -1245,7 +1245,7 @@ RowsVariant mfma_variant(int dt) {
 // The matrix cores take head_dim == value_dim of 64, 128 and 256 with 16-byte
 // aligned rows; any other width, or alignment, the vector kernel.
 RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool aligned) {
-    if (aligned && head_dim == value_dim && tune("rows_mfma", 1) != 0) {
+    if (aligned && head_dim == value_dim) {
         if (head_dim == 64) return mfma_variant<64>(dt);
         if (head_dim == 128) return mfma_variant<128>(dt);
         if (head_dim == 256) return mfma_variant<256>(dt);

@@ -157,3 +157,167 @@ def test_recorded_step(hip, dt):
         assert rel_to_scale(got, want) <= RTOL
         assert bits_equal(got, call(q, k, v, n_kv, HK, window, sinks, dt, [last], kpos))
     plan.destroy()
+
+
+# Calls with enough query vectors for the prompt kernels (128 workgroups and more):
+# every width, and one, two and four waves on the same queries.
+PROMPTS = [(64, 16, 32, 500), (64, 32, 64, 500), (64, 64, 128, 400), (128, 16, 16, 900),
+           (128, 64, 128, 400), (256, 32, 32, 420)]
+PROMPT_IDS = ["-".join(map(str, s)) for s in PROMPTS]
+
+
+def values(rng, *shape):
+    return rng.standard_normal(shape).astype(np.float32)
+
+
+def heads_of(q, HK, heads):
+    """The query heads of the kv heads `heads` (the oracle need not do them all)."""
+    rep = q.shape[1] // HK
+    return np.concatenate([np.arange(h * rep, (h + 1) * rep) for h in heads])
+
+
+def prompt(q, k, v, qpos, window, sinks, scale=0.1, kpos=None, heads=(0, -1)):
+    """(got, want, keep) for the query heads of the kv heads `heads`."""
+    HK, n_kv = k.shape[1], k.shape[0]
+    heads = [h % HK for h in heads]
+    got = call(q, (DA.from_numpy(k), None), (DA.from_numpy(v), None), n_kv, HK, window, sinks, 0,
+               qpos, kpos, scale)
+    keep = R.seen(np.arange(len(q)) if qpos is None else qpos,
+                  np.arange(n_kv) if kpos is None else kpos, window, sinks)
+    at = heads_of(q, HK, heads)
+    return got[:, at], R.attention(q[:, at], k[:, heads], v[:, heads], keep, scale), keep
+
+
+@pytest.mark.parametrize("shape", PROMPTS, ids=PROMPT_IDS)
+def test_prompt_positions(hip, shape):
+    """Consecutive positions from 0 and from the middle of a 32-key tile on; in any
+    order and too far apart for the tiles there is room for; key positions of a
+    ring, shuffled and absent."""
+    D, HK, H, T = shape
+    rng = np.random.default_rng([D, H, T])
+    window, sinks, n_kv = 70, 5, T + 1500
+    k, v, q = values(rng, n_kv, HK, D), values(rng, n_kv, HK, D), values(rng, T, H, D)
+    short = 300
+    ring = np.arange(short)
+    ring[sinks:] = 900 + (ring[sinks:] * 7) % (short - sinks)
+    for qpos, kpos in ((None, None), (np.arange(1217, 1217 + T), None),
+                       (rng.permutation(T) + 900, None), (rng.integers(-5, n_kv + 50, T), None),
+                       (np.full(T, -1), None), (np.full(T, 2**31 - 1), None),
+                       (rng.integers(880, 1250, T), ring), (np.arange(T), rng.permutation(short)),
+                       (np.arange(T) - 40, np.full(short, 2**31 - 1))):
+        n = n_kv if kpos is None else short
+        got, want, keep = prompt(q, k[:n], v[:n], qpos, window, sinks, kpos=kpos)
+        assert np.isfinite(got).all()
+        assert not got[~keep.any(1)].any()
+        if want.any():
+            assert rel_to_scale(got, want) <= RTOL
+
+
+@pytest.mark.parametrize("shape", PROMPTS, ids=PROMPT_IDS)
+def test_prompt_values(hip, shape):
+    """NaN and infinities that nobody keeps stay out; one that the last query keeps
+    reaches it alone, within a tile that others keep keys of."""
+    D, HK, H, T = shape
+    rng = np.random.default_rng([D, H, T, 1])
+    window, sinks, n_kv = 50, 3, T + 100
+    k, v, q = values(rng, n_kv, HK, D), values(rng, n_kv, HK, D), values(rng, T, H, D)
+    qpos = np.arange(n_kv - T, n_kv)
+    hidden = ~R.seen(qpos, np.arange(n_kv), window, sinks).any(0)
+    k[hidden], v[hidden] = np.nan, np.inf
+    got, want, _ = prompt(q, k, v, qpos, window, sinks)
+    assert np.isfinite(got).all()
+    assert rel_to_scale(got, want) <= RTOL
+    v[n_kv - 1] = np.inf
+    k[n_kv - 1, 1] = np.nan
+    got, want, _ = prompt(q[:, :H], k, v, qpos, window, sinks)
+    assert np.isfinite(got[:-1]).all()
+    assert rel_to_scale(got[:-1], want[:-1]) <= RTOL
+    assert not np.isfinite(got[-1]).any()
+    q[T // 2, 0, 1] = np.nan       # a query's own
+    got, want, _ = prompt(q, k, v, qpos, window, sinks)
+    assert np.isnan(got[T // 2, 0]).all()
+    ok = np.ones(T, bool)
+    ok[[T // 2, T - 1]] = False
+    assert rel_to_scale(got[ok], want[ok]) <= RTOL
+
+
+@pytest.mark.parametrize("shape", PROMPTS, ids=PROMPT_IDS)
+@pytest.mark.parametrize("what", ["rows", "dimensions", "tiny", "huge"])
+def test_prompt_ranges(hip, shape, what):
+    """Values far apart in size: each part of the result to its own scale. (Of 50
+    kept values of one size the largest error is a few units of 2^-22 of it, as
+    where all are of a size.)"""
+    D, HK, H, T = shape
+    rng = np.random.default_rng([D, H, T, 2])
+    window, sinks, n_kv = 50, 3, T + 100
+    k, v, q = values(rng, n_kv, HK, D), values(rng, n_kv, HK, D), values(rng, T, H, D)
+    qpos = np.arange(n_kv - T, n_kv)
+    if what == "rows":             # the first keys' and a run's in the middle, sinks too
+        v[:n_kv // 2] *= np.float32(2.0**-30)
+    elif what == "dimensions":
+        v[:, :, ::3] *= np.float32(2.0**-40)
+    elif what == "tiny":
+        v *= np.float32(2.0**-100)
+        k *= np.float32(2.0**-100)
+        q *= np.float32(2.0**60)
+    else:
+        v *= np.float32(2.0**100)
+        k *= np.float32(2.0**60)
+        q *= np.float32(2.0**-60)
+    got, want, _ = prompt(q, k, v, qpos, window, sinks)
+    if what == "rows":
+        # queries that keep small values alone, and those that keep a large one
+        small = np.abs(want).max((1, 2)) < 2.0**-20
+        assert small.any() and not small.all()
+        assert rel_to_scale(got[small], want[small]) <= RTOL
+        assert rel_to_scale(got[~small], want[~small]) <= RTOL
+    elif what == "dimensions":
+        assert rel_to_scale(got[..., ::3], want[..., ::3]) <= RTOL
+        assert rel_to_scale(got[..., 1::3], want[..., 1::3]) <= RTOL
+    else:
+        assert rel_to_scale(got * np.float32(1 / np.abs(want).max()),
+                            want / np.abs(want).max()) <= RTOL
+
+
+@pytest.mark.parametrize("shape", PROMPTS, ids=PROMPT_IDS)
+def test_prompt_large_scores(hip, shape):
+    """Scores of thousands. A score's error in fp32 is at most e = (D + 3) 2^-24 of
+    scale * sum |q k|, a probability's e^(2e) - 1 of it, and the output's that of
+    the largest value, twice (numerator and sum)."""
+    D, HK, H, T = shape
+    rng = np.random.default_rng([D, H, T, 3])
+    window, sinks, n_kv = 50, 3, T + 100
+    k, v, q = values(rng, n_kv, HK, D), values(rng, n_kv, HK, D), values(rng, T, H, D)
+    q *= np.float32(1600 / D**0.5)
+    qpos = np.arange(n_kv - T, n_kv)
+    got, want, keep = prompt(q, k, v, qpos, window, sinks, scale=1.0, heads=(0,))
+    size = np.einsum("thd,kd->thk", np.abs(q[:, :H // HK]).astype(np.float64), np.abs(k[:, 0]))
+    e = (D + 3) * 2.0**-24 * (size * keep[:, None]).max(2)
+    limit = 2 * np.expm1(2 * e) * np.abs(v[:, 0]).max()
+    assert (np.abs(got - want).max(2) <= limit).all()
+
+
+def test_prompt_recorded(hip):
+    """A prompt's chunk recorded; positions and cache rows move on between the
+    replays, which each give the eager call's bits."""
+    rng = np.random.default_rng(50)
+    H, HK, D, T, n_kv, window, sinks = 32, 16, 64, 500, 1600, 200, 4
+    k, v, q = values(rng, n_kv, HK, D), values(rng, n_kv, HK, D), values(rng, T, H, D)
+    dk, dv, dq, out = DA.from_numpy(k), DA.from_numpy(v), DA.from_numpy(q), DA.empty((T, H, D))
+    qp = DA.empty(T, np.int32)
+    plan = Plan()
+    with plan:
+        ops.attention(dq, dk, dv, out, T, H, HK, D, D, n_kv, 0.1, qpos=qp, window=window,
+                      sinks=sinks)
+    for first in (0, 500, 1000, 333):
+        k[first:first + T] *= np.float32(0.5)
+        dk.copy_from(k)
+        qpos = np.arange(first, first + T)
+        qp.copy_from(qpos.astype(np.int32))
+        plan.launch()
+        got = out.numpy()
+        eager, want, _ = prompt(q, k, v, qpos, window, sinks)
+        at = heads_of(q, HK, (0, HK - 1))
+        assert bits_equal(got[:, at], eager)
+        assert rel_to_scale(eager, want) <= RTOL
+    plan.destroy()
