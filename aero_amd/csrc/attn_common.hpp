@@ -53,6 +53,54 @@ typedef unsigned int v2u __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ h2 u32_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
 __device__ __forceinline__ uint32_t h2_u32(h2 h) { return __builtin_bit_cast(uint32_t, h); }
 
+// A reduction over each row of 16 lanes (or 8), and over the lanes c, 16 + c, 32 + c
+// and 48 + c (or 32 apart): every lane has the result, the same bits in all of them. By
+// lane moves of the vector unit: a shuffle through LDS takes some 100 cycles.
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL, typename T, typename Op>
+__device__ __forceinline__ T with_moved(T v, Op op) {
+    return op(v, __builtin_bit_cast(T, lane_moved<CTRL>(__builtin_bit_cast(uint32_t, v))));
+}
+template <typename T, typename Op>
+__device__ __forceinline__ T over_eight(T v, Op op) {
+    v = with_moved<0xb1>(v, op);           // lane ^ 1
+    v = with_moved<0x4e>(v, op);           // lane ^ 2
+    return with_moved<0x141>(v, op);       // 7 - lane: the other four
+}
+template <typename T, typename Op>
+__device__ __forceinline__ T over_row(T v, Op op) {
+    return with_moved<0x140>(over_eight(v, op), op);   // 15 - lane: the other eight
+}
+template <typename T, typename Op>
+__device__ __forceinline__ T over_halves(T v, Op op) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const v2u r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r.x, b = r.y;     // (not cast as they are: that takes x twice)
+    return op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+}
+template <typename T, typename Op>
+__device__ __forceinline__ T over_rows(T v, Op op) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const v2u r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a = r.x, b = r.y;
+    return over_halves(op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b)), op);
+}
+struct Add {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
+};
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ int32_t operator()(int32_t a, int32_t b) const { return max(a, b); }
+};
+struct Min {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); }
+    __device__ __forceinline__ int32_t operator()(int32_t a, int32_t b) const { return min(a, b); }
+};
+
 // the 8 codes of key-slice step s as fp16 (bits 0x6400 or u are 1024 + u), in the
 // order of key_order
 template <int DT>

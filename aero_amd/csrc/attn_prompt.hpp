@@ -68,11 +68,8 @@ __device__ __forceinline__ void call_reach(const AttnParams& p, int32_t* s, int3
             hi = max(hi, q[x]);
         }
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        lo = min(lo, __shfl_xor(lo, off));
-        hi = max(hi, __shfl_xor(hi, off));
-    }
+    lo = over_rows(over_row(lo, Min{}), Min{});
+    hi = over_rows(over_row(hi, Max{}), Max{});
     if ((threadIdx.x & 63) == 0) {
         s[threadIdx.x >> 6] = lo;
         s[4 + (threadIdx.x >> 6)] = hi;
@@ -153,11 +150,8 @@ __global__ __launch_bounds__(256) void prompt_parts_kernel(PromptParams pp) {
                 ak = fmaxf(ak, fabsf(k[i][x][e]));
                 av = fmaxf(av, fabsf(y));
             }
-#pragma unroll
-    for (int off = 4; off >= 1; off >>= 1) {
-        ak = fmaxf(ak, __shfl_xor(ak, off));
-        av = fmaxf(av, __shfl_xor(av, off));
-    }
+    ak = over_eight(ak, Max{});
+    av = over_eight(av, Max{});
     if ((tid & 7) == 0) {
         s_row[0][row] = ak;
         s_row[1][row] = av;
@@ -167,12 +161,9 @@ __global__ __launch_bounds__(256) void prompt_parts_kernel(PromptParams pp) {
     // (32 rows in each half of a wave)
     float kmax = s_row[0][tid & 31], vmax = s_row[1][tid & 31];
     float vmin = vmax > 0.0f ? vmax : INFINITY;
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-        kmax = fmaxf(kmax, __shfl_xor(kmax, off));
-        vmax = fmaxf(vmax, __shfl_xor(vmax, off));
-        vmin = fminf(vmin, __shfl_xor(vmin, off));
-    }
+    kmax = over_rows(over_row(kmax, Max{}), Max{});
+    vmax = over_rows(over_row(vmax, Max{}), Max{});
+    vmin = over_rows(over_row(vmin, Min{}), Min{});
     const int ek = block_exp(kmax), ev = block_exp(vmax);
     const bool finite = s_bad == 0;     // (else the image is not read)
     const float fk = finite ? pow2i(14 - ek) : 0.0f, fv = finite ? pow2i(14 - ev) : 0.0f;
@@ -274,13 +265,8 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
     const uint32_t qrow = tq * (uint32_t)p.n_head + (uint32_t)(kh * p.rep) + uc % (uint32_t)p.rep;
     const int32_t qp = p.qpos ? p.qpos[tq] : (int32_t)tq;
     int32_t qmin = qp, qmax = qp;
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-        qmin = min(qmin, __shfl_xor(qmin, off));
-        qmax = max(qmax, __shfl_xor(qmax, off));
-    }
-    qmin = __builtin_amdgcn_readfirstlane(qmin);
-    qmax = __builtin_amdgcn_readfirstlane(qmax);
+    qmin = __builtin_amdgcn_readfirstlane(over_rows(over_row(qmin, Min{}), Min{}));
+    qmax = __builtin_amdgcn_readfirstlane(over_rows(over_row(qmax, Max{}), Max{}));
 
     // the query, on its way; then its parts, times scale * log2(e) (its product with
     // two floats): dimensions 16 st + 8 h .. + 7 of step st, scaled by a power of two
@@ -308,7 +294,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
                     const float y = fabsf(f[st][x][e]);
                     am = y <= am ? am : (y <= 3.4028235e38f ? y : INFINITY);
                 }
-        am = fmaxf(am, __shfl_xor(am, 32));
+        am = over_halves(am, Max{});
         const float c0 = p.scale * kLog2e;
         const float c1 = __builtin_fmaf(p.scale, kLog2e, -c0) + p.scale * kLog2eLo;
         int eq = block_exp(am * fabsf(c0) * 1.0001f);
@@ -328,8 +314,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
             qlo[st] = __builtin_bit_cast(
                 h8, make_uint4(h2_u32(lo[0]), h2_u32(lo[1]), h2_u32(lo[2]), h2_u32(lo[3])));
         }
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) eq = max(eq, __shfl_xor(eq, off));
+        eq = over_rows(over_row(eq, Max{}), Max{});
         if (lane == 0) s_eq[wave] = eq;
     };
     for (int d = threadIdx.x; d < D; d += 64 * C::NW) s_ch[d] = 0;
@@ -420,12 +405,9 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
         for (int x = threadIdx.x / D + G * CL; x < kt.n; x += G)
             c = max(c, pp.channel[(head0 + min(place(x), pp.cap - 1)) * D + threadIdx.x % D]);
         atomicMax(&s_ch[threadIdx.x % D], c);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) {
-            em = max(em, __shfl_xor(em, off));
-            lo = min(lo, __shfl_xor(lo, off));
-            ekm = max(ekm, __shfl_xor(ekm, off));
-        }
+        em = over_rows(over_row(em, Max{}), Max{});
+        lo = over_rows(over_row(lo, Min{}), Min{});
+        ekm = over_rows(over_row(ekm, Max{}), Max{});
         if (lane == 0) {
             atomicMax(&s_emax, em);
             atomicMin(&s_lomin, lo);
@@ -538,7 +520,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
 #pragma unroll
             for (int y = 3; y < 15; y += 2) tm = max3(tm, s[y], s[y + 1]);
             tm = fmaxf(tm, s[15]);
-            tm = fmaxf(tm, __shfl_xor(tm, 32)) * c;
+            tm = over_halves(tm, Max{}) * c;
             const int mt = tm > -INFINITY ? (int)ceilf(fminf(fmaxf(tm, -1e8f), 1e8f)) : kNoMax;
             if (__any(mt > m + 1)) {
                 const int mn = max(m, mt);
@@ -628,7 +610,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
     }
 
     // the halves of a column added; the groups' sums joined
-    ls += __shfl_xor(ls, 32);
+    ls = over_halves(ls, Add{});
     if constexpr (GK > 1) {
         constexpr int ROW = 64 * (16 * NT + 2);       // floats of a wave's sums
         constexpr int HALF = sizeof(buf0) / (4 * ROW);

@@ -62,6 +62,8 @@ struct Item {
     int32_t s, kh, z;   // sequence, kv head, query tile
     int32_t len;        // keys there are
     int32_t pos0;       // paged: position of token 0
+    bool early;         // paged: id is the page of the table's column threadIdx.x
+    int32_t id;
     KeyTiles kt;
 };
 
@@ -80,13 +82,15 @@ __device__ __forceinline__ float2* part_ml(const RowsParams& p, int vec, int64_t
     return reinterpret_cast<float2*>(p.part + (int64_t)p.parts * vec * p.pitch) + row;
 }
 
-// The page of table column col of sequence s, or -1 (none, or not of the pool)
-__device__ __forceinline__ int32_t page_at(const RowsParams& p, int32_t s, int32_t col) {
-    const int32_t page =
-        col < p.max_pages ? p.table[(int64_t)s * p.max_pages + col] : -1;
+// A table entry, or -1 where it is no page of the pool
+__device__ __forceinline__ int32_t checked_page(const RowsParams& p, int32_t page) {
     const bool ok = page >= 0 && page < p.n_pages;
     if (!ok && p.bad != nullptr) *p.bad = 1;
     return ok ? page : -1;
+}
+// The page of table column col of sequence s, or -1 (none, or not of the pool)
+__device__ __forceinline__ int32_t page_at(const RowsParams& p, int32_t s, int32_t col) {
+    return checked_page(p, col < p.max_pages ? p.table[(int64_t)s * p.max_pages + col] : -1);
 }
 
 // ------------------------------------------------------------ any head width
@@ -170,16 +174,12 @@ struct VecCore {
     }
 
     // positions of the item's rows, least and greatest
-    static __device__ __forceinline__ void reach(const RowsParams& p, int z, int64_t& lo,
-                                                 int64_t& hi) {
-        const int n_vec = p.n_q * p.rep;
-        lo = INT64_MAX;
-        hi = INT64_MIN;
-        for (int i = 0; i < VEC; ++i) {
-            const int t = min(z * VEC + i, n_vec - 1) / p.rep;
-            const int64_t x = p.qpos ? p.qpos[t] : t;
-            lo = min(lo, x);
-            hi = max(hi, x);
+    __device__ __forceinline__ void reach(int64_t& lo, int64_t& hi) const {
+        lo = hi = qp[0];
+#pragma unroll
+        for (int i = 1; i < VEC; ++i) {
+            lo = min(lo, qp[i]);
+            hi = max(hi, qp[i]);
         }
     }
 
@@ -207,7 +207,7 @@ struct VecCore {
                 float d = 0.0f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) d = __builtin_fmaf(q[i][e], kv[e], d);
-                d = group_sum<16>(d);
+                d = over_row(d, Add{});
                 if (key_seen(kp, qp[i], p.window, p.sinks)) {
                     const float s = d * p.scale;
                     const float mn = fmaxf(m[i], s);
@@ -324,8 +324,11 @@ struct Tiles {
             const int shift = p.page_shift - 4;
             place0 = it.kt.page_place(x, shift);
             const int n = it.kt.page_place(x1 - 1, shift) - place0 + 1;
-            for (int i = threadIdx.x; i < n; i += 256)
-                to[i] = page_at(p, it.s, it.kt.column(place0 + i, shift));
+            for (int i = threadIdx.x; i < n; i += 256) {
+                const int32_t col = it.kt.column(place0 + i, shift);
+                to[i] = it.early && col == (int32_t)threadIdx.x ? checked_page(p, it.id)
+                                                                : page_at(p, it.s, col);
+            }
         }
     }
     // (the sinks' and the window's first and last pages may be partly used)
@@ -433,7 +436,7 @@ template <Source SRC>
 struct Columns {
     int rows;            // vectors there are
     int32_t qp, klo;     // kept: kp <= qp and (kp >= klo or kp < sinks)
-    int32_t qmin, klo_max;
+    int32_t qmin, qmax, klo_max;
     bool mixed;          // positions differ
 
     __device__ __forceinline__ Columns(const RowsParams& p, const Item& it, int c) {
@@ -445,14 +448,8 @@ struct Columns {
         qp = SRC == kPaged ? it.pos0 + t : (p.qpos ? p.qpos[t] : t);
         klo = p.window > 0 ? (int32_t)max<int64_t>((int64_t)qp - p.window + 1, INT32_MIN)
                            : INT32_MIN;
-        int32_t lo = qp, hi = qp;
-#pragma unroll
-        for (int off = 8; off >= 1; off >>= 1) {
-            lo = min(lo, __shfl_xor(lo, off, 16));
-            hi = max(hi, __shfl_xor(hi, off, 16));
-        }
-        qmin = __builtin_amdgcn_readfirstlane(lo);
-        const int32_t qmax = __builtin_amdgcn_readfirstlane(hi);
+        qmin = __builtin_amdgcn_readfirstlane(over_row(qp, Min{}));
+        qmax = __builtin_amdgcn_readfirstlane(over_row(qp, Max{}));
         klo_max = p.window > 0 ? (int32_t)max<int64_t>((int64_t)qmax - p.window + 1, INT32_MIN)
                                : INT32_MIN;
         mixed = qmin != qmax;
@@ -493,8 +490,7 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
                                             float ls, const v4f (&acc)[D / 16], int64_t row,
                                             TileShared<D>& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-    ls += __shfl_xor(ls, 16);
-    ls += __shfl_xor(ls, 32);
+    ls = over_rows(ls, Add{});
     __syncthreads();     // (the item before is read)
     if (g == 0) {
         sh.m[wave][c] = m;
@@ -512,9 +508,7 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
         const float mt = fmaxf(fmaxf(sh.m[0][i], sh.m[1][i]), fmaxf(sh.m[2][i], sh.m[3][i]));
         const float w = sh.m[x][i] == -INFINITY ? 0.0f : expf(sh.m[x][i] - mt);
         sh.w[x][i] = w;
-        float lw = sh.l[x][i] * w;
-        lw += __shfl_xor(lw, 16);
-        lw += __shfl_xor(lw, 32);
+        const float lw = over_rows(sh.l[x][i] * w, Add{});
         if (x == 0) {
             sh.mt[i] = mt;
             sh.lt[i] = lw;
@@ -575,18 +569,9 @@ struct F16Core {
 #pragma unroll
         for (int t = 0; t < VS; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    static __device__ __forceinline__ void reach(const RowsParams& p, int z, int64_t& lo,
-                                                 int64_t& hi) {
-        const int u = min(z * 16 + (int)(threadIdx.x & 15), p.n_q * p.rep - 1);
-        const int t = u / p.rep;
-        int32_t a = p.qpos ? p.qpos[t] : t, b = a;
-#pragma unroll
-        for (int off = 8; off >= 1; off >>= 1) {
-            a = min(a, __shfl_xor(a, off, 16));
-            b = max(b, __shfl_xor(b, off, 16));
-        }
-        lo = a;
-        hi = b;
+    __device__ __forceinline__ void reach(int64_t& lo, int64_t& hi) const {
+        lo = col.qmin;
+        hi = col.qmax;
     }
 
     // The queries' parts into LDS: 16 lanes a row, a row's 4 NS operands (step
@@ -613,8 +598,7 @@ struct F16Core {
         for (int i = 0; i < QI; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) qmax = fmaxf(qmax, fabsf(f[i][e]));
-#pragma unroll
-        for (int off = 8; off >= 1; off >>= 1) qmax = fmaxf(qmax, __shfl_xor(qmax, off, 16));
+        qmax = over_row(qmax, Max{});
         int eq = 0;
         if (qmax > 0.0f && qmax <= 3.4028235e38f) frexpf(qmax, &eq);
         const float qsc = ldexpf(1.0f, 14 - eq);
@@ -685,14 +669,9 @@ struct F16Core {
             tm = fmaxf(tm, sc[x]);
             vmax = fmaxf(vmax, vs[x]);
         }
-        tm = fmaxf(tm, __shfl_xor(tm, 16));
-        tm = fmaxf(tm, __shfl_xor(tm, 32));
-        vmax = fmaxf(vmax, __shfl_xor(vmax, 16));
-        vmax = fmaxf(vmax, __shfl_xor(vmax, 32));
-        if (!full) {
-#pragma unroll
-            for (int off = 8; off >= 1; off >>= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, off));
-        }
+        tm = over_rows(tm, Max{});
+        vmax = over_rows(vmax, Max{});
+        if (!full) vmax = over_row(vmax, Max{});
         int ev = 0;
         if (vmax > 0.0f && vmax <= 3.4028235e38f) frexpf(vmax, &ev);
         ev = __builtin_amdgcn_readfirstlane(ev);
@@ -706,8 +685,7 @@ struct F16Core {
             for (int t = 0; t < VS; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) amax = fmaxf(amax, fabsf(acc[t][r]));
-#pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+            amax = over_rows(over_row(amax, Max{}), Max{});
             int ea = -1000;
             if (amax > 0.0f) frexpf(amax, &ea);
             ea = __builtin_amdgcn_readfirstlane(ea);
@@ -769,20 +747,25 @@ struct F16Core {
         const int span = tl.id_tiles(x1 - x0);
         for (int xb = x0; xb < x1; xb += span) {
             const int xe = min(x1, xb + span);
-            __syncthreads();     // (what was in LDS is read)
+            if (xb != x0) __syncthreads();     // (the ids before are read)
             tl.pages(it, xb, xe, sh.ids);
-            if (xb == x0) split_query(f);
-            __syncthreads();
-            qsl = sh.qscale[c];
+            if (SRC == kPaged) __syncthreads();
             typename TL::K ka, kb;
             typename TL::V va, vb;
             int x = xb + 2 * wave;
             typename TL::Place la = tl.locate(it, x, xe), lb = tl.locate(it, x + 1, xe);
-            if (x < xe) {
-                tl.load(ka, la);
-                tl.load(kb, lb);
-                tl.load(va, la);
-                tl.load(vb, lb);
+            // (a wave without a tile loads nothing, but counts as many loads: what the
+            // queries wait for is told from the count)
+            tl.load(ka, la);
+            tl.load(kb, lb);
+            tl.load(va, la);
+            tl.load(vb, lb);
+            // (the queries' parts while the first keys and values are on their way)
+            __builtin_amdgcn_sched_barrier(0);
+            if (xb == x0) {
+                split_query(f);
+                __syncthreads();
+                qsl = sh.qscale[c];
             }
             // the next step's keys are on their way during this one's softmax and
             // value sum, its values during the next scores
@@ -841,9 +824,9 @@ struct F32Core {
 #pragma unroll
         for (int t = 0; t < VS; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    static __device__ __forceinline__ void reach(const RowsParams& p, int z, int64_t& lo,
-                                                 int64_t& hi) {
-        F16Core<1, 64, SRC>::reach(p, z, lo, hi);
+    __device__ __forceinline__ void reach(int64_t& lo, int64_t& hi) const {
+        lo = col.qmin;
+        hi = col.qmax;
     }
 
     __device__ __forceinline__ void scores(const typename TL::K& t, float (&sc)[4]) const {
@@ -889,8 +872,7 @@ struct F32Core {
             leak = col.mixed && __any(leak);
         }
         float tm = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-        tm = fmaxf(tm, __shfl_xor(tm, 16));
-        tm = fmaxf(tm, __shfl_xor(tm, 32));
+        tm = over_rows(tm, Max{});
         // the sums move when a query's maximum passes the reference by 2^8
         if (__any(tm > m + 8.0f)) {
             const float mn = fmaxf(m, tm);
@@ -962,23 +944,23 @@ struct F32Core {
         const int span = tl.id_tiles(x1 - x0);
         for (int xb = x0; xb < x1; xb += span) {
             const int xe = min(x1, xb + span);
-            __syncthreads();     // (what was in LDS is read)
+            if (xb != x0) __syncthreads();     // (the ids before are read)
             tl.pages(it, xb, xe, sh.ids);
+            if (SRC == kPaged) __syncthreads();
+            typename TL::K k;
+            typename TL::V v;
+            int x = xb + wave;
+            typename TL::Place l = tl.locate(it, x, xe);
+            tl.load(k, l);
+            tl.load(v, l);
+            __builtin_amdgcn_sched_barrier(0);
             if (xb == x0) {
 #pragma unroll
                 for (int i = 0; i < QI; ++i) {
                     const int x = 16 * i + (threadIdx.x & 15);
                     sh.q[x >> 2][16 * (x & 3) + row] = f[i];
                 }
-            }
-            __syncthreads();
-            typename TL::K k;
-            typename TL::V v;
-            int x = xb + wave;
-            typename TL::Place l = tl.locate(it, x, xe);
-            if (x < xe) {
-                tl.load(k, l);
-                tl.load(v, l);
+                __syncthreads();
             }
             while (x < xe) {
                 const typename TL::Place n = tl.locate(it, x + 4, xe);
@@ -1033,42 +1015,60 @@ __device__ __forceinline__ int32_t chunks_of(const RowsParams& p, int32_t units,
     return p.target == 0 ? 1 : item_chunks(units, total, p.target);
 }
 
-// Paged: workgroup blockIdx.x's chunk. Every wave finds it by itself: all items'
-// units summed over the lanes, then the chunks of 64 sequences at a time.
+// Chunk b of all: its sequence (-1: there are no so many chunks), its place from
+// that sequence's first on, the parts before that one's, and all items' units. Every
+// wave finds it by itself: the units summed over the lanes, then the chunks of 64
+// sequences at a time.
+struct Chunk {
+    int32_t s, b, part, total;
+};
+
+template <int UNIT>
+__device__ __forceinline__ Chunk find_chunk(const RowsParams& p, int32_t b, int32_t per_seq) {
+    const int lane = threadIdx.x & 63;
+    auto units = [&](int s) __attribute__((always_inline)) {
+        return item_units(seq_tiles(p, seq_len(p, s)).n, UNIT);
+    };
+    Chunk k{-1, b, 0, 0};
+    // (the host keeps the units that the table has room for below 2^31)
+    for (int s = lane; s < p.n_seq; s += 64) k.total += units(s) * per_seq;
+    k.total = __builtin_amdgcn_readlane(wave_scan(k.total), 63);
+    for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
+        const int x = s0 + lane;
+        const int32_t n = x < p.n_seq ? chunks_of(p, units(x), k.total) * per_seq : 0;
+        const int32_t m = n > per_seq ? n : 0;   // (an item of one chunk has no parts)
+        const int32_t upto = wave_scan(n), parts = wave_scan(m);
+        const uint64_t past = __ballot(upto > k.b);
+        if (past != 0) {
+            const int f = __ffsll((unsigned long long)past) - 1;
+            k.s = s0 + f;
+            k.b -= __builtin_amdgcn_readlane(upto - n, f);
+            k.part += __builtin_amdgcn_readlane(parts - m, f);
+            break;
+        }
+        k.b -= __builtin_amdgcn_readlane(upto, 63);
+        k.part += __builtin_amdgcn_readlane(parts, 63);
+    }
+    return k;
+}
+
+// Paged: workgroup blockIdx.x's chunk. Where items are one chunk each, the first
+// columns of its sequence's table are on their way while the length is.
 template <typename Core>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Core::EU))) void
 rows_paged_kernel(RowsParams p) {
     __shared__ typename Core::Shared sh;
-    const int lane = threadIdx.x & 63;
     const int32_t per_seq = p.n_head_kv * p.tiles;
-    // (the host keeps the units that the table has room for below 2^31)
-    int32_t total = 0;
-    for (int s = lane; s < p.n_seq && p.target != 0; s += 64)
-        total += item_units(seq_tiles(p, seq_len(p, s)).n, Core::UNIT) * per_seq;
-    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-    int32_t b = blockIdx.x, part = 0;    // the chunk's place from a sequence's first on
-    int s0 = 0, s = -1;
-    for (; s0 < p.n_seq; s0 += 64) {
-        const int x = s0 + lane;
-        const int32_t n =
-            x < p.n_seq ? chunks_of(p, item_units(seq_tiles(p, seq_len(p, x)).n, Core::UNIT), total) *
-                              per_seq
-                        : 0;
-        const int32_t m = n > per_seq ? n : 0;   // (an item of one chunk has no parts)
-        const int32_t upto = wave_scan(n), parts = wave_scan(m);
-        const uint64_t past = __ballot(upto > b);
-        if (past != 0) {
-            const int f = __ffsll((unsigned long long)past) - 1;
-            s = s0 + f;
-            b -= __builtin_amdgcn_readlane(upto - n, f);
-            part += __builtin_amdgcn_readlane(parts - m, f);
-            break;
-        }
-        b -= __builtin_amdgcn_readlane(upto, 63);
-        part += __builtin_amdgcn_readlane(parts, 63);
-    }
-    if (s < 0) return;
     Item it;
+    it.early = p.target == 0;
+    Chunk k{(int32_t)blockIdx.x / per_seq, (int32_t)blockIdx.x % per_seq, 0, 0};
+    if (p.target == 0)
+        it.id = p.table[(int64_t)k.s * p.max_pages +
+                        min((int32_t)threadIdx.x, p.max_pages - 1)];
+    else
+        k = find_chunk<Core::UNIT>(p, blockIdx.x, per_seq);
+    const int32_t s = k.s, b = k.b, part = k.part, total = k.total;
+    if (s < 0) return;
     it.s = __builtin_amdgcn_readfirstlane(s);
     it.len = __builtin_amdgcn_readfirstlane(seq_len(p, it.s));
     it.pos0 = it.len - p.n_q;
@@ -1101,17 +1101,17 @@ rows_linear_kernel(RowsParams p) {
     it.z = gridDim.z - 1 - blockIdx.z;
     it.len = p.n_kv;
     it.pos0 = 0;
+    Core core(p, it, sh);
     if (p.kpos != nullptr) {
         it.kt = KeyTiles{0, 0, (p.n_kv + 15) / 16};
     } else {
         int64_t lo, hi;
-        Core::reach(p, it.z, lo, hi);
+        core.reach(lo, hi);
         it.kt = key_tiles(uniform64(lo), uniform64(hi), p.n_kv, p.window, p.sinks);
     }
     const int units = item_units(it.kt.n, Core::UNIT);
     const int c = blockIdx.x;
     const int a = chunk_begin(c, p.n_chunks, units), b = chunk_begin(c + 1, p.n_chunks, units);
-    Core core(p, it, sh);
     core.walk(a * Core::UNIT, min(b * Core::UNIT, it.kt.n));
     core.finish(p.n_chunks == 1 ? -1 : (item_index(p, it) * p.n_chunks + c) * Core::VEC);
 }

@@ -93,7 +93,8 @@ AERO_HD int32_t item_chunks(int32_t u, int32_t total, int32_t target) {
 }
 // chunk c of n takes units [chunk_begin(c), chunk_begin(c + 1)) of u
 AERO_HD int32_t chunk_begin(int32_t c, int32_t n, int32_t u) {
-    return (int32_t)((int64_t)c * u / n);
+    const int32_t each = u / n, more = u - each * n;     // (the first `more` take one more)
+    return c * each + (c < more ? c : more);
 }
 
 }  // namespace aero
