@@ -1015,33 +1015,40 @@ __device__ __forceinline__ int32_t chunks_of(const RowsParams& p, int32_t units,
     return p.target == 0 ? 1 : item_chunks(units, total, p.target);
 }
 
-// Chunk b of all: its sequence (-1: there are no so many chunks), its place from
-// that sequence's first on, the parts before that one's, and all items' units. Every
-// wave finds it by itself: the units summed over the lanes, then the chunks of 64
-// sequences at a time.
+// Chunk b of all: its sequence (-1: there are no so many chunks) and that one's
+// length, its place from the sequence's first on, the parts before that one's, and
+// all items' units. Every wave finds it by itself: the units summed over the lanes,
+// then the chunks of 64 sequences at a time.
 struct Chunk {
-    int32_t s, b, part, total;
+    int32_t s, len, b, part, total;
 };
 
 template <int UNIT>
 __device__ __forceinline__ Chunk find_chunk(const RowsParams& p, int32_t b, int32_t per_seq) {
     const int lane = threadIdx.x & 63;
-    auto units = [&](int s) __attribute__((always_inline)) {
-        return item_units(seq_tiles(p, seq_len(p, s)).n, UNIT);
+    auto units = [&](int32_t len) __attribute__((always_inline)) {
+        return item_units(seq_tiles(p, len).n, UNIT);
     };
-    Chunk k{-1, b, 0, 0};
+    auto len_of = [&](int s) __attribute__((always_inline)) {
+        return s < p.n_seq ? seq_len(p, s) : -1;
+    };
+    Chunk k{-1, 0, b, 0, 0};
+    const int32_t len0 = len_of(lane), u0 = units(len0);
     // (the host keeps the units that the table has room for below 2^31)
-    for (int s = lane; s < p.n_seq; s += 64) k.total += units(s) * per_seq;
+    if (len0 >= 0) k.total = u0 * per_seq;
+    for (int s = lane + 64; s < p.n_seq; s += 64) k.total += units(seq_len(p, s)) * per_seq;
     k.total = __builtin_amdgcn_readlane(wave_scan(k.total), 63);
     for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
-        const int x = s0 + lane;
-        const int32_t n = x < p.n_seq ? chunks_of(p, units(x), k.total) * per_seq : 0;
+        const int32_t len = s0 == 0 ? len0 : len_of(s0 + lane);
+        const int32_t n =
+            len >= 0 ? chunks_of(p, s0 == 0 ? u0 : units(len), k.total) * per_seq : 0;
         const int32_t m = n > per_seq ? n : 0;   // (an item of one chunk has no parts)
         const int32_t upto = wave_scan(n), parts = wave_scan(m);
         const uint64_t past = __ballot(upto > k.b);
         if (past != 0) {
             const int f = __ffsll((unsigned long long)past) - 1;
             k.s = s0 + f;
+            k.len = __builtin_amdgcn_readlane(len, f);
             k.b -= __builtin_amdgcn_readlane(upto - n, f);
             k.part += __builtin_amdgcn_readlane(parts - m, f);
             break;
@@ -1061,16 +1068,18 @@ rows_paged_kernel(RowsParams p) {
     const int32_t per_seq = p.n_head_kv * p.tiles;
     Item it;
     it.early = p.target == 0;
-    Chunk k{(int32_t)blockIdx.x / per_seq, (int32_t)blockIdx.x % per_seq, 0, 0};
-    if (p.target == 0)
+    Chunk k{(int32_t)blockIdx.x / per_seq, 0, (int32_t)blockIdx.x % per_seq, 0, 0};
+    if (p.target == 0) {
         it.id = p.table[(int64_t)k.s * p.max_pages +
                         min((int32_t)threadIdx.x, p.max_pages - 1)];
-    else
+        k.len = seq_len(p, k.s);
+    } else {
         k = find_chunk<Core::UNIT>(p, blockIdx.x, per_seq);
+    }
     const int32_t s = k.s, b = k.b, part = k.part, total = k.total;
     if (s < 0) return;
     it.s = __builtin_amdgcn_readfirstlane(s);
-    it.len = __builtin_amdgcn_readfirstlane(seq_len(p, it.s));
+    it.len = __builtin_amdgcn_readfirstlane(k.len);
     it.pos0 = it.len - p.n_q;
     it.kt = seq_tiles(p, it.len);
     const int32_t units = item_units(it.kt.n, Core::UNIT);
