@@ -10,7 +10,8 @@ HBM, every activation kept on the device. Per block:
     q, k, v = h Wq, h Wk, h Wv                    attention_layer.cpp
     q, k = qk_norm(q, k); rope(q, k)              :89-156
     k, v -> KV cache rows kv_len .. kv_len+T-1    :158-200
-    a = attention(q, K, V), causal                :202-225
+    a = attention(q, K, V), causal (window,       :202-225
+        sinks of BlockConfig)
     x += a Wo                                     src/model.cpp:279
     h = rmsnorm(x, ffn_norm)                      :280-282
     x += (act(h Wg) * (h Wu)) Wd                  :166-178, 284
@@ -77,6 +78,10 @@ class BlockConfig:
     v_norm: bool = False
     v_from_k: bool = False
     freq_factors: tuple | None = None
+    # attention's sliding window in keys (0: none; src/transformer.cpp:120-214
+    # takes it too), and how many first positions are kept beside it
+    window: int = 0
+    sinks: int = 0
 
     @classmethod
     def from_shape(cls, s: W.Shape, wtype: int, vocab: int | None = None,
@@ -337,7 +342,7 @@ class LayerStep:
         # causal attention over the cache, then the output projection
         att = self.att.view((T, H * D))
         ops.attention(q, Kc, Vc, att, T, H, HK, D, D, kv_len + T, 1.0 / math.sqrt(D),
-                      qpos=self.pos, stream=s)
+                      qpos=self.pos, window=c.window, stream=s, sinks=c.sinks)
         if c.attn_gate:
             # att *= sigmoid(gate) (src/attention_layer.cpp:262-263)
             ops.act_mul("sigmoid", self.qgate.view((T, H * D)), att, att, stream=s)
