@@ -1410,7 +1410,7 @@ bool sinks_sizes_ok(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv, i
         kv_dt > 2 || (kv_dt == 0 && (head_dim % 4 || value_dim % 4)) ||
         (kv_dt == 2 && (head_dim % 2 || value_dim % 2)) || sinks < 0 ||
         n_kv >= (int64_t(1) << 30) || n_q > (int64_t(1) << 28) / n_head ||
-        n_head_kv > (int64_t(1) << 16)) {
+        n_head_kv > 65535) {
         set_error("attention_sinks: bad sizes (kv_dt=%d n_q=%lld n_head=%lld n_head_kv=%lld "
                   "head_dim=%lld value_dim=%lld n_kv=%lld sinks=%d)", kv_dt, (long long)n_q,
                   (long long)n_head, (long long)n_head_kv, (long long)head_dim,

@@ -1080,6 +1080,8 @@ rows_paged_kernel(RowsParams p) {
     if (s < 0) return;
     it.s = __builtin_amdgcn_readfirstlane(s);
     it.len = __builtin_amdgcn_readfirstlane(k.len);
+    // (a length past the table's room is cut to it)
+    if (p.bad != nullptr && threadIdx.x == 0 && p.lens[it.s] > p.n_kv) *p.bad = 1;
     it.pos0 = it.len - p.n_q;
     it.kt = seq_tiles(p, it.len);
     const int32_t units = item_units(it.kt.n, Core::UNIT);
@@ -1107,7 +1109,13 @@ rows_linear_kernel(RowsParams p) {
     Item it;
     it.s = 0;
     it.kh = blockIdx.y;
-    it.z = gridDim.z - 1 - blockIdx.z;
+    int c = blockIdx.x, z = blockIdx.z;
+    if ((int)gridDim.x != p.n_chunks) {    // (more than 65535 tiles)
+        z += c / p.n_chunks * (int)gridDim.z;
+        c %= p.n_chunks;
+    }
+    if (z >= p.tiles) return;
+    it.z = p.tiles - 1 - z;
     it.len = p.n_kv;
     it.pos0 = 0;
     Core core(p, it, sh);
@@ -1119,7 +1127,6 @@ rows_linear_kernel(RowsParams p) {
         it.kt = key_tiles(uniform64(lo), uniform64(hi), p.n_kv, p.window, p.sinks);
     }
     const int units = item_units(it.kt.n, Core::UNIT);
-    const int c = blockIdx.x;
     const int a = chunk_begin(c, p.n_chunks, units), b = chunk_begin(c + 1, p.n_chunks, units);
     core.walk(a * Core::UNIT, min(b * Core::UNIT, it.kt.n));
     core.finish(p.n_chunks == 1 ? -1 : (item_index(p, it) * p.n_chunks + c) * Core::VEC);
@@ -1269,6 +1276,8 @@ RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool align
 // the chip: 64 sequences in a window of 1024, four kv heads of dim 256, 3 tokens each,
 // int8 38.3 / 29.0, fp32 100 / 80.9; in a window of 4096 cutting is as good.
 constexpr int kWholeKeys = 512, kWholeKeysMany = 2176;
+// (a launch has fewer than 2^32 threads in a row of its grid, 256 a workgroup)
+constexpr int64_t kMostWgs = (1 << 24) - 1;
 
 // Bytes of the parts (16-byte aligned), their (m, l), and the spans
 int64_t rows_workspace(const RowsVariant& k, int64_t parts, int64_t items, int64_t pitch) {
@@ -1288,7 +1297,7 @@ bool join(const RowsVariant& k, int64_t items, const RowsParams& p, hipStream_t 
     int groups = 1;
     while (groups < p.parts / items && 2 * groups * lpr <= 256) groups *= 2;
     const int per = 256 / (lpr * groups);
-    const int64_t grid = items * ((rows + per - 1) / per);
+    const int64_t grid = items * ((rows + per - 1) / per);    // (at most 16 an item)
     const bool many = p.parts / items > 2 * groups;
     return launch("rows_join_kernel",
                   k.vec == 4 ? (many ? rows_join_kernel<4, 8> : rows_join_kernel<4, 2>)
@@ -1351,6 +1360,11 @@ bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t 
     pl.target = pl.cut ? std::min<int64_t>(target, pl.items * units) : 0;
     pl.bytes = pl.cut ? rows_workspace(pl.k, 2 * pl.target, pl.items, (pool.value_dim + 3) / 4 * 4)
                       : 0;
+    if (pl.target + pl.items > kMostWgs || (pl.cut && pl.items * pl.k.vec > kMostWgs)) {
+        set_error("paged_attention: %lld sequences of %lld rows are too many for one call",
+                  (long long)n_seq, (long long)n_vec);
+        return false;
+    }
     return true;
 }
 
@@ -1447,10 +1461,6 @@ bool rows_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_sca
                   (long long)ws_bytes, (long long)pl.bytes);
         return false;
     }
-    if (pl.tiles > 65535 || n_head_kv > 65535 || pl.n_chunks * n_head_kv * pl.tiles > INT_MAX) {
-        set_error("attention_sinks: grid too large");
-        return false;
-    }
     RowsParams p{};
     p.q = q;
     p.out = out;
@@ -1469,8 +1479,8 @@ bool rows_sinks_dev(const float* q, int kv_dt, const void* k, const float* k_sca
     p.scale = scale;
     if (pl.n_chunks > 1) place_workspace(p, pl.k, ws);
     if (!launch(pl.k.name, kpos == nullptr ? pl.k.linear : pl.k.linear_pos,
-                dim3((unsigned)pl.n_chunks, (unsigned)n_head_kv, (unsigned)pl.tiles), dim3(256), 0,
-                s, p))
+                dim3((unsigned)(pl.n_chunks * ((pl.tiles + 65534) / 65535)), (unsigned)n_head_kv,
+                     (unsigned)std::min<int64_t>(pl.tiles, 65535)), dim3(256), 0, s, p))
         return false;
     return pl.n_chunks == 1 || join(pl.k, n_head_kv * pl.tiles, p, s);
 }

@@ -238,7 +238,7 @@ bool rows_io(const aero_kv_pool_t& pool, int64_t layer, float* k, float* v, cons
     if (!pool_ok(pool, what)) return false;
     if (layer < 0 || layer >= pool.n_layers || n_seq < 0 || n_q <= 0 || max_pages <= 0 ||
         max_pages > (int64_t(1) << 30) / pool.page || n_q > (int64_t(1) << 30) ||
-        n_seq > INT_MAX / (n_q * pool.n_head_kv)) {
+        n_seq > ((1 << 26) - 1) / (n_q * pool.n_head_kv)) {   // (a grid row: 2^32 threads)
         set_error("%s: bad sizes (layer=%lld n_seq=%lld n_q=%lld max_pages=%lld)", what,
                   (long long)layer, (long long)n_seq, (long long)n_q, (long long)max_pages);
         return false;

@@ -674,8 +674,8 @@ def paged_attention(pool, layer: int, q: DeviceArray, out: DeviceArray, table: D
     over its pages: q [n_seq, n_q, n_head, head_dim] -> out [n_seq, n_q, n_head,
     value_dim], table and lens as paged_kv_write, the mask as attention with
     window and sinks. Rows without a token, or that see nothing, become zeros;
-    keys of a page id outside the pool are not seen, and bad[0] becomes 1. The
-    launch does not depend on the lengths, so a plan that recorded it stays
+    keys of a page id outside the pool are not seen, and bad[0] becomes 1 (as for
+    a length past the table's room, which is cut to it). The launch does not depend on the lengths, so a plan that recorded it stays
     right as the sequences grow. The workspace is allocated once per size and
     reused: calls on different streams must not overlap."""
     max_pages = _paged(pool, table, lens, n_seq, bad)

@@ -120,6 +120,7 @@ class PagedKV:
         self._refs = np.zeros(pool.n_pages, np.int64)
         self._free = list(range(pool.n_pages))   # a heap: the lowest page first
         self._live: set[int] = set()
+        self._window: dict[int, int] = {}      # of the slots that trim has been at
         self._edits: dict[int, int] = {}
 
     # ------------------------------------------------------------ what there is
@@ -211,20 +212,25 @@ class PagedKV:
             if p >= 0:
                 self._refs[p] += 1
             self._set(d * self.max_pages + c, p)
+        if s in self._window:
+            self._window[d] = self._window[s]
         self._set(self._lens_at(d), n)
         self._flush(stream)
         return d
 
     def truncate(self, slot: int, n: int, stream: Stream | None = None) -> None:
-        """Keep the slot's first n tokens (a rejected guess, a shorter prompt)."""
+        """Keep the slot's first n tokens (a rejected guess, a shorter prompt).
+        Refused where trim has given up a page that the newest of them sees: trim
+        with a window that is longer by what may be taken back."""
         self._check()
         s = self._slot(slot)
         have = self.length(s)
         if n < 0 or n > have:
             raise ValueError(f"slot {s} holds {have} tokens, not {n}")
         page = self.pool.page
-        if n > 0 and self._row(s)[(n - 1) // page] < 0:
-            raise ValueError(f"slot {s}: the page of token {n - 1} was given up by trim")
+        seen = self._row(s)[max(0, n - self._window.get(s, n)) // page: -(-n // page)]
+        if (seen < 0).any():
+            raise ValueError(f"slot {s}: pages that token {n - 1} sees were given up by trim")
         for c in range(-(-n // page), -(-have // page)):
             self._clear(s, c)
         self._set(self._lens_at(s), n)
@@ -238,6 +244,7 @@ class PagedKV:
         s = self._slot(slot)
         if window <= 0 or sinks < 0:
             raise ValueError(f"trim: window {window}, sinks {sinks}")
+        self._window[s] = int(window)
         page, gone = self.pool.page, 0
         for c in range(-(-sinks // page), max(0, self.length(s) - window) // page):
             if self._row(s)[c] >= 0:
@@ -250,6 +257,7 @@ class PagedKV:
         """End a sequence: its slot and the pages that no other one shares."""
         self.truncate(slot, 0, stream)
         self._live.discard(int(slot))
+        self._window.pop(int(slot), None)
 
     def compact(self, stream: Stream | None = None) -> int:
         """Move the pages in use to the front of the pool (in every layer), so

@@ -643,11 +643,12 @@ int aero_hip_attention_sinks(const float* q, int kv_dt, const void* k, const flo
  * int32 on the device, read when the kernel runs: a recorded plan follows the
  * sequences as they grow. lens counts the call's n_q new tokens: token t of
  * sequence s has position lens[s] - n_q + t, and is no token when that is
- * negative (a padding row: lens 0). A length past max_pages * page is taken
- * as that many tokens. Page ids outside the pool are never followed: such a
- * page's keys are not seen, its rows not written and read as zeros, and *bad
- * (int32 on the device, or NULL) is set to 1. No counterpart in the
- * reference, which keeps one contiguous slot a sequence (src/kv.cpp). */
+ * negative (a padding row: lens 0). Page ids outside the pool are never
+ * followed: such a page's keys are not seen, its rows not written and read as
+ * zeros, and *bad (int32 on the device, or NULL) is set to 1; as for a length
+ * past max_pages * page, which the attention takes as that many tokens, and the
+ * rows there. No counterpart in the reference, which keeps one contiguous slot a
+ * sequence (src/kv.cpp). */
 typedef struct aero_kv_pool {
     int kv_dt;
     int64_t page;
@@ -678,7 +679,7 @@ int aero_hip_paged_attention(const aero_kv_pool_t* pool, int64_t layer, const fl
 /* The new tokens' rows k [n_seq, n_q, n_head_kv, head_dim] and v (value_dim)
  * into their pages of one layer, quantised as aero_hip_kv_write; and such rows
  * back as fp32 (code * scale; zeros where there is no token). Sequences that
- * write must not share the pages written. */
+ * write must not share the pages written. n_seq * n_q * n_head_kv < 2^26. */
 int aero_hip_paged_kv_write(const aero_kv_pool_t* pool, int64_t layer, const float* k,
                             const float* v, const int32_t* table, int64_t max_pages,
                             const int32_t* lens, int64_t n_seq, int64_t n_q, int32_t* bad,

@@ -465,3 +465,17 @@ def test_serving_run(hip, dt, window, sinks):
     stream.synchronize()
     assert not kv.lens.numpy().any() and (kv.table.numpy() == -1).all()
     stream.destroy()
+
+
+@pytest.mark.parametrize("dt", [0, 1], ids=["fp32", "int8"])
+def test_lengths_past_the_table(hip, dt):
+    """A length that the table has no room for is cut to the room, and said so."""
+    rng = np.random.default_rng([70, dt])
+    c = Cache(rng, dt, 16, 2, 64, 64, [64, 30])
+    q = rng.standard_normal((2, 1, 4, 64)).astype(np.float32)
+    bad = DA.from_numpy(np.zeros(1, np.int32))
+    table = c.table[:, :4].copy()
+    want = c.attend(q, 0.1, table=table, bad=bad)
+    assert bad.numpy()[0] == 0
+    got = c.attend(q, 0.1, table=table, lens=np.asarray([100, 30], np.int32), bad=bad)
+    assert bad.numpy()[0] == 1 and bits_equal(got, want)

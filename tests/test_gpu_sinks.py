@@ -321,3 +321,18 @@ def test_prompt_recorded(hip):
         assert bits_equal(got[:, at], eager)
         assert rel_to_scale(eager, want) <= RTOL
     plan.destroy()
+
+
+def test_more_tiles_than_a_grid_side(hip):
+    """70,000 tokens of four heads: 70,000 query tiles of one kv head; the rows at
+    both ends and around the 65,535th tile."""
+    rng = np.random.default_rng(60)
+    T, H, D, window, sinks = 70000, 4, 8, 5, 2
+    k, v = cache(rng, T, 1, D, 1), cache(rng, T, 1, D, 1)
+    q = values(rng, T, H, D)
+    qpos = np.arange(T)
+    got = call(q, k, v, T, 1, window, sinks, 1, qpos)
+    at = np.r_[0:40, T - 65535 - 20:T - 65535 + 20, 65515:65555, T - 40:T]
+    want = R.attention(q[at], k[2], v[2], R.seen(qpos[at], qpos, window, sinks), 0.1)
+    assert rel_to_scale(got[at], want) <= RTOL
+    assert np.isfinite(got).all() and np.abs(got).max(2).min() > 0

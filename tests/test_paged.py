@@ -173,13 +173,13 @@ def test_paged_kv_against_a_plain_model(monkeypatch, seed):
     pool = fake_pool()
     m = Model(monkeypatch, pool, 6, 12)
     kv = paged.PagedKV(pool, 6, 12)
-    truth, lost, name = {}, {}, 0
+    truth, lost, wins, name = {}, {}, {}, 0
     for step in range(400):
         what = rng.choice(("add", "append", "append", "append", "fork", "trim", "cut", "free",
                            "compact"))
         if what == "add" and len(truth) < 6:
             s = kv.add()
-            truth[s], lost[s] = [], 0
+            truth[s], lost[s], wins[s] = [], 0, 1 << 30
         elif what == "append" and truth:
             slots = rng.sample(sorted(truth), rng.randint(1, len(truth)))
             n = rng.choice((1, 1, 2, 16, 30))
@@ -199,11 +199,12 @@ def test_paged_kv_against_a_plain_model(monkeypatch, seed):
         elif what == "fork" and truth and len(truth) < 6:
             s = rng.choice(sorted(truth))
             d = kv.fork(s)
-            truth[d], lost[d] = list(truth[s]), lost[s]
+            truth[d], lost[d], wins[d] = list(truth[s]), lost[s], wins[s]
         elif what == "trim" and truth:
             s, w, k = rng.choice(sorted(truth)), rng.choice((5, 20, 40)), rng.choice((0, 4, 16, 20))
             first = truth[s][:k]
             kv.trim(s, w, k)
+            wins[s] = w
             lost[s] = max(lost[s], len(truth[s]) - w)
             if lost[s] > 0:     # what neither this nor a later token sees may be gone
                 truth[s] = [t if i < 0 or i >= lost[s] or m.token(s, i) == t else None
@@ -212,7 +213,8 @@ def test_paged_kv_against_a_plain_model(monkeypatch, seed):
         elif what == "cut" and truth:
             s = rng.choice(sorted(truth))
             n = rng.randint(lost[s] if lost[s] > 0 else 0, len(truth[s]))
-            if n == 0 or m.token(s, n - 1) is not None:
+            # (what the newest token left would see has to be there)
+            if all(m.token(s, i) is not None for i in range(max(0, n - wins[s]), n)):
                 kv.truncate(s, n)
                 del truth[s][n:]
                 lost[s] = min(lost[s], n)
@@ -222,7 +224,7 @@ def test_paged_kv_against_a_plain_model(monkeypatch, seed):
         elif what == "free" and truth:
             s = rng.choice(sorted(truth))
             kv.free(s)
-            del truth[s], lost[s]
+            del truth[s], lost[s], wins[s]
         elif what == "compact":
             kv.compact()
             used = {p for s in truth for p in kv.pages(s) if p >= 0}
@@ -236,6 +238,29 @@ def test_paged_kv_against_a_plain_model(monkeypatch, seed):
         for s in range(6):
             if s not in truth:
                 assert m.dev[m.n + s] == 0 and (m.dev[s * 12:(s + 1) * 12] == -1).all()
+
+
+def test_truncate_after_trim(monkeypatch):
+    """Cut back to where the window is still whole, and to the sinks alone; not
+    into pages given up."""
+    pool = fake_pool()
+    Model(monkeypatch, pool, 2, 12)
+    kv = paged.PagedKV(pool, 2, 12)
+    a = kv.add()
+    kv.append([a], 160)
+    kv.trim(a, 40, 4)                    # tokens 16 .. 111 gone
+    assert kv.pages(a)[1:7] == [-1] * 6 and min(kv.pages(a)[7:]) >= 0
+    b = kv.fork(a)
+    for s in (a, b):
+        with pytest.raises(ValueError):
+            kv.truncate(s, 151)
+        kv.truncate(s, 152)
+    kv.truncate(b, 16)
+    kv.append([b], 1)
+    kv.free(a)
+    a = kv.add()                         # a new sequence in the slot
+    kv.append([a], 60)
+    kv.truncate(a, 1)
 
 
 def test_paged_kv_refusals(monkeypatch):
