@@ -601,6 +601,7 @@ struct F16Core {
         qmax = over_row(qmax, Max{});
         int eq = 0;
         if (qmax > 0.0f && qmax <= 3.4028235e38f) frexpf(qmax, &eq);
+        eq = max(eq, -112);     // (2^(14 - e) is finite; what is smaller keeps its bits)
         const float qsc = ldexpf(1.0f, 14 - eq);
         if ((threadIdx.x & 15) == 0) sh.qscale[row] = ldexpf(p.scale * kLog2e, eq - 14);
 #pragma unroll

@@ -336,3 +336,43 @@ def test_more_tiles_than_a_grid_side(hip):
     want = R.attention(q[at], k[2], v[2], R.seen(qpos[at], qpos, window, sinks), 0.1)
     assert rel_to_scale(got[at], want) <= RTOL
     assert np.isfinite(got).all() and np.abs(got).max(2).min() > 0
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("D", [64, 128, 256, 48])
+@pytest.mark.parametrize("e", [-140, -100, 90])
+def test_sizes_of_queries(hip, dt, D, e):
+    """Queries of 2^e, one row of them zeros, at the scale that undoes it as far as a
+    scale of normal floats can."""
+    rng = np.random.default_rng([D, dt, e + 200])
+    H, HK, T, n_kv, window, sinks = 8, 2, 3, 700, 300, 4
+    k, v = cache(rng, n_kv, HK, D, dt), cache(rng, n_kv, HK, D, dt)
+    q = np.ldexp(values(rng, T, H, D), e).astype(np.float32)
+    q[1, 3] = 0
+    qpos = np.arange(n_kv - T, n_kv)
+    scale = float(np.float32(min(np.ldexp(0.1, -e), 2.0**120)))
+    got = call(q, k, v, n_kv, HK, window, sinks, dt, qpos, scale=scale)
+    keep = R.seen(qpos, np.arange(n_kv), window, sinks)
+    assert rel_to_scale(got, R.attention(q, k[2], v[2], keep, scale)) <= RTOL
+
+
+@pytest.mark.parametrize("dt", [1, 2], ids=["int8", "int4"])
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 5), (256, 2), (128, 70)])
+def test_sizes_of_scales(hip, dt, D, T):
+    """Value scales that fall and rise by 2^40 along the keys, key scales by 2^10:
+    each query to the scale of what it keeps."""
+    rng = np.random.default_rng([D, T, dt, 9])
+    H, HK, n_kv, window, sinks = 8, 2, 900, 64, 3
+    k, v = cache(rng, n_kv, HK, D, dt), cache(rng, n_kv, HK, D, dt)
+    for step, qpos in ((300, np.sort(rng.integers(0, n_kv, T))), (64, np.arange(n_kv - T, n_kv))):
+        ev = -40 * ((np.arange(n_kv) // step) % 2)
+        ek = -10 * ((np.arange(n_kv) // 50) % 2)
+        ks = np.ldexp(k[1].numpy(), ek[:, None]).astype(np.float32)
+        vs = np.ldexp(v[1].numpy(), ev[:, None]).astype(np.float32)
+        K, V = np.ldexp(k[2], ek[:, None, None]), np.ldexp(v[2], ev[:, None, None])
+        q = values(rng, T, H, D)
+        got = call(q, (k[0], DA.from_numpy(ks)), (v[0], DA.from_numpy(vs)), n_kv, HK, window,
+                   sinks, dt, qpos)
+        want = R.attention(q, K, V, R.seen(qpos, np.arange(n_kv), window, sinks), 0.1)
+        for t in range(T):
+            assert rel_to_scale(got[t], want[t]) <= RTOL, (step, t)
