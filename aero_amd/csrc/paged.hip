@@ -51,14 +51,14 @@ struct RowsIo {
 };
 
 // The vector of the pool that row r is; -1: no token, or no page
-__device__ __forceinline__ int64_t pool_vector(const RowsIo& p, int64_t r) {
-    const int64_t tok = r / p.heads;
-    const int h = (int)(r - tok * p.heads);
-    const int64_t s = tok / p.n_q;
+// (rows are fewer than 2^26)
+__device__ __forceinline__ int64_t pool_vector(const RowsIo& p, uint32_t r) {
+    const uint32_t tok = r / (uint32_t)p.heads, h = r - tok * p.heads;
+    const uint32_t s = tok / (uint32_t)p.n_q;
     const int64_t pos = (int64_t)p.lens[s] - p.n_q + (tok - s * p.n_q);
     if (pos < 0) return -1;
     const int64_t col = pos >> p.shift;
-    const int32_t page = col < p.max_pages ? p.table[s * p.max_pages + col] : -1;
+    const int32_t page = col < p.max_pages ? p.table[(int64_t)s * p.max_pages + col] : -1;
     if (page < 0 || page >= p.n_pages) {
         if (p.bad != nullptr) *p.bad = 1;
         return -1;
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(RowsIo p) {
     const bool in = 4 * li < dim;
     const float4 f = in ? *reinterpret_cast<const float4*>(x + 4 * li)
                         : make_float4(0.f, 0.f, 0.f, 0.f);
-    const int64_t vec = pool_vector(p, r);
+    const int64_t vec = pool_vector(p, (uint32_t)r);
     if (vec < 0) return;
     if constexpr (DT == 0) {
         if (in) *reinterpret_cast<float4*>(p.pages[w] + (vec * dim + 4 * li) * 4) = f;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(RowsIo p) {
     const int w = blockIdx.y, dim = p.dim[w], li = threadIdx.x % L;
     const int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
     if (r >= p.n_rows || 4 * li >= dim) return;
-    const int64_t vec = pool_vector(p, r);
+    const int64_t vec = pool_vector(p, (uint32_t)r);
     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
     if (vec >= 0) {
         if constexpr (DT == 0) {
@@ -146,7 +146,7 @@ template <int DT>
 __global__ __launch_bounds__(64) void paged_write_any_kernel(RowsIo p) {
     const int w = blockIdx.y, dim = p.dim[w], lane = threadIdx.x;
     const int64_t r = blockIdx.x;
-    const int64_t vec = pool_vector(p, r);
+    const int64_t vec = pool_vector(p, (uint32_t)r);
     if (vec < 0) return;
     const float* x = p.rows[w] + r * dim;
     if constexpr (DT == 0) {
@@ -176,7 +176,7 @@ template <int DT>
 __global__ __launch_bounds__(64) void paged_read_any_kernel(RowsIo p) {
     const int w = blockIdx.y, dim = p.dim[w], lane = threadIdx.x;
     const int64_t r = blockIdx.x;
-    const int64_t vec = pool_vector(p, r);
+    const int64_t vec = pool_vector(p, (uint32_t)r);
     float* o = p.rows[w] + r * dim;
     const float sc = DT != 0 && vec >= 0 ? p.scales[w][vec] : 0.0f;
     for (int i = lane; i < dim; i += 64) {
