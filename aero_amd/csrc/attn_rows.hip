@@ -273,13 +273,18 @@ constexpr int kIds = 1024;   // page ids a workgroup holds at a time
 // One kv head's tiles in memory, through buffer descriptors: lane offsets within
 // a tile are fixed, the tile's place is wave-uniform, and what lies past the
 // cache's end, or on a bad page, reads as zeros.
-template <int DT, int D, Source SRC>
+//
+// PAD: vectors of fewer than D elements, K's and V's of any two widths in whole
+// pieces (integers: of 8 bytes at most). Pieces past a vector's end read as zeros.
+template <int DT, int D, Source SRC, bool PAD>
 struct Tiles {
-    static constexpr int KVEC = D * kv_bits<DT>() / 8;   // bytes of a vector
+    static constexpr int KVEC = D * kv_bits<DT>() / 8;   // bytes of a vector (PAD: at most)
     static constexpr int KS = D / 4, VS = D / 16;        // elements a lane holds
     static constexpr int KB = KVEC / 4, VB = KVEC / 16;
-    static constexpr int KLB = KB < 16 ? KB : 16, KNI = KB / KLB, KLE = KLB * 8 / kv_bits<DT>();
-    static constexpr int VLB = VB < 16 ? VB : 16, VNI = VB / VLB, VLE = VLB * 8 / kv_bits<DT>();
+    static constexpr int MOST = PAD && DT != 0 ? 8 : 16; // bytes of a piece
+    static constexpr int KLB = KB < MOST ? KB : MOST, KNI = KB / KLB, KLE = KLB * 8 / kv_bits<DT>();
+    static constexpr int VLB = VB < MOST ? VB : MOST, VNI = VB / VLB, VLE = VLB * 8 / kv_bits<DT>();
+    static constexpr uint32_t kPast = 0x7ffffff0u;       // an offset past every end
     // head dimension of element j of lane group g's key slice, value dimension
     // of element t of lane c's value slice: pieces of the lanes interleave, so a
     // load instruction reads whole runs of a vector
@@ -307,14 +312,22 @@ struct Tiles {
 
     const RowsParams& p;
     int kh, g, c;
-    uint32_t stride;     // from a key to the next
+    uint32_t k_bytes, v_bytes;      // of a vector
+    uint32_t k_stride, v_stride;    // from a key to the next
     const int32_t* ids;  // paged: in LDS, the pages of the list from place0 on
     int32_t place0;
 
     __device__ __forceinline__ Tiles(const RowsParams& p_, const int32_t* ids_, int kh_, int g_,
                                      int c_)
         : p(p_), kh(kh_), g(g_), c(c_), ids(ids_) {
-        stride = SRC == kPaged ? KVEC : (uint32_t)(p.n_head_kv * KVEC);
+        k_bytes = PAD ? (uint32_t)p.head_dim * kv_bits<DT>() / 8 : KVEC;
+        v_bytes = PAD ? (uint32_t)p.value_dim * kv_bits<DT>() / 8 : KVEC;
+        k_stride = SRC == kPaged ? k_bytes : p.n_head_kv * k_bytes;
+        v_stride = SRC == kPaged ? v_bytes : p.n_head_kv * v_bytes;
+    }
+    // whether a vector has no piece there
+    static __device__ __forceinline__ bool past(uint32_t at, uint32_t bytes) {
+        return PAD && at >= bytes;
     }
 
     // the ids for places x .. x1 - 1 of the list into LDS (no more than
@@ -378,8 +391,9 @@ struct Tiles {
         }
         return l;
     }
-    __device__ __forceinline__ uint32_t bytes(const Place& l) const {
-        return l.left > 0 ? (uint32_t)(l.left - 1) * stride + KVEC : 0u;
+    static __device__ __forceinline__ uint32_t reach(const Place& l, uint32_t stride,
+                                                     uint32_t bytes) {
+        return l.left > 0 ? (uint32_t)(l.left - 1) * stride + bytes : 0u;
     }
     // scales of keys 4g .. 4g + 3 (paged: a head's scales of a page lie together)
     __device__ __forceinline__ void load_scales(float (&o)[4], const float* s,
@@ -399,10 +413,12 @@ struct Tiles {
         }
     }
     __device__ __forceinline__ void load(K& t, const Place& l) const {
-        const __amdgpu_buffer_rsrc_t r = rsrc(p.k, l.vec * KVEC, bytes(l));
+        const __amdgpu_buffer_rsrc_t r = rsrc(p.k, l.vec * k_bytes, reach(l, k_stride, k_bytes));
 #pragma unroll
-        for (int i = 0; i < KNI; ++i)
-            words<KLB>(r, (uint32_t)c * stride + (uint32_t)((4 * i + g) * KLB), t.k + i * KLB / 4);
+        for (int i = 0; i < KNI; ++i) {
+            const uint32_t at = (4 * i + g) * KLB;
+            words<KLB>(r, past(at, k_bytes) ? kPast : c * k_stride + at, t.k + i * KLB / 4);
+        }
         if constexpr (DT != 0) load_scales(t.s, p.ks, l);
     }
     __device__ __forceinline__ void load(V& t, const Place& l) const {
@@ -414,13 +430,15 @@ struct Tiles {
                 t.kp[r] = (int32_t)__builtin_amdgcn_raw_buffer_load_b32(b, (4 * g + r) * 4, 0, 0);
         }
         if constexpr (DT != 0) load_scales(t.s, p.vs, l);
-        const __amdgpu_buffer_rsrc_t b = rsrc(p.v, l.vec * KVEC, bytes(l));
+        const __amdgpu_buffer_rsrc_t b = rsrc(p.v, l.vec * v_bytes, reach(l, v_stride, v_bytes));
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int i = 0; i < VNI; ++i)
-                words<VLB>(b, (uint32_t)(4 * g + r) * stride + (uint32_t)((16 * i + c) * VLB),
+            for (int i = 0; i < VNI; ++i) {
+                const uint32_t at = (16 * i + c) * VLB;
+                words<VLB>(b, past(at, v_bytes) ? kPast : (4 * g + r) * v_stride + at,
                            t.v[r] + i * VLB / 4);
+            }
     }
 };
 
@@ -485,7 +503,7 @@ struct TileShared {
 // The four waves' (m, l, acc) of a tile joined through LDS; its rows written out
 // (row < 0) or as a part. Lane (g, c) holds acc of query 4g + r, dimension
 // vdim(c, t), and (m, l) of query c, l a share.
-template <typename TL, int D>
+template <typename TL, int D, bool PAD>
 __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it, int rows, float m,
                                             float ls, const v4f (&acc)[D / 16], int64_t row,
                                             TileShared<D>& sh) {
@@ -517,6 +535,7 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
     __syncthreads();
     for (int x = tid; x < rows * (D / 4); x += 256) {
         const int i = x / (D / 4), d = 4 * (x % (D / 4));
+        if (PAD && d >= p.value_dim) continue;
         v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
@@ -529,7 +548,7 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
             const int64_t r = ((int64_t)it.s * p.n_q + u / p.rep) * p.n_head + it.kh * p.rep +
                               u % p.rep;
             const float inv = 1.0f / fmaxf(sh.lt[i], 1e-30f);
-            *reinterpret_cast<v4f*>(p.out + r * D + d) =
+            *reinterpret_cast<v4f*>(p.out + r * (PAD ? p.value_dim : D) + d) =
                 v4f{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
         } else {
             *reinterpret_cast<v4f*>(part_row(p, row + i) + d) = o;
@@ -544,12 +563,12 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
 // (hi, lo = v - hi: 22 bits), so every product is exact and added in fp32. 32 keys
 // a step, scores in log2 units, sums rescaled only when a query's maximum passes
 // the reference by 2^8 or the scales' exponent moves (as attention.hip's kernel).
-template <int DT, int D, Source SRC>
+template <int DT, int D, Source SRC, bool PAD = false>
 struct F16Core {
     static constexpr int VEC = 16;
     static constexpr int UNIT = 8;
     static constexpr int EU = D == 256 ? 2 : 3;
-    using TL = Tiles<DT, D, SRC>;
+    using TL = Tiles<DT, D, SRC, PAD>;
     using Shared = TileShared<D>;
     static constexpr int KS = TL::KS, VS = TL::VS, NS = KS / 8;
 
@@ -583,10 +602,13 @@ struct F16Core {
 #pragma unroll
         for (int i = 0; i < QI; ++i) {
             const int x = min(16 * i + (int)(threadIdx.x & 15), 4 * NS - 1);
-            const float* src = p.q + qrow * D + TL::kdim(x & 3, 8 * (x >> 2));
+            const int d = TL::kdim(x & 3, 8 * (x >> 2));
+            const float* src = p.q + qrow * (PAD ? p.head_dim : D) + d;
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(src + e);
+                const float4 v = PAD && d + e >= p.head_dim
+                                     ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                     : *reinterpret_cast<const float4*>(src + e);
                 f[i][e] = v.x; f[i][e + 1] = v.y; f[i][e + 2] = v.z; f[i][e + 3] = v.w;
             }
         }
@@ -797,17 +819,17 @@ struct F16Core {
         for (int t = 0; t < VS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[t][r] *= back;
-        finish_tile<TL, D>(p, it, col.rows, m * kLn2, ls, acc, row, sh);
+        finish_tile<TL, D, PAD>(p, it, col.rows, m * kLn2, ls, acc, row, sh);
     }
 };
 
 // fp32 caches on the fp32 matrix cores (v_mfma_f32_16x16x4_f32): 16 keys a step.
-template <int D, Source SRC>
+template <int D, Source SRC, bool PAD = false>
 struct F32Core {
     static constexpr int VEC = 16;
     static constexpr int UNIT = 4;
     static constexpr int EU = D == 256 ? 1 : (D == 128 ? 2 : 3);
-    using TL = Tiles<0, D, SRC>;
+    using TL = Tiles<0, D, SRC, PAD>;
     using Shared = TileShared<D>;
     static constexpr int KS = TL::KS, VS = TL::VS;
 
@@ -935,12 +957,14 @@ struct F32Core {
         // the queries into LDS: 16 lanes a row
         constexpr int QI = D / 64;
         const int row = threadIdx.x >> 4;
-        const float* src = p.q + query_row(p, it, row) * D;
+        const float* src = p.q + query_row(p, it, row) * (PAD ? p.head_dim : D);
         v4f f[QI];
 #pragma unroll
         for (int i = 0; i < QI; ++i) {
             const int x = 16 * i + (threadIdx.x & 15);
-            f[i] = *reinterpret_cast<const v4f*>(src + TL::kdim(x & 3, 4 * (x >> 2)));
+            const int d = TL::kdim(x & 3, 4 * (x >> 2));
+            f[i] = PAD && d >= p.head_dim ? v4f{0.f, 0.f, 0.f, 0.f}
+                                          : *reinterpret_cast<const v4f*>(src + d);
         }
         const int span = tl.id_tiles(x1 - x0);
         for (int xb = x0; xb < x1; xb += span) {
@@ -981,7 +1005,7 @@ struct F32Core {
     }
 
     __device__ __forceinline__ void finish(int64_t row) {
-        finish_tile<TL, D>(p, it, col.rows, m * kLn2, ls, acc, row, sh);
+        finish_tile<TL, D, PAD>(p, it, col.rows, m * kLn2, ls, acc, row, sh);
     }
 };
 
@@ -1241,33 +1265,46 @@ RowsVariant vec_variant(int width) {
                        : (width <= 128 ? vec_variant<DT, 8>() : vec_variant<DT, 16>());
 }
 
-template <int DT, int D>
+template <int DT, int D, bool PAD>
 RowsVariant f16_variant() {
     return {"rows_f16_kernel", 16, 8, 256 * F16Core<DT, D, kPaged>::EU,
-            rows_paged_kernel<F16Core<DT, D, kPaged>>, rows_linear_kernel<F16Core<DT, D, kLinear>>,
-            rows_linear_kernel<F16Core<DT, D, kLinearPos>>};
+            rows_paged_kernel<F16Core<DT, D, kPaged, PAD>>,
+            rows_linear_kernel<F16Core<DT, D, kLinear, PAD>>,
+            rows_linear_kernel<F16Core<DT, D, kLinearPos, PAD>>};
 }
 
-template <int D>
+template <int D, bool PAD>
 RowsVariant f32_variant() {
-    return {"rows_f32_kernel", 16, 4, 256 * F32Core<D, kPaged>::EU, rows_paged_kernel<F32Core<D, kPaged>>,
-            rows_linear_kernel<F32Core<D, kLinear>>, rows_linear_kernel<F32Core<D, kLinearPos>>};
+    return {"rows_f32_kernel", 16, 4, 256 * F32Core<D, kPaged>::EU,
+            rows_paged_kernel<F32Core<D, kPaged, PAD>>, rows_linear_kernel<F32Core<D, kLinear, PAD>>,
+            rows_linear_kernel<F32Core<D, kLinearPos, PAD>>};
 }
 
-template <int D>
+template <int D, bool PAD>
 RowsVariant mfma_variant(int dt) {
-    return dt == 0 ? f32_variant<D>() : (dt == 1 ? f16_variant<1, D>() : f16_variant<2, D>());
+    return dt == 0   ? f32_variant<D, PAD>()
+           : dt == 1 ? f16_variant<1, D, PAD>()
+                     : f16_variant<2, D, PAD>();
 }
 
-// The matrix cores take head_dim == value_dim of 64, 128 and 256 with 16-byte
-// aligned rows; any other width, or alignment, the vector kernel.
+template <bool PAD>
+RowsVariant mfma_variant(int dt, int width) {
+    return width <= 64    ? mfma_variant<64, PAD>(dt)
+           : width <= 128 ? mfma_variant<128, PAD>(dt)
+                          : mfma_variant<256, PAD>(dt);
+}
+
+// The matrix cores take 16-byte aligned rows: of 64, 128 and 256 elements as they
+// are, others in the next of these widths where both dims are whole 16-byte pieces
+// (fp32) or 8-byte ones (int8: a multiple of 8, int4: of 16). The rest, the vector
+// kernel.
 RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool aligned) {
-    if (aligned && head_dim == value_dim) {
-        if (head_dim == 64) return mfma_variant<64>(dt);
-        if (head_dim == 128) return mfma_variant<128>(dt);
-        if (head_dim == 256) return mfma_variant<256>(dt);
-    }
     const int width = (int)std::max(head_dim, value_dim);
+    const int whole = dt == 0 ? 4 : (dt == 1 ? 8 : 16);
+    if (aligned && head_dim == value_dim && (width == 64 || width == 128 || width == 256))
+        return mfma_variant<false>(dt, width);
+    if (aligned && head_dim % whole == 0 && value_dim % whole == 0)
+        return mfma_variant<true>(dt, width);
     return dt == 0 ? vec_variant<0>(width) : (dt == 1 ? vec_variant<1>(width) : vec_variant<2>(width));
 }
 

@@ -479,3 +479,24 @@ def test_lengths_past_the_table(hip, dt):
     assert bad.numpy()[0] == 0
     got = c.attend(q, 0.1, table=table, lens=np.asarray([100, 30], np.int32), bad=bad)
     assert bad.numpy()[0] == 1 and bits_equal(got, want)
+
+
+# widths between those of the matrix operands, K and V of two, whole pieces and not
+WIDTHS = [(80, 80), (96, 96), (112, 112), (160, 160), (192, 192), (192, 128), (64, 128), (128, 64),
+          (8, 8), (16, 240), (240, 16), (40, 104), (48, 48), (72, 100), (252, 4), (56, 256),
+          (12, 20), (250, 250), (2, 6)]
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("D,DV", WIDTHS, ids=[f"{a}-{b}" for a, b in WIDTHS])
+def test_widths(hip, D, DV, dt):
+    """Other widths: what lies behind a vector (unused rows are NaN, or NaN scales)
+    and behind a query's does not count."""
+    if dt == 0 and (D % 4 or DV % 4):
+        pytest.skip("fp32 rows are whole 16-byte pieces")
+    rng = np.random.default_rng([D, DV, dt])
+    lens = [700, 0, 1, 33, 5]
+    c = Cache(rng, dt, 16, 3, D, DV, lens)
+    for nq, window, sinks in ((1, 0, 0), (3, 40, 4)):
+        q = rng.standard_normal((len(lens), nq, 15, D)).astype(np.float32)
+        check(c.attend(q, 0.1, window, sinks), c.ref(q, 0.1, window, sinks), lens, nq)

@@ -376,3 +376,27 @@ def test_sizes_of_scales(hip, dt, D, T):
         want = R.attention(q, K, V, R.seen(qpos, np.arange(n_kv), window, sinks), 0.1)
         for t in range(T):
             assert rel_to_scale(got[t], want[t]) <= RTOL, (step, t)
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("D,DV", [(80, 80), (96, 96), (192, 128), (16, 240), (40, 104), (72, 100),
+                                  (8, 8), (252, 4)])
+@pytest.mark.parametrize("T", [1, 37])
+def test_widths(hip, D, DV, T, dt):
+    """Other widths, with and without key positions; values that no query keeps
+    are not finite (fp32)."""
+    rng = np.random.default_rng([D, DV, T, dt])
+    HK, H, n_kv, window, sinks = 3, 6, 650, 300, 5
+    k, v = cache(rng, n_kv, HK, D, dt), cache(rng, n_kv, HK, DV, dt)
+    q = values(rng, T, H, D)
+    qpos = np.arange(n_kv - T, n_kv)
+    keep = R.seen(qpos, np.arange(n_kv), window, sinks)
+    if dt == 0:
+        for x, bad in ((k, np.nan), (v, np.inf)):
+            a = x[0].numpy().copy()
+            a[~keep.any(0)] = bad
+            x[0].copy_from(a)
+    want = R.attention(q, k[2], v[2], keep, 0.1)
+    for kpos in (None, np.arange(n_kv)):
+        got = call(q, k, v, n_kv, HK, window, sinks, dt, qpos, kpos, DV=DV)
+        assert rel_to_scale(got, want) <= RTOL
