@@ -500,3 +500,39 @@ def test_widths(hip, D, DV, dt):
     for nq, window, sinks in ((1, 0, 0), (3, 40, 4)):
         q = rng.standard_normal((len(lens), nq, 15, D)).astype(np.float32)
         check(c.attend(q, 0.1, window, sinks), c.ref(q, 0.1, window, sinks), lens, nq)
+
+
+def shifted(a, by=1):
+    """a on the device, `by` elements behind a 16-byte boundary"""
+    a = np.ascontiguousarray(a)
+    buf = DA.empty(a.size + by, a.dtype)
+    buf.copy_from(np.concatenate([np.zeros(by, a.dtype), a.reshape(-1)]))
+    return buf.view(a.shape, offset_bytes=by * a.itemsize)
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("D,DV", [(128, 128), (64, 32), (256, 256)])
+def test_rows_that_are_not_aligned(hip, D, DV, dt):
+    """Queries, outputs and new rows at any 4-byte address."""
+    rng = np.random.default_rng([D, dt, 71])
+    H, HK, lens, nq = 8, 2, [300, 2, 17], 2
+    c = Cache(rng, dt, 16, HK, D, DV, lens)
+    q = rng.standard_normal((3, nq, H, D)).astype(np.float32)
+    T, L = DA.from_numpy(c.table), DA.from_numpy(c.lens)
+    want = c.ref(q, 0.1, 100, 4)
+    for dq, out in ((shifted(q), DA.empty((3, nq, H, DV))),
+                    (DA.from_numpy(q), shifted(np.ones((3, nq, H, DV), np.float32), 3)),
+                    (shifted(q, 2), shifted(np.ones((3, nq, H, DV), np.float32)))):
+        ops.paged_attention(c.pool, 0, dq, out, T, L, 3, H, 0.1, n_q=nq, window=100, sinks=4)
+        check(out.numpy(), want, lens, nq)
+    k = rng.standard_normal((3, nq, HK, D)).astype(np.float32)
+    v = rng.standard_normal((3, nq, HK, DV)).astype(np.float32)
+    rows = []
+    for move in (DA.from_numpy, shifted):
+        ops.paged_kv_write(c.pool, 0, move(k), move(v), T, L, 3, n_q=nq)
+        ko, vo = move(np.full_like(k, 9)), move(np.full_like(v, 9))
+        ops.paged_kv_read(c.pool, 0, ko, vo, T, L, 3, n_q=nq)
+        rows.append((ko.numpy(), vo.numpy()))
+        ops.paged_kv_write(c.pool, 0, DA.from_numpy(0 * k), DA.from_numpy(0 * v), T, L, 3, n_q=nq)
+    assert bits_equal(rows[0][0], rows[1][0]) and bits_equal(rows[0][1], rows[1][1])
+    assert rows[0][0].any()

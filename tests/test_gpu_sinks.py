@@ -400,3 +400,33 @@ def test_widths(hip, D, DV, T, dt):
     for kpos in (None, np.arange(n_kv)):
         got = call(q, k, v, n_kv, HK, window, sinks, dt, qpos, kpos, DV=DV)
         assert rel_to_scale(got, want) <= RTOL
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("D,T,n_kv", [(128, 2, 300), (64, 600, 700), (256, 1, 2000)])
+def test_rows_that_are_not_aligned(hip, D, T, n_kv, dt):
+    """Queries and outputs at any 4-byte address, codes at any byte (fp32 caches
+    are refused then), prompts among them."""
+    from test_gpu_paged import shifted
+    rng = np.random.default_rng([D, T, dt, 5])
+    HK, H, window, sinks = 16, 32, 100, 4
+    k, v = cache(rng, n_kv, HK, D, dt), cache(rng, n_kv, HK, D, dt)
+    q = values(rng, T, H, D)
+    qpos = np.arange(n_kv - T, n_kv)
+    at = np.r_[0:T:max(1, T // 20), T - 1]
+    want = R.attention(q[at], k[2], v[2], R.seen(qpos[at], np.arange(n_kv), window, sinks), 0.1)
+    dq, qp = DA.from_numpy(q), DA.from_numpy(qpos.astype(np.int32))
+    blank = np.ones((T, H, D), np.float32)
+    for dq, out, dk, dv in ((shifted(q), DA.empty((T, H, D)), k[0], v[0]),
+                            (dq, shifted(blank), k[0], v[0]),
+                            (dq, DA.empty((T, H, D)), shifted(k[0].numpy()), v[0]),
+                            (dq, DA.empty((T, H, D)), k[0], shifted(v[0].numpy()))):
+        run = lambda: ops.attention(dq, dk, dv, out, T, H, HK, D, D, n_kv, 0.1, qpos=qp,
+                                    window=window, kv_dt=dt, k_scale=k[1], v_scale=v[1],
+                                    sinks=sinks)
+        if dt == 0 and (dk is not k[0] or dv is not v[0]):
+            with pytest.raises(Exception, match="aligned"):
+                run()
+            continue
+        run()
+        assert rel_to_scale(out.numpy()[at], want) <= RTOL
