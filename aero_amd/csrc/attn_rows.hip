@@ -20,6 +20,13 @@
 //  * contiguous: every item has n_chunks.
 // The parts of an item of several chunks are joined by rows_join_kernel.
 // Page ids are checked against the pool: tiles of a bad page are not seen.
+//
+// What bounds it (MI355X; 8 kv heads of 128, 4 query heads each): reading the cache.
+// 4 fp32 sequences of up to 50,001 tokens, 887 MB: 159 us, 5.6 TB/s (a copy reaches
+// 4.65). 48 int8 ones of up to 8,192, 282 MB: 70 us, the walk 57 of it at 5.0 TB/s
+// (5 us until the first loads are in, as long again at the end), the join 6. Few keys:
+// memory round trips one after another (length, page ids, keys), about 1 us each, and
+// 1 us for the four waves' sums to meet: 333 tokens 7.5 us, one launch.
 #include "attn_common.hpp"
 #include "paged_sched.hpp"
 #include "paged.hpp"
@@ -95,8 +102,10 @@ __device__ __forceinline__ int32_t page_at(const RowsParams& p, int32_t s, int32
 
 // ------------------------------------------------------------ any head width
 // 16-lane groups own a key each (a 16-key tile a step of the workgroup), lane
-// li of a group elements E li .. of the head; dot products by lane shuffles,
-// four query vectors a workgroup.
+// li of a group elements E li .. of the head; dot products by lane moves, four
+// query vectors a workgroup. For widths and addresses that the matrix operands do not
+// take: bound by its vector steps and element-wise loads. 8 sequences of up to 20,000
+// tokens, 8 kv heads of 80: fp32 138 us here, 66 on the matrix cores, int8 224 / 32.
 template <int DT, int E>
 __device__ __forceinline__ void load_slice(const void* base, const float* scales, int64_t vec,
                                            int dim, int e0, float (&o)[E]) {
@@ -563,6 +572,13 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
 // (hi, lo = v - hi: 22 bits), so every product is exact and added in fp32. 32 keys
 // a step, scores in log2 units, sums rescaled only when a query's maximum passes
 // the reference by 2^8 or the scales' exponent moves (as attention.hip's kernel).
+//
+// A step is about 290 vector and 32 matrix instructions for 8 KB of codes (dim 128):
+// a third of the vector units' time at the memory's rate. So as many waves a SIMD as
+// the registers allow without spilling (EU 3; 2 at dim 256), each with the next step's
+// codes on their way: 96 KB a CU. 64 sequences in a window of 1,024, 4 kv heads of
+// 256, 3 tokens each: 102 MB in 27 us (3.8 TB/s; 22 B/ns a CU, all that the memory
+// gives, but for 5 us at the start).
 template <int DT, int D, Source SRC, bool PAD = false>
 struct F16Core {
     static constexpr int VEC = 16;
@@ -823,7 +839,12 @@ struct F16Core {
     }
 };
 
-// fp32 caches on the fp32 matrix cores (v_mfma_f32_16x16x4_f32): 16 keys a step.
+// fp32 caches on the fp32 matrix cores (v_mfma_f32_16x16x4_f32): 16 keys a step,
+// products and sums in fp32. Keys and values are matrix operands as they are loaded,
+// 16 KB a step and wave at dim 128, so two waves a SIMD (one at dim 256, three at 64)
+// keep enough on the way: 5.6 TB/s over long caches. One token over 2,052 keys, 4 kv
+// heads of 256: 132 workgroups of a step each, 16.8 MB in 11 us and the join's 4.5:
+// one round trip to memory at half of the CUs.
 template <int D, Source SRC, bool PAD = false>
 struct F32Core {
     static constexpr int VEC = 16;
@@ -1159,7 +1180,10 @@ rows_linear_kernel(RowsParams p) {
 
 // The parts of an item's rows joined: `groups` groups of pitch / 4 lanes a row
 // take every groups-th part, then the groups meet in LDS; 256 threads do as many
-// rows as fit. B: parts that a group has in flight.
+// rows as fit. B: parts that a group has in flight. Bound by its launch and one or
+// two round trips (the span, the parts): 4.2-6 us from 8 to 33 parts an item. Joining
+// in the kernel above instead, by an item's last workgroup, takes a counter that
+// starts at zero and a fence a workgroup: faster only where items have few parts.
 template <int VEC, int B>
 __global__ __launch_bounds__(256) void rows_join_kernel(RowsParams p, int32_t rows, int32_t groups) {
     __shared__ float sm[256], sl[256];
