@@ -493,25 +493,23 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2))) void attn_prompt_kernel(P
             key_parts(1);
             const float kf = recs[sub].tile.kf;
             const int ev = __builtin_amdgcn_readfirstlane(recs[sub].tile.ev);
-            v16f s, sl;
+            v16f s;
 #pragma unroll
-            for (int y = 0; y < 16; ++y) s[y] = sl[y] = 0.0f;
+            for (int y = 0; y < 16; ++y) s[y] = 0.0f;
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int st = 0; st < NS; ++st) {
                 if (st + 2 < NS) key_parts(st + 2);
                 __builtin_amdgcn_sched_barrier(0);
-                sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[st % 3], qhi[st], sl, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[st % 3], qhi[st], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[st % 3], qlo[st], s, 0, 0, 0);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[st % 3], qhi[st], s, 0, 0, 0);
-                sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[st % 3], qlo[st], sl, 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_setprio(0);
             value_parts(0);
             value_parts(1);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) s[y] += sl[y];
             // (at least the smallest normal: -inf times c stays -inf)
             const float c = fmaxf(kf * qsc, 1.17549435e-38f);
             if (KPOS || kb + 31 > min(qmin, n_kv - 1) ||
