@@ -20,14 +20,17 @@
 // maximum passes it by 1; probabilities are taken in units of 2^(12 + ev - E), ev
 // the exponent of the tile's values and E that of the walk's: below 2^13 in fp16.
 //
-// Measured (2048 tokens, 32 heads of 128 on 8, window 512): 69 us, the splitting 12 of
+// Measured (2048 tokens, 32 heads of 128 on 8, window 512): 68 us, the splitting 12 of
 // it (latency of 512 workgroups: positions, rows, the dimensions' maxima in LDS), the
-// walk 2.1 us a tile of 256 query vectors, which is 1.2 PFLOP/s of fp16 products with
-// every CU at it, what a large fp16 product reaches; the queries' 33 MB in 5-9 us and
-// the results' 2 us have nothing to overlap with: each CU has one workgroup.
-// 1001 tokens, 14 heads of 64 on 2, window 1024: 28.8 us (6 + 2.1 a step of four
-// tiles): half the matrix steps for the same softmax, so vector steps and LDS reads
-// (128 KB a step) set the time.
+// walk 2.1 us a tile of 256 query vectors; the queries' 33 MB in 5-9 us and the
+// results' 2 us have nothing to overlap with: each CU has one workgroup. What bounds
+// the walk is power: over long windows the matrix cores are busy 62% of the cycles and
+// the clock is at 1.8 GHz, 1.17 PFLOP/s, a large fp16 product's rate. 1001 tokens, 14
+// heads of 64 on 2, window 1024: 28 us, 2.1 a step of four tiles: half the matrix steps
+// for the same softmax and LDS reads (41% at 2.1 GHz). So fewer instructions count (all
+// three products into one accumulator, 16 sums less a tile: 128 -> 120 us in a window of
+// 4096, dim 64), their order does not: the next tile's scores among this one's softmax
+// were no faster.
 //
 // What the parts cannot carry is known before the walk, from each tile's record
 // (exponents, the least of a row's, the largest value of each dimension, whether
