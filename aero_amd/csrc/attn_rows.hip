@@ -60,6 +60,7 @@ struct RowsParams {
     int32_t window, sinks;
     int32_t parts;         // room for
     int32_t target;        // paged: chunks that fill the chip (0: an item is one chunk)
+    int32_t item_tokens;   // paged: tokens that an item has, at most
     int32_t n_chunks;      // contiguous
     float scale;
 };
@@ -1053,8 +1054,9 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 __device__ __forceinline__ int32_t seq_len(const RowsParams& p, int32_t s) {
     return min(max(p.lens[s], 0), p.n_kv);
 }
+// the keys of a sequence's last item (none has many more)
 __device__ __forceinline__ KeyTiles seq_tiles(const RowsParams& p, int32_t len) {
-    return key_tiles((int64_t)len - p.n_q, (int64_t)len - 1, len, p.window, p.sinks);
+    return key_tiles((int64_t)len - p.item_tokens, (int64_t)len - 1, len, p.window, p.sinks);
 }
 
 __device__ __forceinline__ int32_t chunks_of(const RowsParams& p, int32_t units, int32_t total) {
@@ -1129,16 +1131,16 @@ rows_paged_kernel(RowsParams p) {
     // (a length past the table's room is cut to it)
     if (p.bad != nullptr && threadIdx.x == 0 && p.lens[it.s] > p.n_kv) *p.bad = 1;
     it.pos0 = it.len - p.n_q;
-    it.kt = seq_tiles(p, it.len);
-    const int32_t units = item_units(it.kt.n, Core::UNIT);
-    const int32_t chunks = chunks_of(p, units, total);
+    const int32_t chunks = chunks_of(p, item_units(seq_tiles(p, it.len).n, Core::UNIT), total);
     const int32_t item = b / chunks, c = b % chunks;
     it.kh = item / p.tiles;
     it.z = item % p.tiles;
-    // (keys past the tile's own last position are not walked)
-    const int t_last = min(it.z * Core::VEC + Core::VEC - 1, p.n_q * p.rep - 1) / p.rep;
-    const int x1 = min(chunk_begin(c + 1, chunks, units) * Core::UNIT,
-                       it.kt.upto(it.pos0 + t_last));
+    // the keys that the item's own tokens see, in as many chunks (some empty then)
+    it.kt = key_tiles(it.pos0 + it.z * Core::VEC / p.rep,
+                      it.pos0 + min(it.z * Core::VEC + Core::VEC - 1, p.n_q * p.rep - 1) / p.rep,
+                      it.len, p.window, p.sinks);
+    const int32_t units = item_units(it.kt.n, Core::UNIT);
+    const int x1 = min(chunk_begin(c + 1, chunks, units) * Core::UNIT, it.kt.n);
     Core core(p, it, sh);
     core.walk(chunk_begin(c, chunks, units) * Core::UNIT, x1);
     core.finish(chunks == 1 ? -1 : (int64_t)(part + b) * Core::VEC);
@@ -1379,7 +1381,7 @@ int log2_of(int64_t x) {
 // not possible. (Pointers are checked apart.)
 struct PagedPlan {
     RowsVariant k;
-    int64_t tiles, items, target, bytes;
+    int64_t tiles, items, item_tokens, target, bytes;
     bool cut;   // some item may have more than one chunk
 };
 
@@ -1411,9 +1413,11 @@ bool paged_plan(const aero_kv_pool_t& pool, int64_t n_seq, int64_t n_q, int64_t 
                   "work than one call takes", (long long)max_pages, (long long)n_seq);
         return false;
     }
+    const int64_t rep = n_head / pool.n_head_kv;
+    pl.item_tokens = std::min<int64_t>(n_q, (pl.k.vec + rep - 1) / rep + 1);
     // (a window's keys, and what is left of the tiles at the runs' ends)
-    const int64_t seen = window > 0 ? std::min<int64_t>(max_pages * pool.page, (int64_t)window +
-                                                        sinks + n_q + 45)
+    const int64_t seen = window > 0 ? std::min<int64_t>(max_pages * pool.page,
+                                                        (int64_t)window + sinks + pl.item_tokens + 45)
                                     : max_pages * pool.page;
     const int64_t fill = pl.k.workers, most = (seen + 16 * pl.k.unit - 1) / (16 * pl.k.unit);
     pl.cut = most * 16 * pl.k.unit > (2 * pl.items >= fill ? kWholeKeysMany : kWholeKeys);
@@ -1471,6 +1475,7 @@ bool paged_attention_dev(const aero_kv_pool_t& pool, int64_t layer, const float*
     p.tiles = (int32_t)pl.tiles;
     p.window = window; p.sinks = sinks;
     p.target = (int32_t)pl.target;
+    p.item_tokens = (int32_t)pl.item_tokens;
     p.parts = (int32_t)(2 * pl.target);
     p.scale = scale;
     if (pl.cut) place_workspace(p, pl.k, ws);

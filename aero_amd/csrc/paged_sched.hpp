@@ -30,13 +30,6 @@ struct KeyTiles {
     AERO_HD int32_t at(int32_t x) const { return x < n_sink ? x : x - n_sink + first; }
     // the place of tile x (one of the list's)
     AERO_HD int32_t place(int32_t x) const { return x < n_sink ? x : x - first + n_sink; }
-    // the places whose tiles begin at or before position q_hi
-    AERO_HD int32_t upto(int64_t q_hi) const {
-        if (q_hi < 0) return 0;
-        const int64_t t = q_hi >> 4;
-        const int64_t x = t >= first ? t - first + n_sink + 1 : (t + 1 < n_sink ? t + 1 : n_sink);
-        return x < n ? (int32_t)x : n;
-    }
     // a page list with no gaps: the sinks' pages, then the window's; the place
     // there of the page of list place x (shift: log2 of tiles a page)
     AERO_HD int32_t page_place(int32_t x, int shift) const {

@@ -536,3 +536,17 @@ def test_rows_that_are_not_aligned(hip, D, DV, dt):
         ops.paged_kv_write(c.pool, 0, DA.from_numpy(0 * k), DA.from_numpy(0 * v), T, L, 3, n_q=nq)
     assert bits_equal(rows[0][0], rows[1][0]) and bits_equal(rows[0][1], rows[1][1])
     assert rows[0][0].any()
+
+
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["fp32", "int8", "int4"])
+@pytest.mark.parametrize("H,HK,D,page,lens,nq,window,sinks", [
+    (32, 8, 128, 16, [300, 900, 100, 0], 300, 64, 4), (8, 2, 64, 64, [3000, 700], 130, 33, 70),
+    (2, 1, 64, 16, [3000], 20, 1000, 4), (16, 2, 256, 32, [2600, 40], 37, 1500, 0),
+    (24, 1, 128, 16, [1200], 9, 500, 16), (6, 2, 48, 16, [800, 90], 50, 100, 3),
+    (32, 8, 64, 16, [1500, 200], 200, 0, 0)])
+def test_prompts(hip, H, HK, D, page, lens, nq, window, sinks, dt):
+    """Many new tokens at once, windows that most of them do not share."""
+    rng = np.random.default_rng([H, D, nq, dt])
+    c = Cache(rng, dt, page, HK, D, D, lens)
+    q = rng.standard_normal((len(lens), nq, H, D)).astype(np.float32)
+    check(c.attend(q, 0.1, window, sinks), c.ref(q, 0.1, window, sinks), lens, nq)

@@ -18,14 +18,13 @@ SCHED = r"""
 using namespace aero;
 extern "C" {
 int tiles(long long lo, long long hi, long long n_kv, int window, int sinks, int shift, int* out,
-          int* place, int* column, int* upto, long long q) {
+          int* place, int* column) {
     const KeyTiles t = key_tiles(lo, hi, n_kv, window, sinks);
     for (int x = 0; x < t.n; ++x) {
         out[x] = t.at(x);
         place[x] = t.page_place(x, shift);
         column[x] = t.column(place[x], shift);
     }
-    *upto = t.upto(q);
     return t.n;
 }
 int units(int n, int u) { return item_units(n, u); }
@@ -45,17 +44,16 @@ def sched(tmp_path_factory):
                    check=True)
     L = ctypes.CDLL(str(so))
     i64, i32p = ctypes.c_int64, ctypes.POINTER(ctypes.c_int32)
-    L.tiles.argtypes = [i64, i64, i64, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [i32p] * 4 + [i64]
+    L.tiles.argtypes = [i64, i64, i64, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [i32p] * 3
     return L
 
 
 def test_key_tiles_are_those_of_the_seen_keys(sched):
     """Every tile with a key that some position sees is in the list, once and in
     order; tiles between the sinks and the window are not; page places have no
-    gaps and name the tile's own column; upto() cuts after a position's tile."""
+    gaps and name the tile's own column."""
     rng = random.Random(1)
     out, place, col = ((ctypes.c_int32 * 400)() for _ in range(3))
-    upto = ctypes.c_int32()
     for _ in range(4000):
         n_kv = rng.choice((1, 15, 16, 17, 33, 100, 640, rng.randint(1, 2000)))
         window = rng.choice((0, 0, 1, 7, 16, 64, rng.randint(1, 1500)))
@@ -63,8 +61,7 @@ def test_key_tiles_are_those_of_the_seen_keys(sched):
         lo = rng.randint(-3, n_kv + 5)
         hi = lo + rng.choice((0, 0, 1, 5, 40))
         shift = rng.choice((0, 1, 2, 4))
-        q = rng.randint(lo, hi)
-        n = sched.tiles(lo, hi, n_kv, window, sinks, shift, out, place, col, upto, q)
+        n = sched.tiles(lo, hi, n_kv, window, sinks, shift, out, place, col)
         got = list(out[:n])
         need = {j // 16 for p in range(lo, hi + 1) for j in range(min(p + 1, n_kv))
                 if not window or p - j < window or j < sinks}
@@ -76,7 +73,6 @@ def test_key_tiles_are_those_of_the_seen_keys(sched):
         assert list(col[:n]) == [t >> shift for t in got]
         if n:
             assert place[0] == 0 and all(b - a in (0, 1) for a, b in zip(place[:n], place[1:n]))
-        assert upto.value == sum(16 * t <= q for t in got)
 
 
 def test_chunks_cover_every_unit_once(sched):
