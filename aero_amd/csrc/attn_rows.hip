@@ -1226,9 +1226,10 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsParams p, int32_t ro
             A.x *= sc; A.y *= sc; A.z *= sc; A.w *= sc;
 #pragma unroll
             for (int x = 0; x < B; ++x) {
-                // (a part without keys holds zeros; a copy of the last is no part)
-                if (c0 + x * groups >= n || ml[x].x == -INFINITY) continue;
-                const float w = expf(ml[x].x - mb);
+                // (a copy of the last is no part; where all scores are NaN m is -inf too: a
+                // part without keys adds zeros, that one its NaN)
+                if (c0 + x * groups >= n) continue;
+                const float w = ml[x].x == -INFINITY ? 0.0f : expf(ml[x].x - mb);
                 L = __builtin_fmaf(ml[x].y, w, L);
                 A.x = __builtin_fmaf(a[x].x, w, A.x);
                 A.y = __builtin_fmaf(a[x].y, w, A.y);
