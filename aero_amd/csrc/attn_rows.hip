@@ -568,11 +568,18 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
 }
 
 // Integer caches on the fp16 matrix cores (v_mfma_f32_16x16x32_f16): the codes are
-// exact in fp16; q, scaled per query to below 2^15, and the probabilities times
-// the value scales, scaled by the largest value scale so far, go in two fp16 parts
-// (hi, lo = v - hi: 22 bits), so every product is exact and added in fp32. 32 keys
-// a step, scores in log2 units, sums rescaled only when a query's maximum passes
-// the reference by 2^8 or the scales' exponent moves (as attention.hip's kernel).
+// exact in fp16; q, scaled per query to below 2^15, and the weights (probability times
+// value scale) go in two fp16 parts (hi, lo = v - hi: 22 bits), so every product is
+// exact and added in fp32. 32 keys a step, scores in log2 units.
+//
+// A query's weights and sums are in units of 2^(e - 6), e the exponent of its own
+// largest weight so far: the parts' last bit, 2^-24, is 2^-29 of that one or less, and
+// large values of keys that the query does not keep, or that have no weight, cost it
+// nothing. The reference m is a whole number and moves up when a maximum passes it by
+// 8; e goes down with it (the sums stay as they are) and up where a weight passes
+// 2^(e + 9), 2^15 in these units: only then are the sums rescaled. (One exponent a wave
+// from the value scales alone: 0-2% faster, and rows of zeros where a neighbour's were
+// 2^32 times larger.)
 //
 // A step is about 290 vector and 32 matrix instructions for 8 KB of codes (dim 128):
 // a third of the vector units' time at the memory's rate. So as many waves a SIMD as
@@ -594,8 +601,8 @@ struct F16Core {
     Shared& sh;
     int g, c;
     Columns<SRC> col;
-    float m = -INFINITY, ls = 0.0f;
-    int e_acc = -1000;
+    float m = -INFINITY, ls = 0.0f;    // of query c
+    int e_acc = -120;
     v4f acc[VS];
     float qsl;
 
@@ -703,67 +710,49 @@ struct F16Core {
                 vs[x] = keep ? vs[x] : 0.0f;
             }
         }
-        float tm = sc[0], vmax = vs[0];
+        float tm = sc[0];
 #pragma unroll
-        for (int x = 1; x < 8; ++x) {
-            tm = fmaxf(tm, sc[x]);
-            vmax = fmaxf(vmax, vs[x]);
-        }
+        for (int x = 1; x < 8; ++x) tm = fmaxf(tm, sc[x]);
         tm = over_rows(tm, Max{});
-        vmax = over_rows(vmax, Max{});
-        if (!full) vmax = over_row(vmax, Max{});
-        int ev = 0;
-        if (vmax > 0.0f && vmax <= 3.4028235e38f) frexpf(vmax, &ev);
-        ev = __builtin_amdgcn_readfirstlane(ev);
-        int e_new = e_acc;
-        if (ev > e_acc) {
-            e_new = ev;
-        } else if (ev < e_acc - 8) {
-            // down to ev, as far as the sums stay below 2^100
-            float amax = 0.0f;
-#pragma unroll
-            for (int t = 0; t < VS; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) amax = fmaxf(amax, fabsf(acc[t][r]));
-            amax = over_rows(over_row(amax, Max{}), Max{});
-            int ea = -1000;
-            if (amax > 0.0f) frexpf(amax, &ea);
-            ea = __builtin_amdgcn_readfirstlane(ea);
-            e_new = max(ev, e_acc - (100 - ea));
-        }
-        e_new = min(max(e_new, -120), 128);   // 2^(6 - e) and 2^(e - 6) normal
-        if (__any(tm > m + 8.0f) || e_new != e_acc) {
-            const float mn = fmaxf(m, tm);
-            if (e_acc != -1000) {     // (before the first step all sums are zero)
-                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                ls = ls * alpha;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float ar = __shfl(alpha, 4 * g + r);
-#pragma unroll
-                    for (int t = 0; t < VS; ++t) acc[t][r] *= ar;
-                }
-                const int d = e_acc - e_new;
-                if (d != 0) {
-#pragma unroll
-                    for (int t = 0; t < VS; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[t][r] = ldexpf(acc[t][r], d);
-                }
-            }
-            m = mn;
-            e_acc = e_new;
-        }
-        const float msafe = m == -INFINITY ? 0.0f : m;
-        const float psc = pow2i(6 - e_acc);
-        h8 phi, plo;
-        float psum = 0.0f;
+        const bool up = __any(tm > m + 8.0f);
+        const float mn = up ? fmaxf(m, ceilf(tm)) : m;
+        const float msafe = mn == -INFINITY ? 0.0f : mn;
+        float pr[8], psum = 0.0f, wmax = 0.0f;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            const float pr = __builtin_amdgcn_exp2f(sc[x] - msafe);
-            psum += pr;
+            pr[x] = __builtin_amdgcn_exp2f(sc[x] - msafe);
+            psum += pr[x];
+            wmax = fmaxf(wmax, fabsf(pr[x] * vs[x]));
+        }
+        wmax = over_rows(wmax, Max{});
+        // the exponent of the step's largest weight (past fp32: below 2^136)
+        int ew = (int)(__builtin_bit_cast(uint32_t, wmax) >> 23) - 126;
+        ew = ew > 128 ? 136 : ew;
+        // (from -inf on, or past 2^-400, nothing of the sums is left)
+        const float rise = mn > m ? mn - m : 0.0f;
+        const int e_now = e_acc - (int)fminf(rise, 400.0f);
+        const int e_new = min(max(ew > e_now + 9 ? ew : e_now, -120), 128);
+        if (up) ls *= __builtin_amdgcn_exp2f(-rise);
+        if (__any(e_new != e_now)) {
+            const float f = ldexpf(1.0f, e_now - e_new);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float fr = __shfl(f, 4 * g + r);
+#pragma unroll
+                for (int t = 0; t < VS; ++t) acc[t][r] *= fr;
+            }
+        }
+        m = mn;
+        e_acc = e_new;
+        // (2^(6 - e) before or after the value scale, so that no product on the way
+        // leaves fp32)
+        const float psc = pow2i(6 - e_acc);
+        const float pa = e_acc > 0 ? psc : 1.0f, pb = e_acc > 0 ? 1.0f : psc;
+        h8 phi, plo;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
             _Float16 hi, lo;
-            split2(pr * vs[x] * psc, hi, lo);
+            split2(pr[x] * pa * vs[x] * pb, hi, lo);
             phi[x] = hi;
             plo[x] = lo;
         }
@@ -831,11 +820,12 @@ struct F16Core {
     }
 
     __device__ __forceinline__ void finish(int64_t row) {
-        const float back = e_acc < -120 ? 0.0f : pow2i(e_acc - 6);
 #pragma unroll
-        for (int t = 0; t < VS; ++t)
+        for (int r = 0; r < 4; ++r) {
+            const int e = __shfl(e_acc, 4 * g + r) - 6;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][r] *= back;
+            for (int t = 0; t < VS; ++t) acc[t][r] = ldexpf(acc[t][r], e);
+        }
         finish_tile<TL, D, PAD>(p, it, col.rows, m * kLn2, ls, acc, row, sh);
     }
 };
