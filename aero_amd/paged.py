@@ -22,6 +22,7 @@ moving each other.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import heapq
 
@@ -102,7 +103,12 @@ class PagedKV:
 
     One thread and one stream at a time: a page that is given up may be handed
     out again by the next call, which only the stream's order protects. The
-    methods change state by the call and are refused while a plan records."""
+    methods change state by the call and are refused while a plan records.
+
+    A method that raises has changed nothing here. Where it was a launch that
+    failed, the device arrays may hold part of the change until the next append,
+    fork, truncate, trim, free or compact that does not, which writes what they
+    should hold."""
 
     def __init__(self, pool: KvPool, max_seqs: int, max_pages: int):
         if max_seqs <= 0 or max_pages <= 0 or max_pages * pool.page > 1 << 30:
@@ -122,6 +128,7 @@ class PagedKV:
         self._live: set[int] = set()
         self._window: dict[int, int] = {}      # of the slots that trim has been at
         self._edits: dict[int, int] = {}
+        self._undo: list[tuple] = []           # (array, place, value) before a change
 
     # ------------------------------------------------------------ what there is
     @property
@@ -181,41 +188,46 @@ class PagedKV:
                     copies.append((s, old - 1, p))
                     need += 1
             more = -(-(have + n) // page) - old
-            news.append((s, old, more))
+            news.append((s, old, more, have + n))
             need += more
         if need > len(self._free):
             raise OutOfPages(f"append needs {need} pages, {len(self._free)} are free")
-        pairs = []
-        for s, col, p in copies:
-            new = self._take()
-            self._drop(p)
-            self._set(s * self.max_pages + col, new)
-            pairs.append((p, new))
-        for s, old, more in news:
-            for c in range(old, old + more):
-                self._set(s * self.max_pages + c, self._take())
-            self._set(self._lens_at(s), self.length(s) + n)
-        named = set(slots)
-        for s in range(self.max_seqs):
-            self._set(self._lens_at(s) + self.max_seqs, self.length(s) if s in named else 0)
-        if pairs:
-            ops.kv_pages_copy(self.pool, [a for a, _ in pairs], [b for _, b in pairs], stream)
-        self._flush(stream)
+        with self._change(stream):
+            pairs = []
+            for s, col, p in copies:
+                new = self._take()
+                self._drop(p)
+                self._set(s * self.max_pages + col, new)
+                pairs.append((p, new))
+            step = [0] * self.max_seqs
+            for s, old, more, length in news:
+                for c in range(old, old + more):
+                    self._set(s * self.max_pages + c, self._take())
+                self._set(self._lens_at(s), length)
+                step[s] = length
+            for s, length in enumerate(step, self._lens_at(self.max_seqs)):
+                self._set(s, length)
+            if pairs:
+                ops.kv_pages_copy(self.pool, [a for a, _ in pairs], [b for _, b in pairs], stream)
 
     def fork(self, slot: int, stream: Stream | None = None) -> int:
         """A new slot with the same tokens, in the same pages."""
         s = self._slot(slot)
         d = self.add()
         row, n = self._row(s), self.length(s)
-        for c in range(-(-n // self.pool.page)):
-            p = int(row[c])
-            if p >= 0:
-                self._refs[p] += 1
-            self._set(d * self.max_pages + c, p)
+        try:
+            with self._change(stream):
+                for c in range(-(-n // self.pool.page)):
+                    p = int(row[c])
+                    if p >= 0:
+                        self._ref(p, 1)
+                    self._set(d * self.max_pages + c, p)
+                self._set(self._lens_at(d), n)
+        except BaseException:
+            self._live.discard(d)
+            raise
         if s in self._window:
             self._window[d] = self._window[s]
-        self._set(self._lens_at(d), n)
-        self._flush(stream)
         return d
 
     def truncate(self, slot: int, n: int, stream: Stream | None = None) -> None:
@@ -231,11 +243,11 @@ class PagedKV:
         seen = self._row(s)[max(0, n - self._window.get(s, n)) // page: -(-n // page)]
         if (seen < 0).any():
             raise ValueError(f"slot {s}: pages that token {n - 1} sees were given up by trim")
-        for c in range(-(-n // page), -(-have // page)):
-            self._clear(s, c)
-        self._set(self._lens_at(s), n)
-        self._set(self._lens_at(s) + self.max_seqs, 0)
-        self._flush(stream)
+        with self._change(stream):
+            for c in range(-(-n // page), -(-have // page)):
+                self._clear(s, c)
+            self._set(self._lens_at(s), n)
+            self._set(self._lens_at(s) + self.max_seqs, 0)
 
     def trim(self, slot: int, window: int, sinks: int = 0, stream: Stream | None = None) -> int:
         """Give up the pages that neither the newest token nor a later one sees
@@ -244,13 +256,13 @@ class PagedKV:
         s = self._slot(slot)
         if window <= 0 or sinks < 0:
             raise ValueError(f"trim: window {window}, sinks {sinks}")
-        self._window[s] = int(window)
         page, gone = self.pool.page, 0
-        for c in range(-(-sinks // page), max(0, self.length(s) - window) // page):
-            if self._row(s)[c] >= 0:
-                self._clear(s, c)
-                gone += 1
-        self._flush(stream)
+        with self._change(stream):
+            for c in range(-(-sinks // page), max(0, self.length(s) - window) // page):
+                if self._row(s)[c] >= 0:
+                    self._clear(s, c)
+                    gone += 1
+        self._window[s] = int(window)
         return gone
 
     def free(self, slot: int, stream: Stream | None = None) -> None:
@@ -266,20 +278,20 @@ class PagedKV:
         used = self.used_pages
         holes = [p for p in sorted(self._free) if p < used]
         tail = [p for p in range(used, self.pool.n_pages) if self._refs[p] > 0]
-        if not tail:
-            return 0
         to = dict(zip(tail, holes))
-        ops.kv_pages_copy(self.pool, tail, holes, stream)
-        for a, b in to.items():
-            self._refs[b], self._refs[a] = self._refs[a], 0
-        self._free = list(range(used, self.pool.n_pages))
-        for s in self._live:
-            row = self._row(s)
-            for c in range(-(-self.length(s) // self.pool.page)):
-                p = int(row[c])
-                if p in to:
-                    self._set(s * self.max_pages + c, to[p])
-        self._flush(stream)
+        with self._change(stream):
+            if tail:
+                ops.kv_pages_copy(self.pool, tail, holes, stream)
+            for a, b in to.items():
+                self._ref(b, int(self._refs[a]))
+                self._ref(a, -int(self._refs[a]))
+            self._free = list(range(used, self.pool.n_pages))
+            for s in self._live:
+                row = self._row(s)
+                for c in range(-(-self.length(s) // self.pool.page)):
+                    p = int(row[c])
+                    if p in to:
+                        self._set(s * self.max_pages + c, to[p])
         return len(tail)
 
     # ------------------------------------------------------------------ helpers
@@ -299,13 +311,37 @@ class PagedKV:
     def _row(self, s: int) -> np.ndarray:
         return self._host[s * self.max_pages: (s + 1) * self.max_pages]
 
+    @contextlib.contextmanager
+    def _change(self, stream: Stream | None):
+        """A change of tables, lengths and pages, written to the device at its end;
+        taken back where something raises (its edits, of which the device may have
+        some, then become those that write the old values)."""
+        try:
+            yield
+            if self._edits:
+                ops.write_i32(self._dev, sorted(self._edits.items()), stream)
+        except BaseException:
+            for a, at, value in reversed(self._undo):
+                a[at] = value
+            self._free = np.flatnonzero(self._refs == 0).tolist()   # (ascending: a heap)
+            self._edits = {at: int(self._host[at]) for at in self._edits}
+            raise
+        else:
+            self._edits.clear()
+        finally:
+            self._undo.clear()
+
+    def _ref(self, p: int, by: int) -> None:
+        self._undo.append((self._refs, p, int(self._refs[p])))
+        self._refs[p] += by
+
     def _take(self) -> int:
         p = heapq.heappop(self._free)
-        self._refs[p] = 1
+        self._ref(p, 1)
         return p
 
     def _drop(self, p: int) -> None:
-        self._refs[p] -= 1
+        self._ref(p, -1)
         if self._refs[p] == 0:
             heapq.heappush(self._free, p)
 
@@ -317,10 +353,6 @@ class PagedKV:
 
     def _set(self, at: int, value: int) -> None:
         if self._host[at] != value:
+            self._undo.append((self._host, at, int(self._host[at])))
             self._host[at] = value
             self._edits[at] = value
-
-    def _flush(self, stream: Stream | None) -> None:
-        if self._edits:
-            ops.write_i32(self._dev, sorted(self._edits.items()), stream)
-            self._edits.clear()

@@ -283,6 +283,94 @@ def test_paged_kv_refusals(monkeypatch):
         kv.compact()
 
 
+def held(kv):
+    """What a PagedKV says it holds."""
+    return (kv.free_pages, {s: (kv.length(s), kv.pages(s)) for s in range(kv.max_seqs)
+                            if s in kv._live})
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_launch_that_fails_changes_nothing(monkeypatch, seed):
+    """Page copies and table writes that fail, the latter after part of their
+    entries: the call raises, all is as before it, and the next call that succeeds
+    leaves on the device what it should hold, no sequence's tokens lost."""
+    rng = random.Random(seed)
+    pool = fake_pool()
+    m = Model(monkeypatch, pool, 5, 12)
+    kv = paged.PagedKV(pool, 5, 12)
+    truth, name, failed = {}, 0, 0
+    fail = {"copy": False, "edit": False}
+
+    def copy(pool, src, dst, stream=None):
+        if fail["copy"]:
+            raise _lib.AeroHipError("kv_pages_copy")
+        m.copy(pool, src, dst)
+
+    def edit(a, items, stream=None):
+        if fail["edit"]:
+            m.edit(a, items[:rng.randint(0, len(items))])
+            raise _lib.AeroHipError("write_i32")
+        m.edit(a, items)
+
+    monkeypatch.setattr(ops, "kv_pages_copy", copy)
+    monkeypatch.setattr(ops, "write_i32", edit)
+    for step in range(500):
+        fail["copy"], fail["edit"] = rng.random() < 0.3, rng.random() < 0.2
+        what = rng.choice(("add", "append", "append", "append", "fork", "trim", "cut", "free",
+                           "compact"))
+        if what == "add":
+            if len(truth) < 5:
+                truth[kv.add()] = []
+            continue
+        if what != "compact" and not truth:
+            continue
+        s = rng.choice(sorted(truth)) if truth else None
+        before = held(kv)
+        try:
+            if what == "append":
+                slots, n = rng.sample(sorted(truth), rng.randint(1, len(truth))), rng.choice((1, 9, 20))
+                kv.append(slots, n)
+                for t in slots:
+                    for _ in range(n):
+                        m.write(t, len(truth[t]), name)
+                        truth[t].append(name)
+                        name += 1
+            elif what == "fork":
+                d = kv.fork(s)
+                truth[d] = list(truth[s])
+            elif what == "trim":        # (no window is longer than this one)
+                kv.trim(s, 150, 16)
+                gone = max(0, len(truth[s]) - 150) // 16 * 16
+                truth[s][16:gone] = [None] * max(0, gone - 16)
+            elif what == "cut":
+                n = rng.randint(max(0, len(truth[s]) - 5), len(truth[s]))
+                kv.truncate(s, n)
+                del truth[s][n:]
+            elif what == "free":
+                kv.free(s)
+                del truth[s]
+            else:
+                kv.compact()
+        except _lib.AeroHipError:
+            failed += 1
+            assert held(kv) == before, (step, what)
+            continue
+        except (paged.OutOfPages, ValueError):
+            assert held(kv) == before
+            continue
+        assert np.array_equal(m.dev, kv._host), (step, what)
+        for t in range(5):
+            row = kv.pages(t) if t in truth else []
+            assert m.dev[t * 12:(t + 1) * 12].tolist() == row + [-1] * (12 - len(row)), (step, what)
+            assert m.dev[m.n + t] == len(truth.get(t, []))
+        for t, want in truth.items():
+            for i, x in enumerate(want):
+                assert x is None or m.token(t, i) == x, (step, what, t, i)
+        used = {p for t in truth for p in kv.pages(t) if p >= 0}
+        assert kv.used_pages == len(used)
+    assert failed > 20          # (the run did meet failures)
+
+
 # ------------------------------------------------------------------- refusals
 def c_pool(**k):
     d = dict(kv_dt=1, page=16, n_layers=2, n_pages=8, n_head_kv=2, head_dim=64, value_dim=64,
