@@ -1478,6 +1478,8 @@ PromptPlan prompt_plan(int kv_dt, int64_t n_q, int64_t n_head, int64_t n_head_kv
     pl.record = pl.image + n_head_kv * pl.cap * 256 * head_dim;
     pl.channel = pl.record + n_head_kv * pl.cap * (int64_t)sizeof(PromptTile);
     pl.bytes = pl.channel + n_head_kv * pl.cap * head_dim * 4;
+    // (the images are as large as the K and V rows in reach: 0.56 GB for 8 heads of 128
+    // and 65,536 keys)
     if (pl.bytes > (int64_t(4) << 30)) return pl;
     pl.vecs = 32 * waves / gk;
     if ((n_vec + pl.vecs - 1) / pl.vecs > 65535) return pl;

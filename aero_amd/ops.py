@@ -587,8 +587,11 @@ def attention(q: DeviceArray, k: DeviceArray, v: DeviceArray, out: DeviceArray, 
     (src/transformer.cpp:120-214): q [n_q, n_head, head_dim] -> out
     [n_q, n_head, value_dim]; K / V [n_kv, n_head_kv, dim] in kv_dt. A query at
     position qp keeps keys at positions kp <= qp with qp - kp < window (0: all)
-    or kp < sinks. The decode split's workspace is allocated once per size and
-    reused."""
+    or kp < sinks. The workspace grows to the largest call and is kept: calls that
+    overlap on different streams would share its contents. With sinks it is the
+    one of paged_attention, and a prompt over an fp32 cache takes as much of it as
+    the keys and values in reach of its tokens (window + n_q + sinks keys; not
+    above 4 GiB, beyond which, and for few tokens, slower kernels need a few MB)."""
     _need(q, n_q * n_head * head_dim, np.float32, "q")
     _need(out, n_q * n_head * value_dim, np.float32, "out")
     _need(qpos, n_q, np.int32, "qpos")
@@ -675,9 +678,10 @@ def paged_attention(pool, layer: int, q: DeviceArray, out: DeviceArray, table: D
     value_dim], table and lens as paged_kv_write, the mask as attention with
     window and sinks. Rows without a token, or that see nothing, become zeros;
     keys of a page id outside the pool are not seen, and bad[0] becomes 1 (as for
-    a length past the table's room, which is cut to it). The launch does not depend on the lengths, so a plan that recorded it stays
-    right as the sequences grow. The workspace is allocated once per size and
-    reused: calls on different streams must not overlap."""
+    a length past the table's room, which is cut to it). The launch does not
+    depend on the lengths, so a plan that recorded it stays right as the sequences
+    grow. The workspace grows to the largest call and is kept; attention with
+    sinks has the same one: such calls on different streams must not overlap."""
     max_pages = _paged(pool, table, lens, n_seq, bad)
     rows = n_seq * n_q * n_head
     _need(q, rows * pool.head_dim, np.float32, "q")

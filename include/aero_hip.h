@@ -620,7 +620,12 @@ int aero_hip_softmax_rows(const float* x, float* y, int64_t n_rows, int64_t n_co
  * sinks 0 it is aero_hip_attention's call. A cache that keeps the sinks and a
  * ring of the window passes the positions of its slots in kpos. n_kv below
  * 2^30. Workspace: aero_hip_attention_sinks_workspace bytes (-1: bad sizes),
- * 16-byte aligned. No counterpart in the reference. */
+ * 16-byte aligned, its contents free between calls; calls that share it must be
+ * ordered. A prompt over an fp32 cache (128 workgroups of its queries and more)
+ * keeps its keys and values there as matrix operands: as many bytes as the K and V
+ * rows in reach, min(n_kv, window + n_q + sinks), at most 4 GiB, beyond which it
+ * runs on the kernels of the other calls, which need a few MB. No counterpart in
+ * the reference. */
 int64_t aero_hip_attention_sinks_workspace(int kv_dt, int64_t n_q, int64_t n_head,
                                            int64_t n_head_kv, int64_t head_dim,
                                            int64_t value_dim, int64_t n_kv, int window,
