@@ -232,8 +232,8 @@ class PagedKV:
 
     def truncate(self, slot: int, n: int, stream: Stream | None = None) -> None:
         """Keep the slot's first n tokens (a rejected guess, a shorter prompt).
-        Refused where trim has given up a page that the newest of them sees: trim
-        with a window that is longer by what may be taken back."""
+        Refused where trim has given up a page in the last trim's window of the
+        newest of them: trim with a window that is longer by what may be taken back."""
         self._check()
         s = self._slot(slot)
         have = self.length(s)
@@ -251,7 +251,9 @@ class PagedKV:
 
     def trim(self, slot: int, window: int, sinks: int = 0, stream: Stream | None = None) -> int:
         """Give up the pages that neither the newest token nor a later one sees
-        under `window` and `sinks`; the number given up."""
+        under `window` and `sinks`; the number given up. What one call gives up stays
+        so: a later call with more sinks or a longer window does not bring it back
+        (pages() has -1 there, attention does not see those keys and sets its `bad`)."""
         self._check()
         s = self._slot(slot)
         if window <= 0 or sinks < 0:

@@ -259,6 +259,24 @@ def test_truncate_after_trim(monkeypatch):
     kv.truncate(a, 1)
 
 
+def test_trim_with_more_sinks_later(monkeypatch):
+    """First tokens that a trim without sinks gave up stay given up, and show as such;
+    the window decides what may be cut back."""
+    pool = fake_pool()
+    Model(monkeypatch, pool, 2, 12)
+    kv = paged.PagedKV(pool, 2, 12)
+    a = kv.add()
+    kv.append([a], 100)
+    assert kv.trim(a, 40) == 3 and kv.pages(a)[:3] == [-1] * 3
+    assert kv.trim(a, 40, 16) == 0 and kv.pages(a)[:3] == [-1] * 3
+    kv.append([a], 30)
+    assert kv.trim(a, 40, 16) == 2 and kv.pages(a)[:5] == [-1] * 5
+    kv.truncate(a, 120)
+    with pytest.raises(ValueError):
+        kv.truncate(a, 119)
+    assert kv.pages(a)[0] == -1
+
+
 def test_paged_kv_refusals(monkeypatch):
     pool = fake_pool(n_pages=4)
     m = Model(monkeypatch, pool, 2, 3)
