@@ -573,6 +573,13 @@ def kv_write(dt: int, x: DeviceArray, n_tok: int, heads: int, dim: int, q: Devic
                                             as_ptr(scale), _s(stream)), "kv_write")
 
 
+def _int32(value, name: str) -> int:
+    v = int(value)
+    if not -2**31 <= v < 2**31:
+        raise ValueError(f"{name}: {value} is past 32 bits")
+    return v
+
+
 _attn_ws = Workspace("attention chunk partials")
 _rows_ws = Workspace("attention row parts")
 
@@ -605,16 +612,18 @@ def attention(q: DeviceArray, k: DeviceArray, v: DeviceArray, out: DeviceArray, 
             raise ValueError("K / V cache too small")
         _need(k_scale, n_kv * n_head_kv, np.float32, "k_scale")
         _need(v_scale, n_kv * n_head_kv, np.float32, "v_scale")
+    if sinks != 0:
+        window, sinks = _int32(window, "window"), _int32(sinks, "sinks")
     L = _lib.lib()
     if sinks != 0:
-        sizes = (n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, int(window), int(sinks))
+        sizes = (n_q, n_head, n_head_kv, head_dim, value_dim, n_kv, window, sinks)
         wsb = int(L.aero_hip_attention_sinks_workspace(kv_dt, *sizes))
         _lib.check(wsb >= 0, "attention")
         ws = _rows_ws.get(wsb)
         _lib.check(L.aero_hip_attention_sinks(
             q.ptr, kv_dt, k.ptr, as_ptr(k_scale), v.ptr, as_ptr(v_scale), out.ptr, n_q, n_head,
             n_head_kv, head_dim, value_dim, float(scale), as_ptr(qpos), as_ptr(kpos), n_kv,
-            int(window), int(sinks), as_ptr(ws), ws.nbytes if ws is not None else 0, _s(stream)),
+            window, sinks, as_ptr(ws), ws.nbytes if ws is not None else 0, _s(stream)),
             "attention")
         return
     wsb = int(L.aero_hip_attention_workspace(n_q, n_head, n_head_kv, head_dim, value_dim, n_kv))
@@ -686,13 +695,14 @@ def paged_attention(pool, layer: int, q: DeviceArray, out: DeviceArray, table: D
     rows = n_seq * n_q * n_head
     _need(q, rows * pool.head_dim, np.float32, "q")
     _need(out, rows * pool.value_dim, np.float32, "out")
+    window, sinks = _int32(window, "window"), _int32(sinks, "sinks")
     L = _lib.lib()
     wsb = int(L.aero_hip_paged_attention_workspace(pool.ref, n_seq, n_q, n_head, max_pages))
     _lib.check(wsb >= 0, "paged_attention")
     ws = _rows_ws.get(wsb)
     _lib.check(L.aero_hip_paged_attention(
         pool.ref, layer, q.ptr, out.ptr, table.ptr, max_pages, lens.ptr, n_seq, n_q, n_head,
-        float(scale), int(window), int(sinks), as_ptr(bad), as_ptr(ws),
+        float(scale), window, sinks, as_ptr(bad), as_ptr(ws),
         ws.nbytes if ws is not None else 0, _s(stream)), "paged_attention")
 
 

@@ -501,3 +501,16 @@ def test_op_wrappers_check_on_the_host():
                                    n_pages=40, page=16, n_head_kv=2, head_dim=64), **k})
     with pytest.raises(ValueError):
         paged.KvPool(1, fake(40960, np.uint8), fake(40960, np.uint8), 20, 16, 2, 64)
+
+
+@pytest.mark.parametrize("k", [dict(window=1 << 32), dict(window=(1 << 32) + 5),
+                               dict(window=1 << 31), dict(window=64, sinks=1 << 32),
+                               dict(window=64, sinks=(1 << 32) + 4)], ids=str)
+def test_windows_past_32_bits_are_refused(k):
+    """A C int would take their low 32 bits: another window, or none."""
+    pool = fake_pool(dt=ops.KV_INT8)
+    t, n, q = fake((4, 5), np.int32), fake(4, np.int32), fake((4, 1, 4, 64))
+    with pytest.raises(ValueError):
+        ops.paged_attention(pool, 0, q, q, t, n, 4, 4, 1.0, **k)
+    with pytest.raises(ValueError):
+        ops.attention(q, q, q, q, 1, 4, 2, 64, 64, 4, 1.0, **{"sinks": 4, **k})
