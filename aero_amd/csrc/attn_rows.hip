@@ -22,11 +22,11 @@
 // Page ids are checked against the pool: tiles of a bad page are not seen.
 //
 // What bounds it (MI355X; 8 kv heads of 128, 4 query heads each): reading the cache.
-// 4 fp32 sequences of up to 50,001 tokens, 887 MB: 159 us, 5.6 TB/s (a copy reaches
-// 4.65). 48 int8 ones of up to 8,192, 282 MB: 70 us, the walk 57 of it at 5.0 TB/s
-// (5 us until the first loads are in, as long again at the end), the join 6. Few keys:
-// memory round trips one after another (length, page ids, keys), about 1 us each, and
-// 1 us for the four waves' sums to meet: 333 tokens 7.5 us, one launch.
+// 4 fp32 sequences of up to 50,001 tokens, 887 MB: 159 us, 5.6 TB/s (a large copy reaches
+// 4.65, reads alone 6.25). 48 int8 ones of up to 8,192, 282 MB: 70 us, the walk 58 of it
+// at 4.9 TB/s (5 us until the first loads are in, as long again at the end), the join 6.
+// Few keys: memory round trips one after another (length, page ids, keys), about 1 us
+// each, and 1 us for the four waves' sums to meet: 333 tokens 7.5 us, one launch.
 #include "attn_common.hpp"
 #include "paged_sched.hpp"
 #include "paged.hpp"
@@ -581,12 +581,12 @@ __device__ __forceinline__ void finish_tile(const RowsParams& p, const Item& it,
 // from the value scales alone: 0-2% faster, and rows of zeros where a neighbour's were
 // 2^32 times larger.)
 //
-// A step is about 290 vector and 32 matrix instructions for 8 KB of codes (dim 128):
+// A step is about 340 vector and 32 matrix instructions for 8 KB of codes (dim 128):
 // a third of the vector units' time at the memory's rate. So as many waves a SIMD as
 // the registers allow without spilling (EU 3; 2 at dim 256), each with the next step's
 // codes on their way: 96 KB a CU. 64 sequences in a window of 1,024, 4 kv heads of
-// 256, 3 tokens each: 102 MB in 27 us (3.8 TB/s; 22 B/ns a CU, all that the memory
-// gives, but for 5 us at the start).
+// 256, 3 tokens each: 102 MB in 27 us (3.8 TB/s; 22 B/ns a CU, of the 24 of reads
+// alone, but for 5 us at the start).
 template <int DT, int D, Source SRC, bool PAD = false>
 struct F16Core {
     static constexpr int VEC = 16;
@@ -1328,8 +1328,15 @@ RowsVariant pick_variant(int dt, int64_t head_dim, int64_t value_dim, bool align
 // Items of no more keys than this (whole units) are not cut: a unit more takes a
 // workgroup less than the parts and their join do. One sequence of 333 int8 tokens,
 // two kv heads of dim 64: cut 11.9 us, whole 8.5. More where the items fill half of
-// the chip: 64 sequences in a window of 1024, four kv heads of dim 256, 3 tokens each,
-// int8 38.3 / 29.0, fp32 100 / 80.9; in a window of 4096 cutting is as good.
+// the chip. 64 sequences, cut / whole, us, int8 and fp32:
+//   4 kv heads of 256, 3 tokens, window 1024 36.4 / 26.9, 103 / 83.0; 1984 47.6 / 43.1,
+//     147 / 135; 4096 77.0 / 78.3, 246 / 250
+//   8 of 128, one token, window 1024 35.5 / 26.4, 86.7 / 80.9; 1984 47.8 / 45.6, 131 /
+//     135; 4096 76.9 / 83.5, 223 / 253
+//   8 of 128, ragged up to 1024 27.1 / 18.7, 49.4 / 52.2; 2048 36.1 / 30.9, 80.8 / 95.7
+//   4 of 256, ragged up to 1024 26.1 / 22.6, 60.3 / 61.5; 2048 32.5 / 37.6, 92.6 / 112
+// So it holds for items of a length (a window's) and for most int8 batches; ragged fp32
+// ones of up to 2176 tokens lose up to a fifth, the balance that cutting gives.
 constexpr int kWholeKeys = 512, kWholeKeysMany = 2176;
 // (a launch has fewer than 2^32 threads in a row of its grid, 256 a workgroup)
 constexpr int64_t kMostWgs = (1 << 24) - 1;
@@ -1353,8 +1360,10 @@ bool join(const RowsVariant& k, int64_t items, const RowsParams& p, hipStream_t 
     while (groups < p.parts / items && 2 * groups * lpr <= 256) groups *= 2;
     const int per = 256 / (lpr * groups);
     const int64_t grid = items * ((rows + per - 1) / per);    // (at most 16 an item)
-    // (2 or 8 parts of a group in flight: 48 sequences, 8 parts an item in 8 groups 69.9 /
-    // 72.6 us in all; one token over a ring, 33 parts in 4 groups 17.1 / 15.4)
+    // (2 or 8 parts of a group in flight, us in all: 48 sequences of up to 8,192, 8 parts
+    // an item in 8 groups 69.9 / 72.6, at dim 64 21.2 / 21.8, and within 1% at dim 256.
+    // One token over a ring of 2,052, dim 256, 33 parts in 4 groups 17.1 / 15.4; over
+    // 8,192 keys, int8 dim 256 19.5 / 15.7, fp32 dim 64 13.8 / 11.9)
     const bool many = p.parts / items > 2 * groups;
     return launch("rows_join_kernel",
                   k.vec == 4 ? (many ? rows_join_kernel<4, 8> : rows_join_kernel<4, 2>)

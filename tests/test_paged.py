@@ -346,7 +346,8 @@ def test_a_launch_that_fails_changes_nothing(monkeypatch, seed):
         before = held(kv)
         try:
             if what == "append":
-                slots, n = rng.sample(sorted(truth), rng.randint(1, len(truth))), rng.choice((1, 9, 20))
+                slots = rng.sample(sorted(truth), rng.randint(1, len(truth)))
+                n = rng.choice((1, 9, 20))
                 kv.append(slots, n)
                 for t in slots:
                     for _ in range(n):
