@@ -210,6 +210,15 @@ PROTOTYPES = {
                                        c_int64, c_int64, vp, vp]),
     "aero_hip_kv_pages_copy": (c_int, [POINTER(KvPool), vp, vp, c_int64, vp]),
     "aero_hip_write_i32": (c_int, [vp, c_int64, POINTER(c_int64), ip, c_int64, vp]),
+    "aero_hip_mx_quantize": (c_int, [c_int, vp, c_int64, vp, vp, c_int64, c_int64, vp]),
+    "aero_hip_mx_dequant": (c_int, [c_int, vp, vp, vp, c_int64, c_int64, vp]),
+    "aero_hip_rmsnorm_mx": (c_int, [c_int] + [vp] * 6 + [c_int64, c_int64, c_float, c_int, vp]),
+    "aero_hip_act_mul_mx": (c_int, [c_int, c_int, vp, vp, c_int64, vp, vp, c_int64, c_int64, vp]),
+    "aero_hip_mx_weight_bytes": (c_int64, [c_int64, c_int64]),
+    "aero_hip_mx_pack": (c_int, [vp, vp, vp, c_int64, c_int64, c_int64, vp]),
+    "aero_hip_mx_matmul_workspace": (c_int64, [c_int, c_int64, c_int64, c_int64]),
+    "aero_hip_mx_matmul": (c_int, [c_int, vp, vp, vp, c_int64, vp, c_int64, c_int64, c_int64, vp,
+                                   c_int64, vp]),
     "aero_hip_kv_write": (c_int, [c_int, vp, c_int64, c_int64, c_int64, c_int64, c_int64, vp,
                                   vp, vp]),
     "aero_hip_softmax_rows": (c_int, [vp, vp, c_int64, c_int64, vp]),

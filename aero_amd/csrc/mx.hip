@@ -1,0 +1,394 @@
+// Microscaled rows (mx.hpp) from fp32: plain quantisation, RMSNorm with the residual's
+// addition, act(gate) * up, each in one pass that reads its inputs once and writes codes
+// and scales; and the way back.
+//
+// Norms and activations are evaluated in 64 bits and rounded to fp32 once before they are
+// quantised. A code is a decision, and next to the border of two an error of the last bit
+// of 32 turns it: in 64 bits the codes are those of the formula and do not depend on the
+// order of a sum. The arithmetic hides behind the memory: 16384 x 8192 with a residual moves
+// 13 bytes a value, for which the card has about 30 instructions a lane.
+#include "act_ops.hpp"
+#include "mx.hpp"
+
+#pragma clang fp contract(off)
+
+namespace aero {
+namespace {
+
+constexpr int64_t kMaxBlocks = 0x7fffffff;
+
+__device__ __forceinline__ float4 ld4(const float* p, bool vec) {
+    if (vec) return ld_stream(p);
+    return make_float4(p[0], p[1], p[2], p[3]);
+}
+
+// ------------------------------------------------------------- activations
+// act(v) in 64 bits; gelu with the erf polynomial of act_ops.hpp, in a form that does not
+// cancel on the negative side; gelu_tanh by 1 + tanh(z) = 2 / (1 + exp(-2z)).
+template <int KIND>
+__device__ __forceinline__ double act64(double v) {
+    if constexpr (KIND == AERO_ACT_SILU) {
+        return v / (1.0 + exp(-v));
+    } else if constexpr (KIND == AERO_ACT_SIGMOID) {
+        return 1.0 / (1.0 + exp(-v));
+    } else if constexpr (KIND == AERO_ACT_GELU_TANH) {
+        return v / (1.0 + exp(-2.0 * 0.7978845608028654 * (v + 0.044715 * v * v * v)));
+    } else if constexpr (KIND == AERO_ACT_GELU) {
+        const double a = fabs(v * 0.7071067811865476);
+        const double t = 1.0 / (1.0 + 0.3275911 * a);
+        const double p = ((((1.061405429 * t - 1.453152027) * t + 1.421413741) * t
+                           - 0.284496736) * t + 0.254829592) * t * exp(-a * a);
+        return 0.5 * v * (v < 0.0 ? p : 2.0 - p);
+    } else {
+        return v;
+    }
+}
+
+constexpr int kNone = -1;  // no activation, no second input: plain quantisation
+
+// Quad i of rows of nq quads, input rows ld floats apart; 8 consecutive lanes hold a block.
+template <int FMT, int KIND, bool UP>
+__global__ __launch_bounds__(256)
+void mx_rows_kernel(const float* g, const float* u, uint8_t* codes, uint8_t* scales, uint32_t n,
+                    uint32_t nq, int64_t ld, bool vec) {
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= n) return;
+    const uint32_t row = i / nq;
+    const int64_t at = row * ld + 4 * (int64_t)(i - row * nq);
+    float4 h = ld4(g + at, vec);
+    if constexpr (KIND != kNone) {
+        const float4 b = UP ? ld4(u + at, vec) : make_float4(1.f, 1.f, 1.f, 1.f);
+        auto one = [](float x, float y) {
+            const double a = act64<KIND>((double)x);
+            return (float)(UP ? a * (double)y : a);
+        };
+        h = make_float4(one(h.x, b.x), one(h.y, b.y), one(h.z, b.z), one(h.w, b.w));
+    }
+    mx_store<FMT>(h, i, codes, scales);
+}
+
+template <int FMT, int KIND, bool UP>
+bool run_rows(const char* name, const float* g, const float* u, uint8_t* codes, uint8_t* scales,
+              int64_t rows, int64_t cols, int64_t ld, hipStream_t s) {
+    const bool vec = aligned16(g) && (!UP || aligned16(u)) && ld % 4 == 0;
+    const int64_t nq = cols / 4;
+    const int64_t per = (int64_t)1 << 31;             // quads a launch: indices of 32 bits
+    const int64_t step = nq >= per ? 1 : per / nq;
+    for (int64_t r = 0; r < rows; r += step) {
+        const int64_t n = (rows - r < step ? rows - r : step) * nq;
+        if (!launch(name, mx_rows_kernel<FMT, KIND, UP>, dim3((unsigned)((n + 255) / 256)),
+                    dim3(256), 0, s, g + r * ld, UP ? u + r * ld : u,
+                    codes + r * mx_row_bytes(FMT, cols), scales + r * (cols / 32), (uint32_t)n,
+                    (uint32_t)nq, ld, vec))
+            return false;
+    }
+    return true;
+}
+
+template <int FMT>
+bool run_act(int kind, const float* g, const float* u, uint8_t* codes, uint8_t* scales,
+             int64_t rows, int64_t cols, int64_t ld, hipStream_t s) {
+#define AERO_MX_ACT(K)                                                                       \
+    case K:                                                                                  \
+        return u ? run_rows<FMT, K, true>("mx_act_kernel", g, u, codes, scales, rows, cols, ld, s) \
+                 : run_rows<FMT, K, false>("mx_act_kernel", g, u, codes, scales, rows, cols, ld, s)
+    switch (kind) {
+    AERO_MX_ACT(AERO_ACT_SILU);
+    AERO_MX_ACT(AERO_ACT_GELU);
+    AERO_MX_ACT(AERO_ACT_GELU_TANH);
+    AERO_MX_ACT(AERO_ACT_SIGMOID);
+    AERO_MX_ACT(AERO_ACT_IDENTITY);
+    default:
+        set_error("act_mul_mx: unknown kind %d", kind);
+        return false;
+    }
+#undef AERO_MX_ACT
+}
+
+// ------------------------------------------------------------------- norm
+struct MxNorm {
+    const float* x;
+    const float* d;      // residual input, or null
+    float* xo;           // x + d
+    const float* w;      // or null (ones)
+    uint8_t* codes;
+    uint8_t* scales;
+    int64_t cols;
+    float eps;
+    int flags;
+    bool vec;
+};
+
+// Sum over a workgroup of BS lanes, the same bits in every lane.
+template <int BS>
+__device__ __forceinline__ double mx_sum(double v) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    if constexpr (BS > 64) {
+        __shared__ double part[BS / 64];
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int k = 1; k < BS / 64; ++k) v += part[k];
+    }
+    return v;
+}
+
+__device__ __forceinline__ double sq4(float4 v) {
+    return (double)v.x * v.x + (double)v.y * v.y + ((double)v.z * v.z + (double)v.w * v.w);
+}
+
+__device__ __forceinline__ float4 add4(float4 a, float4 b) {
+    return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+
+__device__ __forceinline__ float4 scaled4(float4 v, double inv, const MxNorm& p, int64_t c) {
+    double w[4] = {1.0, 1.0, 1.0, 1.0};
+    if (p.w != nullptr) {
+        const float4 f = p.vec ? *reinterpret_cast<const float4*>(p.w + 4 * c)
+                               : make_float4(p.w[4 * c], p.w[4 * c + 1], p.w[4 * c + 2], p.w[4 * c + 3]);
+        const double one = (p.flags & AERO_NORM_UNIT_OFFSET) ? 1.0 : 0.0;
+        w[0] = f.x + one; w[1] = f.y + one; w[2] = f.z + one; w[3] = f.w + one;
+    }
+    return make_float4((float)(v.x * inv * w[0]), (float)(v.y * inv * w[1]),
+                       (float)(v.z * inv * w[2]), (float)(v.w * inv * w[3]));
+}
+
+// A row a workgroup, V quads of it in each lane's registers; V = 0: rows of any length,
+// read twice.
+template <int FMT, int BS, int V>
+__global__ __launch_bounds__(BS)
+void mx_norm_kernel(MxNorm p) {
+    const int64_t row = blockIdx.x, nq = p.cols / 4, base = row * p.cols;
+    const int t = threadIdx.x;
+    auto quad = [&](int64_t c) {
+        float4 v = ld4(p.x + base + 4 * c, p.vec);
+        if (p.d != nullptr) v = add4(v, ld4(p.d + base + 4 * c, p.vec));
+        return v;
+    };
+    auto put = [&](int64_t c, float4 v) {
+        if (p.d == nullptr) return;
+        float* o = p.xo + base + 4 * c;
+        if (p.vec) {
+            *reinterpret_cast<float4*>(o) = v;
+        } else {
+            o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+        }
+    };
+    constexpr int N = V > 0 ? V : 1;
+    float4 v[N];
+    double ss = 0.0;
+    if constexpr (V > 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int64_t c = t + i * BS;
+            v[i] = c < nq ? quad(c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int64_t c = t + i * BS;
+            if (c < nq) put(c, v[i]);
+            ss += sq4(v[i]);
+        }
+    } else {
+        for (int64_t c = t; c < nq; c += BS) {
+            v[0] = quad(c);
+            put(c, v[0]);
+            ss += sq4(v[0]);
+        }
+    }
+    ss = mx_sum<BS>(ss);
+    const double inv = 1.0 / sqrt(ss / (double)p.cols + (double)p.eps);
+    const int64_t q0 = row * nq;
+    if constexpr (V > 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int64_t c = t + i * BS;
+            if (c < nq) mx_store<FMT>(scaled4(v[i], inv, p, c), q0 + c, p.codes, p.scales);
+        }
+    } else {
+        // the sum comes from where this lane wrote it: xo may be x or d
+        for (int64_t c = t; c < nq; c += BS) {
+            float4 h;
+            if (p.d != nullptr) {
+                const float* o = p.xo + base + 4 * c;
+                h = make_float4(o[0], o[1], o[2], o[3]);
+            } else {
+                h = quad(c);
+            }
+            mx_store<FMT>(scaled4(h, inv, p, c), q0 + c, p.codes, p.scales);
+        }
+    }
+}
+
+template <int FMT, int BS, int V>
+bool launch_norm(const MxNorm& p, int64_t rows, hipStream_t s) {
+    return launch("mx_norm_kernel", mx_norm_kernel<FMT, BS, V>, dim3((unsigned)rows), dim3(BS), 0, s,
+                  p);
+}
+
+template <int FMT>
+bool run_norm(const MxNorm& p, int64_t rows, hipStream_t s) {
+    const int64_t nq = p.cols / 4;
+    if (nq <= 64) return launch_norm<FMT, 64, 1>(p, rows, s);
+    if (nq <= 128) return launch_norm<FMT, 64, 2>(p, rows, s);
+    if (nq <= 256) return launch_norm<FMT, 256, 1>(p, rows, s);
+    if (nq <= 512) return launch_norm<FMT, 256, 2>(p, rows, s);
+    if (nq <= 1024) return launch_norm<FMT, 256, 4>(p, rows, s);
+    if (nq <= 2048) return launch_norm<FMT, 512, 4>(p, rows, s);
+    if (nq <= 4096) return launch_norm<FMT, 1024, 4>(p, rows, s);
+    return launch_norm<FMT, 1024, 0>(p, rows, s);
+}
+
+// --------------------------------------------------------------- the way back
+template <int FMT>
+__global__ __launch_bounds__(256)
+void mx_dequant_kernel(const uint8_t* codes, const uint8_t* scales, float* out, int64_t n, bool vec) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int s = scales[i >> 3];
+    float v[4];
+    if constexpr (FMT == AERO_MX_INT8) {
+        const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf((float)(int8_t)(c >> (8 * k)), s - 133);
+    } else {
+        const uint32_t c = reinterpret_cast<const uint16_t*>(codes)[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            // twice the magnitude: 0 1 2 3 4 6 8 12, a byte each
+            const uint32_t m = __builtin_amdgcn_perm(0x0c080604u, 0x03020100u, (c >> (4 * k)) & 7u) & 255u;
+            const float a = __builtin_amdgcn_ldexpf((float)m, s - 128);
+            v[k] = (c >> (4 * k)) & 8u ? -a : a;
+        }
+    }
+    if (s == 255) v[0] = v[1] = v[2] = v[3] = __builtin_nanf("");
+    if (vec) {
+        const v4f q = {v[0], v[1], v[2], v[3]};
+        __builtin_nontemporal_store(q, reinterpret_cast<v4f*>(out + 4 * i));
+    } else {
+        for (int k = 0; k < 4; ++k) out[4 * i + k] = v[k];
+    }
+}
+
+}  // namespace
+
+bool mx_rows_ok(const char* what, int fmt, const void* codes, const void* scales, int64_t rows,
+                int64_t cols) {
+    if (fmt != AERO_MX_INT8 && fmt != AERO_MX_FP4) {
+        set_error("%s: unknown format %d", what, fmt);
+        return false;
+    }
+    if (codes == nullptr || scales == nullptr || rows < 0 || rows > kMaxBlocks) {
+        set_error("%s: bad arguments", what);
+        return false;
+    }
+    if (cols <= 0 || cols % 32 != 0 || cols > ((int64_t)1 << 31)) {
+        set_error("%s: %lld columns: rows are whole blocks of 32 values", what, (long long)cols);
+        return false;
+    }
+    if ((reinterpret_cast<uintptr_t>(codes) & 3u) != 0) {
+        set_error("%s: codes at a multiple of 4 bytes are needed", what);
+        return false;
+    }
+    return true;
+}
+
+static bool rows_in_ok(const char* what, const float* a, const float* b, int64_t cols, int64_t ld) {
+    if (a == nullptr || ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 3u) != 0) {
+        set_error("%s: bad input pointer", what);
+        return false;
+    }
+    if (ld < cols) {
+        set_error("%s: rows %lld values apart hold no %lld columns", what, (long long)ld,
+                  (long long)cols);
+        return false;
+    }
+    return true;
+}
+
+}  // namespace aero
+
+extern "C" {
+
+int aero_hip_mx_quantize(int fmt, const float* x, int64_t ld, uint8_t* codes, uint8_t* scales,
+                         int64_t rows, int64_t cols, void* stream) {
+    using namespace aero;
+    if (!mx_rows_ok("mx_quantize", fmt, codes, scales, rows, cols) ||
+        !rows_in_ok("mx_quantize", x, nullptr, cols, ld))
+        return 0;
+    if (rows == 0) return 1;
+    const hipStream_t s = (hipStream_t)stream;
+    return (fmt == AERO_MX_INT8
+                ? run_rows<AERO_MX_INT8, kNone, false>("mx_quantize_kernel", x, nullptr, codes, scales,
+                                                       rows, cols, ld, s)
+                : run_rows<AERO_MX_FP4, kNone, false>("mx_quantize_kernel", x, nullptr, codes, scales,
+                                                      rows, cols, ld, s))
+               ? 1 : 0;
+}
+
+int aero_hip_act_mul_mx(int fmt, int kind, const float* gate, const float* up, int64_t ld,
+                        uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, void* stream) {
+    using namespace aero;
+    if (!mx_rows_ok("act_mul_mx", fmt, codes, scales, rows, cols) ||
+        !rows_in_ok("act_mul_mx", gate, up, cols, ld))
+        return 0;
+    if (kind == AERO_ACT_IDENTITY && up == nullptr) {
+        set_error("act_mul_mx: identity needs `up`");
+        return 0;
+    }
+    if (rows == 0) return 1;
+    const hipStream_t s = (hipStream_t)stream;
+    return (fmt == AERO_MX_INT8
+                ? run_act<AERO_MX_INT8>(kind, gate, up, codes, scales, rows, cols, ld, s)
+                : run_act<AERO_MX_FP4>(kind, gate, up, codes, scales, rows, cols, ld, s))
+               ? 1 : 0;
+}
+
+int aero_hip_rmsnorm_mx(int fmt, const float* x, const float* d, float* x_out, const float* w,
+                        uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, float eps,
+                        int flags, void* stream) {
+    using namespace aero;
+    if (!mx_rows_ok("rmsnorm_mx", fmt, codes, scales, rows, cols) ||
+        !rows_in_ok("rmsnorm_mx", x, d, cols, cols) || !rows_in_ok("rmsnorm_mx", x, w, cols, cols))
+        return 0;
+    if ((d == nullptr) != (x_out == nullptr) || (reinterpret_cast<uintptr_t>(x_out) & 3u) != 0) {
+        set_error("rmsnorm_mx: d and x_out go together");
+        return 0;
+    }
+    if (flags & ~AERO_NORM_UNIT_OFFSET) {
+        set_error("rmsnorm_mx: unknown flags %d", flags);
+        return 0;
+    }
+    if (rows == 0) return 1;
+    MxNorm p{x, d, x_out, w, codes, scales, cols, eps, flags,
+             aligned16(x) && aligned16(d) && aligned16(x_out) && aligned16(w)};
+    const hipStream_t s = (hipStream_t)stream;
+    return (fmt == AERO_MX_INT8 ? run_norm<AERO_MX_INT8>(p, rows, s) : run_norm<AERO_MX_FP4>(p, rows, s))
+               ? 1 : 0;
+}
+
+int aero_hip_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, float* out, int64_t rows,
+                        int64_t cols, void* stream) {
+    using namespace aero;
+    if (!mx_rows_ok("mx_dequant", fmt, codes, scales, rows, cols) ||
+        !rows_in_ok("mx_dequant", out, nullptr, cols, cols))
+        return 0;
+    if (rows == 0) return 1;
+    const int64_t n = rows * (cols / 4), blocks = (n + 255) / 256;
+    if (blocks > kMaxBlocks) {
+        set_error("mx_dequant: too many values (%lld rows of %lld)", (long long)rows, (long long)cols);
+        return 0;
+    }
+    const hipStream_t s = (hipStream_t)stream;
+    const dim3 grid((unsigned)blocks), block(256);
+    return (fmt == AERO_MX_INT8
+                ? launch("mx_dequant_kernel", mx_dequant_kernel<AERO_MX_INT8>, grid, block, 0, s, codes,
+                         scales, out, n, aligned16(out))
+                : launch("mx_dequant_kernel", mx_dequant_kernel<AERO_MX_FP4>, grid, block, 0, s, codes,
+                         scales, out, n, aligned16(out)))
+               ? 1 : 0;
+}
+
+}  // extern "C"

@@ -741,6 +741,107 @@ def write_i32(a: DeviceArray, items, stream: Stream | None = None) -> None:
         val.ctypes.data_as(_lib.ip), at.size, _s(stream)), "write_i32")
 
 
+MX_INT8, MX_FP4 = 0, 1
+
+
+def mx_row_bytes(fmt: int, cols: int) -> int:
+    """Bytes of one row's codes in a microscaled format (its scales: cols / 32)."""
+    if fmt not in (MX_INT8, MX_FP4):
+        raise ValueError(f"microscaled format {fmt}")
+    if cols <= 0 or cols % 32:
+        raise ValueError(f"{cols} columns: microscaled rows are whole blocks of 32 values")
+    return cols if fmt == MX_INT8 else cols // 2
+
+
+def _mx_rows(fmt: int, codes: DeviceArray, scales: DeviceArray, rows: int, cols: int) -> None:
+    _need(codes, rows * mx_row_bytes(fmt, cols), np.int8 if fmt == MX_INT8 else np.uint8, "codes")
+    _need(scales, rows * (cols // 32), np.uint8, "scales")
+
+
+def _mx_span(rows: int, cols: int, ld: int) -> int:
+    return (rows - 1) * ld + cols if rows > 0 else 0
+
+
+def mx_quantize(fmt: int, x: DeviceArray, codes: DeviceArray, scales: DeviceArray, rows: int,
+                cols: int, ld: int | None = None, stream: Stream | None = None) -> None:
+    """Rows of x, ld values apart (default cols), in a microscaled format: each 32
+    values of a row as codes under a power of two of their own. MX_INT8: codes int8
+    [rows, cols], worth code/64 of the scale; MX_FP4: uint8 [rows, cols/2], the low
+    nibble first, worth 0 .5 1 1.5 2 3 4 6 with a sign. scales uint8 [rows, cols/32]:
+    2^(s-127), the smallest under which the block's largest value does not pass the
+    format's largest; 255 for a block with NaN or an infinity. Nearest code, halves
+    to even."""
+    ld = cols if ld is None else int(ld)
+    _mx_rows(fmt, codes, scales, rows, cols)
+    _need(x, _mx_span(rows, cols, ld), np.float32, "x")
+    _lib.check(_lib.lib().aero_hip_mx_quantize(fmt, x.ptr, ld, codes.ptr, scales.ptr, rows, cols,
+                                               _s(stream)), "mx_quantize")
+
+
+def mx_dequant(fmt: int, codes: DeviceArray, scales: DeviceArray, out: DeviceArray, rows: int,
+               cols: int, stream: Stream | None = None) -> None:
+    """out [rows, cols] = the fp32 values of microscaled rows."""
+    _mx_rows(fmt, codes, scales, rows, cols)
+    _need(out, rows * cols, np.float32, "out")
+    _lib.check(_lib.lib().aero_hip_mx_dequant(fmt, codes.ptr, scales.ptr, out.ptr, rows, cols,
+                                              _s(stream)), "mx_dequant")
+
+
+def rmsnorm_mx(fmt: int, x: DeviceArray, w: DeviceArray | None, codes: DeviceArray,
+               scales: DeviceArray, rows: int, cols: int, eps: float, unit_offset: bool = False,
+               d: DeviceArray | None = None, x_out: DeviceArray | None = None,
+               stream: Stream | None = None) -> None:
+    """rmsnorm(x') * (w or 1+w) as microscaled rows (mx_quantize), one pass; x' = x +
+    d (stored to x_out, default x) when d is given, else x. The norm is evaluated in
+    64 bits and rounded to fp32 once, so the codes are those of the formula."""
+    if d is not None and x_out is None:
+        x_out = x
+    if d is None and x_out is not None:
+        raise ValueError("rmsnorm_mx: x_out without d")
+    _mx_rows(fmt, codes, scales, rows, cols)
+    for a, name in ((x, "x"), (d, "d"), (x_out, "x_out")):
+        _need(a, rows * cols, np.float32, name)
+    _need(w, cols, np.float32, "w")
+    _lib.check(_lib.lib().aero_hip_rmsnorm_mx(
+        fmt, x.ptr, as_ptr(d), as_ptr(x_out), as_ptr(w), codes.ptr, scales.ptr, rows, cols,
+        float(eps), NORM_UNIT_OFFSET if unit_offset else 0, _s(stream)), "rmsnorm_mx")
+
+
+def act_mul_mx(fmt: int, kind, gate: DeviceArray, up: DeviceArray | None, codes: DeviceArray,
+               scales: DeviceArray, rows: int, cols: int, ld: int | None = None,
+               stream: Stream | None = None) -> None:
+    """act(gate) * up (up None: act(gate)) as microscaled rows (mx_quantize), kinds of
+    act_mul; rows of gate and up ld values apart (default cols): with gate and up the
+    halves of one product's rows, ld is twice cols. In 64 bits, rounded to fp32 once."""
+    k = ACTS[kind] if isinstance(kind, str) else int(kind)
+    ld = cols if ld is None else int(ld)
+    _mx_rows(fmt, codes, scales, rows, cols)
+    _need(gate, _mx_span(rows, cols, ld), np.float32, "gate")
+    _need(up, _mx_span(rows, cols, ld), np.float32, "up")
+    _lib.check(_lib.lib().aero_hip_act_mul_mx(fmt, k, gate.ptr, as_ptr(up), ld, codes.ptr,
+                                              scales.ptr, rows, cols, _s(stream)), "act_mul_mx")
+
+
+_mx_ws = Workspace("microscaled product")
+
+
+def mx_matmul(fmt: int, codes: DeviceArray, scales: DeviceArray, w, y: DeviceArray, n_tok: int,
+              stream: Stream | None = None) -> None:
+    """y [n_tok, w.n_rows] = x W^T in fp32: x microscaled rows [n_tok, w.n_cols] in
+    fmt, w an mx.MxWeight (4 bits). Products and the sums within a block are exact. The
+    workspace grows to the largest call and is kept: calls that overlap on different
+    streams would share its contents."""
+    _mx_rows(fmt, codes, scales, n_tok, w.n_cols)
+    _need(y, n_tok * w.n_rows, np.float32, "y")
+    L = _lib.lib()
+    wsb = int(L.aero_hip_mx_matmul_workspace(fmt, w.n_rows, w.n_cols, n_tok))
+    _lib.check(wsb >= 0, "mx_matmul")
+    ws = _mx_ws.get(wsb)
+    _lib.check(L.aero_hip_mx_matmul(fmt, codes.ptr, scales.ptr, w.buf.ptr, w.buf.nbytes, y.ptr,
+                                    w.n_rows, w.n_cols, n_tok, as_ptr(ws),
+                                    ws.nbytes if ws is not None else 0, _s(stream)), "mx_matmul")
+
+
 def softmax_rows(x: DeviceArray, y: DeviceArray, n_rows: int, n_cols: int,
                  stream: Stream | None = None) -> None:
     """y[r] = softmax(x[r]) (src/tensor.cpp:167-178); y may be x."""

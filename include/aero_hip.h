@@ -703,6 +703,51 @@ int aero_hip_kv_pages_copy(const aero_kv_pool_t* pool, const int32_t* src, const
 int aero_hip_write_i32(int32_t* base, int64_t n_base, const int64_t* at, const int32_t* value,
                        int64_t n, void* stream);
 
+/* Microscaled rows: blocks of 32 consecutive values of a row share a power of two,
+ * 2^(s-127) for the scale byte s (255: the block holds NaN or an infinity and stands
+ * for 32 NaN). AERO_MX_INT8: codes int8, a value is code/64 of the scale; AERO_MX_FP4:
+ * 4 bits (sign, two of exponent, one of mantissa: 0 .5 1 1.5 2 3 4 6), two codes a
+ * byte, the low nibble first. Rows are packed: codes [rows][cols] bytes or
+ * [rows][cols/2], scales [rows][cols/32]; cols a multiple of 32, codes at 4 bytes
+ * (16 for the product). The quantisers take the smallest scale under which the block's
+ * largest magnitude does not pass the format's largest (127/64, 6), 8 bits none below
+ * s = 4 (blocks below 2^-123), and the nearest code, halves to even. No counterpart in
+ * the reference, which quantises cache vectors only (include/aero/kv.hpp:62-126). */
+#define AERO_MX_INT8 0
+#define AERO_MX_FP4  1
+/* Rows of x, ld values apart (ld >= cols). */
+int aero_hip_mx_quantize(int fmt, const float* x, int64_t ld, uint8_t* codes, uint8_t* scales,
+                         int64_t rows, int64_t cols, void* stream);
+/* out [rows][cols] = the values that codes and scales stand for. */
+int aero_hip_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, float* out,
+                        int64_t rows, int64_t cols, void* stream);
+/* rmsnorm(x') * (w, 1 + w with AERO_NORM_UNIT_OFFSET, or 1 where w is NULL), x' = x + d
+ * stored to x_out (which may be x or d; both NULL: x' = x): evaluated in 64 bits,
+ * rounded to fp32 once and quantised as mx_quantize. */
+int aero_hip_rmsnorm_mx(int fmt, const float* x, const float* d, float* x_out, const float* w,
+                        uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, float eps,
+                        int flags, void* stream);
+/* act(gate) * up (up NULL: act(gate)), kinds of aero_hip_act_mul, rows of both ld values
+ * apart (the two halves of one product's rows, for instance); in 64 bits, rounded to
+ * fp32 once and quantised. */
+int aero_hip_act_mul_mx(int fmt, int kind, const float* gate, const float* up, int64_t ld,
+                        uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols,
+                        void* stream);
+/* Weights for the product: 4-bit rows laid out once in the order of its matrix steps,
+ * in aero_hip_mx_weight_bytes bytes (-1: bad sizes) at a 16-byte address. */
+int64_t aero_hip_mx_weight_bytes(int64_t n_rows, int64_t n_cols);
+int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64_t w_bytes,
+                     int64_t n_rows, int64_t n_cols, void* stream);
+/* y[t][n] = sum over k of x[t][k] W[n][k] in fp32, x [n_tok][n_cols] in fmt, W of
+ * mx_pack; products and the sums within a block are exact. Scale bytes of 8-bit rows
+ * below 4 count as 4. Workspace: aero_hip_mx_matmul_workspace bytes (0: none; -1: bad
+ * sizes), 16-byte aligned, its contents free between calls; calls that share it must be
+ * ordered. */
+int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok);
+int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, const void* w,
+                       int64_t w_bytes, float* y, int64_t n_rows, int64_t n_cols, int64_t n_tok,
+                       void* workspace, int64_t ws_bytes, void* stream);
+
 /* Plain fp32 copy kernel (dst = src, n elements): the known-size reference
  * workload used to calibrate HBM byte counters. */
 int aero_hip_copy_f32(const float* src, float* dst, int64_t n, void* stream);

@@ -1,0 +1,385 @@
+"""GPU: microscaled rows (ops.mx_quantize, mx_dequant, rmsnorm_mx, act_mul_mx) and their
+product with 4-bit weights (ops.mx_matmul, mx.MxWeight) against plain 64-bit forms
+(tests/mx_ref.py).
+
+Rows: codes and scales equal, the residual sums and the values read back bit for bit. The
+norms and activations are 64-bit expressions rounded to fp32 once, so both sides round the
+same number but where it lies within some 2^-50 of a border of two fp32 numbers.
+
+Product: its terms are exact, each of a sum's additions rounds to fp32. A step of 64
+columns adds 8 groups of 8 products and the running sum, twice for 8-bit rows (a code's
+halves): 9 K / 32 additions, each off by up to 2^-23 of the running sum, which grows to
+the result's size; as independent errors sqrt(9 K / 32) 2^-24 of the result, in the norm.
+No element further than 2^-20 of the sum of its terms' magnitudes."""
+import numpy as np
+import pytest
+
+import mx_ref as R
+from conftest import bits_equal
+from aero_amd import mx, ops
+from aero_amd.device import DeviceArray as DA, Plan, Stream, synchronize
+
+pytestmark = pytest.mark.gpu
+
+INT8, FP4 = ops.MX_INT8, ops.MX_FP4
+FMTS = [INT8, FP4]
+
+
+def held(fmt, rows, cols, fill=0x5A):
+    codes = np.full((rows, ops.mx_row_bytes(fmt, cols)), fill, np.int8 if fmt == INT8 else np.uint8)
+    return DA.from_numpy(codes), DA.from_numpy(np.full((rows, cols // 32), fill, np.uint8))
+
+
+def same(dc, ds, want):
+    assert np.array_equal(ds.numpy(), want[1])
+    assert np.array_equal(dc.numpy(), want[0])
+
+
+def awkward(rng, rows, cols):
+    """Rows of many sizes with zeros, subnormals, the largest numbers, ties and blocks whose
+    largest value is at, just below and just above a scale's border."""
+    x = (rng.standard_normal((rows, cols)) * np.exp2(rng.integers(-140, 120, (rows, 1)))).astype(np.float32)
+    b = x.reshape(-1, 32)
+    n = len(b)
+    for i in range(0, n, 3):
+        kind = (i // 3) % 8
+        e = np.float32(2.0) ** np.float32(rng.integers(-100, 100))
+        if kind == 0:
+            b[i] = 0
+            b[i, 1::2] = -0.0
+        elif kind == 1:
+            b[i] = (rng.integers(-9, 10, 32) * 2.0 ** -149).astype(np.float32)
+        elif kind == 2:
+            b[i, rng.integers(32)] = np.finfo(np.float32).max
+        elif kind == 3:      # every tie of 8 bits below the largest code
+            b[i] = (rng.integers(-126, 126, 32) + 0.5) / 64 * e
+            b[i, 0] = 127 / 64 * e
+        elif kind == 4:      # and of 4 bits
+            b[i] = rng.choice([.25, .75, 1.25, 1.75, 2.5, 3.5, 5.0, -.25, -5.0, 6.0], 32) * e
+            b[i, 0] = 6 * e
+        elif kind == 5:
+            b[i, 3] = np.nextafter(np.float32(np.abs(b[i]).max()) * 0 + np.float32(127 / 64) * e, np.float32(np.inf))
+        elif kind == 6:
+            b[i] = b[i] * 0 + np.nextafter(np.float32(6) * e, np.float32(np.inf))
+        else:
+            b[i] = b[i] * 0 - np.nextafter(np.float32(6) * e, np.float32(0))
+    return b.reshape(rows, cols)
+
+
+SIZES = [(1, 32), (3, 64), (1, 896), (37, 96), (130, 2560), (5, 14336)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_quantise(hip, fmt, rows, cols):
+    x = awkward(np.random.default_rng(rows + cols), rows, cols)
+    dc, ds = held(fmt, rows, cols)
+    ops.mx_quantize(fmt, DA.from_numpy(x), dc, ds, rows, cols)
+    same(dc, ds, R.quantise(x, fmt))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantise_not_finite(hip, fmt):
+    x = np.random.default_rng(1).standard_normal((6, 96)).astype(np.float32)
+    x[0, 5], x[1, 40], x[2, 95], x[3, 32:64] = np.nan, np.inf, -np.inf, np.nan
+    dc, ds = held(fmt, 6, 96)
+    ops.mx_quantize(fmt, DA.from_numpy(x), dc, ds, 6, 96)
+    want = R.quantise(x, fmt)
+    assert (want[1] == 255).sum() == 4
+    same(dc, ds, want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("off,ld", [(0, 96), (0, 100), (1, 97), (3, 203), (2, 96)])
+def test_quantise_strides_and_addresses(hip, fmt, off, ld):
+    rows, cols = 19, 96
+    rng = np.random.default_rng(ld)
+    flat = rng.standard_normal(off + rows * ld).astype(np.float32)
+    x = np.stack([flat[off + r * ld:off + r * ld + cols] for r in range(rows)])
+    d = DA.from_numpy(flat[:off + (rows - 1) * ld + cols])
+    dc, ds = held(fmt, rows + 1, cols)
+    ops.mx_quantize(fmt, d.view(shape=d.size - off, offset_bytes=4 * off), dc, ds, rows, cols, ld=ld)
+    want = R.quantise(x, fmt)
+    assert np.array_equal(dc.numpy()[:rows], want[0]) and np.array_equal(ds.numpy()[:rows], want[1])
+    assert (dc.numpy()[rows] == 0x5A).all() and (ds.numpy()[rows] == 0x5A).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("off", [0, 1])
+def test_dequant_every_code_and_scale(hip, fmt, off):
+    """Every code under every scale byte, also where the value is an fp32 subnormal, past
+    the largest fp32 number (an infinity, as rounding gives) or NaN."""
+    per = 256 if fmt == INT8 else 32
+    codes = np.tile(np.arange(256, dtype=np.uint8).view(np.int8), (256, 1)) if fmt == INT8 else \
+        np.tile(R.pack(np.arange(32)[None] % 16, FP4), (256, 1))
+    s = np.repeat(np.arange(256, dtype=np.uint8)[:, None], per // 32, 1)
+    out = DA.from_numpy(np.full(256 * per + 8, 7, np.float32))
+    ops.mx_dequant(fmt, DA.from_numpy(codes), DA.from_numpy(s),
+                   out.view(shape=256 * per, offset_bytes=4 * off), 256, per)
+    with np.errstate(over="ignore"):
+        want = R.values(codes, s, fmt).astype(np.float32)
+    got = out.numpy()
+    body = got[off:off + 256 * per].reshape(256, per)
+    assert np.array_equal(np.isnan(body), np.isnan(want))
+    assert bits_equal(np.nan_to_num(body, nan=1), np.nan_to_num(want, nan=1)) or \
+        np.array_equal(body[~np.isnan(body)], want[~np.isnan(want)])
+    assert (got[:off] == 7).all() and (got[off + 256 * per:] == 7).all()
+
+
+NORMS = [(1, 32), (1, 896), (5, 224), (333, 2560), (9, 512), (64, 4096), (3, 8192), (2, 14336),
+         (3, 16384), (2, 16416), (2, 28672)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("add", ["none", "x", "d", "apart"])
+@pytest.mark.parametrize("rows,cols", NORMS)
+def test_norm(hip, fmt, add, rows, cols):
+    rng = np.random.default_rng(rows * 7 + cols)
+    x = (rng.standard_normal((rows, cols)) * np.exp(rng.standard_normal(cols))).astype(np.float32)
+    d = rng.standard_normal((rows, cols)).astype(np.float32)
+    unit = cols % 512 == 0
+    w = None if rows == 2 else (rng.standard_normal(cols) * 0.1 + (not unit)).astype(np.float32)
+    dx, dd = DA.from_numpy(x), DA.from_numpy(d)
+    out = {"none": None, "x": dx, "d": dd, "apart": DA.empty((rows, cols))}[add]
+    dc, ds = held(fmt, rows, cols)
+    ops.rmsnorm_mx(fmt, dx, None if w is None else DA.from_numpy(w), dc, ds, rows, cols, 1e-5,
+                   unit_offset=unit, d=None if add == "none" else dd, x_out=out)
+    total = x if add == "none" else x + d
+    same(dc, ds, R.quantise(R.norm(total, w, 1e-5, unit), fmt))
+    if out is not None:
+        assert bits_equal(out.numpy(), total)
+    for arr, host in ((dx, x), (dd, d)):
+        if arr is not out:
+            assert bits_equal(arr.numpy(), host)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_norm_awkward_rows(hip, fmt):
+    """Zero rows, rows whose squares pass fp32's range, NaN and infinities; odd addresses."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((8, 160)).astype(np.float32)
+    x[0] = 0
+    x[1] *= np.float32(1e30)
+    x[2] *= np.float32(1e-30)
+    x[3, 7] = np.inf
+    x[4, 9] = np.nan
+    x[5, 0] = np.float32(3e38)
+    w = rng.standard_normal(160).astype(np.float32)
+    want = R.quantise(R.norm(x, w, 1e-6, False), fmt)
+    assert (want[1][4] == 255).all() and (want[1][3] == 255).sum() == 1
+    for off in (0, 1):
+        dx = DA.from_numpy(np.concatenate([np.zeros(off, np.float32), x.reshape(-1)]))
+        dw = DA.from_numpy(np.concatenate([np.zeros(off, np.float32), w]))
+        dc, ds = held(fmt, 8, 160)
+        ops.rmsnorm_mx(fmt, dx.view(shape=1280, offset_bytes=4 * off),
+                       dw.view(shape=160, offset_bytes=4 * off), dc, ds, 8, 160, 1e-6)
+        same(dc, ds, want)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh", "identity", "sigmoid"])
+@pytest.mark.parametrize("rows,cols,layout", [(1, 4864, "halves"), (33, 96, "halves"), (7, 320, "own"),
+                                              (5, 64, "odd"), (130, 1024, "own")])
+def test_act(hip, fmt, kind, rows, cols, layout):
+    rng = np.random.default_rng(cols)
+    g, u = ((rng.standard_normal((rows, cols)) * 3).astype(np.float32) for _ in range(2))
+    g[0, :32] = np.linspace(-200, 200, 32)
+    g[0, 32:64] = -30 - np.arange(32)                 # a block of tails only
+    with np.errstate(over="ignore"):
+        want = R.quantise((R.act(kind, g) * u).astype(np.float32), fmt)
+    dc, ds = held(fmt, rows, cols)
+    if layout == "own":
+        ops.act_mul_mx(fmt, kind, DA.from_numpy(g), DA.from_numpy(u), dc, ds, rows, cols)
+    else:
+        gap = 0 if layout == "halves" else 3
+        both = DA.from_numpy(np.concatenate([g, u, np.full((rows, gap), np.nan, np.float32)], 1))
+        ld = 2 * cols + gap
+        ops.act_mul_mx(fmt, kind, both, both.view(shape=both.size - cols, offset_bytes=4 * cols), dc,
+                       ds, rows, cols, ld=ld)
+    same(dc, ds, want)
+    if kind != "identity":
+        ops.act_mul_mx(fmt, kind, DA.from_numpy(g), None, dc, ds, rows, cols)
+        with np.errstate(over="ignore"):
+            same(dc, ds, R.quantise(R.act(kind, g).astype(np.float32), fmt))
+
+
+def test_act_not_finite(hip):
+    g = np.random.default_rng(2).standard_normal((4, 64)).astype(np.float32)
+    u = np.ones_like(g)
+    g[0, 3], g[1, 40], u[2, 5], u[3, 60] = np.nan, np.inf, np.nan, np.float32(3e38)
+    g[3, 60] = 100                                     # 3e40: past fp32
+    dc, ds = held(INT8, 4, 64)
+    ops.act_mul_mx(INT8, "silu", DA.from_numpy(g), DA.from_numpy(u), dc, ds, 4, 64)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = R.quantise((R.act("silu", g) * u).astype(np.float32), INT8)
+    assert (want[1] == 255).sum() == 4
+    same(dc, ds, want)
+
+
+# ------------------------------------------------------------------ product
+def operands(rng, fmt, T, N, K, spread=0):
+    """(x codes, x scales, W codes, W scales) of rows of different sizes."""
+    x = rng.standard_normal((T, K)) * np.exp2(rng.integers(-spread, spread + 1, (T, 1)))
+    x[:, ::97] *= 20
+    w = rng.standard_normal((N, K)) * 0.02
+    return (*R.quantise(x.astype(np.float32), fmt), *R.quantise(w.astype(np.float32), FP4))
+
+
+def product(fmt, xc, xs, wc, ws, stream=None, guard=64):
+    T, N, K = xc.shape[0], wc.shape[0], 32 * xs.shape[1]
+    weight = mx.MxWeight(DA.from_numpy(wc), DA.from_numpy(ws), N, K)
+    y = DA.from_numpy(np.full(T * N + guard, 7.0, np.float32))
+    ops.mx_matmul(fmt, DA.from_numpy(xc), DA.from_numpy(xs), weight, y, T, stream=stream)
+    synchronize()
+    y = y.numpy()
+    assert (y[T * N:] == 7).all()
+    return y[:T * N].reshape(T, N)
+
+
+def near(got, xc, xs, wc, ws, fmt):
+    K = 32 * xs.shape[1]
+    x, w = R.values(xc, xs, fmt), R.values(wc, ws, FP4)
+    want = x @ w.T
+    assert (np.abs(got - want) <= 2.0 ** -20 * (np.abs(x) @ np.abs(w).T) + 2.0 ** -149).all()
+    off = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert off <= np.sqrt(9 * K / 32) * 2.0 ** -24, off
+
+
+PRODUCTS = [(1, 1, 32), (1, 9728, 896), (1, 100, 64), (2, 33, 96), (3, 4096, 160), (5, 50, 992),
+            (16, 257, 512), (17, 31, 2560), (31, 64, 128), (32, 96, 4096), (33, 130, 224),
+            (64, 1000, 1024), (65, 129, 352), (100, 3, 4864), (127, 255, 736), (128, 256, 256),
+            (129, 257, 288), (200, 513, 1056), (256, 512, 2048), (300, 1021, 928), (512, 640, 4096),
+            (513, 300, 544), (1000, 100, 1120)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T,N,K", PRODUCTS)
+def test_product(hip, fmt, T, N, K):
+    print(f"product fmt={fmt} T={T} N={N} K={K}", flush=True)
+    a = operands(np.random.default_rng(T + N + K), fmt, T, N, K, spread=2)
+    near(product(fmt, *a), *a, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_product_any_codes_and_scales(hip, fmt, T):
+    """Random bytes for codes (-128 and both zeros among them), scales over 40 binades."""
+    rng = np.random.default_rng(T)
+    N, K = 70, 480
+    xc = rng.integers(0, 256, (T, ops.mx_row_bytes(fmt, K))).astype(np.uint8)
+    xc = xc.view(np.int8) if fmt == INT8 else xc
+    xs, ws = (rng.integers(107, 147, (n, K // 32)).astype(np.uint8) for n in (T, N))
+    wc = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    got = product(fmt, xc, xs, wc, ws)
+    x, w = R.values(xc, xs, fmt), R.values(wc, ws, FP4)
+    assert (np.abs(got - x @ w.T) <= 2.0 ** -20 * (np.abs(x) @ np.abs(w).T)).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T", [3, 140])
+def test_product_of_not_finite_blocks(hip, fmt, T):
+    """A NaN block makes its token's, or its weight row's, results NaN and no others; scales
+    at both ends of their range meet."""
+    rng = np.random.default_rng(9)
+    N, K = 40, 224
+    xc, xs, wc, ws = operands(rng, fmt, T, N, K)
+    xs[1, 3], ws[7, 6] = 255, 255
+    got = product(fmt, xc, xs, wc, ws)
+    nan = np.isnan(got)
+    assert nan[1].all() and nan[:, 7].all()
+    keep = np.ones((T, N), bool)
+    keep[1], keep[:, 7] = False, False
+    assert not nan[keep].any()
+    xs[1, 3], ws[7, 6] = 127, 127
+    xs[:], ws[:] = 250, 4      # 2^123 * 2^-123
+    got = product(fmt, xc, xs, wc, ws)
+    x, w = R.values(xc, xs, fmt), R.values(wc, ws, FP4)
+    assert (np.abs(got - x @ w.T) <= 2.0 ** -20 * (np.abs(x) @ np.abs(w).T)).all()
+
+
+def test_product_of_nothing(hip):
+    w = mx.MxWeight.from_rows(DA.from_numpy(np.ones((4, 32), np.float32)), 4, 32)
+    y = DA.from_numpy(np.full(4, 7, np.float32))
+    ops.mx_matmul(INT8, *held(INT8, 1, 32), w, y, 0)
+    assert (y.numpy() == 7).all()
+
+
+def test_product_rows_at_odd_addresses(hip):
+    """y anywhere on 4 bytes."""
+    rng = np.random.default_rng(4)
+    for T in (2, 130):
+        a = operands(rng, INT8, T, 64, 256)
+        w = mx.MxWeight(DA.from_numpy(a[2]), DA.from_numpy(a[3]), 64, 256)
+        flat = DA.from_numpy(np.full(T * 64 + 9, 7, np.float32))
+        ops.mx_matmul(INT8, DA.from_numpy(a[0]), DA.from_numpy(a[1]), w,
+                      flat.view(shape=T * 64, offset_bytes=4), T)
+        got = flat.numpy()
+        near(got[1:1 + T * 64].reshape(T, 64), *a, INT8)
+        assert got[0] == 7 and (got[1 + T * 64:] == 7).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_same_call_same_bits(hip, fmt):
+    """The same call twice: the same bits."""
+    a = operands(np.random.default_rng(8), fmt, 150, 300, 1056)
+    assert bits_equal(product(fmt, *a), product(fmt, *a))
+
+
+# ------------------------------------------------------------ as they are used
+def test_feed_forward_in_a_plan(hip):
+    """Residual and norm to 8 bits, gate and up in one product, the activation to 8 bits, the
+    down projection, recorded once and replayed on new inputs on a stream; each step against
+    its formula on the inputs that it had."""
+    rng = np.random.default_rng(11)
+    T, C, F = 70, 256, 416
+    wg, wd = ((rng.standard_normal((n, k)) * k ** -0.5).astype(np.float32)
+              for n, k in ((2 * F, C), (C, F)))
+    nw = rng.standard_normal(C).astype(np.float32)
+    w1 = mx.MxWeight.from_rows(DA.from_numpy(wg), 2 * F, C)
+    w2 = mx.MxWeight.from_rows(DA.from_numpy(wd), C, F)
+    x, d, y = DA.empty((T, C)), DA.empty((T, C)), DA.empty((T, C))
+    both, dw = DA.empty((T, 2 * F)), DA.from_numpy(nw)
+    hc, hs = held(INT8, T, C)
+    ac, as_ = held(INT8, T, F)
+    up = both.view(shape=both.size - F, offset_bytes=4 * F)
+    plan = Plan()
+    with plan:
+        ops.rmsnorm_mx(INT8, x, dw, hc, hs, T, C, 1e-5, d=d)
+        ops.mx_matmul(INT8, hc, hs, w1, both, T)
+        ops.act_mul_mx(INT8, "silu", both, up, ac, as_, T, F, ld=2 * F)
+        ops.mx_matmul(INT8, ac, as_, w2, y, T)
+    stream = Stream()
+    for step in range(3):
+        hx, hd = (rng.standard_normal((T, C)).astype(np.float32) * (step + 1) for _ in range(2))
+        x.copy_from(hx)
+        d.copy_from(hd)
+        plan.launch(stream)
+        stream.synchronize()
+        assert bits_equal(x.numpy(), hx + hd)
+        same(hc, hs, R.quantise(R.norm(hx + hd, nw, 1e-5, False), INT8))
+        near(both.numpy(), hc.numpy(), hs.numpy(), *R.quantise(wg, FP4), INT8)
+        g, u = both.numpy()[:, :F], both.numpy()[:, F:]
+        same(ac, as_, R.quantise((R.act("silu", g) * u).astype(np.float32), INT8))
+        near(y.numpy(), ac.numpy(), as_.numpy(), *R.quantise(wd, FP4), INT8)
+    stream.destroy()
+
+
+def test_plan_keeps_its_workspace(hip):
+    """A plan recorded before a larger call has its own workspace, and gives the same bits."""
+    a = operands(np.random.default_rng(12), INT8, 130, 200, 512)
+    weight = mx.MxWeight(DA.from_numpy(a[2]), DA.from_numpy(a[3]), 200, 512)
+    xc, xs, y = DA.from_numpy(a[0]), DA.from_numpy(a[1]), DA.empty((130, 200))
+    plan = Plan()
+    with plan:
+        ops.mx_matmul(INT8, xc, xs, weight, y, 130)
+    plan.launch()
+    synchronize()
+    first = y.numpy()
+    near(first, *a, INT8)
+    b = operands(np.random.default_rng(13), INT8, 700, 64, 4096)
+    near(product(INT8, *b), *b, INT8)
+    for _ in range(2):
+        y.copy_from(np.zeros((130, 200), np.float32))
+        plan.launch()
+        synchronize()
+        assert bits_equal(y.numpy(), first)

@@ -1,0 +1,121 @@
+"""CPU: refusals of the microscaled ops and their host-side sizes; the plain forms that
+the GPU tests compare with, on values worked out by hand."""
+import numpy as np
+import pytest
+
+import mx_ref as R
+from aero_amd import _lib, ops
+
+
+def test_plain_forms_by_hand():
+    x = np.zeros((1, 32), np.float32)
+    x[0, :6] = [1.984375, -1, 0.0078125, 0.0234375, 3 / 128, -0.0078125]
+    c, s = R.quantise(x, R.INT8)                       # 127/64 just fits 2^0; ties to even
+    assert s[0, 0] == 127 and c[0, :6].tolist() == [127, -64, 0, 2, 2, 0]
+    x[0, 0] = 2
+    c, s = R.quantise(x, R.INT8)
+    assert s[0, 0] == 128 and c[0, :2].tolist() == [64, -32]
+    x[0, :4] = [6, -5, 0.25, 0.75]
+    c, s = R.quantise(x, R.FP4)
+    assert s[0, 0] == 127 and c[0, 0] == 7 | (0x8 | 6) << 4 and c[0, 1] == 0 | 2 << 4
+    assert R.values(c, s, R.FP4)[0, :4].tolist() == [6, -4, 0, 1]
+    x[0, 0] = 6.5
+    assert R.quantise(x, R.FP4)[1][0, 0] == 128
+    x[0, 1] = np.inf
+    assert R.quantise(x, R.FP4)[1][0, 0] == 255 and np.isnan(R.values(*R.quantise(x, R.FP4), R.FP4)).all()
+
+
+def test_sizes():
+    L = _lib.load()
+    assert ops.mx_row_bytes(ops.MX_INT8, 96) == 96 and ops.mx_row_bytes(ops.MX_FP4, 96) == 48
+    for cols in (0, -32, 33, 16):
+        with pytest.raises(ValueError):
+            ops.mx_row_bytes(ops.MX_INT8, cols)
+    with pytest.raises(ValueError):
+        ops.mx_row_bytes(2, 32)
+    assert L.aero_hip_mx_weight_bytes(1, 32) == 2176           # a tile of 32 rows, 128 columns
+    assert L.aero_hip_mx_weight_bytes(33, 160) == 4 * 2176
+    assert L.aero_hip_mx_weight_bytes(28672, 8192) == 28672 * 8192 * 17 // 32
+    for sizes in ((0, 32), (1, 31), (1, 0), (-1, 32), (1, 1 << 25)):
+        assert L.aero_hip_mx_weight_bytes(*sizes) == -1
+    assert L.aero_hip_mx_matmul_workspace(2, 32, 32, 1) == -1
+    assert L.aero_hip_mx_matmul_workspace(0, 32, 33, 1) == -1
+    assert L.aero_hip_mx_matmul_workspace(0, 32, 32, -1) == -1
+    assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 0) >= 0
+
+
+@pytest.mark.parametrize("call,args,reason", [
+    ("mx_quantize", (2, 16, 32, 16, 16, 1, 32, None), "format"),
+    ("mx_quantize", (0, 16, 32, 16, 16, 1, 31, None), "blocks"),
+    ("mx_quantize", (0, 16, 32, 16, 16, 1, 0, None), "blocks"),
+    ("mx_quantize", (0, 16, 32, 16, 16, -1, 32, None), "arguments"),
+    ("mx_quantize", (0, None, 32, 16, 16, 1, 32, None), "input"),
+    ("mx_quantize", (0, 18, 32, 16, 16, 1, 32, None), "input"),
+    ("mx_quantize", (0, 16, 32, None, 16, 1, 32, None), "arguments"),
+    ("mx_quantize", (0, 16, 32, 16, None, 1, 32, None), "arguments"),
+    ("mx_quantize", (0, 16, 32, 18, 16, 1, 32, None), "4 bytes"),
+    ("mx_quantize", (0, 16, 31, 16, 16, 1, 32, None), "apart"),
+    ("mx_dequant", (5, 16, 16, 16, 1, 32, None), "format"),
+    ("mx_dequant", (0, 16, 16, None, 1, 32, None), "input"),
+    ("mx_dequant", (0, 16, 16, 16, 1, 48, None), "blocks"),
+    ("rmsnorm_mx", (0, 16, 16, None, 16, 16, 16, 1, 32, 1e-5, 0, None), "together"),
+    ("rmsnorm_mx", (0, 16, None, 16, 16, 16, 16, 1, 32, 1e-5, 0, None), "together"),
+    ("rmsnorm_mx", (0, 16, None, None, 17, 16, 16, 1, 32, 1e-5, 0, None), "input"),
+    ("rmsnorm_mx", (0, 16, None, None, 16, 16, 16, 1, 32, 1e-5, 2, None), "flags"),
+    ("rmsnorm_mx", (0, 16, None, None, 16, 16, 16, 1, 40, 1e-5, 0, None), "blocks"),
+    ("act_mul_mx", (0, 9, 16, 16, 32, 16, 16, 1, 32, None), "kind"),
+    ("act_mul_mx", (0, 3, 16, None, 32, 16, 16, 1, 32, None), "identity"),
+    ("act_mul_mx", (0, 0, None, 16, 32, 16, 16, 1, 32, None), "input"),
+    ("act_mul_mx", (0, 0, 16, 16, 16, 16, 16, 1, 32, None), "apart"),
+    ("mx_pack", (16, 16, 16, 2175, 1, 32, None), "bytes"),
+    ("mx_pack", (16, 16, 24, 4096, 1, 32, None), "bytes"),
+    ("mx_pack", (16, 16, None, 4096, 1, 32, None), "bytes"),
+    ("mx_pack", (16, 16, 16, 4096, 0, 32, None), "rows"),
+    ("mx_matmul", (0, 16, 16, 16, 2175, 16, 1, 32, 1, None, 0, None), "take"),
+    ("mx_matmul", (0, 20, 16, 16, 2176, 16, 1, 32, 1, None, 0, None), "16-byte"),
+    ("mx_matmul", (0, 16, 16, 16, 2176, None, 1, 32, 1, None, 0, None), "y"),
+    ("mx_matmul", (0, 16, 16, 16, 2176, 18, 1, 32, 1, None, 0, None), "y"),
+    ("mx_matmul", (3, 16, 16, 16, 2176, 16, 1, 32, 1, None, 0, None), "format"),
+    ("mx_matmul", (0, 16, 16, 16, 2176, 16, 1, 32, -1, None, 0, None), "arguments"),
+    ("mx_matmul", (0, 16, 16, 24, 4096, 16, 1, 32, 1, None, 0, None), "take"),
+])
+def test_refusals(call, args, reason):
+    """Refused with a reason before anything is launched: no pointer here is memory."""
+    L = _lib.load()
+    assert getattr(L, "aero_hip_" + call)(*args) == 0
+    assert reason in _lib.last_error(), _lib.last_error()
+
+
+def test_nothing_to_do():
+    L = _lib.load()
+    assert L.aero_hip_mx_quantize(0, 16, 32, 16, 16, 0, 32, None) == 1
+    assert L.aero_hip_mx_dequant(0, 16, 16, 16, 0, 32, None) == 1
+    assert L.aero_hip_rmsnorm_mx(0, 16, None, None, None, 16, 16, 0, 32, 1e-5, 0, None) == 1
+    assert L.aero_hip_act_mul_mx(0, 0, 16, None, 32, 16, 16, 0, 32, None) == 1
+    assert L.aero_hip_mx_matmul(0, 16, 16, 16, 2176, 16, 1, 32, 0, None, 0, None) == 1
+
+
+def test_arrays_are_checked():
+    """Buffers too small or of another type are refused by the Python ops."""
+    def arr(n, dtype):
+        return ops.DeviceArray((n,), dtype, _ptr=16, _owner=False)
+
+    x, c8, c4, s = arr(64, np.float32), arr(64, np.int8), arr(32, np.uint8), arr(2, np.uint8)
+    with pytest.raises(TypeError):
+        ops.mx_quantize(ops.MX_INT8, x, c4, s, 1, 64)
+    with pytest.raises(TypeError):
+        ops.mx_quantize(ops.MX_FP4, x, c8, s, 1, 64)
+    with pytest.raises(ValueError):
+        ops.mx_quantize(ops.MX_INT8, x, c8, s, 2, 64)
+    with pytest.raises(ValueError):
+        ops.mx_quantize(ops.MX_INT8, x, c8, s, 2, 32, ld=33)
+    with pytest.raises(ValueError):
+        ops.mx_dequant(ops.MX_FP4, c4, s, arr(63, np.float32), 1, 64)
+    with pytest.raises(ValueError):
+        ops.rmsnorm_mx(ops.MX_INT8, x, arr(32, np.float32), c8, s, 1, 64, 1e-5)
+    with pytest.raises(ValueError):
+        ops.rmsnorm_mx(ops.MX_INT8, x, None, c8, s, 1, 64, 1e-5, x_out=x)
+    with pytest.raises(ValueError):
+        ops.act_mul_mx(ops.MX_INT8, "silu", x, arr(63, np.float32), c8, s, 1, 64)
+    with pytest.raises(KeyError):
+        ops.act_mul_mx(ops.MX_INT8, "relu", x, x, c8, s, 1, 64)
