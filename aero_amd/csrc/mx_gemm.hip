@@ -14,6 +14,8 @@
 // Weights are laid out once, in the order in which the steps take them: 32 rows, then
 // blocks of 32 columns, then the 32 rows' 16 bytes of a block; a step's operand is 1 KB in
 // one piece. Their scales are a dword (four blocks) a row.
+#include <type_traits>
+
 #include "mx.hpp"
 
 #pragma clang fp contract(off)
@@ -23,9 +25,10 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-constexpr int kF8 = 0, kF4 = 4;  // operand formats of the step
+constexpr int kF8 = 0, kF6 = 2, kF4 = 4;  // operand formats of the step
 
 struct MxGemm {
     const uint8_t* x;    // codes [T][K] or [T][K/2]
@@ -71,7 +74,7 @@ __device__ __forceinline__ void halves(uint32_t c, int& hi, int& lo) {
 
 __device__ __forceinline__ v8i wide(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
-// 32 weight rows and 32 tokens a workgroup, its four waves each every fourth 128 columns,
+// Few tokens: 32 weight rows and up to 32 tokens a workgroup, its four waves each every fourth 128 columns,
 // their sums joined in LDS. Lane l of a step holds row (token) l % 32 and, of 64 columns,
 // block l / 32 of 4-bit operands; of e4m3 ones the bytes 16 (l / 32) .. of either block.
 template <int FMT>
@@ -146,6 +149,277 @@ void mx_gemm_kernel(MxGemm p) {
         if (n + i < p.N) o[i] = v[i];
 }
 
+// ---------------------------------------------------------- many tokens
+// x as operands, once a call: 32 tokens, then steps of 64 columns. 4 bits: as the weights.
+// 8 bits: the halves as 6-bit floats (e2m3), whose steps against 4-bit operands take half
+// the time of e4m3 ones (35 cycles and 64 measured). There too a number 0 .. 15 is its own
+// code (in units of 1/8). A lane's 24 bytes a half lie as 16 and 8, 64 lanes side by side:
+// 1024 + 512 for the high halves, the same for the low ones.
+template <int FMT>
+constexpr int kStepBytes = FMT == AERO_MX_INT8 ? 3072 : 1024;
+
+// 32 codes of 6 bits, the first lowest, from 32 bytes' signs (bit 7) and low halves.
+__device__ __forceinline__ void pack6(const uint32_t (&b)[8], uint32_t (&o)[6]) {
+    uint64_t q[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const uint32_t v = b[i >> 2] >> (8 * (i & 3));
+        const uint64_t c = (v & 15u) | ((v >> 2) & 32u);
+        const int at = 6 * i, w = at >> 6, s = at & 63;
+        q[w] |= c << s;
+        if (s > 58) q[w + 1] |= c >> (64 - s);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        o[2 * i] = (uint32_t)q[i];
+        o[2 * i + 1] = (uint32_t)(q[i] >> 32);
+    }
+}
+
+// One block of one token a lane; tokens and blocks past the end are zeros.
+template <int FMT>
+__global__ __launch_bounds__(256)
+void mx_operand_kernel(const uint8_t* x, const uint8_t* xs, uint8_t* o, uint8_t* os, int64_t T, int KB,
+                       int KP, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int lane = (int)(i & 63), r = lane & 31;
+    const int64_t step = i >> 6, tile = step / (2 * KP);
+    const int kb = 2 * (int)(step - tile * (2 * KP)) + (lane >> 5);
+    const int64_t tok = tile * 32 + r;
+    const bool in = tok < T && kb < KB;
+    const int low = FMT == AERO_MX_INT8 ? 4 : 0;
+    int s = in ? xs[tok * KB + kb] : low;
+    os[((tile * KP + (kb >> 2)) * 32 + r) * 4 + (kb & 3)] = (uint8_t)(s < low ? low : s);
+    uint8_t* to = o + step * kStepBytes<FMT>;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (FMT == AERO_MX_FP4) {
+        reinterpret_cast<uint4*>(to)[lane] =
+            in ? *reinterpret_cast<const uint4*>(x + (tok * KB + kb) * 16) : zero;
+    } else {
+        const uint4* p = reinterpret_cast<const uint4*>(x + (tok * KB + kb) * 32);
+        const uint4 c0 = in ? p[0] : zero, c1 = in ? p[1] : zero;
+        const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        uint32_t hi[8], lo[8], h[6], l[6];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            int a, b;
+            halves(c[k], a, b);
+            hi[k] = (uint32_t)a;
+            lo[k] = (uint32_t)b;
+        }
+        pack6(hi, h);
+        pack6(lo, l);
+        reinterpret_cast<uint4*>(to)[lane] = make_uint4(h[0], h[1], h[2], h[3]);
+        reinterpret_cast<uint2*>(to + 1024)[lane] = make_uint2(h[4], h[5]);
+        reinterpret_cast<uint4*>(to + 1536)[lane] = make_uint4(l[0], l[1], l[2], l[3]);
+        reinterpret_cast<uint2*>(to + 2560)[lane] = make_uint2(l[4], l[5]);
+    }
+}
+
+// A value the compiler knows nothing about. (The host pass has no such registers.)
+template <typename T>
+__device__ __forceinline__ void opaque(T& v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(v));
+#endif
+}
+
+struct MxTiles {
+    const uint8_t* w;    // operand codes and scales of both sides
+    const uint8_t* ws;
+    const uint8_t* x;
+    const uint8_t* xs;
+    float* y;
+    int64_t T, N;
+    int KP, steps;       // 128-column groups, 64-column steps
+    int nt, tt;          // 32-row and 32-token tiles
+    int bn, bt;          // workgroups along each
+    bool vec;
+};
+
+// A workgroup of GN x GT waves, a wave WA weight tiles by XB token tiles of 32. Steps of 64
+// columns go through NB buffers in LDS by direct loads of 1 KB, each wave its share.
+template <int FMT, int WA, int XB, int GN, int GT>
+struct MxShape {
+    static constexpr int NW = GN * GT, TN = WA * GN, TT = XB * GT, NB = 3;
+    static constexpr int XC = kStepBytes<FMT> / 1024;
+    static constexpr int SC = (TN + TT + 7) / 8;                 // pieces of 8 tiles' scales
+    static constexpr int PIECES = TN + TT * XC + SC;
+    static constexpr int LOADS = (PIECES + NW - 1) / NW;
+    static constexpr int XOFF = TN * 1024, SOFF = XOFF + TT * XC * 1024;
+    static constexpr int BYTES = SOFF + SC * 1024;
+};
+
+template <int FMT, int WA, int XB, int GN, int GT, int WAVES>
+__global__ __launch_bounds__(64 * GN * GT, WAVES)
+void mx_tiles_kernel(MxTiles p) {
+    using S = MxShape<FMT, WA, XB, GN, GT>;
+    __shared__ __attribute__((aligned(16))) uint8_t buf0[S::BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t buf1[S::BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t buf2[S::BYTES];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, g = lane >> 5;
+    // each XCD (workgroups go round them in turn) takes a run of neighbouring tiles, the
+    // token tiles of one weight tile one after another
+    const int per = gridDim.x >> 3;
+    const int at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (at >= p.bn * p.bt) return;
+    const int n0 = (at / p.bt) * S::TN, t0 = (at % p.bt) * S::TT;
+
+    // This wave's pieces of a step, the scales' first: where they begin, how far a step goes.
+    // (A piece past the last is the wave's one before once more, to the same place.)
+    static_assert(S::SC <= S::NW, "the scales' pieces are first ones");
+    const uint8_t* src[S::LOADS];
+    int dst[S::LOADS], stride[S::LOADS];
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+        int c = wave + S::NW * i;
+        if (c >= S::PIECES) c -= S::NW;
+        c -= S::SC;
+        dst[i] = c * 1024;
+        if (c < S::TN) {
+            src[i] = p.w + (int64_t)min(n0 + max(c, 0), p.nt - 1) * p.KP * 2048;
+            stride[i] = 1024;
+        } else {
+            const int q = c - S::TN;
+            src[i] = p.x + (int64_t)min(t0 + q / S::XC, p.tt - 1) * p.KP * (2 * kStepBytes<FMT>) +
+                     (q % S::XC) * 1024;
+            stride[i] = kStepBytes<FMT>;
+        }
+    }
+    uint32_t lane16 = lane * 16;
+    opaque(lane16);
+    const uint8_t* first = src[0] + lane16;
+    const int half = wave < S::SC ? 1 : 0;
+    if (wave < S::SC) {       // eight tiles' scales of 128 columns
+        const int k = min(wave * 8 + (lane >> 3), S::TN + S::TT - 1);
+        first = (k < S::TN ? p.ws + (int64_t)min(n0 + k, p.nt - 1) * p.KP * 128
+                           : p.xs + (int64_t)min(t0 + k - S::TN, p.tt - 1) * p.KP * 128) + (lane & 7) * 16;
+        dst[0] = S::SOFF + wave * 1024;
+        stride[0] = 128;
+    }
+    auto fetch = [&](int i, uint8_t* b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < S::LOADS; ++k) {
+            const uint8_t* from = k == 0 ? first + (int64_t)(i >> half) * stride[0]
+                                         : src[k] + (int64_t)i * stride[k] + lane16;
+            uint8_t* to = b + dst[k];
+            __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+        }
+    };
+
+    const int wn = (wave % GN) * WA, wt = (wave / GN) * XB;
+    v16f acc[WA][XB];
+#pragma unroll
+    for (int a = 0; a < WA; ++a)
+#pragma unroll
+        for (int b = 0; b < XB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+
+    // A lane's places in a buffer. (Opaque, so that each stays one register that the buffers
+    // and tiles add constants to.)
+    int oa = wn * 1024 + lane * 16, ox = S::XOFF + wt * kStepBytes<FMT> + lane * 16;
+    int ox8 = ox - lane * 8, osa = S::SOFF + wn * 128 + r * 4, osx = S::SOFF + (S::TN + wt) * 128 + r * 4;
+    opaque(oa);
+    opaque(ox);
+    opaque(ox8);
+    opaque(osa);
+    opaque(osx);
+    auto compute = [&](int i, const uint8_t* buf) __attribute__((always_inline)) {
+        const int sh = 16 * (i & 1) + 8 * g;
+        v4i a[WA];
+        int sa[WA];
+#pragma unroll
+        for (int k = 0; k < WA; ++k) {
+            a[k] = *reinterpret_cast<const v4i*>(buf + oa + k * 1024);
+            sa[k] = (int)(*reinterpret_cast<const uint32_t*>(buf + osa + k * 128) >> sh);
+        }
+#pragma unroll
+        for (int b = 0; b < XB; ++b) {
+            const int at = b * kStepBytes<FMT>;
+            const int sb = (int)(*reinterpret_cast<const uint32_t*>(buf + osx + b * 128) >> sh);
+            if constexpr (FMT == AERO_MX_INT8) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const v4i q = *reinterpret_cast<const v4i*>(buf + ox + at + 1536 * h);
+                    const v2i e = *reinterpret_cast<const v2i*>(buf + ox8 + at + 1536 * h + 1024);
+                    const v4i e4 = __builtin_shufflevector(e, e, 0, 1, -1, -1);
+                    const v8i f = __builtin_shufflevector(q, e4, 0, 1, 2, 3, 4, 5, -1, -1);
+#pragma unroll
+                    for (int k = 0; k < WA; ++k)
+                        acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                            wide(a[k]), f, acc[k][b], kF4, kF6, 0, sa[k], 0, sb - 4 * h);
+                }
+            } else {
+                const v4i q = *reinterpret_cast<const v4i*>(buf + ox + at);
+#pragma unroll
+                for (int k = 0; k < WA; ++k)
+                    acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                        wide(a[k]), wide(q), acc[k][b], kF4, kF4, 0, sa[k], 0, sb);
+            }
+        }
+    };
+    // A step begins when its loads have landed (the next one's may be on their way) and
+    // every wave is done with the step before, whose buffer is then filled again; the last
+    // steps load the last one once more, so that every step is alike. (The marks keep the
+    // copies of this code apart: merged, the compiler could not tell the buffer that is read
+    // from the one that is filled, and would wait for the loads.)
+    auto step = [&](auto k, int i, const uint8_t* b, uint8_t* nb) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt((S::LOADS & 15) | 0x0f70 | ((S::LOADS >> 4) << 14));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        fetch(min(i + 2, p.steps - 1), nb);
+        asm volatile("; buffer %0" ::"n"(decltype(k)::value) : "memory");
+        compute(i, b);
+        asm volatile("; buffer %0 done" ::"n"(decltype(k)::value) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    fetch(0, buf0);
+    fetch(min(1, p.steps - 1), buf1);
+    using K0 = std::integral_constant<int, 0>;
+    using K1 = std::integral_constant<int, 1>;
+    using K2 = std::integral_constant<int, 2>;
+    // (whole rounds of three, then the rest: with an exit after each step the compiler
+    // keeps the sums twice and spills)
+    int i = 0;
+    for (; i + 3 <= p.steps; i += 3) {
+        step(K0{}, i, buf0, buf2);
+        step(K1{}, i + 1, buf1, buf0);
+        step(K2{}, i + 2, buf2, buf1);
+    }
+    if (i < p.steps) step(K0{}, i, buf0, buf2);
+    if (i + 1 < p.steps) step(K1{}, i + 1, buf1, buf0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);       // (no load is on its way when the wave ends)
+
+    constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
+#pragma unroll
+    for (int b = 0; b < XB; ++b) {
+        const int64_t tok = (int64_t)(t0 + wt + b) * 32 + r;
+        if (tok >= p.T) continue;
+#pragma unroll
+        for (int a = 0; a < WA; ++a) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t n = (int64_t)(n0 + wn + a) * 32 + 8 * q + 4 * g;
+                float* o = p.y + tok * p.N + n;
+                const v4f v = {acc[a][b][4 * q] * UNIT, acc[a][b][4 * q + 1] * UNIT,
+                               acc[a][b][4 * q + 2] * UNIT, acc[a][b][4 * q + 3] * UNIT};
+                if (p.vec && n + 4 <= p.N) {
+                    *reinterpret_cast<v4f*>(o) = v;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < p.N) o[i] = v[i];
+                }
+            }
+        }
+    }
+}
+
 int64_t tiles32(int64_t n) { return (n + 31) / 32; }
 
 bool weight_sizes_ok(const char* what, int64_t n_rows, int64_t n_cols) {
@@ -160,6 +434,47 @@ bool weight_sizes_ok(const char* what, int64_t n_rows, int64_t n_cols) {
 
 int64_t weight_codes_bytes(int64_t n_rows, int64_t n_cols) {
     return tiles32(n_rows) * ((n_cols + 127) / 128) * 2048;
+}
+
+// Calls of more tokens go through operands in the workspace.
+constexpr int64_t kFewTokens = 32;
+
+template <int FMT>
+int64_t operand_bytes(int64_t n_tok, int KP) {
+    return tiles32(n_tok) * KP * (2 * kStepBytes<FMT> + 128);
+}
+
+template <int FMT, int WA, int XB, int GN, int GT, int WAVES>
+bool launch_tiles(MxTiles p, hipStream_t s) {
+    using S = MxShape<FMT, WA, XB, GN, GT>;
+    p.bn = (p.nt + S::TN - 1) / S::TN;
+    p.bt = (p.tt + S::TT - 1) / S::TT;
+    const int64_t grid = ((int64_t)p.bn * p.bt + 7) / 8 * 8;
+    if (grid > 0x7fffffff) {
+        set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
+        return false;
+    }
+    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, WAVES>, dim3((unsigned)grid),
+                  dim3(64 * S::NW), 0, s, p);
+}
+
+template <int FMT>
+bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
+    const int64_t tt = tiles32(g.T), nt = tiles32(g.N);
+    uint8_t* o = (uint8_t*)ws;
+    uint8_t* os = o + tt * g.KP * (2 * kStepBytes<FMT>);
+    const int64_t n = tt * 32 * 4 * g.KP, blocks = (n + 255) / 256;
+    if (blocks > 0x7fffffff || nt > 0x7fffffff || tt > 0x7fffffff) {
+        set_error("mx_matmul: %lld tokens are too many", (long long)g.T);
+        return false;
+    }
+    if (!launch("mx_operand_kernel", mx_operand_kernel<FMT>, dim3((unsigned)blocks), dim3(256), 0, s, g.x,
+                g.xs, o, os, g.T, g.KB, g.KP, n))
+        return false;
+    const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, g.vec};
+    const int64_t big = ((nt + 7) / 8) * ((tt + 3) / 4);
+    if (big >= tune("mx_big", 256)) return launch_tiles<FMT, 4, 2, 2, 2, 2>(p, s);
+    return launch_tiles<FMT, 2, 1, 2, 2, 2>(p, s);
 }
 
 }  // namespace
@@ -202,7 +517,10 @@ int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, in
     if ((fmt != AERO_MX_INT8 && fmt != AERO_MX_FP4) || n_tok < 0 ||
         !weight_sizes_ok("mx_matmul_workspace", n_rows, n_cols))
         return -1;
-    return 0;
+    if (n_tok <= kFewTokens) return 0;
+    const int KP = (int)((n_cols + 127) / 128);
+    return fmt == AERO_MX_INT8 ? operand_bytes<AERO_MX_INT8>(n_tok, KP)
+                               : operand_bytes<AERO_MX_FP4>(n_tok, KP);
 }
 
 int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, const void* w,
@@ -223,16 +541,20 @@ int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, con
         return 0;
     }
     if (n_tok == 0) return 1;
-    const int64_t tt = tiles32(n_tok);
-    if (tt > 65535) {
-        set_error("mx_matmul: %lld tokens are too many", (long long)n_tok);
-        return 0;
-    }
     const int KB = (int)(n_cols / 32), KP = (KB + 3) / 4;
     MxGemm p{codes, scales, (const uint8_t*)w, (const uint8_t*)w + weight_codes_bytes(n_rows, n_cols), y,
              n_tok, n_rows, KB, KP, aligned16(y) && n_rows % 4 == 0};
-    const dim3 grid((unsigned)tiles32(n_rows), (unsigned)tt);
     const hipStream_t s = (hipStream_t)stream;
+    if (n_tok > kFewTokens) {
+        const int64_t need = aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok);
+        if (workspace == nullptr || !aligned16(workspace) || ws_bytes < need) {
+            set_error("mx_matmul: the workspace takes %lld bytes at a 16-byte address", (long long)need);
+            return 0;
+        }
+        return (fmt == AERO_MX_INT8 ? run_tiles<AERO_MX_INT8>(p, workspace, s)
+                                    : run_tiles<AERO_MX_FP4>(p, workspace, s)) ? 1 : 0;
+    }
+    const dim3 grid((unsigned)tiles32(n_rows));
     return (fmt == AERO_MX_INT8
                 ? launch("mx_gemm_kernel", mx_gemm_kernel<AERO_MX_INT8>, grid, dim3(256), 0, s, p)
                 : launch("mx_gemm_kernel", mx_gemm_kernel<AERO_MX_FP4>, grid, dim3(256), 0, s, p))

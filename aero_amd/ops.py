@@ -13,7 +13,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from .device import DeviceArray, Stream, Workspace, as_ptr
+from .device import DeviceArray, Stream, Workspace, as_ptr, recording_plan
 
 NORM_UNIT_OFFSET = 1
 NORM_L2 = 2
@@ -830,13 +830,16 @@ def mx_matmul(fmt: int, codes: DeviceArray, scales: DeviceArray, w, y: DeviceArr
     """y [n_tok, w.n_rows] = x W^T in fp32: x microscaled rows [n_tok, w.n_cols] in
     fmt, w an mx.MxWeight (4 bits). Products and the sums within a block are exact. The
     workspace grows to the largest call and is kept: calls that overlap on different
-    streams would share its contents."""
+    streams would share its contents. A plan that records the call holds the weights."""
     _mx_rows(fmt, codes, scales, n_tok, w.n_cols)
     _need(y, n_tok * w.n_rows, np.float32, "y")
     L = _lib.lib()
     wsb = int(L.aero_hip_mx_matmul_workspace(fmt, w.n_rows, w.n_cols, n_tok))
     _lib.check(wsb >= 0, "mx_matmul")
     ws = _mx_ws.get(wsb)
+    plan = recording_plan()
+    if plan is not None:
+        plan.hold(w.buf)
     _lib.check(L.aero_hip_mx_matmul(fmt, codes.ptr, scales.ptr, w.buf.ptr, w.buf.nbytes, y.ptr,
                                     w.n_rows, w.n_cols, n_tok, as_ptr(ws),
                                     ws.nbytes if ws is not None else 0, _s(stream)), "mx_matmul")
