@@ -234,15 +234,15 @@ struct MxTiles {
     int64_t T, N;
     int KP, steps;       // 128-column groups, 64-column steps
     int nt, tt;          // 32-row and 32-token tiles
-    int bn, bt;          // workgroups along each
-    bool vec;
+    int bn, bt, group;   // workgroups along each; token tiles side by side
 };
 
 // A workgroup of GN x GT waves, a wave WA weight tiles by XB token tiles of 32. Steps of 64
-// columns go through NB buffers in LDS by direct loads of 1 KB, each wave its share.
+// columns go through NB buffers in LDS by direct loads of 1 KB, each wave its share, NB - 1
+// steps ahead.
 template <int FMT, int WA, int XB, int GN, int GT>
 struct MxShape {
-    static constexpr int NW = GN * GT, TN = WA * GN, TT = XB * GT, NB = 3;
+    static constexpr int NW = GN * GT, TN = WA * GN, TT = XB * GT;
     static constexpr int XC = kStepBytes<FMT> / 1024;
     static constexpr int SC = (TN + TT + 7) / 8;                 // pieces of 8 tiles' scales
     static constexpr int PIECES = TN + TT * XC + SC;
@@ -251,22 +251,28 @@ struct MxShape {
     static constexpr int BYTES = SOFF + SC * 1024;
 };
 
-template <int FMT, int WA, int XB, int GN, int GT, int WAVES>
+template <int FMT, int WA, int XB, int GN, int GT, int NB, int WAVES>
 __global__ __launch_bounds__(64 * GN * GT, WAVES)
 void mx_tiles_kernel(MxTiles p) {
     using S = MxShape<FMT, WA, XB, GN, GT>;
-    __shared__ __attribute__((aligned(16))) uint8_t buf0[S::BYTES];
-    __shared__ __attribute__((aligned(16))) uint8_t buf1[S::BYTES];
-    __shared__ __attribute__((aligned(16))) uint8_t buf2[S::BYTES];
+    // (arrays of their own: the compiler tells a load into one from a read of another)
+#define AERO_MX_BUF(K) __shared__ __attribute__((aligned(16))) uint8_t b##K[K < NB ? S::BYTES : 16]
+    AERO_MX_BUF(0); AERO_MX_BUF(1); AERO_MX_BUF(2); AERO_MX_BUF(3); AERO_MX_BUF(4); AERO_MX_BUF(5);
+    AERO_MX_BUF(6); AERO_MX_BUF(7); AERO_MX_BUF(8); AERO_MX_BUF(9); AERO_MX_BUF(10); AERO_MX_BUF(11);
+#undef AERO_MX_BUF
+    uint8_t* const bufs[12] = {b0, b1, b2, b3, b4, b5, b6, b7, b8, b9, b10, b11};
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, g = lane >> 5;
-    // each XCD (workgroups go round them in turn) takes a run of neighbouring tiles, the
-    // token tiles of one weight tile one after another
+    // Each XCD (workgroups go round them in turn) takes a run of neighbouring tiles: four
+    // token tiles beside one weight tile, then beside the next, so that what runs at a time
+    // on an XCD shares both sides through its L2.
     const int per = gridDim.x >> 3;
     const int at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (at >= p.bn * p.bt) return;
-    const int n0 = (at / p.bt) * S::TN, t0 = (at % p.bt) * S::TT;
+    const int group = at / (p.group * p.bn), rest = at - group * p.group * p.bn;
+    const int width = min(p.group, p.bt - group * p.group);
+    const int n0 = (rest / width) * S::TN, t0 = (group * p.group + rest % width) * S::TT;
 
     // This wave's pieces of a step, the scales' first: where they begin, how far a step goes.
     // (A piece past the last is the wave's one before once more, to the same place.)
@@ -300,9 +306,9 @@ void mx_tiles_kernel(MxTiles p) {
         dst[0] = S::SOFF + wave * 1024;
         stride[0] = 128;
     }
-    auto fetch = [&](int i, uint8_t* b) __attribute__((always_inline)) {
+    auto fetch = [&](int i, uint8_t* b, int k0, int k1) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < S::LOADS; ++k) {
+        for (int k = k0; k < k1; ++k) {
             const uint8_t* from = k == 0 ? first + (int64_t)(i >> half) * stride[0]
                                          : src[k] + (int64_t)i * stride[k] + lane16;
             uint8_t* to = b + dst[k];
@@ -328,93 +334,102 @@ void mx_tiles_kernel(MxTiles p) {
     opaque(ox8);
     opaque(osa);
     opaque(osx);
-    auto compute = [&](int i, const uint8_t* buf) __attribute__((always_inline)) {
-        const int sh = 16 * (i & 1) + 8 * g;
-        v4i a[WA];
-        int sa[WA];
+    // (the step's operands are read first; the loads of a later step go out between groups of
+    // matrix steps, behind which their issue hides)
+    auto compute = [&](int i, const uint8_t* buf, uint8_t* nb) __attribute__((always_inline)) {
+        constexpr int H = FMT == AERO_MX_INT8 ? 2 : 1, GROUPS = XB * H;
+        const int sh = 16 * (i & 1) + 8 * g, next = min(i + NB - 1, p.steps - 1);
+        v4i a[WA], q[XB][H];
+        v2i e[XB][H];
+        int sa[WA], sb[XB];
 #pragma unroll
-        for (int k = 0; k < WA; ++k) {
-            a[k] = *reinterpret_cast<const v4i*>(buf + oa + k * 1024);
-            sa[k] = (int)(*reinterpret_cast<const uint32_t*>(buf + osa + k * 128) >> sh);
-        }
+        for (int k = 0; k < WA; ++k) a[k] = *reinterpret_cast<const v4i*>(buf + oa + k * 1024);
+#pragma unroll
+        for (int k = 0; k < WA; ++k) sa[k] = *reinterpret_cast<const int*>(buf + osa + k * 128);
 #pragma unroll
         for (int b = 0; b < XB; ++b) {
-            const int at = b * kStepBytes<FMT>;
-            const int sb = (int)(*reinterpret_cast<const uint32_t*>(buf + osx + b * 128) >> sh);
-            if constexpr (FMT == AERO_MX_INT8) {
+            sb[b] = *reinterpret_cast<const int*>(buf + osx + b * 128);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const v4i q = *reinterpret_cast<const v4i*>(buf + ox + at + 1536 * h);
-                    const v2i e = *reinterpret_cast<const v2i*>(buf + ox8 + at + 1536 * h + 1024);
-                    const v4i e4 = __builtin_shufflevector(e, e, 0, 1, -1, -1);
-                    const v8i f = __builtin_shufflevector(q, e4, 0, 1, 2, 3, 4, 5, -1, -1);
+            for (int h = 0; h < H; ++h) {
+                const int at = b * kStepBytes<FMT> + 1536 * h;
+                q[b][h] = *reinterpret_cast<const v4i*>(buf + ox + at);
+                if constexpr (H == 2) e[b][h] = *reinterpret_cast<const v2i*>(buf + ox8 + at + 1024);
+            }
+        }
 #pragma unroll
-                    for (int k = 0; k < WA; ++k)
-                        acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                            wide(a[k]), f, acc[k][b], kF4, kF6, 0, sa[k], 0, sb - 4 * h);
+        for (int k = 0; k < WA; ++k) sa[k] = (int)((uint32_t)sa[k] >> sh);
+#pragma unroll
+        for (int b = 0; b < XB; ++b) sb[b] = (int)((uint32_t)sb[b] >> sh);
+#pragma unroll
+        for (int b = 0; b < XB; ++b)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int n = b * H + h;
+                v8i f;
+                if constexpr (H == 2) {
+                    const v4i e4 = __builtin_shufflevector(e[b][h], e[b][h], 0, 1, -1, -1);
+                    f = __builtin_shufflevector(q[b][h], e4, 0, 1, 2, 3, 4, 5, -1, -1);
+                } else {
+                    f = wide(q[b][h]);
                 }
-            } else {
-                const v4i q = *reinterpret_cast<const v4i*>(buf + ox + at);
 #pragma unroll
                 for (int k = 0; k < WA; ++k)
                     acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                        wide(a[k]), wide(q), acc[k][b], kF4, kF4, 0, sa[k], 0, sb);
+                        f, wide(a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb[b] - 4 * h, 0, sa[k]);
+                __builtin_amdgcn_sched_barrier(0);
+                fetch(next, nb, n * S::LOADS / GROUPS, (n + 1) * S::LOADS / GROUPS);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
     };
-    // A step begins when its loads have landed (the next one's may be on their way) and
+    // A step begins when its loads have landed (the next ones' may be on their way) and
     // every wave is done with the step before, whose buffer is then filled again; the last
     // steps load the last one once more, so that every step is alike. (The marks keep the
     // copies of this code apart: merged, the compiler could not tell the buffer that is read
     // from the one that is filled, and would wait for the loads.)
-    auto step = [&](auto k, int i, const uint8_t* b, uint8_t* nb) __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt((S::LOADS & 15) | 0x0f70 | ((S::LOADS >> 4) << 14));
+    auto step = [&](auto k, int i) __attribute__((always_inline)) {
+        constexpr int K = decltype(k)::value, N = (NB - 2) * S::LOADS;
+        __builtin_amdgcn_s_waitcnt((N & 15) | 0x0f70 | ((N >> 4) << 14));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        fetch(min(i + 2, p.steps - 1), nb);
-        asm volatile("; buffer %0" ::"n"(decltype(k)::value) : "memory");
-        compute(i, b);
-        asm volatile("; buffer %0 done" ::"n"(decltype(k)::value) : "memory");
+        asm volatile("; buffer %0" ::"n"(K) : "memory");
+        compute(i, bufs[K], bufs[(K + NB - 1) % NB]);
+        asm volatile("; buffer %0 done" ::"n"(K) : "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    fetch(0, buf0);
-    fetch(min(1, p.steps - 1), buf1);
-    using K0 = std::integral_constant<int, 0>;
-    using K1 = std::integral_constant<int, 1>;
-    using K2 = std::integral_constant<int, 2>;
-    // (whole rounds of three, then the rest: with an exit after each step the compiler
-    // keeps the sums twice and spills)
+#define AERO_MX_EACH(DO) DO(0) DO(1) DO(2) DO(3) DO(4) DO(5) DO(6) DO(7) DO(8) DO(9) DO(10) DO(11)
+#define AERO_MX_FILL(K) if constexpr (K < NB - 1) fetch(min(K, p.steps - 1), bufs[K], 0, S::LOADS);
+#define AERO_MX_ROUND(K) if constexpr (K < NB) step(std::integral_constant<int, K>{}, i + K);
+#define AERO_MX_REST(K) \
+    if constexpr (K < NB - 1) if (i + K < p.steps) step(std::integral_constant<int, K>{}, i + K);
+    AERO_MX_EACH(AERO_MX_FILL)
+    // (whole rounds, then the rest: with an exit after each step the compiler keeps the sums
+    // twice and spills)
     int i = 0;
-    for (; i + 3 <= p.steps; i += 3) {
-        step(K0{}, i, buf0, buf2);
-        step(K1{}, i + 1, buf1, buf0);
-        step(K2{}, i + 2, buf2, buf1);
+    for (; i + NB <= p.steps; i += NB) {
+        AERO_MX_EACH(AERO_MX_ROUND)
     }
-    if (i < p.steps) step(K0{}, i, buf0, buf2);
-    if (i + 1 < p.steps) step(K1{}, i + 1, buf1, buf0);
+    AERO_MX_EACH(AERO_MX_REST)
+#undef AERO_MX_EACH
+#undef AERO_MX_FILL
+#undef AERO_MX_ROUND
+#undef AERO_MX_REST
     __builtin_amdgcn_s_waitcnt(0x0f70);       // (no load is on its way when the wave ends)
 
     constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
+    // lane l holds column l % 32 of 16 tokens: 128 bytes in one piece for each
 #pragma unroll
-    for (int b = 0; b < XB; ++b) {
-        const int64_t tok = (int64_t)(t0 + wt + b) * 32 + r;
-        if (tok >= p.T) continue;
+    for (int a = 0; a < WA; ++a) {
+        const int64_t n = (int64_t)(n0 + wn + a) * 32 + r;
+        if (n >= p.N) continue;
 #pragma unroll
-        for (int a = 0; a < WA; ++a) {
+        for (int b = 0; b < XB; ++b) {
+            const int64_t t1 = (int64_t)(t0 + wt + b) * 32 + 4 * g;
+            float* o = p.y + t1 * p.N + n;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t n = (int64_t)(n0 + wn + a) * 32 + 8 * q + 4 * g;
-                float* o = p.y + tok * p.N + n;
-                const v4f v = {acc[a][b][4 * q] * UNIT, acc[a][b][4 * q + 1] * UNIT,
-                               acc[a][b][4 * q + 2] * UNIT, acc[a][b][4 * q + 3] * UNIT};
-                if (p.vec && n + 4 <= p.N) {
-                    *reinterpret_cast<v4f*>(o) = v;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (n + i < p.N) o[i] = v[i];
-                }
+            for (int i = 0; i < 16; ++i) {
+                const int t = 8 * (i >> 2) + (i & 3);
+                if (t1 + t < p.T) __builtin_nontemporal_store(acc[a][b][i] * UNIT, o + t * p.N);
             }
         }
     }
@@ -444,7 +459,7 @@ int64_t operand_bytes(int64_t n_tok, int KP) {
     return tiles32(n_tok) * KP * (2 * kStepBytes<FMT> + 128);
 }
 
-template <int FMT, int WA, int XB, int GN, int GT, int WAVES>
+template <int FMT, int WA, int XB, int GN, int GT, int NB, int WAVES>
 bool launch_tiles(MxTiles p, hipStream_t s) {
     using S = MxShape<FMT, WA, XB, GN, GT>;
     p.bn = (p.nt + S::TN - 1) / S::TN;
@@ -454,7 +469,7 @@ bool launch_tiles(MxTiles p, hipStream_t s) {
         set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
         return false;
     }
-    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, WAVES>, dim3((unsigned)grid),
+    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, NB, WAVES>, dim3((unsigned)grid),
                   dim3(64 * S::NW), 0, s, p);
 }
 
@@ -471,10 +486,12 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
     if (!launch("mx_operand_kernel", mx_operand_kernel<FMT>, dim3((unsigned)blocks), dim3(256), 0, s, g.x,
                 g.xs, o, os, g.T, g.KB, g.KP, n))
         return false;
-    const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, g.vec};
+    const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, tune("mx_group", 4)};
     const int64_t big = ((nt + 7) / 8) * ((tt + 3) / 4);
-    if (big >= tune("mx_big", 256)) return launch_tiles<FMT, 4, 2, 2, 2, 2>(p, s);
-    return launch_tiles<FMT, 2, 1, 2, 2, 2>(p, s);
+    if (big >= tune("mx_big", 256)) return launch_tiles<FMT, 4, 2, 2, 2, 3, 2>(p, s);
+    if (tune("mx_nb", 6) == 3) return launch_tiles<FMT, 2, 1, 2, 2, 3, 2>(p, s);
+    if (tune("mx_nb", 6) == 12) return launch_tiles<FMT, 2, 1, 2, 2, 12, 1>(p, s);
+    return launch_tiles<FMT, 2, 1, 2, 2, 6, 2>(p, s);
 }
 
 }  // namespace
