@@ -373,12 +373,14 @@ void mx_tiles_kernel(MxTiles p) {
                     f = wide(q[b][h]);
                 }
 #pragma unroll
-                for (int k = 0; k < WA; ++k)
+                for (int k = 0; k < WA; ++k) {
                     acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
                         f, wide(a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb[b] - 4 * h, 0, sa[k]);
-                __builtin_amdgcn_sched_barrier(0);
-                fetch(next, nb, n * S::LOADS / GROUPS, (n + 1) * S::LOADS / GROUPS);
-                __builtin_amdgcn_sched_barrier(0);
+                    const int at = n * WA + k;
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(next, nb, at * S::LOADS / (GROUPS * WA), (at + 1) * S::LOADS / (GROUPS * WA));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
     };
     // A step begins when its loads have landed (the next ones' may be on their way) and
@@ -424,6 +426,229 @@ void mx_tiles_kernel(MxTiles p) {
         if (n >= p.N) continue;
 #pragma unroll
         for (int b = 0; b < XB; ++b) {
+            const int64_t t1 = (int64_t)(t0 + wt + b) * 32 + 4 * g;
+            float* o = p.y + t1 * p.N + n;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int t = 8 * (i >> 2) + (i & 3);
+                if (t1 + t < p.T) __builtin_nontemporal_store(acc[a][b][i] * UNIT, o + t * p.N);
+            }
+        }
+    }
+}
+
+// The largest calls: 256 weight rows by 256 tokens a workgroup of four waves, each 128 by
+// 128 (its 16 tiles of sums take half of a SIMD's registers: one wave each). LDS carries the
+// tokens only, stages of 128 columns; a wave loads its weights straight into registers, two
+// stages ahead. With both sides in LDS the reads and the direct loads' writes take about as
+// many of its cycles as there are matrix steps; so they take half.
+// A stage is eight groups of matrix steps (four with x in 4 bits). The operands of a group
+// are read while the group before runs, those of a stage's first while the last one of the
+// stage before does: the barrier that a stage begins with stands in front of that.
+template <int FMT>
+struct MxWide {
+    static constexpr int H = FMT == AERO_MX_INT8 ? 2 : 1;        // halves
+    static constexpr int BT = FMT == AERO_MX_INT8 ? 1 : 2;       // token tiles a group
+    static constexpr int GROUPS = 8 / BT;
+    static constexpr int XC = 2 * kStepBytes<FMT> / 1024;        // KB of a token tile's stage
+    static constexpr int PIECES = 8 * XC + 1, LOADS = (PIECES + 3) / 4;
+    static constexpr int SOFF = 8 * XC * 1024, BYTES = SOFF + 1024;
+    static constexpr int VMEM = LOADS + 12;                      // and the weights' loads
+};
+
+template <int FMT>
+__global__ __launch_bounds__(256, 1)
+void mx_wide_kernel(MxTiles p) {
+    using S = MxWide<FMT>;
+    __shared__ __attribute__((aligned(16))) uint8_t b0[S::BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t b1[S::BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t b2[S::BYTES];
+    uint8_t* const bufs[3] = {b0, b1, b2};
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, g = lane >> 5;
+    const int per = gridDim.x >> 3;
+    const int at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (at >= p.bn * p.bt) return;
+    const int group = at / (p.group * p.bn), rest = at - group * p.group * p.bn;
+    const int width = min(p.group, p.bt - group * p.group);
+    const int n0 = (rest / width) * 8, t0 = (group * p.group + rest % width) * 8;
+    const int wn = (wave & 1) * 4, wt = (wave >> 1) * 4;
+
+    // this wave's pieces of a stage's tokens (the first wave's first: their scales), and its
+    // weights
+    uint32_t lane16 = lane * 16, lane4 = r * 4;
+    opaque(lane16);
+    opaque(lane4);
+    const uint8_t* src[S::LOADS];
+    int dst[S::LOADS];
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+        int c = wave + 4 * i;
+        if (c >= S::PIECES) c -= 4;
+        c = max(c - 1, 0);
+        dst[i] = c * 1024;
+        src[i] = p.x + (int64_t)min(t0 + c / S::XC, p.tt - 1) * p.KP * (S::XC * 1024) + (c % S::XC) * 1024;
+    }
+    const uint8_t* first = src[0] + lane16;
+    int first_stride = S::XC * 1024;
+    if (wave == 0) {
+        first = p.xs + (int64_t)min(t0 + (lane >> 3), p.tt - 1) * p.KP * 128 + (lane & 7) * 16;
+        first_stride = 128;
+        dst[0] = S::SOFF;
+    }
+    auto piece = [&](int i, uint8_t* b, int k0, int k1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = k0; k < k1; ++k) {
+            const uint8_t* from = k == 0 ? first + (int64_t)i * first_stride
+                                         : src[k] + (int64_t)i * (S::XC * 1024) + lane16;
+            uint8_t* to = b + dst[k];
+            __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+        }
+    };
+    const uint8_t* wp[4];
+    const uint8_t* wsp[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        const int64_t tile = min(n0 + wn + a, p.nt - 1);
+        wp[a] = p.w + tile * p.KP * 2048;
+        wsp[a] = p.ws + tile * p.KP * 128;
+    }
+    v4i w[3][2][4];
+    int sw[3][4];
+    auto weights = [&](int i, int set, int n) __attribute__((always_inline)) {   // the n-th of 12 loads
+        const int64_t k = i;
+        const int a = n / 3;
+        if (n % 3 < 2)
+            w[set][n % 3][a] = *reinterpret_cast<const v4i*>(wp[a] + k * 2048 + n % 3 * 1024 + lane16);
+        else
+            sw[set][a] = *reinterpret_cast<const int*>(wsp[a] + k * 128 + lane4);
+    };
+    auto load = [&](int i, int set, uint8_t* b, int k0, int k1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = k0; k < k1; ++k) {
+            if (k < S::LOADS)
+                piece(i, b, k, k + 1);
+            else
+                weights(i, set, k - S::LOADS);
+        }
+    };
+
+    v16f acc[4][4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+
+    struct Frag {
+        v4i q[S::BT][S::H];
+        v2i e[S::BT][S::H];
+        int s[S::BT];
+    };
+    int ox = wt * (S::XC * 1024) + lane * 16, ox8 = ox - lane * 8, osx = S::SOFF + wt * 128 + r * 4;
+    opaque(ox);
+    opaque(ox8);
+    opaque(osx);
+    // group n: columns 64 (n / (4 / BT)) .. of the stage, token tiles BT (n % (4 / BT)) ..
+    auto read = [&](Frag& f, const uint8_t* b, int n) __attribute__((always_inline)) {
+        const int j = n / (4 / S::BT), b0 = n % (4 / S::BT) * S::BT;
+#pragma unroll
+        for (int x = 0; x < S::BT; ++x) {
+            const int off = (b0 + x) * (S::XC * 1024) + j * kStepBytes<FMT>;
+#pragma unroll
+            for (int h = 0; h < S::H; ++h) {
+                f.q[x][h] = *reinterpret_cast<const v4i*>(b + ox + off + 1536 * h);
+                if constexpr (S::H == 2)
+                    f.e[x][h] = *reinterpret_cast<const v2i*>(b + ox8 + off + 1536 * h + 1024);
+            }
+            f.s[x] = *reinterpret_cast<const int*>(b + osx + (b0 + x) * 128);
+        }
+    };
+    const int sh0 = 8 * g, sh1 = 16 + 8 * g;
+    Frag f0, f1;
+    auto stage = [&](auto kk, int i) __attribute__((always_inline)) {
+        constexpr int K = decltype(kk)::value, K1 = (K + 1) % 3, K2 = (K + 2) % 3;
+        const int next = min(i + 2, p.KP - 1);
+        int sa[2][4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            sa[0][a] = (int)((uint32_t)sw[K][a] >> sh0);
+            sa[1][a] = (int)((uint32_t)sw[K][a] >> sh1);
+        }
+#pragma unroll
+        for (int n = 0; n < S::GROUPS; ++n) {
+            Frag& cur = n & 1 ? f1 : f0;
+            Frag& nxt = n & 1 ? f0 : f1;
+            const int j = n / (4 / S::BT), b0 = n % (4 / S::BT) * S::BT;
+            if (n + 1 < S::GROUPS) {
+                read(nxt, bufs[K], n + 1);
+            } else {
+                // every wave has read this stage, and the next one has landed
+                __builtin_amdgcn_s_waitcnt((S::VMEM & 15) | 0x0070 | ((S::VMEM >> 4) << 14));
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                asm volatile("; buffer %0" ::"n"(K1) : "memory");
+                read(nxt, bufs[K1], 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < S::BT; ++x)
+#pragma unroll
+                for (int h = 0; h < S::H; ++h) {
+                    v8i f;
+                    if constexpr (S::H == 2) {
+                        const v4i e4 = __builtin_shufflevector(cur.e[x][h], cur.e[x][h], 0, 1, -1, -1);
+                        f = __builtin_shufflevector(cur.q[x][h], e4, 0, 1, 2, 3, 4, 5, -1, -1);
+                    } else {
+                        f = wide(cur.q[x][h]);
+                    }
+                    const int sb = (int)((uint32_t)cur.s[x] >> (j ? sh1 : sh0)) - 4 * h;
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        acc[a][b0 + x] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                            f, wide(w[K][j][a]), acc[a][b0 + x], S::H == 2 ? kF6 : kF4, kF4, 0, sb, 0,
+                            sa[j][a]);
+                        // (one load at a time, each behind a matrix step)
+                        constexpr int M = (S::GROUPS - 1) * 8;
+                        const int m = n * 8 + (x * S::H + h) * 4 + a;
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (m < M) load(next, K2, bufs[K2], m * S::VMEM / M, (m + 1) * S::VMEM / M);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+        }
+    };
+    load(0, 0, b0, 0, S::VMEM);
+    load(min(1, p.KP - 1), 1, b1, 0, S::VMEM);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((S::VMEM & 15) | 0x0f70 | ((S::VMEM >> 4) << 14));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(f0, b0, 0);
+    using K0 = std::integral_constant<int, 0>;
+    using K1 = std::integral_constant<int, 1>;
+    using K2 = std::integral_constant<int, 2>;
+    int i = 0;
+    for (; i + 3 <= p.KP; i += 3) {
+        stage(K0{}, i);
+        stage(K1{}, i + 1);
+        stage(K2{}, i + 2);
+    }
+    if (i < p.KP) stage(K0{}, i);
+    if (i + 1 < p.KP) stage(K1{}, i + 1);
+    __builtin_amdgcn_s_waitcnt(0x0f70);       // (no load is on its way when the wave ends)
+
+    constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        const int64_t n = (int64_t)(n0 + wn + a) * 32 + r;
+        if (n >= p.N) continue;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
             const int64_t t1 = (int64_t)(t0 + wt + b) * 32 + 4 * g;
             float* o = p.y + t1 * p.N + n;
 #pragma unroll
@@ -487,6 +712,14 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
                 g.xs, o, os, g.T, g.KB, g.KP, n))
         return false;
     const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, tune("mx_group", 4)};
+    const int64_t wide = ((nt + 7) / 8) * ((tt + 7) / 8);
+    if (wide >= tune("mx_wide", 200)) {
+        MxTiles q = p;
+        q.bn = (int)((nt + 7) / 8);
+        q.bt = (int)((tt + 7) / 8);
+        return launch("mx_wide_kernel", mx_wide_kernel<FMT>, dim3((unsigned)((wide + 7) / 8 * 8)), dim3(256),
+                      0, s, q);
+    }
     const int64_t big = ((nt + 7) / 8) * ((tt + 3) / 4);
     if (big >= tune("mx_big", 256)) return launch_tiles<FMT, 4, 2, 2, 2, 3, 2>(p, s);
     if (tune("mx_nb", 6) == 3) return launch_tiles<FMT, 2, 1, 2, 2, 3, 2>(p, s);
