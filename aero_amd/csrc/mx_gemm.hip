@@ -74,37 +74,82 @@ __device__ __forceinline__ void halves(uint32_t c, int& hi, int& lo) {
 
 __device__ __forceinline__ v8i wide(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
-// Few tokens: 32 weight rows and up to 32 tokens a workgroup, its four waves each every fourth 128 columns,
-// their sums joined in LDS. Lane l of a step holds row (token) l % 32 and, of 64 columns,
-// block l / 32 of 4-bit operands; of e4m3 ones the bytes 16 (l / 32) .. of either block.
-template <int FMT>
-__global__ __launch_bounds__(256)
-void mx_gemm_kernel(MxGemm p) {
-    __shared__ v4f part[4][4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = lane & 31, g = lane >> 5;
-    const int64_t tile = blockIdx.x, t0 = (int64_t)blockIdx.y * 32;
-    const int64_t tok = t0 + r < p.T ? t0 + r : p.T - 1;
-    const uint8_t* wt = p.w + (tile * (4 * p.KP) * 32 + r) * 16;
-    const uint8_t* wst = p.ws + (tile * p.KP * 32 + r) * 4;
-    const uint8_t* xt = p.x + tok * p.KB * (FMT == AERO_MX_INT8 ? 32 : 16);
-    const uint8_t* xst = p.xs + tok * p.KB;
-    v16f acc;
+// ----------------------------------------------------------- few tokens
+// The weights' bytes count. A workgroup takes 16 WA rows and up to 16 XB tokens; its waves take
+// every NW-th 128 columns, D of them on their way at a time, and x as it lies in memory
+// (16x16x128 steps: lane l holds row or token l % 16, of 4-bit operands block l / 16 of the 128
+// columns, of e4m3 ones the bytes 16 (l / 16) .. of either half of them). The waves' sums are
+// joined in LDS, in the order of the waves.
+template <int FMT, int WA, int XB, int NW, int D>
+__global__ __launch_bounds__(64 * NW)
+void mx_stream_kernel(MxGemm p) {
+    constexpr bool I8 = FMT == AERO_MX_INT8;
+    __shared__ v4f part[NW][XB][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * WA), last = ((p.N + 31) >> 5) * 32 - 16;
+
+    const uint8_t* wt[WA];
+    const uint8_t* wst[WA];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-    const v4i zero = {0, 0, 0, 0};
-    for (int k = wave; k < p.KP; k += 4) {
-        const uint32_t sw = *reinterpret_cast<const uint32_t*>(wst + (int64_t)k * 128);
+    for (int a = 0; a < WA; ++a) {
+        const int64_t n = min(n0 + 16 * a, last), tile = n >> 5;
+        const int row = (int)(n & 31) + r;
+        wt[a] = p.w + ((tile * (4 * p.KP) + q) * 32 + row) * 16;
+        wst[a] = p.ws + (tile * p.KP * 32 + row) * 4 + q;
+    }
+    const uint8_t* xt[XB];
+    const uint8_t* xst[XB];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int k0 = 4 * k + 2 * j, kb = k0 + g;   // the step's first block; this lane's
-            const v4i a = *reinterpret_cast<const v4i*>(wt + (int64_t)kb * 512);
-            const int sa = (int)(sw >> (8 * (2 * j + g)));
-            int sb = kb < p.KB ? xst[kb] : 0;
-            if constexpr (FMT == AERO_MX_INT8) {
-                v4i c0 = zero, c1 = zero;
-                if (k0 < p.KB) c0 = *reinterpret_cast<const v4i*>(xt + k0 * 32 + 16 * g);
-                if (k0 + 1 < p.KB) c1 = *reinterpret_cast<const v4i*>(xt + k0 * 32 + 32 + 16 * g);
+    for (int b = 0; b < XB; ++b) {
+        const int64_t tok = min((int64_t)(16 * b + r), p.T - 1);
+        xt[b] = p.x + tok * p.KB * (I8 ? 32 : 16) + 16 * q;
+        xst[b] = p.xs + tok * p.KB;
+    }
+
+    v4i w[D][WA], x0[D][XB], x1[D][XB];
+    int sw[D][WA], sx[D][XB];
+    auto load = [&](int d, int kk) __attribute__((always_inline)) {
+        const int k = min(kk, p.KP - 1);
+#pragma unroll
+        for (int a = 0; a < WA; ++a) {
+            w[d][a] = *reinterpret_cast<const v4i*>(wt[a] + (int64_t)k * 2048);
+            sw[d][a] = wst[a][(int64_t)k * 128];
+        }
+        // (places past a row's last block: its last one, taken out below)
+        const int kb = 4 * k + q, top = p.KB - 1;
+#pragma unroll
+        for (int b = 0; b < XB; ++b) {
+            if constexpr (I8) {
+                const int k0 = min(4 * k + (q >> 1), top), k1 = min(4 * k + 2 + (q >> 1), top);
+                x0[d][b] = *reinterpret_cast<const v4i*>(xt[b] + 32 * k0 - 32 * (q >> 1));
+                x1[d][b] = *reinterpret_cast<const v4i*>(xt[b] + 32 * k1 - 32 * (q >> 1));
+            } else {
+                x0[d][b] = *reinterpret_cast<const v4i*>(xt[b] + 16 * (min(kb, top) - q));
+            }
+            sx[d][b] = xst[b][min(kb, top)];
+        }
+    };
+    v4f acc[WA][XB];
+#pragma unroll
+    for (int a = 0; a < WA; ++a)
+#pragma unroll
+        for (int b = 0; b < XB; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int d, int k) __attribute__((always_inline)) {
+        const bool whole = 4 * k + 4 <= p.KB;
+        const v4i zero = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < XB; ++b) {
+            int s = sx[d][b];
+            if constexpr (I8) {
+                v4i c0 = x0[d][b], c1 = x1[d][b];
+                s = s < 4 ? 4 : s;
+                if (!whole) {
+                    if (4 * k + (q >> 1) >= p.KB) c0 = zero;
+                    if (4 * k + 2 + (q >> 1) >= p.KB) c1 = zero;
+                    if (4 * k + q >= p.KB) s = 4;
+                }
                 v8i hi, lo;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -114,39 +159,63 @@ void mx_gemm_kernel(MxGemm p) {
                     halves((uint32_t)c1[i], h, l);
                     hi[4 + i] = h; lo[4 + i] = l;
                 }
-                sb = sb < 4 ? 4 : sb;
-                acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), hi, acc, kF4, kF8, 0, sa,
-                                                                      0, sb);
-                acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), lo, acc, kF4, kF8, 0, sa,
-                                                                      0, sb - 4);
+#pragma unroll
+                for (int a = 0; a < WA; ++a)
+                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        wide(w[d][a]), hi, acc[a][b], kF4, kF8, 0, sw[d][a], 0, s);
+#pragma unroll
+                for (int a = 0; a < WA; ++a)
+                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        wide(w[d][a]), lo, acc[a][b], kF4, kF8, 0, sw[d][a], 0, s - 4);
             } else {
-                v4i b = zero;
-                if (kb < p.KB) b = *reinterpret_cast<const v4i*>(xt + kb * 16);
-                acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), acc, kF4, kF4, 0,
-                                                                      sa, 0, sb);
+                v4i c0 = x0[d][b];
+                if (!whole && 4 * k + q >= p.KB) {
+                    c0 = zero;
+                    s = 0;
+                }
+#pragma unroll
+                for (int a = 0; a < WA; ++a)
+                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        wide(w[d][a]), wide(c0), acc[a][b], kF4, kF4, 0, sw[d][a], 0, s);
             }
         }
-    }
+    };
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const v4f v = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-        part[wave][q][lane] = v;
-    }
-    __syncthreads();
-    v4f v = part[0][wave][lane];
+    for (int d = 0; d < D; ++d) load(d, wave + d * NW);
+    for (int k = wave; k < p.KP; k += D * NW) {
 #pragma unroll
-    for (int k = 1; k < 4; ++k) v += part[k][wave][lane];
-    if constexpr (FMT == AERO_MX_INT8) v *= 128.f;   // h 16 / 64 = (h 2^-9) 2^7
-    const int64_t n = tile * 32 + 8 * wave + 4 * g;
-    if (t0 + r >= p.T) return;
-    float* o = p.y + (t0 + r) * p.N + n;
-    if (p.vec && n + 4 <= p.N) {
-        *reinterpret_cast<v4f*>(o) = v;
-        return;
+        for (int d = 0; d < D; ++d) {
+            const int kk = k + d * NW;
+            if (kk < p.KP) compute(d, kk);
+            if (kk + D * NW < p.KP) load(d, kk + D * NW);
+        }
     }
+
+    constexpr float UNIT = I8 ? 128.f : 1.f;            // h 16 / 64 = (h 2^-9) 2^7
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (n + i < p.N) o[i] = v[i];
+    for (int a = 0; a < WA; ++a) {
+        if (a > 0) __syncthreads();
+#pragma unroll
+        for (int b = 0; b < XB; ++b) part[wave][b][lane] = acc[a][b];
+        __syncthreads();
+        const int64_t n = n0 + 16 * a + 4 * q;
+        for (int b = wave; b < XB; b += NW) {
+            v4f v = part[0][b][lane];
+#pragma unroll
+            for (int k = 1; k < NW; ++k) v += part[k][b][lane];
+            v *= UNIT;
+            const int64_t tok = 16 * b + r;
+            if (tok >= p.T) continue;
+            float* o = p.y + tok * p.N + n;
+            if (p.vec && n + 4 <= p.N) {
+                *reinterpret_cast<v4f*>(o) = v;
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < p.N) o[i] = v[i];
+        }
+    }
 }
 
 // ---------------------------------------------------------- many tokens
@@ -158,62 +227,83 @@ void mx_gemm_kernel(MxGemm p) {
 template <int FMT>
 constexpr int kStepBytes = FMT == AERO_MX_INT8 ? 3072 : 1024;
 
-// 32 codes of 6 bits, the first lowest, from 32 bytes' signs (bit 7) and low halves.
+// 32 codes of 6 bits, the first lowest, from bytes of a sign (bit 7) and a number 0 .. 15.
 __device__ __forceinline__ void pack6(const uint32_t (&b)[8], uint32_t (&o)[6]) {
-    uint64_t q[3] = {0, 0, 0};
+    uint32_t d[8];       // four codes each, 24 bits
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const uint32_t v = b[i >> 2] >> (8 * (i & 3));
-        const uint64_t c = (v & 15u) | ((v >> 2) & 32u);
-        const int at = 6 * i, w = at >> 6, s = at & 63;
-        q[w] |= c << s;
-        if (s > 58) q[w + 1] |= c >> (64 - s);
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t c = (b[i] & 0x0F0F0F0Fu) | ((b[i] >> 2) & 0x20202020u);
+        const uint32_t e = (c & 0x003F003Fu) | ((c >> 2) & 0x0FC00FC0u);
+        d[i] = (e & 0xFFFu) | ((e >> 4) & 0xFFF000u);
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        o[2 * i] = (uint32_t)q[i];
-        o[2 * i + 1] = (uint32_t)(q[i] >> 32);
+    for (int i = 0; i < 2; ++i) {
+        o[3 * i] = d[4 * i] | (d[4 * i + 1] << 24);
+        o[3 * i + 1] = (d[4 * i + 1] >> 8) | (d[4 * i + 2] << 16);
+        o[3 * i + 2] = (d[4 * i + 2] >> 16) | (d[4 * i + 3] << 8);
     }
 }
 
-// One block of one token a lane; tokens and blocks past the end are zeros.
+// Two blocks of one token (columns 32 g .. and 64 + 32 g .. of 128) a lane; tokens and blocks
+// past the end are zeros.
 template <int FMT>
 __global__ __launch_bounds__(256)
 void mx_operand_kernel(const uint8_t* x, const uint8_t* xs, uint8_t* o, uint8_t* os, int64_t T, int KB,
                        int KP, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    const int lane = (int)(i & 63), r = lane & 31;
-    const int64_t step = i >> 6, tile = step / (2 * KP);
-    const int kb = 2 * (int)(step - tile * (2 * KP)) + (lane >> 5);
-    const int64_t tok = tile * 32 + r;
-    const bool in = tok < T && kb < KB;
-    const int low = FMT == AERO_MX_INT8 ? 4 : 0;
-    int s = in ? xs[tok * KB + kb] : low;
-    os[((tile * KP + (kb >> 2)) * 32 + r) * 4 + (kb & 3)] = (uint8_t)(s < low ? low : s);
-    uint8_t* to = o + step * kStepBytes<FMT>;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (FMT == AERO_MX_FP4) {
-        reinterpret_cast<uint4*>(to)[lane] =
-            in ? *reinterpret_cast<const uint4*>(x + (tok * KB + kb) * 16) : zero;
-    } else {
-        const uint4* p = reinterpret_cast<const uint4*>(x + (tok * KB + kb) * 32);
-        const uint4 c0 = in ? p[0] : zero, c1 = in ? p[1] : zero;
-        const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        uint32_t hi[8], lo[8], h[6], l[6];
+    constexpr int LOW = kMxLow<FMT>;
+    const int lane = (int)(i & 63), r = lane & 31, g = lane >> 5;
+    const uint32_t group = (uint32_t)(i >> 6), tile = group / (uint32_t)KP;
+    const int k0 = 4 * (int)(group - tile * KP);
+    const int64_t row = (int64_t)tile * 32 + r;
+    // (loads from clamped places, all at once, then what is past the end taken out)
+    const int64_t at = min(row, T - 1) * KB;
+    constexpr int PIECE = FMT == AERO_MX_INT8 ? 2 : 1;      // 16 bytes a block
+    uint4 c[2][PIECE];
+    uint32_t s[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            int a, b;
-            halves(c[k], a, b);
-            hi[k] = (uint32_t)a;
-            lo[k] = (uint32_t)b;
+    for (int j = 0; j < 2; ++j) {
+        const uint4* p = reinterpret_cast<const uint4*>(x) + (at + min(k0 + 2 * j + g, KB - 1)) * PIECE;
+#pragma unroll
+        for (int h = 0; h < PIECE; ++h) c[j][h] = p[h];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = xs[at + min(k0 + k, KB - 1)];
+    const bool in = row < T;
+    uint32_t four = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        four |= (uint32_t)(in && k0 + k < KB && s[k] > (uint32_t)LOW ? s[k] : LOW) << (8 * k);
+    if (g == 0) reinterpret_cast<uint32_t*>(os)[(int64_t)group * 32 + r] = four;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < PIECE; ++h)
+            if (!(in && k0 + 2 * j + g < KB)) c[j][h] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        uint8_t* to = o + (2 * (int64_t)group + j) * kStepBytes<FMT>;
+        if constexpr (FMT == AERO_MX_FP4) {
+            reinterpret_cast<uint4*>(to)[lane] = c[j][0];
+        } else {
+            const uint4 a = c[j][0], b = c[j][PIECE - 1];
+            const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            uint32_t hi[8], lo[8], h[6], l[6];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                int e, f;
+                halves(v[k], e, f);
+                hi[k] = (uint32_t)e;
+                lo[k] = (uint32_t)f;
+            }
+            pack6(hi, h);
+            pack6(lo, l);
+            reinterpret_cast<uint4*>(to)[lane] = make_uint4(h[0], h[1], h[2], h[3]);
+            reinterpret_cast<uint2*>(to + 1024)[lane] = make_uint2(h[4], h[5]);
+            reinterpret_cast<uint4*>(to + 1536)[lane] = make_uint4(l[0], l[1], l[2], l[3]);
+            reinterpret_cast<uint2*>(to + 2560)[lane] = make_uint2(l[4], l[5]);
         }
-        pack6(hi, h);
-        pack6(lo, l);
-        reinterpret_cast<uint4*>(to)[lane] = make_uint4(h[0], h[1], h[2], h[3]);
-        reinterpret_cast<uint2*>(to + 1024)[lane] = make_uint2(h[4], h[5]);
-        reinterpret_cast<uint4*>(to + 1536)[lane] = make_uint4(l[0], l[1], l[2], l[3]);
-        reinterpret_cast<uint2*>(to + 2560)[lane] = make_uint2(l[4], l[5]);
     }
 }
 
@@ -237,24 +327,29 @@ struct MxTiles {
     int bn, bt, group;   // workgroups along each; token tiles side by side
 };
 
-// A workgroup of GN x GT waves, a wave WA weight tiles by XB token tiles of 32. Steps of 64
-// columns go through NB buffers in LDS by direct loads of 1 KB, each wave its share, NB - 1
-// steps ahead.
-template <int FMT, int WA, int XB, int GN, int GT>
+// A workgroup of GN x GT waves, a wave WA weight tiles by XB token tiles of 32; with GK = 2
+// two such sets of waves, one for the first 64 of every 128 columns, one for the others, whose
+// sums are joined at the end: as many waves on tiles of the same size. Stages of 64 GK columns
+// go through NB buffers in LDS by direct loads of 1 KB, each wave its share, NB - 1 stages
+// ahead.
+template <int FMT, int WA, int XB, int GN, int GT, int GK, bool WD>
 struct MxShape {
-    static constexpr int NW = GN * GT, TN = WA * GN, TT = XB * GT;
-    static constexpr int XC = kStepBytes<FMT> / 1024;
-    static constexpr int SC = (TN + TT + 7) / 8;                 // pieces of 8 tiles' scales
-    static constexpr int PIECES = TN + TT * XC + SC;
+    static constexpr int NW = GN * GT * GK, TN = WA * GN, TT = XB * GT;
+    static constexpr int TL = WD ? 0 : TN;                       // weight tiles that go through LDS
+    static constexpr int XS = kStepBytes<FMT> * GK;              // bytes of a token tile's stage
+    static constexpr int XC = XS / 1024;
+    static constexpr int SC = (TL + TT + 7) / 8;                 // pieces of 8 tiles' scales
+    static constexpr int PIECES = TL * GK + TT * XC + SC;
     static constexpr int LOADS = (PIECES + NW - 1) / NW;
-    static constexpr int XOFF = TN * 1024, SOFF = XOFF + TT * XC * 1024;
+    static constexpr int XOFF = TL * GK * 1024, SOFF = XOFF + TT * XS;
     static constexpr int BYTES = SOFF + SC * 1024;
+    static constexpr int VMEM = LOADS + (WD ? 2 * WA : 0);       // a wave's loads of a stage
 };
 
-template <int FMT, int WA, int XB, int GN, int GT, int NB, int WAVES>
-__global__ __launch_bounds__(64 * GN * GT, WAVES)
+template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, bool WD, int WAVES>
+__global__ __launch_bounds__(64 * GN * GT * GK, WAVES)
 void mx_tiles_kernel(MxTiles p) {
-    using S = MxShape<FMT, WA, XB, GN, GT>;
+    using S = MxShape<FMT, WA, XB, GN, GT, GK, WD>;
     // (arrays of their own: the compiler tells a load into one from a read of another)
 #define AERO_MX_BUF(K) __shared__ __attribute__((aligned(16))) uint8_t b##K[K < NB ? S::BYTES : 16]
     AERO_MX_BUF(0); AERO_MX_BUF(1); AERO_MX_BUF(2); AERO_MX_BUF(3); AERO_MX_BUF(4); AERO_MX_BUF(5);
@@ -285,24 +380,25 @@ void mx_tiles_kernel(MxTiles p) {
         if (c >= S::PIECES) c -= S::NW;
         c -= S::SC;
         dst[i] = c * 1024;
-        if (c < S::TN) {
-            src[i] = p.w + (int64_t)min(n0 + max(c, 0), p.nt - 1) * p.KP * 2048;
-            stride[i] = 1024;
+        if (c < S::TL * GK) {
+            const int q = max(c, 0);
+            src[i] = p.w + (int64_t)min(n0 + q / GK, p.nt - 1) * p.KP * 2048 + q % GK * 1024;
+            stride[i] = 1024 * GK;
         } else {
-            const int q = c - S::TN;
+            const int q = max(c - S::TL * GK, 0);
             src[i] = p.x + (int64_t)min(t0 + q / S::XC, p.tt - 1) * p.KP * (2 * kStepBytes<FMT>) +
                      (q % S::XC) * 1024;
-            stride[i] = kStepBytes<FMT>;
+            stride[i] = S::XS;
         }
     }
     uint32_t lane16 = lane * 16;
     opaque(lane16);
     const uint8_t* first = src[0] + lane16;
-    const int half = wave < S::SC ? 1 : 0;
+    const int half = GK == 1 && wave < S::SC ? 1 : 0;
     if (wave < S::SC) {       // eight tiles' scales of 128 columns
-        const int k = min(wave * 8 + (lane >> 3), S::TN + S::TT - 1);
-        first = (k < S::TN ? p.ws + (int64_t)min(n0 + k, p.nt - 1) * p.KP * 128
-                           : p.xs + (int64_t)min(t0 + k - S::TN, p.tt - 1) * p.KP * 128) + (lane & 7) * 16;
+        const int k = min(wave * 8 + (lane >> 3), S::TL + S::TT - 1);
+        first = (k < S::TL ? p.ws + (int64_t)min(n0 + k, p.nt - 1) * p.KP * 128
+                           : p.xs + (int64_t)min(t0 + k - S::TL, p.tt - 1) * p.KP * 128) + (lane & 7) * 16;
         dst[0] = S::SOFF + wave * 1024;
         stride[0] = 128;
     }
@@ -316,7 +412,39 @@ void mx_tiles_kernel(MxTiles p) {
         }
     };
 
-    const int wn = (wave % GN) * WA, wt = (wave / GN) * XB;
+    const int kg = GK == 1 ? 0 : wave / (GN * GT);
+    const int wn = (wave % GN) * WA, wt = (wave / GN % GT) * XB;
+    const int stages = GK == 1 ? p.steps : p.KP;
+    // (weights that go straight into registers, a ring of stages)
+    v4i wr[WD ? NB : 1][WA];
+    int wsr[WD ? NB : 1][WA];
+    const uint8_t* wp[WA];
+    const uint8_t* wsp[WA];
+    uint32_t row4 = r * 4;
+    opaque(row4);
+#pragma unroll
+    for (int k = 0; k < WA; ++k) {
+        const int64_t tile = min(n0 + wn + k, p.nt - 1);
+        wp[k] = p.w + tile * p.KP * 2048 + kg * 1024;
+        wsp[k] = p.ws + tile * p.KP * 128;
+    }
+    // loads k0 .. k1 of stage i: this wave's pieces into b, its weights into slot s
+    auto load = [&](int i, uint8_t* b, int s, int k0, int k1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = k0; k < k1; ++k) {
+            __builtin_amdgcn_sched_barrier(0);    // (in this order: the waits below count them)
+            if (k < S::LOADS) {
+                fetch(i, b, k, k + 1);
+            } else if constexpr (WD) {
+                const int a = (k - S::LOADS) / 2;
+                if ((k - S::LOADS) % 2 == 0)
+                    wr[s][a] = *reinterpret_cast<const v4i*>(wp[a] + (int64_t)i * (1024 * GK) + lane16);
+                else
+                    wsr[s][a] = *reinterpret_cast<const int*>(wsp[a] + (int64_t)(GK == 1 ? i >> 1 : i) * 128 + row4);
+            }
+        }
+    };
+
     v16f acc[WA][XB];
 #pragma unroll
     for (int a = 0; a < WA; ++a)
@@ -327,88 +455,119 @@ void mx_tiles_kernel(MxTiles p) {
 
     // A lane's places in a buffer. (Opaque, so that each stays one register that the buffers
     // and tiles add constants to.)
-    int oa = wn * 1024 + lane * 16, ox = S::XOFF + wt * kStepBytes<FMT> + lane * 16;
-    int ox8 = ox - lane * 8, osa = S::SOFF + wn * 128 + r * 4, osx = S::SOFF + (S::TN + wt) * 128 + r * 4;
+    int oa = (wn * GK + kg) * 1024 + lane * 16;
+    int ox = S::XOFF + wt * S::XS + kg * kStepBytes<FMT> + lane * 16;
+    int ox8 = ox - lane * 8, osa = S::SOFF + wn * 128 + r * 4, osx = S::SOFF + (S::TL + wt) * 128 + r * 4;
     opaque(oa);
     opaque(ox);
     opaque(ox8);
     opaque(osa);
     opaque(osx);
-    // (the step's operands are read first; the loads of a later step go out between groups of
-    // matrix steps, behind which their issue hides)
-    auto compute = [&](int i, const uint8_t* buf, uint8_t* nb) __attribute__((always_inline)) {
-        constexpr int H = FMT == AERO_MX_INT8 ? 2 : 1, GROUPS = XB * H;
-        const int sh = 16 * (i & 1) + 8 * g, next = min(i + NB - 1, p.steps - 1);
-        v4i a[WA], q[XB][H];
-        v2i e[XB][H];
-        int sa[WA], sb[XB];
+    constexpr int H = FMT == AERO_MX_INT8 ? 2 : 1, GROUPS = XB * H;
+    struct Operands {
+        v4i a[WA];
+        v8i x[XB][H];        // (4-bit: the first four)
+        int sa[WA], sb[XB];  // dwords of four blocks' scales
+    };
+    auto read = [&](Operands& f, const uint8_t* buf) __attribute__((always_inline)) {
+        if constexpr (!WD) {
 #pragma unroll
-        for (int k = 0; k < WA; ++k) a[k] = *reinterpret_cast<const v4i*>(buf + oa + k * 1024);
+            for (int k = 0; k < WA; ++k) f.a[k] = *reinterpret_cast<const v4i*>(buf + oa + k * GK * 1024);
 #pragma unroll
-        for (int k = 0; k < WA; ++k) sa[k] = *reinterpret_cast<const int*>(buf + osa + k * 128);
-#pragma unroll
-        for (int b = 0; b < XB; ++b) {
-            sb[b] = *reinterpret_cast<const int*>(buf + osx + b * 128);
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                const int at = b * kStepBytes<FMT> + 1536 * h;
-                q[b][h] = *reinterpret_cast<const v4i*>(buf + ox + at);
-                if constexpr (H == 2) e[b][h] = *reinterpret_cast<const v2i*>(buf + ox8 + at + 1024);
-            }
+            for (int k = 0; k < WA; ++k) f.sa[k] = *reinterpret_cast<const int*>(buf + osa + k * 128);
         }
 #pragma unroll
-        for (int k = 0; k < WA; ++k) sa[k] = (int)((uint32_t)sa[k] >> sh);
-#pragma unroll
-        for (int b = 0; b < XB; ++b) sb[b] = (int)((uint32_t)sb[b] >> sh);
-#pragma unroll
-        for (int b = 0; b < XB; ++b)
+        for (int b = 0; b < XB; ++b) {
+            f.sb[b] = *reinterpret_cast<const int*>(buf + osx + b * 128);
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const int n = b * H + h;
-                v8i f;
+                const int at = b * S::XS + 1536 * h;
+                const v4i q = *reinterpret_cast<const v4i*>(buf + ox + at);
                 if constexpr (H == 2) {
-                    const v4i e4 = __builtin_shufflevector(e[b][h], e[b][h], 0, 1, -1, -1);
-                    f = __builtin_shufflevector(q[b][h], e4, 0, 1, 2, 3, 4, 5, -1, -1);
+                    const v2i e = *reinterpret_cast<const v2i*>(buf + ox8 + at + 1024);
+                    const v4i e4 = __builtin_shufflevector(e, e, 0, 1, -1, -1);
+                    f.x[b][h] = __builtin_shufflevector(q, e4, 0, 1, 2, 3, 4, 5, -1, -1);
                 } else {
-                    f = wide(q[b][h]);
+                    f.x[b][h] = wide(q);
                 }
+            }
+        }
+    };
+    // the matrix steps; the loads of a later stage go out behind them, one at a time
+    auto multiply = [&](auto kk, const Operands& f, int i, uint8_t* nb) __attribute__((always_inline)) {
+        constexpr int K = decltype(kk)::value;
+        const int next = min(i + NB - 1, stages - 1);
+        const int sh = 16 * (GK == 1 ? i & 1 : kg) + 8 * g;
+        int sa[WA];
+#pragma unroll
+        for (int k = 0; k < WA; ++k) sa[k] = (int)((uint32_t)(WD ? wsr[WD ? K : 0][k] : f.sa[k]) >> sh);
+#pragma unroll
+        for (int b = 0; b < XB; ++b) {
+            const int sb = (int)((uint32_t)f.sb[b] >> sh);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int k = 0; k < WA; ++k) {
                     acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                        f, wide(a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb[b] - 4 * h, 0, sa[k]);
-                    const int at = n * WA + k;
+                        f.x[b][h], wide(WD ? wr[WD ? K : 0][k] : f.a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 4 * h, 0, sa[k]);
+                    const int at = (b * H + h) * WA + k;
                     __builtin_amdgcn_sched_barrier(0);
-                    fetch(next, nb, at * S::LOADS / (GROUPS * WA), (at + 1) * S::LOADS / (GROUPS * WA));
+                    load(next, nb, WD ? (K + NB - 1) % NB : 0, at * S::VMEM / (GROUPS * WA),
+                         (at + 1) * S::VMEM / (GROUPS * WA));
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            }
+        }
     };
+    Operands even, odd;
     // A step begins when its loads have landed (the next ones' may be on their way) and
     // every wave is done with the step before, whose buffer is then filled again; the last
     // steps load the last one once more, so that every step is alike. (The marks keep the
     // copies of this code apart: merged, the compiler could not tell the buffer that is read
     // from the one that is filled, and would wait for the loads.)
     auto step = [&](auto k, int i) __attribute__((always_inline)) {
-        constexpr int K = decltype(k)::value, N = (NB - 2) * S::LOADS;
+        constexpr int K = decltype(k)::value, R = PIPE ? (K + 1) % NB : K;
+        constexpr int N = (PIPE ? NB - 3 : NB - 2) * S::VMEM;
         __builtin_amdgcn_s_waitcnt((N & 15) | 0x0f70 | ((N >> 4) << 14));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        asm volatile("; buffer %0" ::"n"(K) : "memory");
-        compute(i, bufs[K], bufs[(K + NB - 1) % NB]);
-        asm volatile("; buffer %0 done" ::"n"(K) : "memory");
+        asm volatile("; buffer %0" ::"n"(R) : "memory");
+        if constexpr (PIPE) {
+            if constexpr (K % 2 == 0) {
+                read(odd, bufs[R]);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(k, even, i, bufs[(K + NB - 1) % NB]);
+            } else {
+                read(even, bufs[R]);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(k, odd, i, bufs[(K + NB - 1) % NB]);
+            }
+        } else {
+            read(even, bufs[K]);
+            multiply(k, even, i, bufs[(K + NB - 1) % NB]);
+        }
+        asm volatile("; buffer %0 done" ::"n"(R) : "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
 #define AERO_MX_EACH(DO) DO(0) DO(1) DO(2) DO(3) DO(4) DO(5) DO(6) DO(7) DO(8) DO(9) DO(10) DO(11)
-#define AERO_MX_FILL(K) if constexpr (K < NB - 1) fetch(min(K, p.steps - 1), bufs[K], 0, S::LOADS);
+#define AERO_MX_FILL(K) if constexpr (K < NB - 1) load(min(K, stages - 1), bufs[K], WD ? K : 0, 0, S::VMEM);
 #define AERO_MX_ROUND(K) if constexpr (K < NB) step(std::integral_constant<int, K>{}, i + K);
 #define AERO_MX_REST(K) \
-    if constexpr (K < NB - 1) if (i + K < p.steps) step(std::integral_constant<int, K>{}, i + K);
+    if constexpr (K < NB - 1) if (i + K < stages) step(std::integral_constant<int, K>{}, i + K);
     AERO_MX_EACH(AERO_MX_FILL)
+    if constexpr (PIPE) {
+        static_assert(NB >= 4 && NB % 2 == 0, "two sets of operands in turn, two stages ahead of the loads");
+        constexpr int N = (NB - 2) * S::VMEM;
+        __builtin_amdgcn_s_waitcnt((N & 15) | 0x0f70 | ((N >> 4) << 14));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(even, bufs[0]);
+    }
     // (whole rounds, then the rest: with an exit after each step the compiler keeps the sums
     // twice and spills)
     int i = 0;
-    for (; i + NB <= p.steps; i += NB) {
+    for (; i + NB <= stages; i += NB) {
         AERO_MX_EACH(AERO_MX_ROUND)
     }
     AERO_MX_EACH(AERO_MX_REST)
@@ -420,242 +579,50 @@ void mx_tiles_kernel(MxTiles p) {
 
     constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
     // lane l holds column l % 32 of 16 tokens: 128 bytes in one piece for each
-#pragma unroll
-    for (int a = 0; a < WA; ++a) {
+    auto put = [&](int a, int b, const v16f& v) __attribute__((always_inline)) {
         const int64_t n = (int64_t)(n0 + wn + a) * 32 + r;
-        if (n >= p.N) continue;
+        const int64_t t1 = (int64_t)(t0 + wt + b) * 32 + 4 * g;
+        if (n >= p.N) return;
+        float* o = p.y + t1 * p.N + n;
 #pragma unroll
-        for (int b = 0; b < XB; ++b) {
-            const int64_t t1 = (int64_t)(t0 + wt + b) * 32 + 4 * g;
-            float* o = p.y + t1 * p.N + n;
+        for (int i = 0; i < 16; ++i) {
+            const int t = 8 * (i >> 2) + (i & 3);
+            if (t1 + t < p.T) __builtin_nontemporal_store(v[i] * UNIT, o + t * p.N);
+        }
+    };
+    if constexpr (GK == 1) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int t = 8 * (i >> 2) + (i & 3);
-                if (t1 + t < p.T) __builtin_nontemporal_store(acc[a][b][i] * UNIT, o + t * p.N);
+        for (int a = 0; a < WA; ++a)
+#pragma unroll
+            for (int b = 0; b < XB; ++b) put(a, b, acc[a][b]);
+    } else {
+        // each set of waves ends with half of the tiles, the other's sums of them passed
+        // through LDS
+        constexpr int HALF = WA * XB / 2;
+        static_assert(WA * XB % 2 == 0, "half of the tiles each");
+        __shared__ v4f join[S::NW][4][64];
+        v4f* mine = &join[wave][0][lane];
+        const v4f* other = &join[wave ^ (GN * GT)][0][lane];
+#pragma unroll
+        for (int m = 0; m < HALF; ++m) {
+            const v16f &lo = acc[m / XB][m % XB], &up = acc[(m + HALF) / XB][(m + HALF) % XB];
+            if (m > 0) __syncthreads();
+            const v16f give = kg ? lo : up;
+            v16f sum = kg ? up : lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const v4f q = {give[4 * i], give[4 * i + 1], give[4 * i + 2], give[4 * i + 3]};
+                mine[64 * i] = q;
             }
-        }
-    }
-}
-
-// The largest calls: 256 weight rows by 256 tokens a workgroup of four waves, each 128 by
-// 128 (its 16 tiles of sums take half of a SIMD's registers: one wave each). LDS carries the
-// tokens only, stages of 128 columns; a wave loads its weights straight into registers, two
-// stages ahead. With both sides in LDS the reads and the direct loads' writes take about as
-// many of its cycles as there are matrix steps; so they take half.
-// A stage is eight groups of matrix steps (four with x in 4 bits). The operands of a group
-// are read while the group before runs, those of a stage's first while the last one of the
-// stage before does: the barrier that a stage begins with stands in front of that.
-template <int FMT>
-struct MxWide {
-    static constexpr int H = FMT == AERO_MX_INT8 ? 2 : 1;        // halves
-    static constexpr int BT = FMT == AERO_MX_INT8 ? 1 : 2;       // token tiles a group
-    static constexpr int GROUPS = 8 / BT;
-    static constexpr int XC = 2 * kStepBytes<FMT> / 1024;        // KB of a token tile's stage
-    static constexpr int PIECES = 8 * XC + 1, LOADS = (PIECES + 3) / 4;
-    static constexpr int SOFF = 8 * XC * 1024, BYTES = SOFF + 1024;
-    static constexpr int VMEM = LOADS + 12;                      // and the weights' loads
-};
-
-template <int FMT>
-__global__ __launch_bounds__(256, 1)
-void mx_wide_kernel(MxTiles p) {
-    using S = MxWide<FMT>;
-    __shared__ __attribute__((aligned(16))) uint8_t b0[S::BYTES];
-    __shared__ __attribute__((aligned(16))) uint8_t b1[S::BYTES];
-    __shared__ __attribute__((aligned(16))) uint8_t b2[S::BYTES];
-    uint8_t* const bufs[3] = {b0, b1, b2};
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 31, g = lane >> 5;
-    const int per = gridDim.x >> 3;
-    const int at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (at >= p.bn * p.bt) return;
-    const int group = at / (p.group * p.bn), rest = at - group * p.group * p.bn;
-    const int width = min(p.group, p.bt - group * p.group);
-    const int n0 = (rest / width) * 8, t0 = (group * p.group + rest % width) * 8;
-    const int wn = (wave & 1) * 4, wt = (wave >> 1) * 4;
-
-    // this wave's pieces of a stage's tokens (the first wave's first: their scales), and its
-    // weights
-    uint32_t lane16 = lane * 16, lane4 = r * 4;
-    opaque(lane16);
-    opaque(lane4);
-    const uint8_t* src[S::LOADS];
-    int dst[S::LOADS];
+            __syncthreads();
 #pragma unroll
-    for (int i = 0; i < S::LOADS; ++i) {
-        int c = wave + 4 * i;
-        if (c >= S::PIECES) c -= 4;
-        c = max(c - 1, 0);
-        dst[i] = c * 1024;
-        src[i] = p.x + (int64_t)min(t0 + c / S::XC, p.tt - 1) * p.KP * (S::XC * 1024) + (c % S::XC) * 1024;
-    }
-    const uint8_t* first = src[0] + lane16;
-    int first_stride = S::XC * 1024;
-    if (wave == 0) {
-        first = p.xs + (int64_t)min(t0 + (lane >> 3), p.tt - 1) * p.KP * 128 + (lane & 7) * 16;
-        first_stride = 128;
-        dst[0] = S::SOFF;
-    }
-    auto piece = [&](int i, uint8_t* b, int k0, int k1) __attribute__((always_inline)) {
+            for (int i = 0; i < 4; ++i) {
+                const v4f q = other[64 * i];
 #pragma unroll
-        for (int k = k0; k < k1; ++k) {
-            const uint8_t* from = k == 0 ? first + (int64_t)i * first_stride
-                                         : src[k] + (int64_t)i * (S::XC * 1024) + lane16;
-            uint8_t* to = b + dst[k];
-            __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-        }
-    };
-    const uint8_t* wp[4];
-    const uint8_t* wsp[4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-        const int64_t tile = min(n0 + wn + a, p.nt - 1);
-        wp[a] = p.w + tile * p.KP * 2048;
-        wsp[a] = p.ws + tile * p.KP * 128;
-    }
-    v4i w[3][2][4];
-    int sw[3][4];
-    auto weights = [&](int i, int set, int n) __attribute__((always_inline)) {   // the n-th of 12 loads
-        const int64_t k = i;
-        const int a = n / 3;
-        if (n % 3 < 2)
-            w[set][n % 3][a] = *reinterpret_cast<const v4i*>(wp[a] + k * 2048 + n % 3 * 1024 + lane16);
-        else
-            sw[set][a] = *reinterpret_cast<const int*>(wsp[a] + k * 128 + lane4);
-    };
-    auto load = [&](int i, int set, uint8_t* b, int k0, int k1) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = k0; k < k1; ++k) {
-            if (k < S::LOADS)
-                piece(i, b, k, k + 1);
-            else
-                weights(i, set, k - S::LOADS);
-        }
-    };
-
-    v16f acc[4][4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
-
-    struct Frag {
-        v4i q[S::BT][S::H];
-        v2i e[S::BT][S::H];
-        int s[S::BT];
-    };
-    int ox = wt * (S::XC * 1024) + lane * 16, ox8 = ox - lane * 8, osx = S::SOFF + wt * 128 + r * 4;
-    opaque(ox);
-    opaque(ox8);
-    opaque(osx);
-    // group n: columns 64 (n / (4 / BT)) .. of the stage, token tiles BT (n % (4 / BT)) ..
-    auto read = [&](Frag& f, const uint8_t* b, int n) __attribute__((always_inline)) {
-        const int j = n / (4 / S::BT), b0 = n % (4 / S::BT) * S::BT;
-#pragma unroll
-        for (int x = 0; x < S::BT; ++x) {
-            const int off = (b0 + x) * (S::XC * 1024) + j * kStepBytes<FMT>;
-#pragma unroll
-            for (int h = 0; h < S::H; ++h) {
-                f.q[x][h] = *reinterpret_cast<const v4i*>(b + ox + off + 1536 * h);
-                if constexpr (S::H == 2)
-                    f.e[x][h] = *reinterpret_cast<const v2i*>(b + ox8 + off + 1536 * h + 1024);
+                for (int k = 0; k < 4; ++k) sum[4 * i + k] += q[k];
             }
-            f.s[x] = *reinterpret_cast<const int*>(b + osx + (b0 + x) * 128);
-        }
-    };
-    const int sh0 = 8 * g, sh1 = 16 + 8 * g;
-    Frag f0, f1;
-    auto stage = [&](auto kk, int i) __attribute__((always_inline)) {
-        constexpr int K = decltype(kk)::value, K1 = (K + 1) % 3, K2 = (K + 2) % 3;
-        const int next = min(i + 2, p.KP - 1);
-        int sa[2][4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            sa[0][a] = (int)((uint32_t)sw[K][a] >> sh0);
-            sa[1][a] = (int)((uint32_t)sw[K][a] >> sh1);
-        }
-#pragma unroll
-        for (int n = 0; n < S::GROUPS; ++n) {
-            Frag& cur = n & 1 ? f1 : f0;
-            Frag& nxt = n & 1 ? f0 : f1;
-            const int j = n / (4 / S::BT), b0 = n % (4 / S::BT) * S::BT;
-            if (n + 1 < S::GROUPS) {
-                read(nxt, bufs[K], n + 1);
-            } else {
-                // every wave has read this stage, and the next one has landed
-                __builtin_amdgcn_s_waitcnt((S::VMEM & 15) | 0x0070 | ((S::VMEM >> 4) << 14));
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                asm volatile("; buffer %0" ::"n"(K1) : "memory");
-                read(nxt, bufs[K1], 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int x = 0; x < S::BT; ++x)
-#pragma unroll
-                for (int h = 0; h < S::H; ++h) {
-                    v8i f;
-                    if constexpr (S::H == 2) {
-                        const v4i e4 = __builtin_shufflevector(cur.e[x][h], cur.e[x][h], 0, 1, -1, -1);
-                        f = __builtin_shufflevector(cur.q[x][h], e4, 0, 1, 2, 3, 4, 5, -1, -1);
-                    } else {
-                        f = wide(cur.q[x][h]);
-                    }
-                    const int sb = (int)((uint32_t)cur.s[x] >> (j ? sh1 : sh0)) - 4 * h;
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        acc[a][b0 + x] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                            f, wide(w[K][j][a]), acc[a][b0 + x], S::H == 2 ? kF6 : kF4, kF4, 0, sb, 0,
-                            sa[j][a]);
-                        // (one load at a time, each behind a matrix step)
-                        constexpr int M = (S::GROUPS - 1) * 8;
-                        const int m = n * 8 + (x * S::H + h) * 4 + a;
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (m < M) load(next, K2, bufs[K2], m * S::VMEM / M, (m + 1) * S::VMEM / M);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-        }
-    };
-    load(0, 0, b0, 0, S::VMEM);
-    load(min(1, p.KP - 1), 1, b1, 0, S::VMEM);
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt((S::VMEM & 15) | 0x0f70 | ((S::VMEM >> 4) << 14));
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    read(f0, b0, 0);
-    using K0 = std::integral_constant<int, 0>;
-    using K1 = std::integral_constant<int, 1>;
-    using K2 = std::integral_constant<int, 2>;
-    int i = 0;
-    for (; i + 3 <= p.KP; i += 3) {
-        stage(K0{}, i);
-        stage(K1{}, i + 1);
-        stage(K2{}, i + 2);
-    }
-    if (i < p.KP) stage(K0{}, i);
-    if (i + 1 < p.KP) stage(K1{}, i + 1);
-    __builtin_amdgcn_s_waitcnt(0x0f70);       // (no load is on its way when the wave ends)
-
-    constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-        const int64_t n = (int64_t)(n0 + wn + a) * 32 + r;
-        if (n >= p.N) continue;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int64_t t1 = (int64_t)(t0 + wt + b) * 32 + 4 * g;
-            float* o = p.y + t1 * p.N + n;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int t = 8 * (i >> 2) + (i & 3);
-                if (t1 + t < p.T) __builtin_nontemporal_store(acc[a][b][i] * UNIT, o + t * p.N);
-            }
+            const int tile = kg ? m + HALF : m;
+            put(tile / XB, tile % XB, sum);
         }
     }
 }
@@ -677,16 +644,52 @@ int64_t weight_codes_bytes(int64_t n_rows, int64_t n_cols) {
 }
 
 // Calls of more tokens go through operands in the workspace.
-constexpr int64_t kFewTokens = 32;
+const int64_t kFewTokens = tune("mx_few", 32);
 
 template <int FMT>
 int64_t operand_bytes(int64_t n_tok, int KP) {
     return tiles32(n_tok) * KP * (2 * kStepBytes<FMT> + 128);
 }
 
-template <int FMT, int WA, int XB, int GN, int GT, int NB, int WAVES>
+template <int FMT, int WA, int XB, int NW, int D>
+bool launch_stream(const MxGemm& p, hipStream_t s) {
+    return launch("mx_stream_kernel", mx_stream_kernel<FMT, WA, XB, NW, D>,
+                  dim3((unsigned)((p.N + 16 * WA - 1) / (16 * WA))), dim3(64 * NW), 0, s, p);
+}
+
+template <int FMT>
+bool run_stream(const MxGemm& p, hipStream_t s) {
+    const int c = tune("mx_str", 0);
+    if (p.T <= 16) {
+        switch (c) {
+        case 1: return launch_stream<FMT, 1, 1, 4, 4>(p, s);
+        case 2: return launch_stream<FMT, 2, 1, 8, 2>(p, s);
+        case 3: return launch_stream<FMT, 2, 1, 4, 4>(p, s);
+        case 4: return launch_stream<FMT, 1, 1, 16, 2>(p, s);
+        case 5: return launch_stream<FMT, 1, 1, 8, 2>(p, s);
+        default: return launch_stream<FMT, 1, 1, 8, 4>(p, s);
+        }
+    }
+    if (p.T <= 32) {
+        switch (c) {
+        case 1: return launch_stream<FMT, 1, 2, 8, 2>(p, s);
+        case 2: return launch_stream<FMT, 4, 2, 8, 2>(p, s);
+        case 3: return launch_stream<FMT, 2, 2, 4, 4>(p, s);
+        default: return launch_stream<FMT, 2, 2, 8, 2>(p, s);
+        }
+    }
+    switch (c) {
+    case 1: return launch_stream<FMT, 1, 4, 8, 2>(p, s);
+    case 2: return launch_stream<FMT, 2, 4, 8, 2>(p, s);
+    case 3: return launch_stream<FMT, 4, 4, 4, 2>(p, s);
+    case 4: return launch_stream<FMT, 2, 4, 8, 1>(p, s);
+    default: return launch_stream<FMT, 4, 4, 8, 2>(p, s);
+    }
+}
+
+template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, bool WD, int WAVES>
 bool launch_tiles(MxTiles p, hipStream_t s) {
-    using S = MxShape<FMT, WA, XB, GN, GT>;
+    using S = MxShape<FMT, WA, XB, GN, GT, GK, WD>;
     p.bn = (p.nt + S::TN - 1) / S::TN;
     p.bt = (p.tt + S::TT - 1) / S::TT;
     const int64_t grid = ((int64_t)p.bn * p.bt + 7) / 8 * 8;
@@ -694,7 +697,7 @@ bool launch_tiles(MxTiles p, hipStream_t s) {
         set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
         return false;
     }
-    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, NB, WAVES>, dim3((unsigned)grid),
+    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, GK, NB, PIPE, WD, WAVES>, dim3((unsigned)grid),
                   dim3(64 * S::NW), 0, s, p);
 }
 
@@ -703,8 +706,8 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
     const int64_t tt = tiles32(g.T), nt = tiles32(g.N);
     uint8_t* o = (uint8_t*)ws;
     uint8_t* os = o + tt * g.KP * (2 * kStepBytes<FMT>);
-    const int64_t n = tt * 32 * 4 * g.KP, blocks = (n + 255) / 256;
-    if (blocks > 0x7fffffff || nt > 0x7fffffff || tt > 0x7fffffff) {
+    const int64_t n = tt * 64 * g.KP, blocks = (n + 255) / 256;
+    if (n >> 6 > 0x7fffffff || nt > 0x7fffffff || tt > 0x7fffffff) {
         set_error("mx_matmul: %lld tokens are too many", (long long)g.T);
         return false;
     }
@@ -712,19 +715,19 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
                 g.xs, o, os, g.T, g.KB, g.KP, n))
         return false;
     const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, tune("mx_group", 4)};
-    const int64_t wide = ((nt + 7) / 8) * ((tt + 7) / 8);
-    if (wide >= tune("mx_wide", 200)) {
-        MxTiles q = p;
-        q.bn = (int)((nt + 7) / 8);
-        q.bt = (int)((tt + 7) / 8);
-        return launch("mx_wide_kernel", mx_wide_kernel<FMT>, dim3((unsigned)((wide + 7) / 8 * 8)), dim3(256),
-                      0, s, q);
-    }
     const int64_t big = ((nt + 7) / 8) * ((tt + 3) / 4);
-    if (big >= tune("mx_big", 256)) return launch_tiles<FMT, 4, 2, 2, 2, 3, 2>(p, s);
-    if (tune("mx_nb", 6) == 3) return launch_tiles<FMT, 2, 1, 2, 2, 3, 2>(p, s);
-    if (tune("mx_nb", 6) == 12) return launch_tiles<FMT, 2, 1, 2, 2, 12, 1>(p, s);
-    return launch_tiles<FMT, 2, 1, 2, 2, 6, 2>(p, s);
+    const int c = tune("mx_cfg", big >= 256 ? 0 : 1);
+    switch (c) {
+    case 0: return launch_tiles<FMT, 4, 2, 2, 2, 1, 3, false, false, 2>(p, s);
+    case 1: return launch_tiles<FMT, 2, 1, 2, 2, 2, 6, true, false, 2>(p, s);
+    case 2: return launch_tiles<FMT, 1, 2, 4, 1, 2, 6, true, true, 2>(p, s);
+    case 3: return launch_tiles<FMT, 1, 2, 4, 1, 2, 4, true, true, 2>(p, s);
+    case 4: return launch_tiles<FMT, 2, 1, 1, 2, 2, 6, true, false, 1>(p, s);
+    case 5: return launch_tiles<FMT, 1, 2, 2, 1, 2, 6, true, true, 1>(p, s);
+    case 6: return launch_tiles<FMT, 2, 2, 2, 1, 2, 6, true, true, 1>(p, s);
+    case 7: return launch_tiles<FMT, 2, 2, 4, 1, 2, 6, true, true, 2>(p, s);
+    default: return launch_tiles<FMT, 2, 1, 2, 2, 2, 6, true, true, 2>(p, s);
+    }
 }
 
 }  // namespace
@@ -804,11 +807,7 @@ int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, con
         return (fmt == AERO_MX_INT8 ? run_tiles<AERO_MX_INT8>(p, workspace, s)
                                     : run_tiles<AERO_MX_FP4>(p, workspace, s)) ? 1 : 0;
     }
-    const dim3 grid((unsigned)tiles32(n_rows));
-    return (fmt == AERO_MX_INT8
-                ? launch("mx_gemm_kernel", mx_gemm_kernel<AERO_MX_INT8>, grid, dim3(256), 0, s, p)
-                : launch("mx_gemm_kernel", mx_gemm_kernel<AERO_MX_FP4>, grid, dim3(256), 0, s, p))
-               ? 1 : 0;
+    return (fmt == AERO_MX_INT8 ? run_stream<AERO_MX_INT8>(p, s) : run_stream<AERO_MX_FP4>(p, s)) ? 1 : 0;
 }
 
 }  // extern "C"
