@@ -332,24 +332,22 @@ struct MxTiles {
 // sums are joined at the end: as many waves on tiles of the same size. Stages of 64 GK columns
 // go through NB buffers in LDS by direct loads of 1 KB, each wave its share, NB - 1 stages
 // ahead.
-template <int FMT, int WA, int XB, int GN, int GT, int GK, bool WD>
+template <int FMT, int WA, int XB, int GN, int GT, int GK>
 struct MxShape {
     static constexpr int NW = GN * GT * GK, TN = WA * GN, TT = XB * GT;
-    static constexpr int TL = WD ? 0 : TN;                       // weight tiles that go through LDS
     static constexpr int XS = kStepBytes<FMT> * GK;              // bytes of a token tile's stage
     static constexpr int XC = XS / 1024;
-    static constexpr int SC = (TL + TT + 7) / 8;                 // pieces of 8 tiles' scales
-    static constexpr int PIECES = TL * GK + TT * XC + SC;
+    static constexpr int SC = (TN + TT + 7) / 8;                 // pieces of 8 tiles' scales
+    static constexpr int PIECES = TN * GK + TT * XC + SC;
     static constexpr int LOADS = (PIECES + NW - 1) / NW;
-    static constexpr int XOFF = TL * GK * 1024, SOFF = XOFF + TT * XS;
+    static constexpr int XOFF = TN * GK * 1024, SOFF = XOFF + TT * XS;
     static constexpr int BYTES = SOFF + SC * 1024;
-    static constexpr int VMEM = LOADS + (WD ? 2 * WA : 0);       // a wave's loads of a stage
 };
 
-template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, bool WD, int WAVES>
+template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, int WAVES>
 __global__ __launch_bounds__(64 * GN * GT * GK, WAVES)
 void mx_tiles_kernel(MxTiles p) {
-    using S = MxShape<FMT, WA, XB, GN, GT, GK, WD>;
+    using S = MxShape<FMT, WA, XB, GN, GT, GK>;
     // (arrays of their own: the compiler tells a load into one from a read of another)
 #define AERO_MX_BUF(K) __shared__ __attribute__((aligned(16))) uint8_t b##K[K < NB ? S::BYTES : 16]
     AERO_MX_BUF(0); AERO_MX_BUF(1); AERO_MX_BUF(2); AERO_MX_BUF(3); AERO_MX_BUF(4); AERO_MX_BUF(5);
@@ -371,7 +369,7 @@ void mx_tiles_kernel(MxTiles p) {
 
     // This wave's pieces of a step, the scales' first: where they begin, how far a step goes.
     // (A piece past the last is the wave's one before once more, to the same place.)
-    static_assert(S::SC <= S::NW, "the scales' pieces are first ones");
+    static_assert(S::SC <= S::NW && S::PIECES >= S::NW, "each wave has a piece, the scales' are first ones");
     const uint8_t* src[S::LOADS];
     int dst[S::LOADS], stride[S::LOADS];
 #pragma unroll
@@ -380,12 +378,12 @@ void mx_tiles_kernel(MxTiles p) {
         if (c >= S::PIECES) c -= S::NW;
         c -= S::SC;
         dst[i] = c * 1024;
-        if (c < S::TL * GK) {
+        if (c < S::TN * GK) {
             const int q = max(c, 0);
             src[i] = p.w + (int64_t)min(n0 + q / GK, p.nt - 1) * p.KP * 2048 + q % GK * 1024;
             stride[i] = 1024 * GK;
         } else {
-            const int q = max(c - S::TL * GK, 0);
+            const int q = max(c - S::TN * GK, 0);
             src[i] = p.x + (int64_t)min(t0 + q / S::XC, p.tt - 1) * p.KP * (2 * kStepBytes<FMT>) +
                      (q % S::XC) * 1024;
             stride[i] = S::XS;
@@ -396,15 +394,16 @@ void mx_tiles_kernel(MxTiles p) {
     const uint8_t* first = src[0] + lane16;
     const int half = GK == 1 && wave < S::SC ? 1 : 0;
     if (wave < S::SC) {       // eight tiles' scales of 128 columns
-        const int k = min(wave * 8 + (lane >> 3), S::TL + S::TT - 1);
-        first = (k < S::TL ? p.ws + (int64_t)min(n0 + k, p.nt - 1) * p.KP * 128
-                           : p.xs + (int64_t)min(t0 + k - S::TL, p.tt - 1) * p.KP * 128) + (lane & 7) * 16;
+        const int k = min(wave * 8 + (lane >> 3), S::TN + S::TT - 1);
+        first = (k < S::TN ? p.ws + (int64_t)min(n0 + k, p.nt - 1) * p.KP * 128
+                           : p.xs + (int64_t)min(t0 + k - S::TN, p.tt - 1) * p.KP * 128) + (lane & 7) * 16;
         dst[0] = S::SOFF + wave * 1024;
         stride[0] = 128;
     }
     auto fetch = [&](int i, uint8_t* b, int k0, int k1) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = k0; k < k1; ++k) {
+            __builtin_amdgcn_sched_barrier(0);     // (in this order: the waits below count them)
             const uint8_t* from = k == 0 ? first + (int64_t)(i >> half) * stride[0]
                                          : src[k] + (int64_t)i * stride[k] + lane16;
             uint8_t* to = b + dst[k];
@@ -415,36 +414,6 @@ void mx_tiles_kernel(MxTiles p) {
     const int kg = GK == 1 ? 0 : wave / (GN * GT);
     const int wn = (wave % GN) * WA, wt = (wave / GN % GT) * XB;
     const int stages = GK == 1 ? p.steps : p.KP;
-    // (weights that go straight into registers, a ring of stages)
-    v4i wr[WD ? NB : 1][WA];
-    int wsr[WD ? NB : 1][WA];
-    const uint8_t* wp[WA];
-    const uint8_t* wsp[WA];
-    uint32_t row4 = r * 4;
-    opaque(row4);
-#pragma unroll
-    for (int k = 0; k < WA; ++k) {
-        const int64_t tile = min(n0 + wn + k, p.nt - 1);
-        wp[k] = p.w + tile * p.KP * 2048 + kg * 1024;
-        wsp[k] = p.ws + tile * p.KP * 128;
-    }
-    // loads k0 .. k1 of stage i: this wave's pieces into b, its weights into slot s
-    auto load = [&](int i, uint8_t* b, int s, int k0, int k1) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = k0; k < k1; ++k) {
-            __builtin_amdgcn_sched_barrier(0);    // (in this order: the waits below count them)
-            if (k < S::LOADS) {
-                fetch(i, b, k, k + 1);
-            } else if constexpr (WD) {
-                const int a = (k - S::LOADS) / 2;
-                if ((k - S::LOADS) % 2 == 0)
-                    wr[s][a] = *reinterpret_cast<const v4i*>(wp[a] + (int64_t)i * (1024 * GK) + lane16);
-                else
-                    wsr[s][a] = *reinterpret_cast<const int*>(wsp[a] + (int64_t)(GK == 1 ? i >> 1 : i) * 128 + row4);
-            }
-        }
-    };
-
     v16f acc[WA][XB];
 #pragma unroll
     for (int a = 0; a < WA; ++a)
@@ -457,7 +426,7 @@ void mx_tiles_kernel(MxTiles p) {
     // and tiles add constants to.)
     int oa = (wn * GK + kg) * 1024 + lane * 16;
     int ox = S::XOFF + wt * S::XS + kg * kStepBytes<FMT> + lane * 16;
-    int ox8 = ox - lane * 8, osa = S::SOFF + wn * 128 + r * 4, osx = S::SOFF + (S::TL + wt) * 128 + r * 4;
+    int ox8 = ox - lane * 8, osa = S::SOFF + wn * 128 + r * 4, osx = S::SOFF + (S::TN + wt) * 128 + r * 4;
     opaque(oa);
     opaque(ox);
     opaque(ox8);
@@ -470,12 +439,10 @@ void mx_tiles_kernel(MxTiles p) {
         int sa[WA], sb[XB];  // dwords of four blocks' scales
     };
     auto read = [&](Operands& f, const uint8_t* buf) __attribute__((always_inline)) {
-        if constexpr (!WD) {
 #pragma unroll
-            for (int k = 0; k < WA; ++k) f.a[k] = *reinterpret_cast<const v4i*>(buf + oa + k * GK * 1024);
+        for (int k = 0; k < WA; ++k) f.a[k] = *reinterpret_cast<const v4i*>(buf + oa + k * GK * 1024);
 #pragma unroll
-            for (int k = 0; k < WA; ++k) f.sa[k] = *reinterpret_cast<const int*>(buf + osa + k * 128);
-        }
+        for (int k = 0; k < WA; ++k) f.sa[k] = *reinterpret_cast<const int*>(buf + osa + k * 128);
 #pragma unroll
         for (int b = 0; b < XB; ++b) {
             f.sb[b] = *reinterpret_cast<const int*>(buf + osx + b * 128);
@@ -494,13 +461,12 @@ void mx_tiles_kernel(MxTiles p) {
         }
     };
     // the matrix steps; the loads of a later stage go out behind them, one at a time
-    auto multiply = [&](auto kk, const Operands& f, int i, uint8_t* nb) __attribute__((always_inline)) {
-        constexpr int K = decltype(kk)::value;
+    auto multiply = [&](const Operands& f, int i, uint8_t* nb) __attribute__((always_inline)) {
         const int next = min(i + NB - 1, stages - 1);
         const int sh = 16 * (GK == 1 ? i & 1 : kg) + 8 * g;
         int sa[WA];
 #pragma unroll
-        for (int k = 0; k < WA; ++k) sa[k] = (int)((uint32_t)(WD ? wsr[WD ? K : 0][k] : f.sa[k]) >> sh);
+        for (int k = 0; k < WA; ++k) sa[k] = (int)((uint32_t)f.sa[k] >> sh);
 #pragma unroll
         for (int b = 0; b < XB; ++b) {
             const int sb = (int)((uint32_t)f.sb[b] >> sh);
@@ -509,11 +475,10 @@ void mx_tiles_kernel(MxTiles p) {
 #pragma unroll
                 for (int k = 0; k < WA; ++k) {
                     acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                        f.x[b][h], wide(WD ? wr[WD ? K : 0][k] : f.a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 4 * h, 0, sa[k]);
+                        f.x[b][h], wide(f.a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 4 * h, 0, sa[k]);
                     const int at = (b * H + h) * WA + k;
                     __builtin_amdgcn_sched_barrier(0);
-                    load(next, nb, WD ? (K + NB - 1) % NB : 0, at * S::VMEM / (GROUPS * WA),
-                         (at + 1) * S::VMEM / (GROUPS * WA));
+                    fetch(next, nb, at * S::LOADS / (GROUPS * WA), (at + 1) * S::LOADS / (GROUPS * WA));
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
@@ -526,7 +491,7 @@ void mx_tiles_kernel(MxTiles p) {
     // from the one that is filled, and would wait for the loads.)
     auto step = [&](auto k, int i) __attribute__((always_inline)) {
         constexpr int K = decltype(k)::value, R = PIPE ? (K + 1) % NB : K;
-        constexpr int N = (PIPE ? NB - 3 : NB - 2) * S::VMEM;
+        constexpr int N = (PIPE ? NB - 3 : NB - 2) * S::LOADS;
         __builtin_amdgcn_s_waitcnt((N & 15) | 0x0f70 | ((N >> 4) << 14));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -536,28 +501,28 @@ void mx_tiles_kernel(MxTiles p) {
             if constexpr (K % 2 == 0) {
                 read(odd, bufs[R]);
                 __builtin_amdgcn_sched_barrier(0);
-                multiply(k, even, i, bufs[(K + NB - 1) % NB]);
+                multiply(even, i, bufs[(K + NB - 1) % NB]);
             } else {
                 read(even, bufs[R]);
                 __builtin_amdgcn_sched_barrier(0);
-                multiply(k, odd, i, bufs[(K + NB - 1) % NB]);
+                multiply(odd, i, bufs[(K + NB - 1) % NB]);
             }
         } else {
             read(even, bufs[K]);
-            multiply(k, even, i, bufs[(K + NB - 1) % NB]);
+            multiply(even, i, bufs[(K + NB - 1) % NB]);
         }
         asm volatile("; buffer %0 done" ::"n"(R) : "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
 #define AERO_MX_EACH(DO) DO(0) DO(1) DO(2) DO(3) DO(4) DO(5) DO(6) DO(7) DO(8) DO(9) DO(10) DO(11)
-#define AERO_MX_FILL(K) if constexpr (K < NB - 1) load(min(K, stages - 1), bufs[K], WD ? K : 0, 0, S::VMEM);
+#define AERO_MX_FILL(K) if constexpr (K < NB - 1) fetch(min(K, stages - 1), bufs[K], 0, S::LOADS);
 #define AERO_MX_ROUND(K) if constexpr (K < NB) step(std::integral_constant<int, K>{}, i + K);
 #define AERO_MX_REST(K) \
     if constexpr (K < NB - 1) if (i + K < stages) step(std::integral_constant<int, K>{}, i + K);
     AERO_MX_EACH(AERO_MX_FILL)
     if constexpr (PIPE) {
         static_assert(NB >= 4 && NB % 2 == 0, "two sets of operands in turn, two stages ahead of the loads");
-        constexpr int N = (NB - 2) * S::VMEM;
+        constexpr int N = (NB - 2) * S::LOADS;
         __builtin_amdgcn_s_waitcnt((N & 15) | 0x0f70 | ((N >> 4) << 14));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -600,13 +565,19 @@ void mx_tiles_kernel(MxTiles p) {
         // through LDS
         constexpr int HALF = WA * XB / 2;
         static_assert(WA * XB % 2 == 0, "half of the tiles each");
-        __shared__ v4f join[S::NW][4][64];
-        v4f* mine = &join[wave][0][lane];
-        const v4f* other = &join[wave ^ (GN * GT)][0][lane];
+        // (a tile a wave, in the buffers where three of them hold that)
+        constexpr bool FITS = (S::NW + 2) / 3 * 4096 <= S::BYTES;
+        __shared__ v4f own[FITS ? 1 : S::NW * 256];
+        auto room = [&](int x) {
+            if constexpr (!FITS) return own + x * 256 + lane;
+            return reinterpret_cast<v4f*>(x % 3 == 0 ? b0 : x % 3 == 1 ? b1 : b2) + x / 3 * 256 + lane;
+        };
+        v4f* mine = room(wave);
+        const v4f* other = room(wave ^ (GN * GT));
 #pragma unroll
         for (int m = 0; m < HALF; ++m) {
             const v16f &lo = acc[m / XB][m % XB], &up = acc[(m + HALF) / XB][(m + HALF) % XB];
-            if (m > 0) __syncthreads();
+            __syncthreads();
             const v16f give = kg ? lo : up;
             v16f sum = kg ? up : lo;
 #pragma unroll
@@ -643,8 +614,10 @@ int64_t weight_codes_bytes(int64_t n_rows, int64_t n_cols) {
     return tiles32(n_rows) * ((n_cols + 127) / 128) * 2048;
 }
 
-// Calls of more tokens go through operands in the workspace.
-const int64_t kFewTokens = tune("mx_few", 32);
+// Calls that run on the few-token kernel; the others go through operands in the workspace. Up to
+// 32 tokens: at 24 tokens of 14336 x 4096 12.1 us and 13.0, of 4096 x 4096 7.4 and 12.2, but at 32
+// of 28672 x 8192 42 and 31, where x comes from the L2 once for each 64 rows.
+bool few_tokens(int64_t n_tok, int64_t n_rows) { return n_tok <= 16 || (n_tok <= 32 && n_rows < 20480); }
 
 template <int FMT>
 int64_t operand_bytes(int64_t n_tok, int KP) {
@@ -657,39 +630,27 @@ bool launch_stream(const MxGemm& p, hipStream_t s) {
                   dim3((unsigned)((p.N + 16 * WA - 1) / (16 * WA))), dim3(64 * NW), 0, s, p);
 }
 
+// Weight tiles a wave and waves a workgroup of the few-token kernel: more tiles share x (and, in
+// 8 bits, its halves), more workgroups keep more of the chip busy. Measured, us, with 16 (32) rows
+// a workgroup: 4096 x 4096, one token, 4.1 (5.0); 14336 x 4096, 8 tokens, 12.1 (8.7); 28672 x 8192,
+// one token, 31 (27); with 17 to 32 tokens, 16 / 32 / 64 rows: 4096 x 4096 7.4 / 8.8 / 11.3, 8192 x
+// 8192 18 / 12.8 / 16, 14336 x 4096 22 / 16.7 / 12.1. Short rows (up to 12 groups of 128 columns)
+// leave little for eight waves: 9728 x 896, one token, 3.3 with four of them and 3.7, 24 tokens 5.4
+// with 16 rows and one group on its way, 7.9 with 32 rows.
 template <int FMT>
 bool run_stream(const MxGemm& p, hipStream_t s) {
-    const int c = tune("mx_str", 0);
-    if (p.T <= 16) {
-        switch (c) {
-        case 1: return launch_stream<FMT, 1, 1, 4, 4>(p, s);
-        case 2: return launch_stream<FMT, 2, 1, 8, 2>(p, s);
-        case 3: return launch_stream<FMT, 2, 1, 4, 4>(p, s);
-        case 4: return launch_stream<FMT, 1, 1, 16, 2>(p, s);
-        case 5: return launch_stream<FMT, 1, 1, 8, 2>(p, s);
-        default: return launch_stream<FMT, 1, 1, 8, 4>(p, s);
-        }
+    if (p.T > 16) {
+        if (p.N >= 12288) return launch_stream<FMT, 4, 2, 8, 2>(p, s);
+        if (p.N >= 6144 && p.KP > 12) return launch_stream<FMT, 2, 2, 8, 2>(p, s);
+        return launch_stream<FMT, 1, 2, 8, 1>(p, s);
     }
-    if (p.T <= 32) {
-        switch (c) {
-        case 1: return launch_stream<FMT, 1, 2, 8, 2>(p, s);
-        case 2: return launch_stream<FMT, 4, 2, 8, 2>(p, s);
-        case 3: return launch_stream<FMT, 2, 2, 4, 4>(p, s);
-        default: return launch_stream<FMT, 2, 2, 8, 2>(p, s);
-        }
-    }
-    switch (c) {
-    case 1: return launch_stream<FMT, 1, 4, 8, 2>(p, s);
-    case 2: return launch_stream<FMT, 2, 4, 8, 2>(p, s);
-    case 3: return launch_stream<FMT, 4, 4, 4, 2>(p, s);
-    case 4: return launch_stream<FMT, 2, 4, 8, 1>(p, s);
-    default: return launch_stream<FMT, 4, 4, 8, 2>(p, s);
-    }
+    if (p.N >= 12288) return launch_stream<FMT, 2, 1, 8, 2>(p, s);
+    return p.KP <= 12 ? launch_stream<FMT, 1, 1, 4, 2>(p, s) : launch_stream<FMT, 1, 1, 8, 2>(p, s);
 }
 
-template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, bool WD, int WAVES>
+template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, int WAVES>
 bool launch_tiles(MxTiles p, hipStream_t s) {
-    using S = MxShape<FMT, WA, XB, GN, GT, GK, WD>;
+    using S = MxShape<FMT, WA, XB, GN, GT, GK>;
     p.bn = (p.nt + S::TN - 1) / S::TN;
     p.bt = (p.tt + S::TT - 1) / S::TT;
     const int64_t grid = ((int64_t)p.bn * p.bt + 7) / 8 * 8;
@@ -697,7 +658,7 @@ bool launch_tiles(MxTiles p, hipStream_t s) {
         set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
         return false;
     }
-    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, GK, NB, PIPE, WD, WAVES>, dim3((unsigned)grid),
+    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, GK, NB, PIPE, WAVES>, dim3((unsigned)grid),
                   dim3(64 * S::NW), 0, s, p);
 }
 
@@ -715,18 +676,33 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
                 g.xs, o, os, g.T, g.KB, g.KP, n))
         return false;
     const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, tune("mx_group", 4)};
-    const int64_t big = ((nt + 7) / 8) * ((tt + 3) / 4);
-    const int c = tune("mx_cfg", big >= 256 ? 0 : 1);
-    switch (c) {
-    case 0: return launch_tiles<FMT, 4, 2, 2, 2, 1, 3, false, false, 2>(p, s);
-    case 1: return launch_tiles<FMT, 2, 1, 2, 2, 2, 6, true, false, 2>(p, s);
-    case 2: return launch_tiles<FMT, 1, 2, 4, 1, 2, 6, true, true, 2>(p, s);
-    case 3: return launch_tiles<FMT, 1, 2, 4, 1, 2, 4, true, true, 2>(p, s);
-    case 4: return launch_tiles<FMT, 2, 1, 1, 2, 2, 6, true, false, 1>(p, s);
-    case 5: return launch_tiles<FMT, 1, 2, 2, 1, 2, 6, true, true, 1>(p, s);
-    case 6: return launch_tiles<FMT, 2, 2, 2, 1, 2, 6, true, true, 1>(p, s);
-    case 7: return launch_tiles<FMT, 2, 2, 4, 1, 2, 6, true, true, 2>(p, s);
-    default: return launch_tiles<FMT, 2, 1, 2, 2, 2, 6, true, true, 2>(p, s);
+    // The tiles by what a round of them takes: microseconds for 128 columns and the workgroups
+    // that run at a time, measured at one round (512 x 28672, 512 x 6144, 512 x 4096, 32 x 28672
+    // and 48 x 4096 results).
+    struct Tiles {
+        int n, t, slots;
+        float cost[2];       // 8 bits, 4 bits
+    };
+    static const Tiles kTiles[5] = {{8, 4, 512, {1.9f, 1.12f}}, {8, 2, 256, {0.58f, 0.58f}},
+                                    {4, 2, 256, {0.40f, 0.31f}}, {4, 1, 256, {0.30f, 0.21f}},
+                                    {2, 1, 256, {0.23f, 0.12f}}};
+    int best = 0;
+    float least = 0.f;
+    for (int i = 0; i < 5; ++i) {
+        const Tiles& c = kTiles[i];
+        const int64_t n = ((nt + c.n - 1) / c.n) * ((tt + c.t - 1) / c.t);
+        const float cost = (float)((n + c.slots - 1) / c.slots) * c.cost[FMT == AERO_MX_INT8 ? 0 : 1];
+        if (i == 0 || cost < least) {
+            best = i;
+            least = cost;
+        }
+    }
+    switch (tune("mx_cfg", best)) {
+    case 0: return launch_tiles<FMT, 4, 2, 2, 2, 1, 3, false, 2>(p, s);
+    case 1: return launch_tiles<FMT, 4, 1, 2, 2, 2, 4, true, 2>(p, s);
+    case 2: return launch_tiles<FMT, 2, 1, 2, 2, 2, 6, true, 2>(p, s);
+    case 3: return launch_tiles<FMT, 2, 1, 2, 1, 2, 6, true, 1>(p, s);
+    default: return launch_tiles<FMT, 2, 1, 1, 1, 2, 6, true, 1>(p, s);
     }
 }
 
@@ -770,7 +746,7 @@ int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, in
     if ((fmt != AERO_MX_INT8 && fmt != AERO_MX_FP4) || n_tok < 0 ||
         !weight_sizes_ok("mx_matmul_workspace", n_rows, n_cols))
         return -1;
-    if (n_tok <= kFewTokens) return 0;
+    if (few_tokens(n_tok, n_rows)) return 0;
     const int KP = (int)((n_cols + 127) / 128);
     return fmt == AERO_MX_INT8 ? operand_bytes<AERO_MX_INT8>(n_tok, KP)
                                : operand_bytes<AERO_MX_FP4>(n_tok, KP);
@@ -798,7 +774,7 @@ int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, con
     MxGemm p{codes, scales, (const uint8_t*)w, (const uint8_t*)w + weight_codes_bytes(n_rows, n_cols), y,
              n_tok, n_rows, KB, KP, aligned16(y) && n_rows % 4 == 0};
     const hipStream_t s = (hipStream_t)stream;
-    if (n_tok > kFewTokens) {
+    if (!few_tokens(n_tok, n_rows)) {
         const int64_t need = aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok);
         if (workspace == nullptr || !aligned16(workspace) || ws_bytes < need) {
             set_error("mx_matmul: the workspace takes %lld bytes at a 16-byte address", (long long)need);
