@@ -44,6 +44,55 @@ __device__ __forceinline__ double act64(double v) {
     }
 }
 
+// exp2(hi + lo), lo small, to 2^-22 (the hardware's exp2 is within 2^-23).
+__device__ __forceinline__ float exp2_split(float hi, float lo) {
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return __builtin_fmaf(e, lo * 0.693147182f, e);
+}
+
+// act(v) in 32 bits, to a relative kActOff<KIND>, the later product with `up` and the rounding
+// included; ok becomes false where it may be further off (far in the negative tail). The
+// arguments of exp are kept in two parts: as one fp32 number their rounding alone would be |v|
+// 2^-24 of the result. Hardware exp2 and reciprocal: 2^-23 each.
+//   silu, sigmoid: 2^-22 (exp) + 2^-24 (1 + e) + 2^-23 (reciprocal) + 2^-23 (two products)
+//   gelu_tanh: the same, its argument from 64 bits
+//   gelu: the polynomial's terms are up to 4.5 times its value and it follows t 3.5 times
+//   relatively: 14 2^-23 with t's own 2^-22, on the negative side in full
+template <int KIND>
+constexpr float kActOff = KIND == AERO_ACT_GELU ? 0x1p-18f : 0x1p-20f;
+
+template <int KIND>
+__device__ __forceinline__ float act32(float v, bool& ok) {
+    constexpr float L = 1.44269502f, LO = 1.92596303e-8f;       // log2(e)
+    if constexpr (KIND == AERO_ACT_SILU || KIND == AERO_ACT_SIGMOID) {
+        const float hi = -v * L;
+        const float e = exp2_split(hi, __builtin_fmaf(-v, L, -hi) - v * LO);
+        ok = ok && hi < 90.f;
+        const float s = __builtin_amdgcn_rcpf(1.f + e);
+        return KIND == AERO_ACT_SILU ? v * s : s;
+    } else if constexpr (KIND == AERO_ACT_GELU_TANH) {
+        const double x = (double)v;
+        const double t = x * __builtin_fma(x * x, -2.0 * 0.7978845608028654 * 1.4426950408889634 * 0.044715,
+                                           -2.0 * 0.7978845608028654 * 1.4426950408889634);
+        const float hi = (float)t;
+        ok = ok && hi < 90.f;
+        return v * __builtin_amdgcn_rcpf(1.f + exp2_split(hi, (float)(t - (double)hi)));
+    } else {
+        const float a = fabsf(v) * 0.707106769f;
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, a, 1.f));
+        float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+        p = __builtin_fmaf(p, t, 1.421413741f);
+        p = __builtin_fmaf(p, t, -0.284496736f);
+        p = __builtin_fmaf(p, t, 0.254829592f);
+        // exp(-v^2 / 2)
+        const float s = v * v, s2 = __builtin_fmaf(v, v, -s), hi = s * (-0.5f * L);
+        const float lo = __builtin_fmaf(s, -0.5f * L, -hi) - 0.5f * (s * LO + s2 * L);
+        ok = ok && (v > 0.f || hi > -90.f);
+        p = p * t * exp2_split(hi, lo);
+        return 0.5f * v * (v < 0.f ? p : 2.f - p);
+    }
+}
+
 constexpr int kNone = -1;  // no activation, no second input: plain quantisation
 
 // Quad i of rows of nq quads, input rows ld floats apart; 8 consecutive lanes hold a block.
@@ -56,13 +105,28 @@ void mx_rows_kernel(const float* g, const float* u, uint8_t* codes, uint8_t* sca
     const uint32_t row = i / nq;
     const int64_t at = row * ld + 4 * (int64_t)(i - row * nq);
     float4 h = ld4(g + at, vec);
-    if constexpr (KIND != kNone) {
-        const float4 b = UP ? ld4(u + at, vec) : make_float4(1.f, 1.f, 1.f, 1.f);
-        auto one = [](float x, float y) {
-            const double a = act64<KIND>((double)x);
-            return (float)(UP ? a * (double)y : a);
+    if constexpr (KIND == AERO_ACT_IDENTITY) {
+        const float4 b = ld4(u + at, vec);      // (a product's fp32 rounding is its only one)
+        h = make_float4(h.x * b.x, h.y * b.y, h.z * b.z, h.w * b.w);
+    } else if constexpr (KIND != kNone) {
+        const float4 x = h, b = UP ? ld4(u + at, vec) : make_float4(1.f, 1.f, 1.f, 1.f);
+        // In 32 bits first: where no border of codes is near any value of the wave, they are the
+        // formula's. In 64 bits for all, 512 x 14336 took 17.4 us (silu), 512 x 14336 x 9 bytes
+        // without the activation 12.0.
+        bool ok = true;
+        auto fast = [&](float v, float w) {
+            const float a = act32<KIND>(v, ok);
+            return UP ? a * w : a;
         };
-        h = make_float4(one(h.x, b.x), one(h.y, b.y), one(h.z, b.z), one(h.w, b.w));
+        h = make_float4(fast(x.x, b.x), fast(x.y, b.y), fast(x.z, b.z), fast(x.w, b.w));
+        ok = mx_sure<FMT>(h, mx_amax(h), kActOff<KIND>) && ok;
+        if (__any(!ok)) {
+            auto one = [](float v, float w) {
+                const double a = act64<KIND>((double)v);
+                return (float)(UP ? a * (double)w : a);
+            };
+            h = make_float4(one(x.x, b.x), one(x.y, b.y), one(x.z, b.z), one(x.w, b.w));
+        }
     }
     mx_store<FMT>(h, i, codes, scales);
 }
@@ -119,11 +183,23 @@ struct MxNorm {
     bool vec;
 };
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xf, 0xf, true);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 // Sum over a workgroup of BS lanes, the same bits in every lane.
 template <int BS>
 __device__ __forceinline__ double mx_sum(double v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    v = dpp_add<0xB1>(v);       // lane ^ 1, ^ 2, then mirrored in 8 and in 16
+    v = dpp_add<0x4E>(v);
+    v = dpp_add<0x141>(v);
+    v = dpp_add<0x140>(v);
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
     if constexpr (BS > 64) {
         __shared__ double part[BS / 64];
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
@@ -143,94 +219,101 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) {
     return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 
-__device__ __forceinline__ float4 scaled4(float4 v, double inv, const MxNorm& p, int64_t c) {
-    double w[4] = {1.0, 1.0, 1.0, 1.0};
-    if (p.w != nullptr) {
-        const float4 f = p.vec ? *reinterpret_cast<const float4*>(p.w + 4 * c)
-                               : make_float4(p.w[4 * c], p.w[4 * c + 1], p.w[4 * c + 2], p.w[4 * c + 3]);
-        const double one = (p.flags & AERO_NORM_UNIT_OFFSET) ? 1.0 : 0.0;
-        w[0] = f.x + one; w[1] = f.y + one; w[2] = f.z + one; w[3] = f.w + one;
-    }
-    return make_float4((float)(v.x * inv * w[0]), (float)(v.y * inv * w[1]),
-                       (float)(v.z * inv * w[2]), (float)(v.w * inv * w[3]));
+__device__ __forceinline__ float4 scaled4(float4 v, double inv, float4 w, double one) {
+    return make_float4((float)(v.x * inv * (w.x + one)), (float)(v.y * inv * (w.y + one)),
+                       (float)(v.z * inv * (w.z + one)), (float)(v.w * inv * (w.w + one)));
 }
 
-// A row a workgroup, V quads of it in each lane's registers; V = 0: rows of any length,
-// read twice.
-template <int FMT, int BS, int V>
+__device__ __forceinline__ double norm_inv(double ss, const MxNorm& p) {
+    return 1.0 / sqrt(ss / (double)p.cols + (double)p.eps);
+}
+
+// A row a workgroup, V quads of it in each lane's registers. Loads are unconditional, from
+// clamped places (a branch around a load waits for those before it). With a residual and up to
+// four quads the weights are loaded with the row, otherwise beside each store: as in the fp32
+// norm, whose stores the loads behind them would wait for (512 x 4096 with a residual 7.0 us
+// without, 6.4 with; 64 x 28672, eight quads, 13.0 and 23.2).
+template <int FMT, int BS, int V, bool ADD>
 __global__ __launch_bounds__(BS)
 void mx_norm_kernel(MxNorm p) {
-    const int64_t row = blockIdx.x, nq = p.cols / 4, base = row * p.cols;
-    const int t = threadIdx.x;
-    auto quad = [&](int64_t c) {
-        float4 v = ld4(p.x + base + 4 * c, p.vec);
-        if (p.d != nullptr) v = add4(v, ld4(p.d + base + 4 * c, p.vec));
-        return v;
+    constexpr bool EARLY = ADD && V <= 4;
+    const int64_t row = blockIdx.x, base = row * p.cols;
+    const int nq = (int)(p.cols / 4), t = threadIdx.x;
+    const double one = p.w != nullptr && (p.flags & AERO_NORM_UNIT_OFFSET) ? 1.0 : 0.0;
+    float4 v[V], d[V], w[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = min(t + i * BS, nq - 1);
+        v[i] = ld_stream(p.x + base + 4 * c);
+        if constexpr (ADD) d[i] = ld_stream(p.d + base + 4 * c);
+    }
+    auto weights = [&](int c) {
+        return p.w != nullptr ? reinterpret_cast<const float4*>(p.w)[c] : make_float4(1.f, 1.f, 1.f, 1.f);
     };
-    auto put = [&](int64_t c, float4 v) {
-        if (p.d == nullptr) return;
-        float* o = p.xo + base + 4 * c;
-        if (p.vec) {
-            *reinterpret_cast<float4*>(o) = v;
-        } else {
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = weights(min(t + i * BS, nq - 1));
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const bool in = t + i * BS < nq;
+        if constexpr (ADD) {
+            v[i] = add4(v[i], d[i]);
+            if (in) {
+                const v4f q = {v[i].x, v[i].y, v[i].z, v[i].w};
+                __builtin_nontemporal_store(q, reinterpret_cast<v4f*>(p.xo + base) + t + i * BS);
+            }
+        }
+        ss += in ? sq4(v[i]) : 0.0;
+    }
+    const double inv = norm_inv(mx_sum<BS>(ss), p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = t + i * BS;
+        if (c < nq)
+            mx_store<FMT>(scaled4(v[i], inv, EARLY ? w[i] : weights(c), one), row * nq + c, p.codes, p.scales);
+    }
+}
+
+// Rows of any length and at any address, read twice.
+template <int FMT>
+__global__ __launch_bounds__(256)
+void mx_norm_any_kernel(MxNorm p) {
+    const int64_t row = blockIdx.x, nq = p.cols / 4, base = row * p.cols;
+    const double one = p.w != nullptr && (p.flags & AERO_NORM_UNIT_OFFSET) ? 1.0 : 0.0;
+    double ss = 0.0;
+    for (int64_t c = threadIdx.x; c < nq; c += 256) {
+        float4 v = ld4(p.x + base + 4 * c, false);
+        if (p.d != nullptr) {
+            v = add4(v, ld4(p.d + base + 4 * c, false));
+            float* o = p.xo + base + 4 * c;
             o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
         }
-    };
-    constexpr int N = V > 0 ? V : 1;
-    float4 v[N];
-    double ss = 0.0;
-    if constexpr (V > 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int64_t c = t + i * BS;
-            v[i] = c < nq ? quad(c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int64_t c = t + i * BS;
-            if (c < nq) put(c, v[i]);
-            ss += sq4(v[i]);
-        }
-    } else {
-        for (int64_t c = t; c < nq; c += BS) {
-            v[0] = quad(c);
-            put(c, v[0]);
-            ss += sq4(v[0]);
-        }
+        ss += sq4(v);
     }
-    ss = mx_sum<BS>(ss);
-    const double inv = 1.0 / sqrt(ss / (double)p.cols + (double)p.eps);
-    const int64_t q0 = row * nq;
-    if constexpr (V > 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int64_t c = t + i * BS;
-            if (c < nq) mx_store<FMT>(scaled4(v[i], inv, p, c), q0 + c, p.codes, p.scales);
-        }
-    } else {
-        // the sum comes from where this lane wrote it: xo may be x or d
-        for (int64_t c = t; c < nq; c += BS) {
-            float4 h;
-            if (p.d != nullptr) {
-                const float* o = p.xo + base + 4 * c;
-                h = make_float4(o[0], o[1], o[2], o[3]);
-            } else {
-                h = quad(c);
-            }
-            mx_store<FMT>(scaled4(h, inv, p, c), q0 + c, p.codes, p.scales);
-        }
+    const double inv = norm_inv(mx_sum<256>(ss), p);
+    // (the sum comes from where this lane wrote it: xo may be x or d)
+    const float* from = p.d != nullptr ? p.xo : p.x;
+    for (int64_t c = threadIdx.x; c < nq; c += 256) {
+        const float4 w = p.w != nullptr ? ld4(p.w + 4 * c, false) : make_float4(1.f, 1.f, 1.f, 1.f);
+        const float* q = from + base + 4 * c;
+        mx_store<FMT>(scaled4(make_float4(q[0], q[1], q[2], q[3]), inv, w, one), row * nq + c, p.codes, p.scales);
     }
 }
 
 template <int FMT, int BS, int V>
 bool launch_norm(const MxNorm& p, int64_t rows, hipStream_t s) {
-    return launch("mx_norm_kernel", mx_norm_kernel<FMT, BS, V>, dim3((unsigned)rows), dim3(BS), 0, s,
-                  p);
+    return launch("mx_norm_kernel",
+                  p.d != nullptr ? mx_norm_kernel<FMT, BS, V, true> : mx_norm_kernel<FMT, BS, V, false>,
+                  dim3((unsigned)rows), dim3(BS), 0, s, p);
 }
 
 template <int FMT>
 bool run_norm(const MxNorm& p, int64_t rows, hipStream_t s) {
     const int64_t nq = p.cols / 4;
+    if (!p.vec || nq > 8192)
+        return launch("mx_norm_any_kernel", mx_norm_any_kernel<FMT>, dim3((unsigned)rows), dim3(256), 0, s, p);
     if (nq <= 64) return launch_norm<FMT, 64, 1>(p, rows, s);
     if (nq <= 128) return launch_norm<FMT, 64, 2>(p, rows, s);
     if (nq <= 256) return launch_norm<FMT, 256, 1>(p, rows, s);
@@ -238,7 +321,7 @@ bool run_norm(const MxNorm& p, int64_t rows, hipStream_t s) {
     if (nq <= 1024) return launch_norm<FMT, 256, 4>(p, rows, s);
     if (nq <= 2048) return launch_norm<FMT, 512, 4>(p, rows, s);
     if (nq <= 4096) return launch_norm<FMT, 1024, 4>(p, rows, s);
-    return launch_norm<FMT, 1024, 0>(p, rows, s);
+    return launch_norm<FMT, 1024, 8>(p, rows, s);
 }
 
 // --------------------------------------------------------------- the way back

@@ -71,17 +71,48 @@ __device__ __forceinline__ uint32_t mx_codes(float4 h, uint32_t s) {
 
 // One lane's four values of a block held by 8 lanes: codes to codes[quad], the scale
 // (by the first lane) to scales[quad / 8].
-template <int FMT>
-__device__ __forceinline__ void mx_store(float4 h, int64_t quad, uint8_t* codes, uint8_t* scales) {
+__device__ __forceinline__ uint32_t mx_amax(float4 h) {
     const uint32_t ax = mx_abs_bits(h.x), ay = mx_abs_bits(h.y);
     const uint32_t az = mx_abs_bits(h.z), aw = mx_abs_bits(h.w);
-    const uint32_t s = mx_scale<FMT>(mx_max8(max(max(ax, ay), max(az, aw))));
+    return mx_max8(max(max(ax, ay), max(az, aw)));
+}
+
+template <int FMT>
+__device__ __forceinline__ void mx_store(float4 h, int64_t quad, uint8_t* codes, uint8_t* scales) {
+    const uint32_t s = mx_scale<FMT>(mx_amax(h));
     const uint32_t c = mx_codes<FMT>(h, s);
     if constexpr (FMT == AERO_MX_INT8)
         reinterpret_cast<uint32_t*>(codes)[quad] = c;
     else
         reinterpret_cast<uint16_t*>(codes)[quad] = (uint16_t)c;
     if ((quad & 7) == 0) scales[quad >> 3] = (uint8_t)s;
+}
+
+// Whether four values that are only known to a relative d, and the block's largest of which
+// mx_max8 gives amax, have the codes they seem to: no border between two codes, nor one of
+// the scale, lies within d of any of them. (d counts the rounding to fp32, too.)
+template <int FMT>
+__device__ __forceinline__ bool mx_sure(float4 h, uint32_t amax, float d) {
+    if (amax == 0u) return true;          // (what 32 bits lose below 2^-149 has code 0)
+    const float top = __builtin_bit_cast(float, amax);
+    const uint32_t s = mx_scale<FMT>(amax);
+    // (a block near the subnormals, where errors are not relative, is not sure)
+    bool sure = s != 255u && top > 0x1p-100f && mx_scale<FMT>(mx_abs_bits(top * (1.f - d))) == mx_scale<FMT>(mx_abs_bits(top * (1.f + d)));
+    if constexpr (FMT == AERO_MX_INT8) {
+        const int e = 133 - (int)s;
+        float far = 0.f;     // the largest |distance to the code| + |code| d, half a code at a border
+        auto one = [&](float v) {
+            const float q = __builtin_amdgcn_ldexpf(v, e);
+            const float f = q - __builtin_rintf(q);
+            far = fmaxf(far, __builtin_fmaf(fabsf(q), d, fabsf(f)));
+        };
+        one(h.x); one(h.y); one(h.z); one(h.w);
+        return sure && far < 0.5f;
+    } else {
+        const float lo = 1.f - d, hi = 1.f + d;
+        return sure && mx_codes<FMT>(make_float4(h.x * lo, h.y * lo, h.z * lo, h.w * lo), s) ==
+                           mx_codes<FMT>(make_float4(h.x * hi, h.y * hi, h.z * hi, h.w * hi), s);
+    }
 }
 
 inline int64_t mx_row_bytes(int fmt, int64_t cols) { return fmt == AERO_MX_FP4 ? cols / 2 : cols; }

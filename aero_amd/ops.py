@@ -41,8 +41,16 @@ def _s(stream: Stream | None):
     return None if stream is None else stream.handle
 
 
+_KNOWN = {t: (np.dtype(t), np.dtype(t).itemsize)
+          for t in (np.float32, np.int32, np.uint32, np.int8, np.uint8)}
+
+
 def _need(arr, nelem: int, dtype, name: str):
     if arr is None:
+        return
+    known = _KNOWN.get(dtype)        # (the common case: every op checks each of its arrays)
+    if known is not None and type(arr) is DeviceArray and arr.dtype is known[0] and \
+            arr.nbytes >= nelem * known[1]:
         return
     if not isinstance(arr, DeviceArray):
         raise TypeError(f"{name}: expected a DeviceArray, got {type(arr).__name__}")

@@ -127,7 +127,7 @@ def test_dequant_every_code_and_scale(hip, fmt, off):
 
 
 NORMS = [(1, 32), (1, 896), (5, 224), (333, 2560), (9, 512), (64, 4096), (3, 8192), (2, 14336),
-         (3, 16384), (2, 16416), (2, 28672)]
+         (3, 16384), (2, 16416), (2, 28672), (2, 32800)]
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -201,6 +201,34 @@ def test_act(hip, fmt, kind, rows, cols, layout):
         ops.act_mul_mx(fmt, kind, DA.from_numpy(g), None, dc, ds, rows, cols)
         with np.errstate(over="ignore"):
             same(dc, ds, R.quantise(R.act(kind, g).astype(np.float32), fmt))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh", "sigmoid"])
+def test_act_next_to_borders(hip, fmt, kind):
+    """Values that lie within a few fp32 steps of a border between two codes, or of the scale:
+    `up` is such a border over the activation, moved by up to 40 steps either way. Tails, tiny
+    blocks and zeros too."""
+    rng = np.random.default_rng(21)
+    rows, cols = 64, 1024
+    g = (rng.standard_normal((rows, cols)) * 4).astype(np.float32)
+    a = R.act(kind, g)
+    if fmt == INT8:
+        border = (rng.integers(-126, 126, (rows, cols)) + 0.5) / 64
+    else:
+        border = rng.choice([.25, .75, 1.25, 1.75, 2.5, 3.5, 5.0], (rows, cols))
+    border[:, ::32] = R.TOP[fmt]
+    border *= np.exp2(np.repeat(rng.integers(-90, 90, (rows, cols // 32)), 32, 1))
+    border[-8:] *= 2.0 ** -140
+    u = border / np.where(a == 0, 1, a) * (1 + rng.integers(-40, 41, (rows, cols)) * 2.0 ** -24)
+    u = np.clip(u, -3e38, 3e38).astype(np.float32)
+    u[5], u[6, ::2] = 0, -0.0
+    g[7] = np.float32(-90)
+    with np.errstate(over="ignore", under="ignore"):
+        want = R.quantise((R.act(kind, g) * u).astype(np.float32), fmt)
+    dc, ds = held(fmt, rows, cols)
+    ops.act_mul_mx(fmt, kind, DA.from_numpy(g), DA.from_numpy(u), dc, ds, rows, cols)
+    same(dc, ds, want)
 
 
 def test_act_not_finite(hip):
