@@ -75,7 +75,8 @@ __device__ __forceinline__ void halves(uint32_t c, int& hi, int& lo) {
 __device__ __forceinline__ v8i wide(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
 // ----------------------------------------------------------- few tokens
-// The weights' bytes count. A workgroup takes 16 WA rows and up to 16 XB tokens; its waves take
+// The weights' bytes count: 28672 x 8192 for one token takes 27 us, 4.9 TB/s; small calls are a
+// launch and its round trips (9728 x 896: 3.3 us). A workgroup takes 16 WA rows and up to 16 XB tokens; its waves take
 // every NW-th 128 columns, D of them on their way at a time, and x as it lies in memory
 // (16x16x128 steps: lane l holds row or token l % 16, of 4-bit operands block l / 16 of the 128
 // columns, of e4m3 ones the bytes 16 (l / 16) .. of either half of them). The waves' sums are
@@ -329,9 +330,21 @@ struct MxTiles {
 
 // A workgroup of GN x GT waves, a wave WA weight tiles by XB token tiles of 32; with GK = 2
 // two such sets of waves, one for the first 64 of every 128 columns, one for the others, whose
-// sums are joined at the end: as many waves on tiles of the same size. Stages of 64 GK columns
-// go through NB buffers in LDS by direct loads of 1 KB, each wave its share, NB - 1 stages
-// ahead.
+// sums are joined at the end: as many waves on tiles of the same size (512 x 4096 x 14336 on
+// 128 x 64 tiles: 61 us with one set, 51 with two). Stages of 64 GK columns go through NB
+// buffers in LDS by direct loads of 1 KB, each wave its share, NB - 1 stages ahead. With PIPE a
+// stage's operands are read into registers while the one before is multiplied.
+//
+// What bounds the large tiles (256 x 128, two workgroups a CU) is power: with the matrix steps
+// busy 51% of the time the clock is down to 1.73 GHz (steps alone, from registers, run at 1.9),
+// and a product of 2048 x 28672 x 4096, twice as many steps as 4-bit x would take, is at 1.9-2.0
+// PFLOP/s (243-256 us; x in 4 bits 3.2). The loads take 106 us of it when nothing else runs, the
+// steps and LDS reads 155, the stores 35, past the caches (42 through them). The smaller
+// tiles move more bytes a result: 128 x 64 loads 21 KB for 128 columns, about 500 of a CU's
+// cycles (1 KB in 25 whatever it is), beside 480 of LDS and 280 of matrix steps, and a stage
+// takes 800. Measured and not kept: 256 x 256 tiles with the weights straight into registers
+// (282 us, one wave a SIMD), the smaller tiles so (the same times), and on x as it lies, its
+// halves as e4m3 made in registers (71 us where this takes 51: steps of twice the length).
 template <int FMT, int WA, int XB, int GN, int GT, int GK>
 struct MxShape {
     static constexpr int NW = GN * GT * GK, TN = WA * GN, TT = XB * GT;
@@ -351,15 +364,16 @@ void mx_tiles_kernel(MxTiles p) {
     // (arrays of their own: the compiler tells a load into one from a read of another)
 #define AERO_MX_BUF(K) __shared__ __attribute__((aligned(16))) uint8_t b##K[K < NB ? S::BYTES : 16]
     AERO_MX_BUF(0); AERO_MX_BUF(1); AERO_MX_BUF(2); AERO_MX_BUF(3); AERO_MX_BUF(4); AERO_MX_BUF(5);
-    AERO_MX_BUF(6); AERO_MX_BUF(7); AERO_MX_BUF(8); AERO_MX_BUF(9); AERO_MX_BUF(10); AERO_MX_BUF(11);
 #undef AERO_MX_BUF
-    uint8_t* const bufs[12] = {b0, b1, b2, b3, b4, b5, b6, b7, b8, b9, b10, b11};
+    static_assert(NB >= 3 && NB <= 6, "");
+    uint8_t* const bufs[6] = {b0, b1, b2, b3, b4, b5};
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, g = lane >> 5;
     // Each XCD (workgroups go round them in turn) takes a run of neighbouring tiles: four
     // token tiles beside one weight tile, then beside the next, so that what runs at a time
-    // on an XCD shares both sides through its L2.
+    // on an XCD shares both sides through its L2 (2048 x 28672 x 4096: 278 us with sixteen,
+    // 274 with four; 8192 x 4096 x 4096 184 and 172).
     const int per = gridDim.x >> 3;
     const int at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (at >= p.bn * p.bt) return;
@@ -514,7 +528,7 @@ void mx_tiles_kernel(MxTiles p) {
         asm volatile("; buffer %0 done" ::"n"(R) : "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-#define AERO_MX_EACH(DO) DO(0) DO(1) DO(2) DO(3) DO(4) DO(5) DO(6) DO(7) DO(8) DO(9) DO(10) DO(11)
+#define AERO_MX_EACH(DO) DO(0) DO(1) DO(2) DO(3) DO(4) DO(5)
 #define AERO_MX_FILL(K) if constexpr (K < NB - 1) fetch(min(K, stages - 1), bufs[K], 0, S::LOADS);
 #define AERO_MX_ROUND(K) if constexpr (K < NB) step(std::integral_constant<int, K>{}, i + K);
 #define AERO_MX_REST(K) \
@@ -675,10 +689,12 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
     if (!launch("mx_operand_kernel", mx_operand_kernel<FMT>, dim3((unsigned)blocks), dim3(256), 0, s, g.x,
                 g.xs, o, os, g.T, g.KB, g.KP, n))
         return false;
-    const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, tune("mx_group", 4)};
-    // The tiles by what a round of them takes: microseconds for 128 columns and the workgroups
-    // that run at a time, measured at one round (512 x 28672, 512 x 6144, 512 x 4096, 32 x 28672
-    // and 48 x 4096 results).
+    const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, 4};
+    // The tiles by what rounds of them take: the workgroups that run at a time, and microseconds
+    // for 128 columns of such a round, measured (8 bits: 512 x 28672, 512 x 6144, 512 x 4096, 32 x
+    // 28672 and 48 x 4096 results; 4 bits: 2048 x 28672 and 1500 x 5120). All five on the same
+    // call, us: 512 x 4096 x 14336 113 / 58 / 49 / 59 / 60, 512 x 6144 x 4096 42 / 26 / 32 / 34 /
+    // 35, 512 x 28672 x 4096 73 / 88 / 102 / 131 / 136, 64 x 4096 x 4096 38 / 22 / 16 / 13 / 13.
     struct Tiles {
         int n, t, slots;
         float cost[2];       // 8 bits, 4 bits
@@ -697,7 +713,7 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
             least = cost;
         }
     }
-    switch (tune("mx_cfg", best)) {
+    switch (tune("mx_tiles", best)) {
     case 0: return launch_tiles<FMT, 4, 2, 2, 2, 1, 3, false, 2>(p, s);
     case 1: return launch_tiles<FMT, 4, 1, 2, 2, 2, 4, true, 2>(p, s);
     case 2: return launch_tiles<FMT, 2, 1, 2, 2, 2, 6, true, 2>(p, s);

@@ -13,7 +13,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import _lib, ops
-from .device import DeviceArray, Stream, synchronize
+from .device import DeviceArray, Stream, recording_plan, synchronize
 
 
 class MxWeight:
@@ -23,6 +23,8 @@ class MxWeight:
     def __init__(self, codes: DeviceArray, scales: DeviceArray, n_rows: int, n_cols: int,
                  stream: Stream | None = None):
         ops._mx_rows(ops.MX_FP4, codes, scales, n_rows, n_cols)
+        if recording_plan() is not None:
+            raise RuntimeError("MxWeight: weights are laid out once, not in a plan")
         L = _lib.lib()
         nbytes = int(L.aero_hip_mx_weight_bytes(n_rows, n_cols))
         _lib.check(nbytes > 0, "MxWeight")
@@ -34,6 +36,8 @@ class MxWeight:
     @classmethod
     def from_rows(cls, x: DeviceArray, n_rows: int, n_cols: int) -> "MxWeight":
         """Quantised from fp32 rows (ops.mx_quantize); complete when this returns."""
+        if recording_plan() is not None:
+            raise RuntimeError("MxWeight: weights are laid out once, not in a plan")
         codes = DeviceArray.empty(n_rows * ops.mx_row_bytes(ops.MX_FP4, n_cols), np.uint8)
         scales = DeviceArray.empty(n_rows * (n_cols // 32), np.uint8)
         ops.mx_quantize(ops.MX_FP4, x, codes, scales, n_rows, n_cols)

@@ -734,14 +734,16 @@ int aero_hip_act_mul_mx(int fmt, int kind, const float* gate, const float* up, i
                         uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols,
                         void* stream);
 /* Weights for the product: 4-bit rows laid out once in the order of its matrix steps,
- * in aero_hip_mx_weight_bytes bytes (-1: bad sizes) at a 16-byte address. */
+ * in aero_hip_mx_weight_bytes bytes (-1: bad sizes) at a 16-byte address. At most 2^24
+ * columns. */
 int64_t aero_hip_mx_weight_bytes(int64_t n_rows, int64_t n_cols);
 int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64_t w_bytes,
                      int64_t n_rows, int64_t n_cols, void* stream);
 /* y[t][n] = sum over k of x[t][k] W[n][k] in fp32, x [n_tok][n_cols] in fmt, W of
  * mx_pack; products and the sums within a block are exact. Scale bytes of 8-bit rows
- * below 4 count as 4. Workspace: aero_hip_mx_matmul_workspace bytes (0: none; -1: bad
- * sizes), 16-byte aligned, its contents free between calls; calls that share it must be
+ * below 4 count as 4. Workspace: aero_hip_mx_matmul_workspace bytes (none up to 16 tokens,
+ * or 32 with fewer than 20480 rows; then about 1.6 bytes a value of x in 8 bits and 0.53
+ * in 4; -1: bad sizes), 16-byte aligned, its contents free between calls; calls that share it must be
  * ordered. */
 int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok);
 int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, const void* w,

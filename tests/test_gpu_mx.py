@@ -17,7 +17,7 @@ import pytest
 import mx_ref as R
 from conftest import bits_equal
 from aero_amd import mx, ops
-from aero_amd.device import DeviceArray as DA, Plan, Stream, synchronize
+from aero_amd.device import DeviceArray as DA, Plan, Stream, synchronize, tune_set
 
 pytestmark = pytest.mark.gpu
 
@@ -277,7 +277,8 @@ PRODUCTS = [(1, 1, 32), (1, 9728, 896), (1, 100, 64), (2, 33, 96), (3, 4096, 160
             (16, 257, 512), (17, 31, 2560), (31, 64, 128), (32, 96, 4096), (33, 130, 224),
             (64, 1000, 1024), (65, 129, 352), (100, 3, 4864), (127, 255, 736), (128, 256, 256),
             (129, 257, 288), (200, 513, 1056), (256, 512, 2048), (300, 1021, 928), (512, 640, 4096),
-            (513, 300, 544), (1000, 100, 1120)]
+            (513, 300, 544), (1000, 100, 1120), (9, 12300, 160),
+            (20, 12290, 96), (24, 6200, 1760), (18, 20490, 64)]
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -286,6 +287,20 @@ def test_product(hip, fmt, T, N, K):
     print(f"product fmt={fmt} T={T} N={N} K={K}", flush=True)
     a = operands(np.random.default_rng(T + N + K), fmt, T, N, K, spread=2)
     near(product(fmt, *a), *a, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("tiles", range(5))
+@pytest.mark.parametrize("T,N,K", [(33, 300, 32), (97, 261, 96), (130, 270, 160), (300, 513, 1632)])
+def test_product_on_every_tile(hip, fmt, tiles, T, N, K):
+    """Each size of tile, with one stage, fewer stages than buffers and more."""
+    print(f"product fmt={fmt} tiles={tiles} T={T} N={N} K={K}", flush=True)
+    a = operands(np.random.default_rng(tiles + T), fmt, T, N, K, spread=2)
+    tune_set("mx_tiles", tiles)
+    try:
+        near(product(fmt, *a), *a, fmt)
+    finally:
+        tune_set("mx_tiles", None)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -390,6 +405,62 @@ def test_feed_forward_in_a_plan(hip):
         same(ac, as_, R.quantise((R.act("silu", g) * u).astype(np.float32), INT8))
         near(y.numpy(), ac.numpy(), as_.numpy(), *R.quantise(wd, FP4), INT8)
     stream.destroy()
+
+
+def test_on_a_stream_of_its_own(hip):
+    """Every op on another stream than the null one, in order behind one another."""
+    rng = np.random.default_rng(15)
+    T, C, N = 40, 288, 70
+    x, d = (rng.standard_normal((T, C)).astype(np.float32) for _ in range(2))
+    wr = rng.standard_normal((N, C)).astype(np.float32)
+    weight = mx.MxWeight.from_rows(DA.from_numpy(wr), N, C)
+    dx, dd, y, back = DA.from_numpy(x), DA.from_numpy(d), DA.empty((T, N)), DA.empty((T, C))
+    c, s = held(INT8, T, C)
+    q, qs = held(FP4, T, C)
+    a, as_ = held(INT8, T, C)
+    stream = Stream()
+    ops.rmsnorm_mx(INT8, dx, None, c, s, T, C, 1e-5, d=dd, stream=stream)
+    ops.mx_matmul(INT8, c, s, weight, y, T, stream=stream)
+    ops.mx_dequant(INT8, c, s, back, T, C, stream=stream)
+    ops.mx_quantize(FP4, back, q, qs, T, C, stream=stream)
+    ops.act_mul_mx(INT8, "silu", back, dx, a, as_, T, C, stream=stream)
+    stream.synchronize()
+    stream.destroy()
+    want = R.quantise(R.norm(x + d, None, 1e-5, False), INT8)
+    same(c, s, want)
+    near(y.numpy(), *want, *R.quantise(wr, FP4), INT8)
+    values = R.values(*want, INT8).astype(np.float32)
+    assert bits_equal(back.numpy(), values)
+    same(q, qs, R.quantise(values, FP4))
+    same(a, as_, R.quantise((R.act("silu", values) * (x + d)).astype(np.float32), INT8))
+
+
+def test_weights_are_not_laid_out_in_a_plan(hip):
+    codes, scales = held(FP4, 4, 32)
+    x = DA.from_numpy(np.ones((4, 32), np.float32))
+    plan = Plan()
+    with plan:
+        with pytest.raises(RuntimeError):
+            mx.MxWeight(codes, scales, 4, 32)
+        with pytest.raises(RuntimeError):
+            mx.MxWeight.from_rows(x, 4, 32)
+    assert len(plan) == 0
+
+
+def test_plan_holds_the_weights(hip):
+    """The weights of a recorded product stay while the plan does."""
+    a = operands(np.random.default_rng(14), INT8, 3, 64, 128)
+    weight = mx.MxWeight(DA.from_numpy(a[2]), DA.from_numpy(a[3]), 64, 128)
+    xc, xs, y = DA.from_numpy(a[0]), DA.from_numpy(a[1]), DA.empty((3, 64))
+    plan = Plan()
+    with plan:
+        ops.mx_matmul(INT8, xc, xs, weight, y, 3)
+    del weight
+    others = [DA.from_numpy(np.full(64 * 128, 255, np.uint8)) for _ in range(8)]
+    plan.launch()
+    synchronize()
+    near(y.numpy(), *a, INT8)
+    del others
 
 
 def test_plan_keeps_its_workspace(hip):

@@ -41,7 +41,11 @@ def test_sizes():
     assert L.aero_hip_mx_matmul_workspace(2, 32, 32, 1) == -1
     assert L.aero_hip_mx_matmul_workspace(0, 32, 33, 1) == -1
     assert L.aero_hip_mx_matmul_workspace(0, 32, 32, -1) == -1
-    assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 0) >= 0
+    assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 0) == 0
+    assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 32) == 0
+    assert L.aero_hip_mx_matmul_workspace(0, 32, 160, 33) == 2 * 2 * (2 * 3072 + 128)
+    assert L.aero_hip_mx_matmul_workspace(1, 32, 160, 33) == 2 * 2 * (2 * 1024 + 128)
+    assert L.aero_hip_mx_matmul_workspace(0, 20480, 32, 17) == 2 * 3072 + 128
 
 
 @pytest.mark.parametrize("call,args,reason", [
@@ -78,6 +82,9 @@ def test_sizes():
     ("mx_matmul", (3, 16, 16, 16, 2176, 16, 1, 32, 1, None, 0, None), "format"),
     ("mx_matmul", (0, 16, 16, 16, 2176, 16, 1, 32, -1, None, 0, None), "arguments"),
     ("mx_matmul", (0, 16, 16, 24, 4096, 16, 1, 32, 1, None, 0, None), "take"),
+    ("mx_matmul", (0, 16, 16, 16, 2176, 16, 1, 32, 33, None, 0, None), "workspace"),
+    ("mx_matmul", (1, 16, 16, 16, 2176, 16, 1, 32, 33, 16, 2 * 2176 - 1, None), "workspace"),
+    ("mx_matmul", (0, 16, 16, 16, 2176, 16, 1, 32, 33, 24, 1 << 20, None), "workspace"),
 ])
 def test_refusals(call, args, reason):
     """Refused with a reason before anything is launched: no pointer here is memory."""
