@@ -226,7 +226,7 @@ void mx_stream_kernel(MxGemm p) {
 // code (in units of 1/8). A lane's 24 bytes a half lie as 16 and 8, 64 lanes side by side:
 // 1024 + 512 for the high halves, the same for the low ones.
 template <int FMT>
-constexpr int kStepBytes = FMT == AERO_MX_INT8 ? 3072 : 1024;
+constexpr int kStepBytes = FMT == AERO_MX_INT8 ? 2 * (1024 + 512) : 1024;
 
 // 32 codes of 6 bits, the first lowest, from bytes of a sign (bit 7) and a number 0 .. 15.
 __device__ __forceinline__ void pack6(const uint32_t (&b)[8], uint32_t (&o)[6]) {

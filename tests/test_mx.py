@@ -43,9 +43,9 @@ def test_sizes():
     assert L.aero_hip_mx_matmul_workspace(0, 32, 32, -1) == -1
     assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 0) == 0
     assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 32) == 0
-    assert L.aero_hip_mx_matmul_workspace(0, 32, 160, 33) == 2 * 2 * (2 * 3072 + 128)
+    assert L.aero_hip_mx_matmul_workspace(0, 32, 160, 33) == 2 * 2 * (4 * 1536 + 128)
     assert L.aero_hip_mx_matmul_workspace(1, 32, 160, 33) == 2 * 2 * (2 * 1024 + 128)
-    assert L.aero_hip_mx_matmul_workspace(0, 20480, 32, 17) == 2 * 3072 + 128
+    assert L.aero_hip_mx_matmul_workspace(0, 20480, 32, 17) == 4 * 1536 + 128
 
 
 @pytest.mark.parametrize("call,args,reason", [
