@@ -116,6 +116,8 @@ void mx_rows_kernel(const float* g, const float* u, uint8_t* codes, uint8_t* sca
         bool ok = true;
         auto fast = [&](float v, float w) {
             const float a = act32<KIND>(v, ok);
+            // (a subnormal act(v) has lost bits that a large w would show)
+            if (UP && KIND != AERO_ACT_SIGMOID) ok = ok && (fabsf(v) > 0x1p-100f || v == 0.f);
             return UP ? a * w : a;
         };
         h = make_float4(fast(x.x, b.x), fast(x.y, b.y), fast(x.z, b.z), fast(x.w, b.w));

@@ -759,9 +759,11 @@ int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64
 
 int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok) {
     using namespace aero;
-    if ((fmt != AERO_MX_INT8 && fmt != AERO_MX_FP4) || n_tok < 0 ||
-        !weight_sizes_ok("mx_matmul_workspace", n_rows, n_cols))
+    if ((fmt != AERO_MX_INT8 && fmt != AERO_MX_FP4) || n_tok < 0 || n_tok > 0x7fffffff) {
+        set_error("mx_matmul_workspace: format %d, %lld tokens", fmt, (long long)n_tok);
         return -1;
+    }
+    if (!weight_sizes_ok("mx_matmul_workspace", n_rows, n_cols)) return -1;
     if (few_tokens(n_tok, n_rows)) return 0;
     const int KP = (int)((n_cols + 127) / 128);
     return fmt == AERO_MX_INT8 ? operand_bytes<AERO_MX_INT8>(n_tok, KP)

@@ -231,6 +231,24 @@ def test_act_next_to_borders(hip, fmt, kind):
     same(dc, ds, want)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh", "sigmoid"])
+def test_act_of_subnormals_times_large(hip, fmt, kind):
+    """act(gate) below fp32's normal numbers, of which fp32 would keep a few bits or none,
+    brought back by `up`."""
+    rng = np.random.default_rng(22)
+    rows, cols = 16, 256
+    g = (rng.integers(-9, 10, (rows, cols)) * 2.0 ** -149).astype(np.float32)
+    g[4:8] = (rng.standard_normal((4, cols)) * 2.0 ** -130).astype(np.float32)
+    g[8:12, ::3] = (rng.standard_normal((4, 86)) * 2.0 ** -110).astype(np.float32)
+    g[12:] = np.where(rng.random((4, cols)) < .03, np.float32(2.0 ** -149), np.float32(0))
+    u = (rng.standard_normal((rows, cols)) * np.exp2(rng.integers(20, 120, (rows, 1)))).astype(np.float32)
+    want = R.quantise((R.act(kind, g) * u).astype(np.float32), fmt)
+    dc, ds = held(fmt, rows, cols)
+    ops.act_mul_mx(fmt, kind, DA.from_numpy(g), DA.from_numpy(u), dc, ds, rows, cols)
+    same(dc, ds, want)
+
+
 def test_act_not_finite(hip):
     g = np.random.default_rng(2).standard_normal((4, 64)).astype(np.float32)
     u = np.ones_like(g)

@@ -41,6 +41,7 @@ def test_sizes():
     assert L.aero_hip_mx_matmul_workspace(2, 32, 32, 1) == -1
     assert L.aero_hip_mx_matmul_workspace(0, 32, 33, 1) == -1
     assert L.aero_hip_mx_matmul_workspace(0, 32, 32, -1) == -1
+    assert L.aero_hip_mx_matmul_workspace(1, 32, 1 << 24, 1 << 60) == -1
     assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 0) == 0
     assert L.aero_hip_mx_matmul_workspace(0, 32, 32, 32) == 0
     assert L.aero_hip_mx_matmul_workspace(0, 32, 160, 33) == 2 * 2 * (4 * 1536 + 128)
