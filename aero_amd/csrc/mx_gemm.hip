@@ -328,23 +328,49 @@ struct MxTiles {
     int bn, bt, group;   // workgroups along each; token tiles side by side
 };
 
-// A workgroup of GN x GT waves, a wave WA weight tiles by XB token tiles of 32; with GK = 2
-// two such sets of waves, one for the first 64 of every 128 columns, one for the others, whose
-// sums are joined at the end: as many waves on tiles of the same size (512 x 4096 x 14336 on
-// 128 x 64 tiles: 61 us with one set, 51 with two). Stages of 64 GK columns go through NB
-// buffers in LDS by direct loads of 1 KB, each wave its share, NB - 1 stages ahead. With PIPE a
-// stage's operands are read into registers while the one before is multiplied.
+// A workgroup's place. Each XCD (workgroups go round them in turn) takes a run of neighbouring
+// tiles: four token tiles beside one weight tile, then beside the next, so that what runs at a time
+// on an XCD shares both sides through its L2 (2048 x 28672 x 4096: 278 us with sixteen, 274 with
+// four; 8192 x 4096 x 4096 184 and 172).
+__device__ __forceinline__ bool tile_of(const MxTiles& p, int& n, int& t) {
+    const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (at >= p.bn * p.bt) return false;
+    const int group = at / (p.group * p.bn), rest = at - group * p.group * p.bn;
+    const int width = min(p.group, p.bt - group * p.group);
+    n = rest / width;
+    t = group * p.group + rest % width;
+    return true;
+}
+
+// A tile of 32 x 32 sums: lane l holds column l % 32 of 16 tokens, 128 bytes of y in one piece for
+// each.
+template <int FMT>
+__device__ __forceinline__ void store_tile(const MxTiles& p, int nt, int tt, const v16f& v) {
+    constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
+    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)nt * 32 + (lane & 31), t1 = (int64_t)tt * 32 + 4 * (lane >> 5);
+    if (n >= p.N) return;
+    float* o = p.y + t1 * p.N + n;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int t = 8 * (i >> 2) + (i & 3);
+        if (t1 + t < p.T) __builtin_nontemporal_store(v[i] * UNIT, o + t * p.N);
+    }
+}
+
+// Large tiles (256 x 128 and 256 x 64 results). A workgroup of GN x GT waves, a wave WA weight
+// tiles by XB token tiles of 32; with GK = 2 two such sets of waves, one for the first 64 of every
+// 128 columns, one for the others, whose sums are joined at the end: as many waves on tiles half
+// the size. Stages of 64 GK columns go through NB buffers in LDS by direct loads of 1 KB, each wave
+// its share, NB - 1 stages ahead. With PIPE a stage's operands are read into registers while the
+// one before is multiplied.
 //
-// What bounds the large tiles (256 x 128, two workgroups a CU) is power: with the matrix steps
-// busy 51% of the time the clock is down to 1.73 GHz (steps alone, from registers, run at 1.9),
-// and a product of 2048 x 28672 x 4096, twice as many steps as 4-bit x would take, is at 1.9-2.0
-// PFLOP/s (243-256 us; x in 4 bits 3.2). The loads take 106 us of it when nothing else runs, the
-// steps and LDS reads 155, the stores 35, past the caches (42 through them). The smaller
-// tiles move more bytes a result: 128 x 64 loads 21 KB for 128 columns, about 500 of a CU's
-// cycles (1 KB in 25 whatever it is), beside 480 of LDS and 280 of matrix steps, and a stage
-// takes 800. Measured and not kept: 256 x 256 tiles with the weights straight into registers
-// (282 us, one wave a SIMD), the smaller tiles so (the same times), and on x as it lies, its
-// halves as e4m3 made in registers (71 us where this takes 51: steps of twice the length).
+// What bounds 256 x 128 (two workgroups a CU) is power: with the matrix steps busy 51% of the time
+// the clock is down to 1.73 GHz (steps alone, from registers, run at 1.9), and a product of
+// 2048 x 28672 x 4096, twice as many steps as 4-bit x would take, is at 1.9-2.0 PFLOP/s (243-256 us;
+// x in 4 bits 3.2). The loads take 106 us of it when nothing else runs, the steps and LDS reads
+// 155, the stores 35, past the caches (42 through them). Measured and not kept: 256 x 256 tiles
+// with the weights straight into registers (282 us, one wave a SIMD).
 template <int FMT, int WA, int XB, int GN, int GT, int GK>
 struct MxShape {
     static constexpr int NW = GN * GT * GK, TN = WA * GN, TT = XB * GT;
@@ -357,29 +383,23 @@ struct MxShape {
     static constexpr int BYTES = SOFF + SC * 1024;
 };
 
-template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, int WAVES>
-__global__ __launch_bounds__(64 * GN * GT * GK, WAVES)
+template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE>
+__global__ __launch_bounds__(64 * GN * GT * GK, 2)
 void mx_tiles_kernel(MxTiles p) {
     using S = MxShape<FMT, WA, XB, GN, GT, GK>;
     // (arrays of their own: the compiler tells a load into one from a read of another)
 #define AERO_MX_BUF(K) __shared__ __attribute__((aligned(16))) uint8_t b##K[K < NB ? S::BYTES : 16]
-    AERO_MX_BUF(0); AERO_MX_BUF(1); AERO_MX_BUF(2); AERO_MX_BUF(3); AERO_MX_BUF(4); AERO_MX_BUF(5);
+    AERO_MX_BUF(0); AERO_MX_BUF(1); AERO_MX_BUF(2); AERO_MX_BUF(3);
 #undef AERO_MX_BUF
-    static_assert(NB >= 3 && NB <= 6, "");
-    uint8_t* const bufs[6] = {b0, b1, b2, b3, b4, b5};
+    static_assert(NB == 3 || NB == 4, "");
+    uint8_t* const bufs[4] = {b0, b1, b2, b3};
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, g = lane >> 5;
-    // Each XCD (workgroups go round them in turn) takes a run of neighbouring tiles: four
-    // token tiles beside one weight tile, then beside the next, so that what runs at a time
-    // on an XCD shares both sides through its L2 (2048 x 28672 x 4096: 278 us with sixteen,
-    // 274 with four; 8192 x 4096 x 4096 184 and 172).
-    const int per = gridDim.x >> 3;
-    const int at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (at >= p.bn * p.bt) return;
-    const int group = at / (p.group * p.bn), rest = at - group * p.group * p.bn;
-    const int width = min(p.group, p.bt - group * p.group);
-    const int n0 = (rest / width) * S::TN, t0 = (group * p.group + rest % width) * S::TT;
+    int n0, t0;
+    if (!tile_of(p, n0, t0)) return;
+    n0 *= S::TN;
+    t0 *= S::TT;
 
     // This wave's pieces of a step, the scales' first: where they begin, how far a step goes.
     // (A piece past the last is the wave's one before once more, to the same place.)
@@ -528,7 +548,7 @@ void mx_tiles_kernel(MxTiles p) {
         asm volatile("; buffer %0 done" ::"n"(R) : "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-#define AERO_MX_EACH(DO) DO(0) DO(1) DO(2) DO(3) DO(4) DO(5)
+#define AERO_MX_EACH(DO) DO(0) DO(1) DO(2) DO(3)
 #define AERO_MX_FILL(K) if constexpr (K < NB - 1) fetch(min(K, stages - 1), bufs[K], 0, S::LOADS);
 #define AERO_MX_ROUND(K) if constexpr (K < NB) step(std::integral_constant<int, K>{}, i + K);
 #define AERO_MX_REST(K) \
@@ -556,18 +576,8 @@ void mx_tiles_kernel(MxTiles p) {
 #undef AERO_MX_REST
     __builtin_amdgcn_s_waitcnt(0x0f70);       // (no load is on its way when the wave ends)
 
-    constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
-    // lane l holds column l % 32 of 16 tokens: 128 bytes in one piece for each
     auto put = [&](int a, int b, const v16f& v) __attribute__((always_inline)) {
-        const int64_t n = (int64_t)(n0 + wn + a) * 32 + r;
-        const int64_t t1 = (int64_t)(t0 + wt + b) * 32 + 4 * g;
-        if (n >= p.N) return;
-        float* o = p.y + t1 * p.N + n;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = 8 * (i >> 2) + (i & 3);
-            if (t1 + t < p.T) __builtin_nontemporal_store(v[i] * UNIT, o + t * p.N);
-        }
+        store_tile<FMT>(p, n0 + wn + a, t0 + wt + b, v);
     };
     if constexpr (GK == 1) {
 #pragma unroll
@@ -579,11 +589,9 @@ void mx_tiles_kernel(MxTiles p) {
         // through LDS
         constexpr int HALF = WA * XB / 2;
         static_assert(WA * XB % 2 == 0, "half of the tiles each");
-        // (a tile a wave, in the buffers where three of them hold that)
-        constexpr bool FITS = (S::NW + 2) / 3 * 4096 <= S::BYTES;
-        __shared__ v4f own[FITS ? 1 : S::NW * 256];
+        // (a tile a wave, in the first three buffers)
+        static_assert((S::NW + 2) / 3 * 4096 <= S::BYTES, "room for a tile a wave");
         auto room = [&](int x) {
-            if constexpr (!FITS) return own + x * 256 + lane;
             return reinterpret_cast<v4f*>(x % 3 == 0 ? b0 : x % 3 == 1 ? b1 : b2) + x / 3 * 256 + lane;
         };
         v4f* mine = room(wave);
@@ -610,6 +618,154 @@ void mx_tiles_kernel(MxTiles p) {
             put(tile / XB, tile % XB, sum);
         }
     }
+}
+
+// Smaller tiles: 32 WA rows by 32 XB tokens, the columns split over the waves. Every NW-th 128
+// columns are one wave's, so that each operand is loaded once, straight into the registers of the
+// one wave that multiplies it, and LDS holds nothing but the waves' sums at the end. D groups of
+// 128 columns are in registers: one is multiplied, and behind each of its steps goes a load or two
+// of the group D - 1 ahead (loads in one piece before the steps: 512 x 4096 x 14336 in 43.5 us, so
+// 42.1, 512 x 28672 x 4096 on the same tiles 100 and 88).
+//
+// What bounds it is the way from the L2 to the CUs: 128 x 64 results take 21 KB for 128 columns, and
+// 256 workgroups get 18 TB/s (303 ns a group, 512 x 4096 x 14336), about 30 bytes a cycle each; the
+// matrix steps would take half of that. For 64 tokens of 28672 x 8192 HBM is the other bound (3.6
+// TB/s on 224 CUs). The same tiles through LDS, with two sets of waves: 512 x 4096 x 14336 50.5 us
+// here 42.1, 333 x 2560 x 10240 in 4 bits 18.0 and 14.7, 48 x 4096 x 14336 26.8 and 19.8, 100 x 4096 x
+// 4096 13.4 and 11.1, 64 x 28672 x 8192 39.9 and 38.9: there each byte crossed LDS three to four
+// times. Eight waves instead of four: 64 x 64 results 56 for 54, 64 x 32 65 for 62.
+template <int FMT, int WA, int XB, int NW, int D>
+__global__ __launch_bounds__(64 * NW, NW / 4)
+void mx_split_kernel(MxTiles p) {
+    constexpr int H = FMT == AERO_MX_INT8 ? 2 : 1, TILES = WA * XB;
+    __shared__ v4f part[NW][TILES][4][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, g = lane >> 5;
+    int n0, t0;
+    if (!tile_of(p, n0, t0)) return;
+    n0 *= WA;
+    t0 *= XB;
+
+    const uint8_t *w[WA], *ws[WA], *x[XB], *xs[XB];
+#pragma unroll
+    for (int a = 0; a < WA; ++a) {
+        const int64_t n = min(n0 + a, p.nt - 1);
+        w[a] = p.w + n * p.KP * 2048;
+        ws[a] = p.ws + n * p.KP * 128;
+    }
+#pragma unroll
+    for (int b = 0; b < XB; ++b) {
+        const int64_t t = min(t0 + b, p.tt - 1);
+        x[b] = p.x + t * p.KP * (2 * kStepBytes<FMT>);
+        xs[b] = p.xs + t * p.KP * 128;
+    }
+    struct Group {
+        v4i w[2][WA];
+        v8i x[2][XB][H];
+        int sw[WA], sx[XB];
+    };
+    Group f[D];
+    // load l of a group: the scales, then the operands in the order of the steps
+    constexpr int XL = 2 * H - (H == 1), STEP = WA + XB * XL, LOADS = WA + XB + 2 * STEP;
+    auto load = [&](Group& f, int k, int l) __attribute__((always_inline)) {
+        if (l < WA) {
+            f.sw[l] = *reinterpret_cast<const int*>(ws[l] + (int64_t)k * 128 + r * 4);
+        } else if (l < WA + XB) {
+            f.sx[l - WA] = *reinterpret_cast<const int*>(xs[l - WA] + (int64_t)k * 128 + r * 4);
+        } else {
+            const int j = (l - WA - XB) / STEP, i = (l - WA - XB) % STEP;
+            if (i < WA) {
+                f.w[j][i] = *reinterpret_cast<const v4i*>(w[i] + (int64_t)k * 2048 + j * 1024 + lane * 16);
+            } else {
+                const int b = (i - WA) / XL, h = (i - WA) % XL / (H == 2 ? 2 : 1), e = (i - WA) % XL % 2;
+                const uint8_t* q = x[b] + ((int64_t)k * 2 + j) * kStepBytes<FMT> + 1536 * h;
+                if (H == 2 && e == 1) {
+                    const v2i v = *reinterpret_cast<const v2i*>(q + 1024 + lane * 8);
+                    const v8i e8 = __builtin_shufflevector(v, v, 0, 1, -1, -1, -1, -1, -1, -1);
+                    f.x[j][b][h] = __builtin_shufflevector(f.x[j][b][h], e8, 0, 1, 2, 3, 8, 9, -1, -1);
+                } else {
+                    f.x[j][b][h] = wide(*reinterpret_cast<const v4i*>(q + lane * 16));
+                }
+            }
+        }
+    };
+    v16f acc[WA][XB];
+#pragma unroll
+    for (int a = 0; a < WA; ++a)
+#pragma unroll
+        for (int b = 0; b < XB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+    // the matrix steps of a group; the loads of a later one go out behind them
+    auto compute = [&](const Group& f, Group& nf, int k, bool more) __attribute__((always_inline)) {
+        constexpr int M = 2 * XB * H * WA;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int sh = 16 * j + 8 * g;
+#pragma unroll
+            for (int b = 0; b < XB; ++b) {
+                const int sb = (int)((uint32_t)f.sx[b] >> sh);
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int a = 0; a < WA; ++a) {
+                        acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                            f.x[j][b][h], wide(f.w[j][a]), acc[a][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 4 * h, 0,
+                            (int)((uint32_t)f.sw[a] >> sh));
+                        const int m = ((j * XB + b) * H + h) * WA + a;
+                        if (more) {
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int l = m * LOADS / M; l < (m + 1) * LOADS / M; ++l) load(nf, k, l);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+            }
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) {
+            load(f[d], min(wave + d * NW, p.KP - 1), l);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    int k = wave;
+    for (; k + (D - 1) * NW < p.KP; k += D * NW) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            compute(f[d], f[(d + D - 1) % D], min(k + (d + D - 1) * NW, p.KP - 1), true);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < D - 1; ++d)
+        if (k + d * NW < p.KP) compute(f[d], f[d], 0, false);
+
+    // each tile's sums by one wave, the others' through LDS
+#pragma unroll
+    for (int m = 0; m < TILES; ++m)
+        if (m % NW != wave) {
+            const v16f v = acc[m / XB][m % XB];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[wave][m][i][lane] = v4f{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < TILES; ++m)
+        if (m % NW == wave) {
+            v16f v = acc[m / XB][m % XB];
+#pragma unroll
+            for (int o = 1; o < NW; ++o)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v4f q = part[(wave + o) % NW][m][i][lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[4 * i + e] += q[e];
+                }
+            store_tile<FMT>(p, n0 + m / XB, t0 + m % XB, v);
+        }
 }
 
 int64_t tiles32(int64_t n) { return (n + 31) / 32; }
@@ -662,7 +818,7 @@ bool run_stream(const MxGemm& p, hipStream_t s) {
     return p.KP <= 12 ? launch_stream<FMT, 1, 1, 4, 2>(p, s) : launch_stream<FMT, 1, 1, 8, 2>(p, s);
 }
 
-template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE, int WAVES>
+template <int FMT, int WA, int XB, int GN, int GT, int GK, int NB, bool PIPE>
 bool launch_tiles(MxTiles p, hipStream_t s) {
     using S = MxShape<FMT, WA, XB, GN, GT, GK>;
     p.bn = (p.nt + S::TN - 1) / S::TN;
@@ -672,8 +828,20 @@ bool launch_tiles(MxTiles p, hipStream_t s) {
         set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
         return false;
     }
-    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, GK, NB, PIPE, WAVES>, dim3((unsigned)grid),
+    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, GK, NB, PIPE>, dim3((unsigned)grid),
                   dim3(64 * S::NW), 0, s, p);
+}
+
+template <int FMT, int WA, int XB, int NW, int D>
+bool launch_split(MxTiles p, hipStream_t s) {
+    p.bn = (p.nt + WA - 1) / WA;
+    p.bt = (p.tt + XB - 1) / XB;
+    const int64_t grid = ((int64_t)p.bn * p.bt + 7) / 8 * 8;
+    if (grid > 0x7fffffff) {
+        set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
+        return false;
+    }
+    return launch("mx_split_kernel", mx_split_kernel<FMT, WA, XB, NW, D>, dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
 }
 
 template <int FMT>
@@ -691,34 +859,37 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
         return false;
     const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, 4};
     // The tiles by what rounds of them take: the workgroups that run at a time, and microseconds
-    // for 128 columns of such a round, measured (8 bits: 512 x 28672, 512 x 6144, 512 x 4096, 32 x
-    // 28672 and 48 x 4096 results; 4 bits: 2048 x 28672 and 1500 x 5120). All five on the same
-    // call, us: 512 x 4096 x 14336 113 / 58 / 49 / 59 / 60, 512 x 6144 x 4096 42 / 26 / 32 / 34 /
-    // 35, 512 x 28672 x 4096 73 / 88 / 102 / 131 / 136, 64 x 4096 x 4096 38 / 22 / 16 / 13 / 13.
+    // of such a round, for each 128 columns and beside them, fitted to measured calls. All six on
+    // the same call, us: 512 x 28672 x 4096 73 / 88 / 88 / 108 / 104 / 108, 512 x 6144 x 4096 42 / 27 /
+    // 29 / 29 / 27 / 29, 512 x 4096 x 14336 113 / 58 / 42 / 54 / 49 / 62, 300 x 9728 x 896 17 / 13 / 16 /
+    // 16 / 16 / 15, 64 x 4096 x 4096 38 / 22 / 16 / 12 / 12 / 10; in 4 bits 333 x 2560 x 10240 (the
+    // last four) 20 / 15 / 16 / 17, 1500 x 5120 x 2048 21 / 23 / 28 / 24 / 26 / 26.
     struct Tiles {
         int n, t, slots;
-        float cost[2];       // 8 bits, 4 bits
+        float each[2], once[2];      // 8 bits, 4 bits
     };
-    static const Tiles kTiles[5] = {{8, 4, 512, {1.9f, 1.12f}}, {8, 2, 256, {0.58f, 0.58f}},
-                                    {4, 2, 256, {0.40f, 0.31f}}, {4, 1, 256, {0.30f, 0.21f}},
-                                    {2, 1, 256, {0.23f, 0.12f}}};
+    static const Tiles kTiles[6] = {{8, 4, 512, {1.75f, 1.1f}, {5.f, 1.f}},     {8, 2, 256, {0.57f, 0.39f}, {4.5f, 3.3f}},
+                                    {4, 2, 256, {0.31f, 0.15f}, {2.5f, 3.8f}},  {2, 2, 256, {0.21f, 0.1f}, {2.4f, 1.4f}},
+                                    {4, 1, 256, {0.2f, 0.12f}, {2.2f, 1.4f}},   {2, 1, 256, {0.118f, 0.075f}, {1.f, 0.5f}}};
+    constexpr int F = FMT == AERO_MX_INT8 ? 0 : 1;
     int best = 0;
     float least = 0.f;
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < 6; ++i) {
         const Tiles& c = kTiles[i];
         const int64_t n = ((nt + c.n - 1) / c.n) * ((tt + c.t - 1) / c.t);
-        const float cost = (float)((n + c.slots - 1) / c.slots) * c.cost[FMT == AERO_MX_INT8 ? 0 : 1];
+        const float cost = (float)((n + c.slots - 1) / c.slots) * (c.each[F] * g.KP + c.once[F]);
         if (i == 0 || cost < least) {
             best = i;
             least = cost;
         }
     }
     switch (tune("mx_tiles", best)) {
-    case 0: return launch_tiles<FMT, 4, 2, 2, 2, 1, 3, false, 2>(p, s);
-    case 1: return launch_tiles<FMT, 4, 1, 2, 2, 2, 4, true, 2>(p, s);
-    case 2: return launch_tiles<FMT, 2, 1, 2, 2, 2, 6, true, 2>(p, s);
-    case 3: return launch_tiles<FMT, 2, 1, 2, 1, 2, 6, true, 1>(p, s);
-    default: return launch_tiles<FMT, 2, 1, 1, 1, 2, 6, true, 1>(p, s);
+    case 0: return launch_tiles<FMT, 4, 2, 2, 2, 1, 3, false>(p, s);
+    case 1: return launch_tiles<FMT, 4, 1, 2, 2, 2, 4, true>(p, s);
+    case 2: return launch_split<FMT, 4, 2, 4, 2>(p, s);
+    case 3: return launch_split<FMT, 2, 2, 4, 3>(p, s);
+    case 4: return launch_split<FMT, 4, 1, 4, 3>(p, s);
+    default: return launch_split<FMT, 2, 1, 4, 3>(p, s);
     }
 }
 

@@ -308,7 +308,7 @@ def test_product(hip, fmt, T, N, K):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("tiles", range(5))
+@pytest.mark.parametrize("tiles", range(6))
 @pytest.mark.parametrize("T,N,K", [(33, 300, 32), (97, 261, 96), (130, 270, 160), (300, 513, 1632)])
 def test_product_on_every_tile(hip, fmt, tiles, T, N, K):
     """Each size of tile, with one stage, fewer stages than buffers and more."""
