@@ -75,7 +75,7 @@ __device__ __forceinline__ void halves(uint32_t c, int& hi, int& lo) {
 __device__ __forceinline__ v8i wide(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
 // ----------------------------------------------------------- few tokens
-// The weights' bytes count: 28672 x 8192 for one token takes 27 us, 4.9 TB/s; small calls are a
+// The weights' bytes count: 28672 x 8192 for one token takes 28 us, 4.5 TB/s; small calls are a
 // launch and its round trips (9728 x 896: 3.3 us). A workgroup takes 16 WA rows and up to 16 XB tokens; its waves take
 // every NW-th 128 columns, D of them on their way at a time, and x as it lies in memory
 // (16x16x128 steps: lane l holds row or token l % 16, of 4-bit operands block l / 16 of the 128
@@ -625,15 +625,17 @@ void mx_tiles_kernel(MxTiles p) {
 // one wave that multiplies it, and LDS holds nothing but the waves' sums at the end. D groups of
 // 128 columns are in registers: one is multiplied, and behind each of its steps goes a load or two
 // of the group D - 1 ahead (loads in one piece before the steps: 512 x 4096 x 14336 in 43.5 us, so
-// 42.1, 512 x 28672 x 4096 on the same tiles 100 and 88).
+// in 42.1, 512 x 28672 x 4096 on the same tiles 100 and 88).
 //
 // What bounds it is the way from the L2 to the CUs: 128 x 64 results take 21 KB for 128 columns, and
 // 256 workgroups get 18 TB/s (303 ns a group, 512 x 4096 x 14336), about 30 bytes a cycle each; the
 // matrix steps would take half of that. For 64 tokens of 28672 x 8192 HBM is the other bound (3.6
 // TB/s on 224 CUs). The same tiles through LDS, with two sets of waves: 512 x 4096 x 14336 50.5 us
-// here 42.1, 333 x 2560 x 10240 in 4 bits 18.0 and 14.7, 48 x 4096 x 14336 26.8 and 19.8, 100 x 4096 x
+// and 42.1, 333 x 2560 x 10240 in 4 bits 18.0 and 14.7, 48 x 4096 x 14336 26.8 and 19.8, 100 x 4096 x
 // 4096 13.4 and 11.1, 64 x 28672 x 8192 39.9 and 38.9: there each byte crossed LDS three to four
-// times. Eight waves instead of four: 64 x 64 results 56 for 54, 64 x 32 65 for 62.
+// times. Eight waves instead of four: 64 x 64 results 56 us for 54 (512 x 4096 x 14336), 64 x 32 65
+// for 62. Weights by loads that pass the caches: 64 x 28672 x 8192 41.4, the others a tenth to a
+// third slower, as their weights no longer come from the last-level cache.
 template <int FMT, int WA, int XB, int NW, int D>
 __global__ __launch_bounds__(64 * NW, NW / 4)
 void mx_split_kernel(MxTiles p) {
@@ -863,7 +865,7 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
     // the same call, us: 512 x 28672 x 4096 73 / 88 / 88 / 108 / 104 / 108, 512 x 6144 x 4096 42 / 27 /
     // 29 / 29 / 27 / 29, 512 x 4096 x 14336 113 / 58 / 42 / 54 / 49 / 62, 300 x 9728 x 896 17 / 13 / 16 /
     // 16 / 16 / 15, 64 x 4096 x 4096 38 / 22 / 16 / 12 / 12 / 10; in 4 bits 333 x 2560 x 10240 (the
-    // last four) 20 / 15 / 16 / 17, 1500 x 5120 x 2048 21 / 23 / 28 / 24 / 26 / 26.
+    // last four) 20 / 15 / 16 / 18, 1500 x 5120 x 2048 21 / 23 / 28 / 24 / 26 / 26.
     struct Tiles {
         int n, t, slots;
         float each[2], once[2];      // 8 bits, 4 bits
