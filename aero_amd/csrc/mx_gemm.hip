@@ -787,8 +787,9 @@ int64_t weight_codes_bytes(int64_t n_rows, int64_t n_cols) {
 }
 
 // Calls that run on the few-token kernel; the others go through operands in the workspace. Up to
-// 32 tokens: at 24 tokens of 14336 x 4096 12.1 us and 13.0, of 4096 x 4096 7.4 and 12.2, but at 32
-// of 28672 x 8192 42 and 31, where x comes from the L2 once for each 64 rows.
+// 32 tokens: at 24 tokens of 4096 x 4096 7.5 us and 9.6, of 1024 x 2048 4.7 and 7.9, of 14336 x 4096
+// 12.0 and 11.2 (x in 4 bits 9.2 and 9.8), but at 32 of 28672 x 8192 42 and 30, where x comes from
+// the L2 once for each 64 rows.
 bool few_tokens(int64_t n_tok, int64_t n_rows) { return n_tok <= 16 || (n_tok <= 32 && n_rows < 20480); }
 
 template <int FMT>
