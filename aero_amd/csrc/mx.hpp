@@ -6,8 +6,9 @@
 //
 // The scale is the smallest power of two under which the block's largest magnitude
 // does not pass the format's largest (127/64, 6): nothing is cut off, and no value is
-// off by more than half a step. 8-bit rows keep s >= 4, so that the product can give
-// the low half of a code a scale byte of its own, s - 4.
+// off by more than half a step (in 8 bits, past 2^127 * 127/64, where no scale is left, the
+// largest code stands in). 8-bit rows keep s >= 4, so that the product can give the low half
+// of a code a scale byte of its own, down to s - 4.
 #pragma once
 #include "common.hpp"
 #include "aero_hip.h"

@@ -8,8 +8,12 @@
 // with 4-bit weights have 8 bits and one exponent range, so the step's sums lose nothing:
 // against 64 bits 1e-7 of the result. The same steps on e4m3 activations keep about 14 bits
 // of each sum of eight products, whose exponents differ (5e-5 measured on random codes): that
-// is why 8 bits are whole numbers here. l has the scale of h divided by 16, the scale byte
-// less 4.
+// is why 8 bits are whole numbers here.
+//
+// Sums are in units of y itself. In larger ones (y / 128 would follow from the codes as they
+// are) a sum near 2^-126 would be a subnormal number and lose bits that y has. So the halves'
+// scale bytes take what their codes leave out: h / 4 of the scale s is the code 2h of e2m3 at s,
+// and of e4m3 at s + 6, l / 64 the code l at s - 3 and s + 3.
 //
 // Weights are laid out once, in the order in which the steps take them: 32 rows, then
 // blocks of 32 columns, then the 32 rows' 16 bytes of a block; a step's operand is 1 KB in
@@ -64,12 +68,21 @@ void mx_pack_kernel(const uint8_t* codes, const uint8_t* scales, uint8_t* w, uin
     ws[((tile * KP + (kb >> 2)) * 32 + r) * 4 + (kb & 3)] = s;
 }
 
-// The halves of four 8-bit codes as e4m3 bytes.
+// The halves of four 8-bit codes: bytes of a sign and 2h (0 .. 16), of a sign and l.
 __device__ __forceinline__ void halves(uint32_t c, int& hi, int& lo) {
     const uint32_t s = c & 0x80808080u, t = s >> 7;
     const uint32_t mag = (c ^ ((s - t) | s)) + t;
-    hi = (int)(((mag >> 4) & 0x0F0F0F0Fu) | s);
+    hi = (int)(((mag >> 3) & 0x1E1E1E1Eu) | s);
     lo = (int)((mag & 0x0F0F0F0Fu) | s);
+}
+
+// Bytes of a sign and a number v = 0 .. 15 as e4m3 numbers v / 4: below 8 by table, from
+// there 2^1 and three bits.
+__device__ __forceinline__ int quarters(int b) {
+    const uint32_t v = (uint32_t)b & 0x07070707u, top = (uint32_t)b & 0x08080808u;
+    const uint32_t large = (top << 4) | ((top << 4) - (top >> 3));      // 0xFF where v is 8 or more
+    const uint32_t small = __builtin_amdgcn_perm(0x3E3C3A38u, 0x34302800u, v);
+    return (int)((large & (0x40404040u | v)) | (~large & small) | ((uint32_t)b & 0x80808080u));
 }
 
 __device__ __forceinline__ v8i wide(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
@@ -151,6 +164,7 @@ void mx_stream_kernel(MxGemm p) {
                     if (4 * k + 2 + (q >> 1) >= p.KB) c1 = zero;
                     if (4 * k + q >= p.KB) s = 4;
                 }
+                int sh = min(s + 6, 255), sl = s + 3;
                 v8i hi, lo;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -160,14 +174,25 @@ void mx_stream_kernel(MxGemm p) {
                     halves((uint32_t)c1[i], h, l);
                     hi[4 + i] = h; lo[4 + i] = l;
                 }
+                // (no scale byte for s + 6: blocks from 2^121 on, whose halves go in as h / 4 and
+                // l / 4 of s and s - 4)
+                if (__any(s > 248 && s != 255)) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        hi[i] = quarters((hi[i] & 0x1E1E1E1E) >> 1 | (hi[i] & (int)0x80808080));
+                        lo[i] = quarters(lo[i]);
+                    }
+                    sh = s;
+                    sl = s - 4;
+                }
 #pragma unroll
                 for (int a = 0; a < WA; ++a)
                     acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                        wide(w[d][a]), hi, acc[a][b], kF4, kF8, 0, sw[d][a], 0, s);
+                        wide(w[d][a]), hi, acc[a][b], kF4, kF8, 0, sw[d][a], 0, sh);
 #pragma unroll
                 for (int a = 0; a < WA; ++a)
                     acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                        wide(w[d][a]), lo, acc[a][b], kF4, kF8, 0, sw[d][a], 0, s - 4);
+                        wide(w[d][a]), lo, acc[a][b], kF4, kF8, 0, sw[d][a], 0, sl);
             } else {
                 v4i c0 = x0[d][b];
                 if (!whole && 4 * k + q >= p.KB) {
@@ -192,7 +217,6 @@ void mx_stream_kernel(MxGemm p) {
         }
     }
 
-    constexpr float UNIT = I8 ? 128.f : 1.f;            // h 16 / 64 = (h 2^-9) 2^7
 #pragma unroll
     for (int a = 0; a < WA; ++a) {
         if (a > 0) __syncthreads();
@@ -204,7 +228,6 @@ void mx_stream_kernel(MxGemm p) {
             v4f v = part[0][b][lane];
 #pragma unroll
             for (int k = 1; k < NW; ++k) v += part[k][b][lane];
-            v *= UNIT;
             const int64_t tok = 16 * b + r;
             if (tok >= p.T) continue;
             float* o = p.y + tok * p.N + n;
@@ -222,18 +245,18 @@ void mx_stream_kernel(MxGemm p) {
 // ---------------------------------------------------------- many tokens
 // x as operands, once a call: 32 tokens, then steps of 64 columns. 4 bits: as the weights.
 // 8 bits: the halves as 6-bit floats (e2m3), whose steps against 4-bit operands take half
-// the time of e4m3 ones (35 cycles and 64 measured). There too a number 0 .. 15 is its own
+// the time of e4m3 ones (35 cycles and 64 measured). There too a number 0 .. 16 is its own
 // code (in units of 1/8). A lane's 24 bytes a half lie as 16 and 8, 64 lanes side by side:
 // 1024 + 512 for the high halves, the same for the low ones.
 template <int FMT>
 constexpr int kStepBytes = FMT == AERO_MX_INT8 ? 2 * (1024 + 512) : 1024;
 
-// 32 codes of 6 bits, the first lowest, from bytes of a sign (bit 7) and a number 0 .. 15.
+// 32 codes of 6 bits, the first lowest, from bytes of a sign (bit 7) and a number 0 .. 16.
 __device__ __forceinline__ void pack6(const uint32_t (&b)[8], uint32_t (&o)[6]) {
     uint32_t d[8];       // four codes each, 24 bits
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t c = (b[i] & 0x0F0F0F0Fu) | ((b[i] >> 2) & 0x20202020u);
+        const uint32_t c = (b[i] & 0x1F1F1F1Fu) | ((b[i] >> 2) & 0x20202020u);
         const uint32_t e = (c & 0x003F003Fu) | ((c >> 2) & 0x0FC00FC0u);
         d[i] = (e & 0xFFFu) | ((e >> 4) & 0xFFF000u);
     }
@@ -344,9 +367,7 @@ __device__ __forceinline__ bool tile_of(const MxTiles& p, int& n, int& t) {
 
 // A tile of 32 x 32 sums: lane l holds column l % 32 of 16 tokens, 128 bytes of y in one piece for
 // each.
-template <int FMT>
 __device__ __forceinline__ void store_tile(const MxTiles& p, int nt, int tt, const v16f& v) {
-    constexpr float UNIT = FMT == AERO_MX_INT8 ? 2.f : 1.f;      // h 16 / 64 = (h / 8) 2
     const int lane = threadIdx.x & 63;
     const int64_t n = (int64_t)nt * 32 + (lane & 31), t1 = (int64_t)tt * 32 + 4 * (lane >> 5);
     if (n >= p.N) return;
@@ -354,7 +375,7 @@ __device__ __forceinline__ void store_tile(const MxTiles& p, int nt, int tt, con
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int t = 8 * (i >> 2) + (i & 3);
-        if (t1 + t < p.T) __builtin_nontemporal_store(v[i] * UNIT, o + t * p.N);
+        if (t1 + t < p.T) __builtin_nontemporal_store(v[i], o + t * p.N);
     }
 }
 
@@ -509,7 +530,7 @@ void mx_tiles_kernel(MxTiles p) {
 #pragma unroll
                 for (int k = 0; k < WA; ++k) {
                     acc[k][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                        f.x[b][h], wide(f.a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 4 * h, 0, sa[k]);
+                        f.x[b][h], wide(f.a[k]), acc[k][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 3 * h, 0, sa[k]);
                     const int at = (b * H + h) * WA + k;
                     __builtin_amdgcn_sched_barrier(0);
                     fetch(next, nb, at * S::LOADS / (GROUPS * WA), (at + 1) * S::LOADS / (GROUPS * WA));
@@ -577,7 +598,7 @@ void mx_tiles_kernel(MxTiles p) {
     __builtin_amdgcn_s_waitcnt(0x0f70);       // (no load is on its way when the wave ends)
 
     auto put = [&](int a, int b, const v16f& v) __attribute__((always_inline)) {
-        store_tile<FMT>(p, n0 + wn + a, t0 + wt + b, v);
+        store_tile(p, n0 + wn + a, t0 + wt + b, v);
     };
     if constexpr (GK == 1) {
 #pragma unroll
@@ -713,7 +734,7 @@ void mx_split_kernel(MxTiles p) {
 #pragma unroll
                     for (int a = 0; a < WA; ++a) {
                         acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                            f.x[j][b][h], wide(f.w[j][a]), acc[a][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 4 * h, 0,
+                            f.x[j][b][h], wide(f.w[j][a]), acc[a][b], H == 2 ? kF6 : kF4, kF4, 0, sb - 3 * h, 0,
                             (int)((uint32_t)f.sw[a] >> sh));
                         const int m = ((j * XB + b) * H + h) * WA + a;
                         if (more) {
@@ -766,7 +787,7 @@ void mx_split_kernel(MxTiles p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[4 * i + e] += q[e];
                 }
-            store_tile<FMT>(p, n0 + m / XB, t0 + m % XB, v);
+            store_tile(p, n0 + m / XB, t0 + m % XB, v);
         }
 }
 

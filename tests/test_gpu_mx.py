@@ -500,3 +500,68 @@ def test_plan_keeps_its_workspace(hip):
         plan.launch()
         synchronize()
         assert bits_equal(y.numpy(), first)
+
+
+# ------------------------------------------- products at the ends of fp32's range
+def whole(rng, fmt, T, N, K, unit):
+    """Random codes whose scales make every product a whole number of 2^unit: (operands,
+    sums in those units). The sums stay below 2^24, so that every partial sum is exact in
+    fp32 wherever 2^unit and the result are in its range, subnormal or not."""
+    xc = rng.integers(0, 256, (T, ops.mx_row_bytes(fmt, K))).astype(np.uint8)
+    xc = xc.view(np.int8) if fmt == INT8 else xc
+    wc = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    one = np.full((T, K // 32), 127, np.uint8), np.full((N, K // 32), 127, np.uint8)
+    low = 2.0 ** (-7 if fmt == INT8 else -2)          # 1/64 or 1/2, times 1/2
+    x, w = R.values(xc, one[0], fmt), R.values(wc, one[1], FP4)
+    sums = (x @ w.T) / low
+    assert (np.abs(x) @ np.abs(w).T / low < 2 ** 24).all()
+    total = 254 + unit + (7 if fmt == INT8 else 2)    # of the two scale bytes
+    return xc, wc, sums, total
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T,tiles", [(1, None), (13, None), (20, None), (32, None)] +
+                         [(40, k) for k in range(6)])
+@pytest.mark.parametrize("unit,x_scale", [(-149, 4), (-149, 60), (-149, 100), (-143, 30), (-135, 50),
+                                          (100, 247), (100, 248), (100, 249), (100, 254),
+                                          (0, 249), (20, 254)])
+def test_product_at_the_ends_of_the_range(hip, fmt, T, tiles, unit, x_scale):
+    """Sums of whole numbers of 2^unit come out exact down to fp32's last subnormal bit and
+    up to the largest scales, alike for every number of tokens."""
+    print(f"ends fmt={fmt} T={T} tiles={tiles} unit={unit} x_scale={x_scale}", flush=True)
+    N, K = 70, 352
+    rng = np.random.default_rng(T + x_scale)
+    xc, wc, sums, total = whole(rng, fmt, T, N, K, unit)
+    xs, ws = np.full((T, K // 32), x_scale, np.uint8), np.full((N, K // 32), total - x_scale, np.uint8)
+    assert 0 <= total - x_scale <= 254
+    tune_set("mx_tiles", tiles)
+    try:
+        got = product(fmt, xc, xs, wc, ws)
+    finally:
+        tune_set("mx_tiles", None)
+    assert bits_equal(got + np.float32(0), (sums * 2.0 ** unit).astype(np.float32) + np.float32(0))
+
+
+@pytest.mark.parametrize("T,tiles", [(1, None), (13, None), (32, None)] + [(40, k) for k in range(6)])
+def test_product_of_scales_far_apart(hip, T, tiles):
+    """Blocks of one token at both ends of the scales, tokens that are NaN, tiny or large
+    beside each other: 8-bit rows whose every block has a scale of its own."""
+    print(f"far apart T={T} tiles={tiles}", flush=True)
+    N, K = 40, 416
+    rng = np.random.default_rng(T)
+    xc = rng.integers(-128, 128, (T, K)).astype(np.int8)
+    xs = rng.choice(np.array([4, 5, 120, 247, 248, 249, 252, 254], np.uint8), (T, K // 32))
+    wc = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    ws = rng.integers(0, 110, (N, K // 32)).astype(np.uint8)
+    xs[T // 2, 7] = 255
+    tune_set("mx_tiles", tiles)
+    try:
+        got = product(INT8, xc, xs, wc, ws)
+    finally:
+        tune_set("mx_tiles", None)
+    ok = np.arange(T) != T // 2
+    assert np.isnan(got[T // 2]).all() and not np.isnan(got[ok]).any()
+    x, w = R.values(xc, xs, INT8)[ok], R.values(wc, ws, FP4)
+    # the terms' own bound, and half a last bit for each addition of what is subnormal
+    room = 2.0 ** -20 * (np.abs(x) @ np.abs(w).T) + 9 * K / 32 * 2.0 ** -150
+    assert (np.abs(got[ok] - x @ w.T) <= room).all()
