@@ -807,11 +807,44 @@ int64_t weight_codes_bytes(int64_t n_rows, int64_t n_cols) {
     return tiles32(n_rows) * ((n_cols + 127) / 128) * 2048;
 }
 
+// Rows that a workgroup of the few-token kernel takes. More of them share x (and, in 8 bits, its
+// halves), more workgroups keep more of the chip busy. Measured, us, with 16 (32) rows: 4096 x
+// 4096, one token, 4.1 (5.0); 14336 x 4096, 8 tokens, 12.1 (8.7); 28672 x 8192, one token, 31 (27);
+// with 17 to 32 tokens, 16 / 32 / 64 rows: 4096 x 4096 7.4 / 8.8 / 11.3, 8192 x 8192 18 / 12.8 /
+// 16, 14336 x 4096 22 / 16.7 / 12.1. Short rows (up to 12 groups of 128 columns) leave little for
+// eight waves: 9728 x 896, 24 tokens, 5.4 with 16 rows and one group on its way, 7.9 with 32 rows.
+int stream_rows(int64_t n_tok, int64_t n_rows, int KP) {
+    if (n_tok > 16) return n_rows >= 12288 ? 64 : n_rows >= 6144 && KP > 12 ? 32 : 16;
+    return n_rows >= 12288 ? 32 : 16;
+}
+
 // Calls that run on the few-token kernel; the others go through operands in the workspace. Up to
-// 32 tokens: at 24 tokens of 4096 x 4096 7.5 us and 9.6, of 1024 x 2048 4.7 and 7.9, of 14336 x 4096
-// 12.0 and 11.2 (x in 4 bits 9.2 and 9.8), but at 32 of 28672 x 8192 42 and 30, where x comes from
-// the L2 once for each 64 rows.
-bool few_tokens(int64_t n_tok, int64_t n_rows) { return n_tok <= 16 || (n_tok <= 32 && n_rows < 20480); }
+// 16 tokens all, from 17 to 32 while rounds of workgroups on the CUs * tokens * columns stay below
+// a limit: the tiles take a launch more (6 us in all), and then less for each column. Measured
+// for 17 / 24 / 32 tokens, us on the few-token kernel and on tiles:
+//   8 bits, 16 rows: 4096 x 14336 16.9, 18.7 / 19.9, 18.8 / 23.3, 19.0; 4096 x 8192 10.8, 13.1 /
+//     12.5, 13.4 / 14.3, 13.5; in two rounds 5120 x 2560 7.2, 8.0 / 7.9, 8.2 / 9.1, 8.4 and 5120 x
+//     4096 11.0, 9.6 / 13.0, 9.9 / 15.0, 10.0
+//   8 bits, 32 rows: 8192 x 4096 8.5, 10.1 / 9.4, 10.4 / 10.2, 10.6; 8192 x 8192 13.2, 13.8 / 15.3,
+//     13.9 / 16.8, 14.2; in two rounds 8224 x 2048 8.8, 7.9 / 9.9, 8.2 / 11.0, 8.4
+//   8 bits, 64 rows: 16384 x 2048 7.6, 9.3 / 8.1, 9.6 / 8.5, 9.9; 14336 x 4096 11.2, 10.9 / 12.1, 11.2 /
+//     12.7, 11.4; in two rounds 16416 x 512 8.6, 7.4 / 9.0, 7.6 / 9.6, 7.9, 20000 x 8192 32.0, 19.7 /
+//     35.2, 19.9 / 39.0, 23.1
+//   4 bits, 16 rows: 4096 x 14336 11.2, 12.7 / 13.8, 12.8 / 16.4, 13.1; in two rounds 5120 x 2560 4.8, 6.1 /
+//     5.4, 6.3 / 6.2, 6.4 and 5120 x 4096 7.3, 7.3 / 9.1, 7.5 / 10.2, 7.6
+//   4 bits, 32 rows: 8192 x 8192 9.2, 10.4 / 10.7, 10.5 / 11.9, 10.7; in two rounds 8224 x 2048 5.4,
+//     6.1 / 6.2, 6.4 / 6.9, 6.5
+//   4 bits, 64 rows: 16384 x 8192 14.2, 15.1 / 14.9, 15.2 / 16.0, 15.4; in two rounds 16416 x 512 7.2,
+//     6.3 / 7.4, 6.1 / 7.8, 6.2
+bool few_tokens(int fmt, int64_t n_tok, int64_t n_rows, int64_t n_cols) {
+    if (n_tok <= 16) return true;
+    if (n_tok > 32) return false;
+    // thousands: one round, more of them; by rows a workgroup (16, 32, 64)
+    static const int kLimit[2][3][2] = {{{290, 130}, {150, 0}, {66, 0}}, {{290, 165}, {200, 100}, {230, 0}}};
+    const int rows = stream_rows(n_tok, n_rows, (int)((n_cols + 127) / 128)), cus = cu_count();
+    const int64_t rounds = ((n_rows + rows - 1) / rows + cus - 1) / cus;
+    return rounds * n_tok * n_cols <= 1000 * (int64_t)kLimit[fmt == AERO_MX_INT8 ? 0 : 1][rows >> 5][rounds > 1];
+}
 
 template <int FMT>
 int64_t operand_bytes(int64_t n_tok, int KP) {
@@ -824,21 +857,15 @@ bool launch_stream(const MxGemm& p, hipStream_t s) {
                   dim3((unsigned)((p.N + 16 * WA - 1) / (16 * WA))), dim3(64 * NW), 0, s, p);
 }
 
-// Weight tiles a wave and waves a workgroup of the few-token kernel: more tiles share x (and, in
-// 8 bits, its halves), more workgroups keep more of the chip busy. Measured, us, with 16 (32) rows
-// a workgroup: 4096 x 4096, one token, 4.1 (5.0); 14336 x 4096, 8 tokens, 12.1 (8.7); 28672 x 8192,
-// one token, 31 (27); with 17 to 32 tokens, 16 / 32 / 64 rows: 4096 x 4096 7.4 / 8.8 / 11.3, 8192 x
-// 8192 18 / 12.8 / 16, 14336 x 4096 22 / 16.7 / 12.1. Short rows (up to 12 groups of 128 columns)
-// leave little for eight waves: 9728 x 896, one token, 3.3 with four of them and 3.7, 24 tokens 5.4
-// with 16 rows and one group on its way, 7.9 with 32 rows.
+// (eight waves a workgroup; four on short rows: 9728 x 896, one token, 3.3 us and 3.7)
 template <int FMT>
 bool run_stream(const MxGemm& p, hipStream_t s) {
+    const int rows = stream_rows(p.T, p.N, p.KP);
     if (p.T > 16) {
-        if (p.N >= 12288) return launch_stream<FMT, 4, 2, 8, 2>(p, s);
-        if (p.N >= 6144 && p.KP > 12) return launch_stream<FMT, 2, 2, 8, 2>(p, s);
-        return launch_stream<FMT, 1, 2, 8, 1>(p, s);
+        if (rows == 64) return launch_stream<FMT, 4, 2, 8, 2>(p, s);
+        return rows == 32 ? launch_stream<FMT, 2, 2, 8, 2>(p, s) : launch_stream<FMT, 1, 2, 8, 1>(p, s);
     }
-    if (p.N >= 12288) return launch_stream<FMT, 2, 1, 8, 2>(p, s);
+    if (rows == 32) return launch_stream<FMT, 2, 1, 8, 2>(p, s);
     return p.KP <= 12 ? launch_stream<FMT, 1, 1, 4, 2>(p, s) : launch_stream<FMT, 1, 1, 8, 2>(p, s);
 }
 
@@ -965,7 +992,7 @@ int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, in
         return -1;
     }
     if (!weight_sizes_ok("mx_matmul_workspace", n_rows, n_cols)) return -1;
-    if (few_tokens(n_tok, n_rows)) return 0;
+    if (few_tokens(fmt, n_tok, n_rows, n_cols)) return 0;
     const int KP = (int)((n_cols + 127) / 128);
     return fmt == AERO_MX_INT8 ? operand_bytes<AERO_MX_INT8>(n_tok, KP)
                                : operand_bytes<AERO_MX_FP4>(n_tok, KP);
@@ -993,7 +1020,7 @@ int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, con
     MxGemm p{codes, scales, (const uint8_t*)w, (const uint8_t*)w + weight_codes_bytes(n_rows, n_cols), y,
              n_tok, n_rows, KB, KP, aligned16(y) && n_rows % 4 == 0};
     const hipStream_t s = (hipStream_t)stream;
-    if (!few_tokens(n_tok, n_rows)) {
+    if (!few_tokens(fmt, n_tok, n_rows, n_cols)) {
         const int64_t need = aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok);
         if (workspace == nullptr || !aligned16(workspace) || ws_bytes < need) {
             set_error("mx_matmul: the workspace takes %lld bytes at a 16-byte address", (long long)need);

@@ -742,9 +742,9 @@ int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64
 /* y[t][n] = sum over k of x[t][k] W[n][k] in fp32, x [n_tok][n_cols] in fmt, W of
  * mx_pack; products and the sums within a block are exact. Scale bytes of 8-bit rows
  * below 4 count as 4. Workspace: aero_hip_mx_matmul_workspace bytes (none up to 16 tokens,
- * or 32 with fewer than 20480 rows; then about 1.6 bytes a value of x in 8 bits and 0.53
- * in 4; -1: bad sizes), 16-byte aligned, its contents free between calls; calls that share it must be
- * ordered. */
+ * and up to 32 for small weights; then about 1.6 bytes a value of x in 8 bits and 0.53 in 4;
+ * -1: bad sizes), 16-byte aligned, its contents free between calls; calls that share it must
+ * be ordered. */
 int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok);
 int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, const void* w,
                        int64_t w_bytes, float* y, int64_t n_rows, int64_t n_cols, int64_t n_tok,

@@ -127,3 +127,27 @@ def test_arrays_are_checked():
         ops.act_mul_mx(ops.MX_INT8, "silu", x, arr(63, np.float32), c8, s, 1, 64)
     with pytest.raises(KeyError):
         ops.act_mul_mx(ops.MX_INT8, "relu", x, x, c8, s, 1, 64)
+
+
+@pytest.mark.parametrize("fmt,n_tok,n_rows,n_cols,few", [
+    # us on the few-token kernel (which takes no workspace) and on tiles
+    (0, 16, 1 << 20, 8192, True),
+    (0, 17, 20000, 8192, False),          # 32.0, 19.7: a second round of workgroups
+    (0, 32, 20000, 8192, False),          # 39.0, 23.1
+    (1, 24, 18432, 4096, False),          # 16.5, 11.4
+    (0, 24, 5120, 5120, False),           # 15.3, 11.0
+    (0, 24, 10240, 4096, False),          # 16.2, 10.5
+    (0, 32, 4096, 14336, False),          # 23.3, 19.0
+    (0, 17, 4096, 14336, True),           # 16.9, 18.7
+    (0, 24, 14336, 4096, False),          # 12.2, 11.3
+    (1, 24, 14336, 4096, True),           # 9.4, 9.9
+    (0, 32, 16384, 2048, True),           # 8.5, 9.9
+    (0, 32, 4096, 4096, True),            # 8.6, 9.8
+    (0, 32, 9728, 896, True),             # 6.1, 7.3
+    (1, 32, 5120, 2560, True),            # 6.2, 6.4
+    (0, 33, 32, 32, False),
+])
+def test_which_calls_are_few_tokens(fmt, n_tok, n_rows, n_cols, few):
+    """The rule between the product's two ways, on a chip of 256 CUs, at sizes where the
+    other one was measured to be slower."""
+    assert (_lib.load().aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok) == 0) == few
