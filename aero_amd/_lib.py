@@ -217,6 +217,7 @@ PROTOTYPES = {
     "aero_hip_mx_weight_bytes": (c_int64, [c_int64, c_int64]),
     "aero_hip_mx_pack": (c_int, [vp, vp, vp, c_int64, c_int64, c_int64, vp]),
     "aero_hip_mx_matmul_workspace": (c_int64, [c_int, c_int64, c_int64, c_int64]),
+    "aero_hip_mx_matmul_tiles": (c_int, [c_int, c_int64, c_int64, c_int64]),
     "aero_hip_mx_matmul": (c_int, [c_int, vp, vp, vp, c_int64, vp, c_int64, c_int64, c_int64, vp,
                                    c_int64, vp]),
     "aero_hip_kv_write": (c_int, [c_int, vp, c_int64, c_int64, c_int64, c_int64, c_int64, vp,

@@ -895,6 +895,45 @@ bool launch_split(MxTiles p, hipStream_t s) {
     return launch("mx_split_kernel", mx_split_kernel<FMT, WA, XB, NW, D>, dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
 }
 
+// The tiles by what rounds of them take: the workgroups that run at a time, and microseconds of
+// such a round, for each 128 columns and beside them, fitted to measured calls. All six on the same
+// call, us: 512 x 28672 x 4096 73 / 88 / 88 / 108 / 104 / 108, 512 x 6144 x 4096 42 / 27 / 29 / 29 / 27 /
+// 29, 512 x 4096 x 14336 113 / 58 / 42 / 54 / 49 / 62, 300 x 9728 x 896 17 / 13 / 16 / 16 / 16 / 15, 64 x 4096
+// x 4096 38 / 22 / 16 / 12 / 12 / 10; in 4 bits 333 x 2560 x 10240 (the last four) 20 / 15 / 16 / 18,
+// 1500 x 5120 x 2048 21 / 23 / 28 / 24 / 26 / 26.
+int best_tiles(int fmt, int64_t T, int64_t N, int KP) {
+    struct Tiles {
+        int n, t, per_cu;
+        float each[2], once[2];      // 8 bits, 4 bits
+    };
+    static const Tiles kTiles[6] = {{8, 4, 2, {1.75f, 1.1f}, {5.f, 1.f}},     {8, 2, 1, {0.57f, 0.39f}, {4.5f, 3.3f}},
+                                    {4, 2, 1, {0.31f, 0.15f}, {2.5f, 3.8f}},  {2, 2, 1, {0.21f, 0.1f}, {2.4f, 1.4f}},
+                                    {4, 1, 1, {0.2f, 0.12f}, {2.2f, 1.4f}},   {2, 1, 1, {0.118f, 0.075f}, {1.f, 0.5f}}};
+    const int F = fmt == AERO_MX_INT8 ? 0 : 1;
+    const int64_t tt = tiles32(T), nt = tiles32(N), cus = cu_count();
+    // The largest run two to a CU. A last round of one each has a time of its own: 1932 x 3456 x 3488
+    // in 4 bits 27.4 us, 28.8 on the best of the others; 1609 x 2624 x 1344 22.7 and 24.6. (For up to
+    // 512 columns it stands above the time of a whole round, which is then set too low, its stores
+    // left out; no choice hangs on that, and the lower of the two would be wrong for small calls:
+    // 128 x 14336 x 128 in 4 bits 9.4 on these tiles, 8.1 on 64 x 32.)
+    const float alone = F == 0 ? 1.f * KP + 6.f : 0.65f * KP + 3.f;
+    int best = 0;
+    float least = 0.f;
+    for (int i = 0; i < 6; ++i) {
+        const Tiles& c = kTiles[i];
+        const int64_t n = ((nt + c.n - 1) / c.n) * ((tt + c.t - 1) / c.t);
+        const int64_t slots = c.per_cu * cus, last = n % slots;
+        const float round = c.each[F] * KP + c.once[F];
+        const float cost = (float)(n / slots) * round +
+                           (last == 0 ? 0.f : i == 0 && last <= cus ? alone : round);
+        if (i == 0 || cost < least) {
+            best = i;
+            least = cost;
+        }
+    }
+    return best;
+}
+
 template <int FMT>
 bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
     const int64_t tt = tiles32(g.T), nt = tiles32(g.N);
@@ -909,38 +948,7 @@ bool run_tiles(const MxGemm& g, void* ws, hipStream_t s) {
                 g.xs, o, os, g.T, g.KB, g.KP, n))
         return false;
     const MxTiles p{g.w, g.ws, o, os, g.y, g.T, g.N, g.KP, (g.KB + 1) / 2, (int)nt, (int)tt, 0, 0, 4};
-    // The tiles by what rounds of them take: the workgroups that run at a time, and microseconds
-    // of such a round, for each 128 columns and beside them, fitted to measured calls. All six on
-    // the same call, us: 512 x 28672 x 4096 73 / 88 / 88 / 108 / 104 / 108, 512 x 6144 x 4096 42 / 27 /
-    // 29 / 29 / 27 / 29, 512 x 4096 x 14336 113 / 58 / 42 / 54 / 49 / 62, 300 x 9728 x 896 17 / 13 / 16 /
-    // 16 / 16 / 15, 64 x 4096 x 4096 38 / 22 / 16 / 12 / 12 / 10; in 4 bits 333 x 2560 x 10240 (the
-    // last four) 20 / 15 / 16 / 18, 1500 x 5120 x 2048 21 / 23 / 28 / 24 / 26 / 26.
-    struct Tiles {
-        int n, t, slots;
-        float each[2], once[2];      // 8 bits, 4 bits
-    };
-    static const Tiles kTiles[6] = {{8, 4, 512, {1.75f, 1.1f}, {5.f, 1.f}},     {8, 2, 256, {0.57f, 0.39f}, {4.5f, 3.3f}},
-                                    {4, 2, 256, {0.31f, 0.15f}, {2.5f, 3.8f}},  {2, 2, 256, {0.21f, 0.1f}, {2.4f, 1.4f}},
-                                    {4, 1, 256, {0.2f, 0.12f}, {2.2f, 1.4f}},   {2, 1, 256, {0.118f, 0.075f}, {1.f, 0.5f}}};
-    constexpr int F = FMT == AERO_MX_INT8 ? 0 : 1;
-    // (The largest run two to a CU. A last round of one each is shorter: 1932 x 3456 x 3488 in 4
-    // bits 27.4 us, 28.8 on the best of the others; 1609 x 2624 x 1344 22.7 and 24.6.)
-    const float alone = FMT == AERO_MX_INT8 ? 1.f * g.KP + 6.f : 0.65f * g.KP + 3.f;
-    int best = 0;
-    float least = 0.f;
-    for (int i = 0; i < 6; ++i) {
-        const Tiles& c = kTiles[i];
-        const int64_t n = ((nt + c.n - 1) / c.n) * ((tt + c.t - 1) / c.t);
-        const float round = c.each[F] * g.KP + c.once[F];
-        const int64_t last = n % c.slots;
-        const float cost = (float)(n / c.slots) * round +
-                           (last == 0 ? 0.f : i == 0 && last <= c.slots / 2 ? alone : round);
-        if (i == 0 || cost < least) {
-            best = i;
-            least = cost;
-        }
-    }
-    switch (tune("mx_tiles", best)) {
+    switch (tune("mx_tiles", best_tiles(FMT, g.T, g.N, g.KP))) {
     case 0: return launch_tiles<FMT, 4, 2, 2, 2, 1, 3, false>(p, s);
     case 1: return launch_tiles<FMT, 4, 1, 2, 2, 2, 4, true>(p, s);
     case 2: return launch_split<FMT, 4, 2, 4, 2>(p, s);
@@ -996,6 +1004,13 @@ int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, in
     const int KP = (int)((n_cols + 127) / 128);
     return fmt == AERO_MX_INT8 ? operand_bytes<AERO_MX_INT8>(n_tok, KP)
                                : operand_bytes<AERO_MX_FP4>(n_tok, KP);
+}
+
+int aero_hip_mx_matmul_tiles(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok) {
+    using namespace aero;
+    if (aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok) < 0) return -1;
+    if (few_tokens(fmt, n_tok, n_rows, n_cols)) return 6;
+    return best_tiles(fmt, n_tok, n_rows, (int)((n_cols + 127) / 128));
 }
 
 int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, const void* w,

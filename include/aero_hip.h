@@ -746,6 +746,10 @@ int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64
  * -1: bad sizes), 16-byte aligned, its contents free between calls; calls that share it must
  * be ordered. */
 int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok);
+/* Which kernel such a call takes: 0 .. 5 tiles of 256 x 128, 256 x 64, 128 x 64, 64 x 64,
+ * 128 x 32, 64 x 32 results (the knob mx_tiles in its place), 6 the one for few tokens; -1:
+ * bad sizes. */
+int aero_hip_mx_matmul_tiles(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok);
 int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, const void* w,
                        int64_t w_bytes, float* y, int64_t n_rows, int64_t n_cols, int64_t n_tok,
                        void* workspace, int64_t ws_bytes, void* stream);

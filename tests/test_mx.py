@@ -151,3 +151,13 @@ def test_which_calls_are_few_tokens(fmt, n_tok, n_rows, n_cols, few):
     """The rule between the product's two ways, on a chip of 256 CUs, at sizes where the
     other one was measured to be slower."""
     assert (_lib.load().aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok) == 0) == few
+
+
+@pytest.mark.parametrize("fmt,n_tok,n_rows,n_cols,tiles", [
+    (0, 2048, 28672, 4096, 0), (1, 2048, 28672, 4096, 0), (0, 512, 6144, 4096, 1), (0, 512, 4096, 14336, 2),
+    (1, 333, 2560, 10240, 3), (0, 70, 40000, 2048, 4), (1, 64, 4096, 4096, 5), (1, 128, 14336, 128, 5),
+    (0, 1, 4096, 4096, 6), (0, 20, 4096, 4096, 6), (1, 0, 64, 64, 6),
+    (0, 1, 4096, 4095, -1), (0, 1, 0, 64, -1), (2, 1, 64, 64, -1), (0, -1, 64, 64, -1)])
+def test_which_tiles(fmt, n_tok, n_rows, n_cols, tiles):
+    """What the rule takes on a chip of 256 CUs."""
+    assert _lib.load().aero_hip_mx_matmul_tiles(fmt, n_rows, n_cols, n_tok) == tiles
