@@ -16,7 +16,7 @@ import pytest
 
 import mx_ref as R
 from conftest import bits_equal
-from aero_amd import mx, ops
+from aero_amd import _lib, mx, ops
 from aero_amd.device import DeviceArray as DA, Plan, Stream, synchronize, tune_set
 
 pytestmark = pytest.mark.gpu
@@ -565,3 +565,79 @@ def test_product_of_scales_far_apart(hip, T, tiles):
     # the terms' own bound, and half a last bit for each addition of what is subnormal
     room = 2.0 ** -20 * (np.abs(x) @ np.abs(w).T) + 9 * K / 32 * 2.0 ** -150
     assert (np.abs(got[ok] - x @ w.T) <= room).all()
+
+
+# ------------------------------------------------ every tile as calls come to it
+def tiles_of(fmt, T, N, K):
+    return _lib.lib().aero_hip_mx_matmul_tiles(fmt, N, K, T)
+
+
+@pytest.mark.parametrize("fmt,tiles,T,N,K", [
+    (INT8, 0, 1859, 9163, 704), (INT8, 0, 2047, 6003, 1056), (INT8, 1, 525, 6207, 3680),
+    (INT8, 1, 263, 7397, 288), (INT8, 2, 835, 1637, 1376), (INT8, 4, 259, 3401, 4704),
+    (INT8, 3, 1031, 897, 1984), (INT8, 4, 707, 815, 2880), (INT8, 4, 35, 9321, 672),
+    (INT8, 4, 141, 4219, 2112), (FP4, 0, 2139, 9101, 1184), (FP4, 0, 2137, 2339, 2400),
+    (FP4, 1, 453, 6511, 960), (FP4, 2, 131, 10657, 2496), (FP4, 3, 181, 3149, 4032),
+    (FP4, 3, 33, 8393, 992), (FP4, 4, 65, 8653, 1984), (FP4, 5, 577, 3363, 6080)])
+def test_product_on_the_tiles_of_its_size(hip, fmt, tiles, T, N, K):
+    """Sizes that the rule itself sends to each size of tile: more workgroups than run at a
+    time, more token tiles than lie side by side, long and ragged sums."""
+    print(f"product fmt={fmt} tiles={tiles} T={T} N={N} K={K}", flush=True)
+    assert tiles_of(fmt, T, N, K) == tiles
+    a = operands(np.random.default_rng(T + N + K), fmt, T, N, K, spread=2)
+    near(product(fmt, *a), *a, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("tiles", range(6))
+@pytest.mark.parametrize("T,N,K", [(645, 265, 4128), (673, 530, 4256)])
+def test_long_sums_on_every_tile(hip, fmt, tiles, T, N, K):
+    print(f"long fmt={fmt} tiles={tiles} T={T} N={N} K={K}", flush=True)
+    a = operands(np.random.default_rng(tiles + T), fmt, T, N, K, spread=2)
+    tune_set("mx_tiles", tiles)
+    try:
+        near(product(fmt, *a), *a, fmt)
+    finally:
+        tune_set("mx_tiles", None)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("tiles", range(6))
+def test_any_codes_on_every_tile(hip, fmt, tiles):
+    """Random bytes for codes and scales, and NaN blocks: their token's, and their weight
+    row's, results are NaN and no others."""
+    print(f"codes fmt={fmt} tiles={tiles}", flush=True)
+    rng = np.random.default_rng(tiles)
+    T, N, K = 150, 290, 608
+    xc = rng.integers(0, 256, (T, ops.mx_row_bytes(fmt, K))).astype(np.uint8)
+    xc = xc.view(np.int8) if fmt == INT8 else xc
+    xs, ws = (rng.integers(107, 147, (n, K // 32)).astype(np.uint8) for n in (T, N))
+    wc = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    xs[1, 3], xs[149, 18], ws[7, 6], ws[289, 0] = 255, 255, 255, 255
+    tune_set("mx_tiles", tiles)
+    try:
+        got = product(fmt, xc, xs, wc, ws)
+    finally:
+        tune_set("mx_tiles", None)
+    nan = np.zeros((T, N), bool)
+    nan[[1, 149]], nan[:, [7, 289]] = True, True
+    assert np.array_equal(np.isnan(got), nan)
+    x, w = (np.nan_to_num(R.values(*a)) for a in ((xc, xs, fmt), (wc, ws, FP4)))
+    ok = ~nan
+    assert (np.abs(got - x @ w.T)[ok] <= (2.0 ** -20 * (np.abs(x) @ np.abs(w).T))[ok]).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_dequant_bit_for_bit(hip, fmt):
+    """Every code under every scale byte, the sign of zeros too."""
+    per = 256 if fmt == INT8 else 32
+    codes = np.tile(np.arange(256, dtype=np.uint8).view(np.int8), (256, 1)) if fmt == INT8 else \
+        np.tile(R.pack(np.arange(32)[None] % 16, FP4), (256, 1))
+    s = np.repeat(np.arange(256, dtype=np.uint8)[:, None], per // 32, 1)
+    out = DA.empty((256, per))
+    ops.mx_dequant(fmt, DA.from_numpy(codes), DA.from_numpy(s), out, 256, per)
+    with np.errstate(over="ignore"):
+        want = R.values(codes, s, fmt).astype(np.float32)
+    got = out.numpy()
+    assert np.isnan(got[255]).all() and not np.isnan(got[:255]).any()
+    assert bits_equal(got[:255], want[:255])
