@@ -15,7 +15,7 @@
 namespace aero {
 namespace {
 
-constexpr int64_t kMaxBlocks = 0x7fffffff;
+constexpr int64_t kMaxRows = 0x7fffffff;
 
 __device__ __forceinline__ float4 ld4(const float* p, bool vec) {
     if (vec) return ld_stream(p);
@@ -138,8 +138,7 @@ bool run_rows(const char* name, const float* g, const float* u, uint8_t* codes, 
               int64_t rows, int64_t cols, int64_t ld, hipStream_t s) {
     const bool vec = aligned16(g) && (!UP || aligned16(u)) && ld % 4 == 0;
     const int64_t nq = cols / 4;
-    const int64_t per = (int64_t)1 << 31;             // quads a launch: indices of 32 bits
-    const int64_t step = nq >= per ? 1 : per / nq;
+    const int64_t step = kMxLanes / nq;
     for (int64_t r = 0; r < rows; r += step) {
         const int64_t n = (rows - r < step ? rows - r : step) * nq;
         if (!launch(name, mx_rows_kernel<FMT, KIND, UP>, dim3((unsigned)((n + 255) / 256)),
@@ -304,18 +303,37 @@ void mx_norm_any_kernel(MxNorm p) {
     }
 }
 
+// A workgroup of bs lanes a row.
+template <int FMT>
+bool launch_rows(const char* name, void (*kernel)(MxNorm), int bs, const MxNorm& p, int64_t rows, hipStream_t s) {
+    const int64_t step = kMxLanes / bs;
+    for (int64_t r = 0; r < rows; r += step) {
+        MxNorm q = p;
+        q.x += r * p.cols;
+        if (p.d != nullptr) {
+            q.d += r * p.cols;
+            q.xo += r * p.cols;
+        }
+        q.codes += r * mx_row_bytes(FMT, p.cols);
+        q.scales += r * (p.cols / 32);
+        if (!launch(name, kernel, dim3((unsigned)(rows - r < step ? rows - r : step)), dim3((unsigned)bs), 0, s, q))
+            return false;
+    }
+    return true;
+}
+
 template <int FMT, int BS, int V>
 bool launch_norm(const MxNorm& p, int64_t rows, hipStream_t s) {
-    return launch("mx_norm_kernel",
-                  p.d != nullptr ? mx_norm_kernel<FMT, BS, V, true> : mx_norm_kernel<FMT, BS, V, false>,
-                  dim3((unsigned)rows), dim3(BS), 0, s, p);
+    return launch_rows<FMT>("mx_norm_kernel",
+                            p.d != nullptr ? mx_norm_kernel<FMT, BS, V, true> : mx_norm_kernel<FMT, BS, V, false>,
+                            BS, p, rows, s);
 }
 
 template <int FMT>
 bool run_norm(const MxNorm& p, int64_t rows, hipStream_t s) {
     const int64_t nq = p.cols / 4;
     if (!p.vec || nq > 8192)
-        return launch("mx_norm_any_kernel", mx_norm_any_kernel<FMT>, dim3((unsigned)rows), dim3(256), 0, s, p);
+        return launch_rows<FMT>("mx_norm_any_kernel", mx_norm_any_kernel<FMT>, 256, p, rows, s);
     if (nq <= 64) return launch_norm<FMT, 64, 1>(p, rows, s);
     if (nq <= 128) return launch_norm<FMT, 64, 2>(p, rows, s);
     if (nq <= 256) return launch_norm<FMT, 256, 1>(p, rows, s);
@@ -357,6 +375,17 @@ void mx_dequant_kernel(const uint8_t* codes, const uint8_t* scales, float* out, 
     }
 }
 
+template <int FMT>
+bool run_dequant(const uint8_t* codes, const uint8_t* scales, float* out, int64_t n, hipStream_t s) {
+    for (int64_t i = 0; i < n; i += kMxLanes) {
+        const int64_t m = n - i < kMxLanes ? n - i : kMxLanes;
+        if (!launch("mx_dequant_kernel", mx_dequant_kernel<FMT>, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, s,
+                    codes + mx_row_bytes(FMT, 4 * i), scales + i / 8, out + 4 * i, m, aligned16(out)))
+            return false;
+    }
+    return true;
+}
+
 }  // namespace
 
 bool mx_rows_ok(const char* what, int fmt, const void* codes, const void* scales, int64_t rows,
@@ -365,7 +394,7 @@ bool mx_rows_ok(const char* what, int fmt, const void* codes, const void* scales
         set_error("%s: unknown format %d", what, fmt);
         return false;
     }
-    if (codes == nullptr || scales == nullptr || rows < 0 || rows > kMaxBlocks) {
+    if (codes == nullptr || scales == nullptr || rows < 0 || rows > kMaxRows) {
         set_error("%s: bad arguments", what);
         return false;
     }
@@ -461,18 +490,10 @@ int aero_hip_mx_dequant(int fmt, const uint8_t* codes, const uint8_t* scales, fl
         !rows_in_ok("mx_dequant", out, nullptr, cols, cols))
         return 0;
     if (rows == 0) return 1;
-    const int64_t n = rows * (cols / 4), blocks = (n + 255) / 256;
-    if (blocks > kMaxBlocks) {
-        set_error("mx_dequant: too many values (%lld rows of %lld)", (long long)rows, (long long)cols);
-        return 0;
-    }
+    const int64_t n = rows * (cols / 4);
     const hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)blocks), block(256);
-    return (fmt == AERO_MX_INT8
-                ? launch("mx_dequant_kernel", mx_dequant_kernel<AERO_MX_INT8>, grid, block, 0, s, codes,
-                         scales, out, n, aligned16(out))
-                : launch("mx_dequant_kernel", mx_dequant_kernel<AERO_MX_FP4>, grid, block, 0, s, codes,
-                         scales, out, n, aligned16(out)))
+    return (fmt == AERO_MX_INT8 ? run_dequant<AERO_MX_INT8>(codes, scales, out, n, s)
+                                : run_dequant<AERO_MX_FP4>(codes, scales, out, n, s))
                ? 1 : 0;
 }
 

@@ -116,6 +116,10 @@ __device__ __forceinline__ bool mx_sure(float4 h, uint32_t amax, float d) {
     }
 }
 
+// Lanes of one launch: HIP takes fewer than 2^32, and the kernels here count quads of a launch in
+// 32 bits. Larger calls are several launches.
+constexpr int64_t kMxLanes = (int64_t)1 << 31;
+
 inline int64_t mx_row_bytes(int fmt, int64_t cols) { return fmt == AERO_MX_FP4 ? cols / 2 : cols; }
 
 // What every call over rows checks first.

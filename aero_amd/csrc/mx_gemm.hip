@@ -50,8 +50,8 @@ struct MxGemm {
 // smallest scale.
 __global__ __launch_bounds__(256)
 void mx_pack_kernel(const uint8_t* codes, const uint8_t* scales, uint8_t* w, uint8_t* ws, int64_t rows,
-                    int KB, int KP, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                    int KB, int KP, int64_t first, int64_t n) {
+    const int64_t i = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const int r = (int)(i & 31);
     const int64_t tile = (i >> 5) / (4 * KP);
@@ -851,10 +851,18 @@ int64_t operand_bytes(int64_t n_tok, int KP) {
     return tiles32(n_tok) * KP * (2 * kStepBytes<FMT> + 128);
 }
 
+// Workgroups of one launch: fewer than 2^32 lanes.
+bool grid_ok(int64_t T, int64_t N, int64_t grid, int lanes) {
+    if (grid * lanes <= 0xffffffff) return true;
+    set_error("mx_matmul: %lld x %lld results are too many", (long long)T, (long long)N);
+    return false;
+}
+
 template <int FMT, int WA, int XB, int NW, int D>
 bool launch_stream(const MxGemm& p, hipStream_t s) {
-    return launch("mx_stream_kernel", mx_stream_kernel<FMT, WA, XB, NW, D>,
-                  dim3((unsigned)((p.N + 16 * WA - 1) / (16 * WA))), dim3(64 * NW), 0, s, p);
+    const int64_t grid = (p.N + 16 * WA - 1) / (16 * WA);
+    return grid_ok(p.T, p.N, grid, 64 * NW) &&
+           launch("mx_stream_kernel", mx_stream_kernel<FMT, WA, XB, NW, D>, dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
 }
 
 // (eight waves a workgroup; four on short rows: 9728 x 896, one token, 3.3 us and 3.7)
@@ -875,11 +883,8 @@ bool launch_tiles(MxTiles p, hipStream_t s) {
     p.bn = (p.nt + S::TN - 1) / S::TN;
     p.bt = (p.tt + S::TT - 1) / S::TT;
     const int64_t grid = ((int64_t)p.bn * p.bt + 7) / 8 * 8;
-    if (grid > 0x7fffffff) {
-        set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
-        return false;
-    }
-    return launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, GK, NB, PIPE>, dim3((unsigned)grid),
+    return grid_ok(p.T, p.N, grid, 64 * S::NW) &&
+           launch("mx_tiles_kernel", mx_tiles_kernel<FMT, WA, XB, GN, GT, GK, NB, PIPE>, dim3((unsigned)grid),
                   dim3(64 * S::NW), 0, s, p);
 }
 
@@ -888,11 +893,8 @@ bool launch_split(MxTiles p, hipStream_t s) {
     p.bn = (p.nt + WA - 1) / WA;
     p.bt = (p.tt + XB - 1) / XB;
     const int64_t grid = ((int64_t)p.bn * p.bt + 7) / 8 * 8;
-    if (grid > 0x7fffffff) {
-        set_error("mx_matmul: %lld x %lld results are too many", (long long)p.T, (long long)p.N);
-        return false;
-    }
-    return launch("mx_split_kernel", mx_split_kernel<FMT, WA, XB, NW, D>, dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
+    return grid_ok(p.T, p.N, grid, 64 * NW) &&
+           launch("mx_split_kernel", mx_split_kernel<FMT, WA, XB, NW, D>, dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
 }
 
 // The tiles by what rounds of them take: the workgroups that run at a time, and microseconds of
@@ -981,16 +983,16 @@ int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64
         return 0;
     }
     const int KB = (int)(n_cols / 32), KP = (KB + 3) / 4;
-    const int64_t n = tiles32(n_rows) * 32 * 4 * KP, blocks = (n + 255) / 256;
-    if (blocks > 0x7fffffff) {
-        set_error("mx_pack: %lld rows of %lld columns are too many", (long long)n_rows,
-                  (long long)n_cols);
-        return 0;
-    }
+    const int64_t n = tiles32(n_rows) * 32 * 4 * KP;
     uint8_t* codes_out = (uint8_t*)w;
-    return launch("mx_pack_kernel", mx_pack_kernel, dim3((unsigned)blocks), dim3(256), 0,
-                  (hipStream_t)stream, codes, scales, codes_out,
-                  codes_out + weight_codes_bytes(n_rows, n_cols), n_rows, KB, KP, n) ? 1 : 0;
+    for (int64_t i = 0; i < n; i += kMxLanes) {
+        const int64_t m = n - i < kMxLanes ? n - i : kMxLanes;
+        if (!launch("mx_pack_kernel", mx_pack_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0,
+                    (hipStream_t)stream, codes, scales, codes_out,
+                    codes_out + weight_codes_bytes(n_rows, n_cols), n_rows, KB, KP, i, n))
+            return 0;
+    }
+    return 1;
 }
 
 int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok) {

@@ -641,3 +641,47 @@ def test_dequant_bit_for_bit(hip, fmt):
     got = out.numpy()
     assert np.isnan(got[255]).all() and not np.isnan(got[:255]).any()
     assert bits_equal(got[:255], want[:255])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_norm_of_more_rows_than_a_launch_takes(hip, fmt):
+    """2^26 + 3 rows of 32 values, 2^32 lanes and more: rows on both sides of what one launch
+    takes, and the last."""
+    rows, cols = (1 << 26) + 3, 32
+    x = DA.empty((rows, cols))
+    ops.fill_f32(x, 1.0)
+    codes = DA.empty((rows, ops.mx_row_bytes(fmt, cols)), np.int8 if fmt == INT8 else np.uint8)
+    scales = DA.empty((rows, 1), np.uint8)
+    rng = np.random.default_rng(3)
+    at = [0, (1 << 25) - 2, rows - 4]          # four rows each, none of them twice
+    h = rng.standard_normal((len(at), 4, cols)).astype(np.float32)
+    for r, v in zip(at, h):
+        x.view(shape=(4, cols), offset_bytes=r * 4 * cols).copy_from(v)
+    ops.rmsnorm_mx(fmt, x, None, codes, scales, rows, cols, 1e-5)
+    synchronize()
+    per = ops.mx_row_bytes(fmt, cols)
+    for r, v in zip(at, h):
+        same(codes.view(shape=(4, per), offset_bytes=r * per), scales.view(shape=(4, 1), offset_bytes=r),
+             R.quantise(R.norm(v, None, 1e-5, False), fmt))
+
+
+def test_dequant_of_more_values_than_a_launch_takes(hip):
+    """2^33 values and some: 34 GB written in two launches."""
+    cols = 1 << 13
+    rows = (1 << 20) + 5
+    codes, scales = DA.empty((rows, cols // 2), np.uint8), DA.empty((rows, cols // 32), np.uint8)
+    out = DA.empty((rows, cols))
+    rng = np.random.default_rng(4)
+    at = [0, (1 << 20) - 2, rows - 2]
+    for r in at:
+        x = rng.standard_normal((2, cols)).astype(np.float32)
+        c, s = R.quantise(x, FP4)
+        codes.view(shape=c.shape, offset_bytes=r * c.shape[1]).copy_from(c)
+        scales.view(shape=s.shape, offset_bytes=r * s.shape[1]).copy_from(s)
+    ops.mx_dequant(FP4, codes, scales, out, rows, cols)
+    synchronize()
+    for r in at:
+        c = codes.view(shape=(2, cols // 2), offset_bytes=r * (cols // 2)).numpy()
+        s = scales.view(shape=(2, cols // 32), offset_bytes=r * (cols // 32)).numpy()
+        got = out.view(shape=(2, cols), offset_bytes=r * 4 * cols).numpy()
+        assert bits_equal(got, R.values(c, s, FP4).astype(np.float32))

@@ -161,3 +161,45 @@ def test_which_calls_are_few_tokens(fmt, n_tok, n_rows, n_cols, few):
 def test_which_tiles(fmt, n_tok, n_rows, n_cols, tiles):
     """What the rule takes on a chip of 256 CUs."""
     assert _lib.load().aero_hip_mx_matmul_tiles(fmt, n_rows, n_cols, n_tok) == tiles
+
+
+def recorded(call):
+    """Launches of a call that is recorded, not run: no pointer here is memory."""
+    L = _lib.load()
+    plan = L.aero_hip_plan_create()
+    assert L.aero_hip_plan_begin(plan)
+    try:
+        call()
+    finally:
+        L.aero_hip_plan_end(plan)
+        n = L.aero_hip_plan_size(plan)
+        L.aero_hip_plan_destroy(plan)
+    return n
+
+
+def test_more_lanes_than_a_launch_takes():
+    """A launch has fewer than 2^32 lanes; larger calls are several."""
+    L = _lib.load()
+    for rows, cols, n in ((1 << 25, 32, 1), ((1 << 25) + 1, 32, 2), (1 << 26, 32, 2), ((1 << 26) + 1, 512, 3),
+                          (1 << 23, 1024, 1), ((1 << 23) + 1, 1024, 2), (1 << 21, 16384, 1), ((1 << 22) + 1, 16384, 3)):
+        assert recorded(lambda: _lib.check(L.aero_hip_rmsnorm_mx(
+            0, 16, None, None, None, 16, 16, rows, cols, 1e-5, 0, None), "norm")) == n
+    for addr, rows, n in ((16, 1 << 25, 1), (20, 1 << 25, 4)):         # not at 16 bytes: 256 lanes a row
+        assert recorded(lambda: _lib.check(L.aero_hip_rmsnorm_mx(
+            1, addr, None, None, None, 16, 16, rows, 32, 1e-5, 0, None), "norm")) == n
+    for rows, n in ((1 << 28, 1), ((1 << 28) + 1, 2), ((1 << 30) + 1, 5)):
+        assert recorded(lambda: _lib.check(L.aero_hip_mx_dequant(0, 16, 16, 16, rows, 32, None), "dequant")) == n
+        assert recorded(lambda: _lib.check(L.aero_hip_mx_quantize(1, 16, 32, 16, 16, rows, 32, None), "quantize")) == n
+    for rows, cols, n in ((1 << 24, 4096, 1), ((1 << 24) + 1, 4096, 2), ((1 << 26) - 1, 4096, 4)):
+        assert recorded(lambda: _lib.check(L.aero_hip_mx_pack(
+            16, 16, 16, 1 << 60, rows, cols, None), "pack")) == n
+
+
+@pytest.mark.parametrize("n_tok,n_rows,n", [(1, 1 << 27, 1),
+                                           (16, (1 << 28) - 32, 1), (1, 1 << 28, 0), (20, 1 << 31, 2)])
+def test_products_with_more_rows_than_a_launch_takes(n_tok, n_rows, n):
+    L, ok = _lib.load(), []
+    launches = recorded(lambda: ok.append(L.aero_hip_mx_matmul(
+        0, 16, 16, 16, 1 << 60, 16, n_rows, 32, n_tok, 16, 1 << 60, None)))
+    assert ok == [n > 0]
+    assert launches == n if n else "too many" in _lib.last_error()
