@@ -5,10 +5,10 @@
 // 8-bit x goes through in two halves. A code c = sign * (16 h + l), h and l in 0 .. 15
 // (h up to 8): as 8-bit floats (e4m3) the numbers 0 .. 15 times 2^-9 are the codes 0 .. 15
 // themselves, subnormals and first normals, so a half is a mask and a sign. Its products
-// with 4-bit weights have 8 bits and one exponent range, so the step's sums lose nothing:
-// against 64 bits 1e-7 of the result. The same steps on e4m3 activations keep about 14 bits
-// of each sum of eight products, whose exponents differ (5e-5 measured on random codes): that
-// is why 8 bits are whole numbers here.
+// with 4-bit weights have 8 bits and one exponent range, so a step's sums of eight products
+// lose nothing; added up in fp32, 1e-7 of the result against 64 bits. The same steps on e4m3
+// activations keep about 14 bits of each sum of eight products, whose exponents differ (5e-5
+// measured on random codes): that is why 8 bits are whole numbers here.
 //
 // Sums are in units of y itself. In larger ones (y / 128 would follow from the codes as they
 // are) a sum near 2^-126 would be a subnormal number and lose bits that y has. So the halves'
@@ -392,12 +392,14 @@ __device__ __forceinline__ void store_tile(const MxTiles& p, int nt, int tt, con
 // its share, NB - 1 stages ahead. With PIPE a stage's operands are read into registers while the
 // one before is multiplied.
 //
-// What bounds 256 x 128 (two workgroups a CU) is power: with the matrix steps busy 51% of the time
-// the clock is down to 1.73 GHz (steps alone, from registers, run at 1.9), and a product of
-// 2048 x 28672 x 4096, twice as many steps as 4-bit x would take, is at 1.9-2.0 PFLOP/s (243-256 us;
-// x in 4 bits 3.2). The loads take 106 us of it when nothing else runs, the steps and LDS reads
-// 155, the stores 35, past the caches (42 through them). Measured and not kept: 256 x 256 tiles
-// with the weights straight into registers (282 us, one wave a SIMD).
+// 256 x 128 (two workgroups a CU, two waves a SIMD): 2048 x 28672 x 4096 in 243-256 us, 1.9-2.0
+// PFLOP/s in twice as many steps as 4-bit x takes (150-156, 3.1). Its steps alone would take 131 at
+// the rate they reach from registers (7.3 PFLOP/s, 1.9 GHz). No one thing bounds it: the clock is
+// down to 1.75 GHz (a tenth), the fourth round of workgroups is half full (an eighth), and within a
+// round the parts overlap only in part: loads alone take 106 us, steps and LDS reads 155, stores 35,
+// past the caches (42 through them). Counters: matrix steps busy 52% of the time, LDS reads 24%,
+// a wave waits to issue 49% of its time and for data or the others at the barrier 23%. Measured and
+// not kept: 256 x 256 tiles with the weights straight into registers (282 us, one wave a SIMD).
 template <int FMT, int WA, int XB, int GN, int GT, int GK>
 struct MxShape {
     static constexpr int NW = GN * GT * GK, TN = WA * GN, TT = XB * GT;
@@ -919,11 +921,12 @@ int best_tiles(int fmt, int64_t T, int64_t N, int KP) {
                                     {4, 1, 1, {0.2f, 0.12f}, {2.2f, 1.4f}},   {2, 1, 1, {0.118f, 0.075f}, {1.f, 0.5f}}};
     const int F = fmt == AERO_MX_INT8 ? 0 : 1;
     const int64_t tt = tiles32(T), nt = tiles32(N), cus = cu_count();
-    // The largest run two to a CU. A last round of one each has a time of its own: 1932 x 3456 x 3488
-    // in 4 bits 27.4 us, 28.8 on the best of the others; 1609 x 2624 x 1344 22.7 and 24.6. (For up to
-    // 512 columns it stands above the time of a whole round, which is then set too low, its stores
-    // left out; no choice hangs on that, and the lower of the two would be wrong for small calls:
-    // 128 x 14336 x 128 in 4 bits 9.4 on these tiles, 8.1 on 64 x 32.)
+    // The largest run two to a CU. A last round of one each has a time of its own: 1939 x 3200 x
+    // 12512 in 4 bits 71.7 us, 75.8 on the best of the others; 1932 x 3456 x 3488 28.6 and 28.4, 1609 x
+    // 2624 x 1344 15.3 and 15.3. (For up to 512 columns it stands above the time of a whole round,
+    // which is then set too low, its stores left out; no choice hangs on that, and the lower of the
+    // two would be wrong for small calls: 128 x 14336 x 128 in 4 bits 9.4 on these tiles, 8.1 on 64
+    // x 32.)
     const float alone = F == 0 ? 1.f * KP + 6.f : 0.65f * KP + 3.f;
     int best = 0;
     float least = 0.f;

@@ -836,9 +836,9 @@ _mx_ws = Workspace("microscaled product")
 def mx_matmul(fmt: int, codes: DeviceArray, scales: DeviceArray, w, y: DeviceArray, n_tok: int,
               stream: Stream | None = None) -> None:
     """y [n_tok, w.n_rows] = x W^T in fp32: x microscaled rows [n_tok, w.n_cols] in
-    fmt, w an mx.MxWeight (4 bits). Products and the sums within a block are exact. The
-    workspace grows to the largest call and is kept: calls that overlap on different
-    streams would share its contents. A plan that records the call holds the weights."""
+    fmt, w an mx.MxWeight (4 bits). Products are exact, their sums in fp32. The workspace
+    grows to the largest call and is kept: calls that overlap on different streams would
+    share its contents. A plan that records the call holds the weights."""
     _mx_rows(fmt, codes, scales, n_tok, w.n_cols)
     _need(y, n_tok * w.n_rows, np.float32, "y")
     L = _lib.lib()

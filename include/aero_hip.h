@@ -711,7 +711,8 @@ int aero_hip_write_i32(int32_t* base, int64_t n_base, const int64_t* at, const i
  * [rows][cols/2], scales [rows][cols/32]; cols a multiple of 32, codes at 4 bytes
  * (16 for the product). The quantisers take the smallest scale under which the block's
  * largest magnitude does not pass the format's largest (127/64, 6), 8 bits none below
- * s = 4 (blocks below 2^-123), and the nearest code, halves to even. No counterpart in
+ * s = 4 (blocks below 2^-123) and none above 254 (past 2^127 * 127/64 the largest code
+ * stands in), and the nearest code, halves to even. No counterpart in
  * the reference, which quantises cache vectors only (include/aero/kv.hpp:62-126). */
 #define AERO_MX_INT8 0
 #define AERO_MX_FP4  1
@@ -740,8 +741,8 @@ int64_t aero_hip_mx_weight_bytes(int64_t n_rows, int64_t n_cols);
 int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64_t w_bytes,
                      int64_t n_rows, int64_t n_cols, void* stream);
 /* y[t][n] = sum over k of x[t][k] W[n][k] in fp32, x [n_tok][n_cols] in fmt, W of
- * mx_pack; products and the sums within a block are exact. Scale bytes of 8-bit rows
- * below 4 count as 4. Workspace: aero_hip_mx_matmul_workspace bytes (none up to 16 tokens,
+ * mx_pack; products are exact, their sums in fp32: sqrt(9 n_cols / 32) 2^-24 of the result,
+ * subnormal results to their last bit. Scale bytes of 8-bit rows below 4 count as 4. Workspace: aero_hip_mx_matmul_workspace bytes (none up to 16 tokens,
  * and up to 32 for small weights; then about 1.6 bytes a value of x in 8 bits and 0.53 in 4;
  * -1: bad sizes), 16-byte aligned, its contents free between calls; calls that share it must
  * be ordered. */
