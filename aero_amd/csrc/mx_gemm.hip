@@ -1046,9 +1046,11 @@ int aero_hip_mx_matmul(int fmt, const uint8_t* codes, const uint8_t* scales, con
     MxGemm p{codes, scales, (const uint8_t*)w, (const uint8_t*)w + weight_codes_bytes(n_rows, n_cols), y,
              n_tok, n_rows, KB, KP, aligned16(y) && n_rows % 4 == 0};
     const hipStream_t s = (hipStream_t)stream;
-    if (!few_tokens(fmt, n_tok, n_rows, n_cols)) {
-        const int64_t need = aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok);
-        if (workspace == nullptr || !aligned16(workspace) || ws_bytes < need) {
+    const int64_t need = aero_hip_mx_matmul_workspace(fmt, n_rows, n_cols, n_tok);
+    const bool room = workspace != nullptr && aligned16(workspace) && ws_bytes >= need;
+    // (without a workspace the few-token kernel takes all that it can)
+    if (!few_tokens(fmt, n_tok, n_rows, n_cols) && (room || n_tok > 32)) {
+        if (!room) {
             set_error("mx_matmul: the workspace takes %lld bytes at a 16-byte address", (long long)need);
             return 0;
         }

@@ -745,7 +745,7 @@ int aero_hip_mx_pack(const uint8_t* codes, const uint8_t* scales, void* w, int64
  * subnormal results to their last bit. Scale bytes of 8-bit rows below 4 count as 4. Workspace: aero_hip_mx_matmul_workspace bytes (none up to 16 tokens,
  * and up to 32 for small weights; then about 1.6 bytes a value of x in 8 bits and 0.53 in 4;
  * -1: bad sizes), 16-byte aligned, its contents free between calls; calls that share it must
- * be ordered. */
+ * be ordered. Calls of up to 32 tokens also run without one, some of them slower. */
 int64_t aero_hip_mx_matmul_workspace(int fmt, int64_t n_rows, int64_t n_cols, int64_t n_tok);
 /* Which kernel such a call takes: 0 .. 5 tiles of 256 x 128, 256 x 64, 128 x 64, 64 x 64,
  * 128 x 32, 64 x 32 results (the knob mx_tiles in its place), 6 the one for few tokens; -1:

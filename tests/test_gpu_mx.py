@@ -685,3 +685,21 @@ def test_dequant_of_more_values_than_a_launch_takes(hip):
         s = scales.view(shape=(2, cols // 32), offset_bytes=r * (cols // 32)).numpy()
         got = out.view(shape=(2, cols), offset_bytes=r * 4 * cols).numpy()
         assert bits_equal(got, R.values(c, s, FP4).astype(np.float32))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("T,N,K", [(24, 4112, 4128), (32, 20500, 96), (17, 8230, 2080), (32, 100, 14336)])
+def test_product_without_a_workspace(hip, fmt, T, N, K):
+    """Calls of up to 32 tokens that the rule sends to tiles, on the few-token kernel."""
+    print(f"no workspace fmt={fmt} T={T} N={N} K={K}", flush=True)
+    assert 0 <= tiles_of(fmt, T, N, K) < 6 or K == 2080
+    a = operands(np.random.default_rng(T + N + K), fmt, T, N, K, spread=2)
+    d = [DA.from_numpy(v) for v in a]
+    w = mx.MxWeight(d[2], d[3], N, K)
+    y = DA.from_numpy(np.full(T * N + 64, 7.0, np.float32))
+    _lib.check(_lib.lib().aero_hip_mx_matmul(fmt, d[0].ptr, d[1].ptr, w.buf.ptr, w.buf.nbytes, y.ptr, N, K, T,
+                                             None, 0, None), "mx_matmul")
+    synchronize()
+    got = y.numpy()
+    assert (got[T * N:] == 7).all()
+    near(got[:T * N].reshape(T, N), *a, fmt)

@@ -203,3 +203,16 @@ def test_products_with_more_rows_than_a_launch_takes(n_tok, n_rows, n):
         0, 16, 16, 16, 1 << 60, 16, n_rows, 32, n_tok, 16, 1 << 60, None)))
     assert ok == [n > 0]
     assert launches == n if n else "too many" in _lib.last_error()
+
+
+@pytest.mark.parametrize("n_tok,n_rows,n_cols,ws,launches", [
+    (24, 5120, 5120, True, 2), (24, 5120, 5120, False, 1), (32, 40960, 8192, False, 1), (17, 64, 64, True, 1),
+    (17, 64, 64, False, 1), (33, 64, 64, True, 2), (33, 64, 64, False, 0)])
+def test_few_tokens_without_a_workspace(n_tok, n_rows, n_cols, ws, launches):
+    """Up to 32 tokens need no workspace, whichever kernel the rule would take with one."""
+    L, ok = _lib.load(), []
+    n = recorded(lambda: ok.append(L.aero_hip_mx_matmul(
+        0, 16, 16, 16, 1 << 60, 16, n_rows, n_cols, n_tok, 16 if ws else None, 1 << 60 if ws else 0, None)))
+    assert ok == [launches > 0] and n == launches
+    if not launches:
+        assert "workspace" in _lib.last_error()
